@@ -77,13 +77,43 @@ enum tt_op {
     TT_OP_REDUCE_MAX = 17,
     TT_OP_STEP = 18,    /* x > 0 ? 1 : 0, the ReLU derivative mask (gradient.cpp:200-222) */
     TT_OP_RESHAPE = 19, /* row-major reshape (a view) */
-    TT_OP_EXPAND = 20   /* broadcast_to the node's shape (a view) */
+    TT_OP_EXPAND = 20,  /* broadcast_to the node's shape (a view) */
+    /* Sequence operators (no reference OpType).  Their numbers, and operands beyond
+     * TT_MAX_NODE_INPUTS, are in the tt_op_attrs that tt_node.data points to.  All
+     * operands are float32 except `tokens` (int32); padding is a negative token: the
+     * position's logits are not read, its value and its gradient are 0. */
+    TT_OP_GATED_SCAN = 21,      /* (gate, x[, init]): h[t] = gate[t]*h[t-1] + x[t] along axis dim0,
+                                 * h[-1] = init (or 0).  gate and x have the node's shape, init has it
+                                 * without the axis. */
+    TT_OP_SCAN_LAST = 22,       /* (h): the state after the last step of a TT_OP_GATED_SCAN node, its
+                                 * shape without the axis (init, or 0, when there are no steps) */
+    TT_OP_TOKEN_LOGPROB = 23,   /* (logits[..., V], tokens[...]): log softmax(logits)[token] */
+    TT_OP_POLICY_LOSS = 24,     /* (logits, tokens, old, advantage[, ref]), all but logits of the tokens'
+                                 * shape; f = {clip_low, clip_high, kl}.  Per token, with p the token's
+                                 * log-probability, r = exp(p - old), A = advantage:
+                                 *   -min(r*A, clamp(r, 1-clip_low, 1+clip_high)*A)
+                                 *   + kl*(exp(ref - p) - (ref - p) - 1) */
+    TT_OP_PREFERENCE_LOSS = 25  /* (logits[N, 2, T, V], tokens[N, 2, T], ref[N, 2, T]); f = {beta,
+                                 * smoothing}.  Per pair, with S(j) the sum over answer j's tokens of
+                                 * p - ref and z = beta*(S(0) - S(1)):
+                                 *   -(1-smoothing)*log sigmoid(z) - smoothing*log sigmoid(-z) */
 };
 
-enum tt_dtype { TT_FLOAT32 = 0, TT_FLOAT64 = 1 }; /* include/tinytensor/core/dtype.hpp:10-13 */
+/* include/tinytensor/core/dtype.hpp:10-13; TT_INT32 (token ids) is taken by graph inputs, views
+ * of them and the `tokens` operands above only. */
+enum tt_dtype { TT_FLOAT32 = 0, TT_FLOAT64 = 1, TT_INT32 = 2 };
 
 #define TT_MAX_RANK 8
 #define TT_MAX_NODE_INPUTS 2
+
+/* Attributes of the sequence operators (TT_OP_GATED_SCAN and later), read through tt_node.data.
+ * A node without numbers and with at most TT_MAX_NODE_INPUTS operands may leave it NULL. */
+#define TT_MAX_OPERANDS 5
+typedef struct tt_op_attrs {
+    int32_t more_inputs[TT_MAX_OPERANDS - TT_MAX_NODE_INPUTS]; /* operands 2..num_inputs-1, earlier entries too */
+    int32_t reserved;                                          /* 0 */
+    float f[4];                                                /* the operator's numbers */
+} tt_op_attrs;
 
 /* One graph node, the C image of tinytensor::Node (include/tinytensor/graph/node.hpp). */
 typedef struct tt_node {
@@ -94,11 +124,12 @@ typedef struct tt_node {
     int32_t rank;
     int64_t shape[TT_MAX_RANK];
     int64_t id;                         /* the reference node id, printed as %id in IR text */
-    int64_t dim0, dim1;                 /* Transpose */
+    int64_t dim0, dim1;                 /* Transpose; dim0 also: GatedScan axis */
     int32_t num_axes;                   /* Reduce*: 0 = all axes */
     int32_t keepdims;
     int64_t axes[TT_MAX_RANK];
-    const void* data;                   /* Constant: numel*itemsize bytes, row-major (copied) */
+    const void* data;                   /* Constant: numel*itemsize bytes, row-major (copied);
+                                         * sequence operators: a tt_op_attrs */
     const char* name;                   /* Input name, may be NULL */
     const char* expr;                   /* FusedElementwise expression, may be NULL */
 } tt_node;
@@ -118,7 +149,8 @@ typedef struct tt_compile_options {
     const char* cache_dir;     /* kernel cache directory; NULL or "" = no disk cache */
     int32_t grad_loss;         /* -1, or the node index of a loss to differentiate */
     int32_t num_grad_wrt;      /* with grad_loss: gradients of loss w.r.t. these nodes are */
-    const int32_t* grad_wrt;   /*   appended to the program outputs, in this order */
+    const int32_t* grad_wrt;   /*   appended to the program outputs, in this order
+                                *   (TT_FLAG_GRAD_SEED: one more entry, the seed node) */
     int32_t flags;             /* TT_FLAG_* */
 } tt_compile_options;
 
@@ -131,6 +163,9 @@ typedef struct tt_compile_options {
 #define TT_FLAG_SERIAL 8          /* every launch on the run's stream, one after another (by
                                      default two adjacent independent GEMMs run side by side
                                      on a second stream of the program) */
+#define TT_FLAG_GRAD_SEED 16      /* grad_wrt holds num_grad_wrt + 1 entries; the last one is a node of
+                                     the loss's shape whose value stands for the loss's own gradient
+                                     (instead of ones): vector-Jacobian products */
 
 typedef struct tt_program tt_program;
 
@@ -173,7 +208,10 @@ int tt_program_output_shape(const tt_program* p, int32_t index, int32_t* rank, i
 int tt_program_run(tt_program* p, const void* const* inputs, void* const* outputs, int32_t where,
                    void* stream);
 /* Synchronises the program's last stream and reads its device status word
- * (0 = fine; nonzero = a bounded wait gave up).  Returns TT_ERR_DEVICE_STATUS then. */
+ * (0 = fine; TT_STATUS_BAD_TOKEN = a token id outside the vocabulary, whose position's
+ * value and gradient are NaN; anything else = a bounded wait gave up).  Returns
+ * TT_ERR_DEVICE_STATUS when it is nonzero and clears it. */
+#define TT_STATUS_BAD_TOKEN 0x400
 int tt_program_status(tt_program* p, int32_t* device_status);
 /* Per-launch profiling (Profiler::record_node for compiled mode): when enabled, each
  * run records CUDA events around every launch on the run's stream; enabling resets the

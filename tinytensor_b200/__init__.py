@@ -47,16 +47,22 @@ from .graph import (  # noqa: F401
     exp,
     float32,
     float64,
+    gated_scan,
+    int32,
     matmul,
     max,
     mean,
     mul,
     neg,
+    policy_loss,
+    preference_loss,
     relu,
+    scan_last,
     sigmoid,
     sub,
     sum,
     tanh,
+    token_logprob,
     transpose,
 )
 from .optim import SGD  # noqa: F401

@@ -13,17 +13,19 @@ LIB_PATH = os.path.join(_HERE, "lib", "libtt_cuda.so")
 
 TT_MAX_RANK = 8
 TT_MAX_NODE_INPUTS = 2
+TT_MAX_OPERANDS = 5
 TT_DP_ID_BYTES = 128
 
 # op codes (reference OpType order, then additions)
 OP_INPUT, OP_CONSTANT, OP_ADD, OP_SUB, OP_MUL, OP_DIV, OP_RELU, OP_SIGMOID = range(8)
 OP_MATMUL, OP_TRANSPOSE, OP_REDUCE_SUM, OP_REDUCE_MEAN, OP_OUTPUT, OP_FUSED = range(8, 14)
 OP_EXP, OP_NEG, OP_TANH, OP_REDUCE_MAX, OP_STEP, OP_RESHAPE, OP_EXPAND = range(14, 21)
+OP_GATED_SCAN, OP_SCAN_LAST, OP_TOKEN_LOGPROB, OP_POLICY_LOSS, OP_PREFERENCE_LOSS = range(21, 26)
 
 HOST, DEVICE = 0, 1
 H2D, D2H, D2D = 1, 2, 3
 INFO_ORIGINAL_IR, INFO_OPTIMIZED_IR, INFO_SOURCE, INFO_PLAN, INFO_CUBIN_PATH = range(5)
-FLAG_NO_FUSION, FLAG_NO_GEMM_FUSION, FLAG_HOST_ONLY, FLAG_SERIAL = 1, 2, 4, 8
+FLAG_NO_FUSION, FLAG_NO_GEMM_FUSION, FLAG_HOST_ONLY, FLAG_SERIAL, FLAG_GRAD_SEED = 1, 2, 4, 8, 16
 
 
 class TinyTensorError(Exception):
@@ -67,7 +69,8 @@ class RuntimeExecutionError(TinyTensorError):
 
 
 class DeviceStatusError(RuntimeExecutionError):
-    """A kernel gave up a bounded wait and reported it through the status word."""
+    """A kernel gave up a bounded wait, or met a token id outside the vocabulary, and
+    reported it through the status word."""
 
 
 class NoDeviceError(RuntimeExecutionError):
@@ -92,6 +95,14 @@ _STATUS = {
     11: ValueError,
     12: CommError,
 }
+
+
+class TTOpAttrs(ctypes.Structure):
+    _fields_ = [
+        ("more_inputs", ctypes.c_int32 * (TT_MAX_OPERANDS - TT_MAX_NODE_INPUTS)),
+        ("reserved", ctypes.c_int32),
+        ("f", ctypes.c_float * 4),
+    ]
 
 
 class TTNode(ctypes.Structure):

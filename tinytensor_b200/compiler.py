@@ -16,8 +16,8 @@ from collections.abc import Mapping, Sequence
 import numpy as np
 
 from . import _lib
-from ._lib import RuntimeExecutionError, ShapeError, TypeError
-from .graph import Graph, Node
+from ._lib import IRError, RuntimeExecutionError, ShapeError, TypeError
+from .graph import Graph, Node, float32, int32
 
 __all__ = ["compile", "compile_gradients", "CompiledProgram", "gradients", "Tensor", "tensor",
            "DeviceBuffer", "Stream", "Event", "CudaGraph", "launch_count"]
@@ -158,25 +158,50 @@ class CudaGraph:
             self.handle = None
 
 
-class DeviceBuffer:
-    """A float32 device allocation (cudaMalloc) with a shape."""
+_NUMPY = {float32: np.float32, int32: np.int32}  # what device buffers hold
 
-    def __init__(self, shape, pinned_host=False):
+
+def _numpy_dtype(dtype):
+    if dtype not in _NUMPY:
+        raise TypeError(f"buffers hold float32 or int32, not {dtype}")
+    return _NUMPY[dtype]
+
+
+def _to_int32(a):
+    """`a` as an int32 array; refuses values that are not whole numbers of that range."""
+    a = np.asarray(a)
+    if a.dtype == np.int32:
+        return np.ascontiguousarray(a).reshape(a.shape)
+    if a.dtype.kind not in "iu":
+        raise TypeError(f"int32 data is made from whole numbers, not {a.dtype}")
+    if a.size and (int(a.min()) < -2**31 or int(a.max()) >= 2**31):
+        raise TypeError("a value does not fit int32")
+    return np.array(a, dtype=np.int32, order="C")
+
+
+class DeviceBuffer:
+    """A float32 (or int32, for token ids) device allocation (cudaMalloc) with a shape."""
+
+    def __init__(self, shape, pinned_host=False, dtype=float32):
+        self._np = _numpy_dtype(dtype)
+        self.dtype = dtype
         self.shape = [int(d) for d in shape]
         self.nbytes = int(np.prod(self.shape, dtype=np.int64)) * 4
         p = ctypes.c_void_p()
         _lib.check(_lib.lib.tt_device_alloc(self.nbytes, ctypes.byref(p)))
         self.ptr = p.value
 
+    def _host(self, arr):
+        return _to_int32(arr) if self.dtype == int32 else np.ascontiguousarray(arr, dtype=np.float32)
+
     @classmethod
-    def from_numpy(cls, arr, stream=None):
-        arr = np.ascontiguousarray(arr, dtype=np.float32)
-        b = cls(arr.shape)
+    def from_numpy(cls, arr, stream=None, dtype=float32):
+        b = cls(np.shape(arr) if dtype == int32 else np.ascontiguousarray(arr, dtype=np.float32).shape, dtype=dtype)
         b.copy_from(arr, stream)
         return b
 
     def copy_from(self, arr, stream=None):
-        arr = np.ascontiguousarray(arr, dtype=np.float32)
+        arr = self._host(arr)
         if arr.nbytes != self.nbytes:
             raise ShapeError(f"copy of {arr.nbytes} bytes into a {self.nbytes}-byte buffer")
         h = stream.handle if stream is not None else None
@@ -184,7 +209,7 @@ class DeviceBuffer:
         _lib.check(_lib.lib.tt_stream_sync(h))
 
     def numpy(self, stream=None):
-        out = np.empty(self.shape, dtype=np.float32)
+        out = np.empty(self.shape, dtype=self._np)
         h = stream.handle if stream is not None else None
         _lib.check(_lib.lib.tt_memcpy(out.ctypes.data, self.ptr, self.nbytes, _lib.D2H, h))
         _lib.check(_lib.lib.tt_stream_sync(h))
@@ -203,15 +228,17 @@ class DeviceBuffer:
 
 
 class PinnedBuffer:
-    """Page-locked host float32 array (cudaMallocHost), usable as a numpy array."""
+    """Page-locked host float32 (or int32) array (cudaMallocHost), usable as a numpy array."""
 
-    def __init__(self, shape):
+    def __init__(self, shape, dtype=float32):
+        ctype = ctypes.c_int32 if _numpy_dtype(dtype) is np.int32 else ctypes.c_float
+        self.dtype = dtype
         self.shape = [int(d) for d in shape]
         n = int(np.prod(self.shape, dtype=np.int64))
         p = ctypes.c_void_p()
         _lib.check(_lib.lib.tt_host_alloc(max(4, n * 4), ctypes.byref(p)))
         self.ptr = p.value
-        self.array = np.ctypeslib.as_array(ctypes.cast(p, ctypes.POINTER(ctypes.c_float)), shape=(max(1, n),))[:n]
+        self.array = np.ctypeslib.as_array(ctypes.cast(p, ctypes.POINTER(ctype)), shape=(max(1, n),))[:n]
         self.array = self.array.reshape(self.shape)
 
     def __del__(self):
@@ -281,8 +308,8 @@ class CompiledProgram:
             if isinstance(v, Tensor):
                 v = v.numpy()
             # converted to the node dtype like tensor(v, dtype=expected_dtype) (compiler.py:31-45);
-            # the device computes in float32
-            a = np.array(v, dtype=np.float32, order="C", copy=None)  # 0-d stays 0-d
+            # the device computes in float32, token ids are int32
+            a = _to_int32(v) if n.dtype == int32 else np.array(v, dtype=np.float32, order="C", copy=None)  # 0-d stays 0-d
             if list(a.shape) != n.shape:
                 raise ShapeError(f"Input %{n.id} shape mismatch: expected {n.shape} but got {list(a.shape)}")
             arrays.append(a)
@@ -312,6 +339,9 @@ class CompiledProgram:
         ko = [getattr(x, "ptr", x) for x in outputs]
         cached = self._dev_args
         if cached is None or cached[0] != ki or cached[1] != ko:
+            for n, x in zip(self._inputs, inputs):
+                if (getattr(x, "dtype", n.dtype) == int32) != (n.dtype == int32):
+                    raise TypeError(f"Input %{n.id} is {n.dtype}, its buffer {x.dtype}")
             ip = (ctypes.c_void_p * max(1, len(ki)))(*ki)
             op = (ctypes.c_void_p * max(1, len(ko)))(*ko)
             cached = self._dev_args = (ki, ko, ip, op)
@@ -376,7 +406,7 @@ class CompiledProgram:
         return out
 
 
-def _compile(graph, outputs, optimize, cache_dir, grad_loss=None, wrt=(), device=0, flags=0):
+def _compile(graph, outputs, optimize, cache_dir, grad_loss=None, wrt=(), device=0, flags=0, seed=None):
     if outputs is not None:
         for o in outputs:
             graph.mark_output(o)
@@ -389,10 +419,11 @@ def _compile(graph, outputs, optimize, cache_dir, grad_loss=None, wrt=(), device
     cdir_b = cdir.encode() if cdir else None
     opt.cache_dir = cdir_b
     opt.grad_loss = -1 if grad_loss is None else grad_loss.index
-    wrt_arr = (ctypes.c_int32 * max(1, len(wrt)))(*[n.index for n in wrt])
+    targets = [n.index for n in wrt] + ([] if seed is None else [seed.index])
+    wrt_arr = (ctypes.c_int32 * max(1, len(targets)))(*targets)
     opt.num_grad_wrt = len(wrt)
     opt.grad_wrt = wrt_arr
-    opt.flags = int(flags)
+    opt.flags = int(flags) | (0 if seed is None else _lib.FLAG_GRAD_SEED)
     h = ctypes.c_void_p()
     _lib.check(_lib.lib.tt_compile(ctypes.byref(g), ctypes.byref(opt), ctypes.byref(h)))
     return CompiledProgram(graph, outs, h.value, wrt)
@@ -413,14 +444,19 @@ def compile(graph: Graph, outputs: Sequence[Node] | None = None, mode: str = "cu
 
 def compile_gradients(graph: Graph, loss: Node, wrt: Sequence[Node], outputs: Sequence[Node] | None = None,
                       optimize: bool = True, cache_dir: str | None = None, device: int = 0,
-                      flags: int = 0) -> CompiledProgram:
+                      flags: int = 0, seed: Node | None = None) -> CompiledProgram:
     """Compiles forward + symbolic backward: program outputs are `outputs` (default
-    [loss]) followed by d loss / d w for every w in `wrt`, in order."""
+    [loss]) followed by d loss / d w for every w in `wrt`, in order.  `seed`, a node of
+    the loss's shape, stands for the gradient of the loss itself (ones when None): the
+    results are then the vector-Jacobian products of a loss of any shape."""
+    if seed is not None and seed._graph is not graph:
+        raise IRError("Node belongs to a different graph")
     outs = [loss] if outputs is None else list(outputs)
     g2 = graph  # outputs are marked on the graph, as tt.compile does
     for o in outs:
         g2.mark_output(o)
-    return _compile(g2, None, optimize, cache_dir, grad_loss=loss, wrt=list(wrt), device=device, flags=flags)
+    return _compile(g2, None, optimize, cache_dir, grad_loss=loss, wrt=list(wrt), device=device, flags=flags,
+                    seed=seed)
 
 
 def gradients(graph: Graph, loss: Node, inputs: Mapping, mode: str = "cuda", cache_dir: str | None = None):
@@ -428,7 +464,7 @@ def gradients(graph: Graph, loss: Node, inputs: Mapping, mode: str = "cuda", cac
 
     The reference evaluates this eagerly on the host (src/autodiff/gradient.cpp); here
     the backward pass is emitted as graph nodes and run as one compiled GPU program."""
-    wrt = [n for n in inputs.keys() if isinstance(n, Node)]
+    wrt = [n for n in inputs.keys() if isinstance(n, Node) and n.dtype != int32]  # token ids have none
     key = (loss.index, tuple(n.index for n in wrt), graph._version)
     cache = graph.__dict__.setdefault("_grad_programs", {}) if hasattr(graph, "__dict__") else {}
     prog = cache.get(key)

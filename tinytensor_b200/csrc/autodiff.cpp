@@ -105,8 +105,19 @@ struct Builder {
 
 }  // namespace
 
-void append_gradients(Graph& g, int loss, const std::vector<int>& wrt) {
+void append_gradients(Graph& g, int loss, const std::vector<int>& wrt, int seed) {
     if (loss < 0 || static_cast<size_t>(loss) >= g.nodes.size()) fail(TT_ERR_INVALID, "loss node out of range");
+    if (seed != -1) {
+        if (seed < 0 || static_cast<size_t>(seed) >= g.nodes.size()) fail(TT_ERR_INVALID, "seed node out of range");
+        if (g.nodes[static_cast<size_t>(seed)].shape != g.nodes[static_cast<size_t>(loss)].shape)
+            fail(TT_ERR_SHAPE, "the seed must have the loss's shape " + shape_str(g.nodes[static_cast<size_t>(loss)].shape) +
+                                   ", got " + shape_str(g.nodes[static_cast<size_t>(seed)].shape));
+        if (g.nodes[static_cast<size_t>(seed)].dtype != g.nodes[static_cast<size_t>(loss)].dtype)
+            fail(TT_ERR_TYPE, "the seed must have the loss's dtype");
+    }
+    for (int w : wrt)
+        if (w >= 0 && static_cast<size_t>(w) < g.nodes.size() && g.nodes[static_cast<size_t>(w)].dtype == TT_INT32)
+            fail(TT_ERR_TYPE, "token ids have no gradient");
     const size_t nfwd = static_cast<size_t>(loss) + 1;  // nodes after the loss cannot reach it
     Builder b{g};
     std::unordered_map<int, int> grads;
@@ -118,8 +129,25 @@ void append_gradients(Graph& g, int loss, const std::vector<int>& wrt) {
             it->second = b.mk(TT_OP_ADD, {it->second, contrib});
     };
 
-    // Seed dL/dL = ones(loss.shape) (gradient.cpp:131).
-    {
+    // Gradients of scan states: of a whole GatedScan (grads) and of its last state alone
+    // (last_grads), which enters the same backward scan as its first carry.
+    std::unordered_map<int, int> last_grads;
+    auto backward = [&](int op, std::vector<int> in, int64_t axis, std::vector<int64_t> has, std::vector<float> attr) {
+        Node q;
+        q.op = op;
+        q.in = std::move(in);
+        q.dim0 = axis;
+        q.axes = std::move(has);
+        q.attr = std::move(attr);
+        q.id = g.next_id;
+        infer_shape(g, q);
+        return g.add(std::move(q));
+    };
+
+    // Seed dL/dL = ones(loss.shape) (gradient.cpp:131), or the caller's seed.
+    if (seed >= 0) {
+        grads[loss] = seed;
+    } else {
         int one = b.scalar(1.0f, b.dtype(loss));
         grads[loss] = b.view(TT_OP_EXPAND, one, b.shape(loss));
     }
@@ -127,8 +155,9 @@ void append_gradients(Graph& g, int loss, const std::vector<int>& wrt) {
     for (size_t ii = nfwd; ii-- > 0;) {
         int i = static_cast<int>(ii);
         auto git = grads.find(i);
-        if (git == grads.end()) continue;
-        const int gidx = git->second;
+        const auto lit = last_grads.find(i);
+        if (git == grads.end() && lit == last_grads.end()) continue;
+        const int gidx = git == grads.end() ? -1 : git->second;  // -1: a scan reached through its last state only
         const Node n = g.nodes[ii];  // copy: g.nodes grows below
         const int dt = n.dtype;
         switch (n.op) {
@@ -219,6 +248,37 @@ void append_gradients(Graph& g, int loss, const std::vector<int>& wrt) {
                 int scaled = b.mk(TT_OP_MUL, {gidx, b.scalar(factor, dt)});
                 int gs = n.keepdims ? scaled : b.view(TT_OP_RESHAPE, scaled, b.kept_shape(n, ash));
                 accumulate(n.in[0], b.view(TT_OP_EXPAND, gs, ash));
+                break;
+            }
+            case TT_OP_SCAN_LAST: {
+                auto l = last_grads.find(n.in[0]);
+                if (l == last_grads.end()) last_grads[n.in[0]] = gidx;
+                else l->second = b.mk(TT_OP_ADD, {l->second, gidx});
+                break;
+            }
+            case TT_OP_GATED_SCAN: {
+                // u[t] = g[t] + gate[t+1]*u[t+1] (g_last enters at the last step): dx = u,
+                // dgate[t] = u[t]*h[t-1], dinit = gate[0]*u[0]
+                std::vector<int> ops{n.in[0]};
+                const bool has_last = lit != last_grads.end(), has_init = n.in.size() > 2;
+                if (gidx >= 0) ops.push_back(gidx);
+                if (has_last) ops.push_back(lit->second);
+                const std::vector<int64_t> has{gidx >= 0, has_last, has_init};
+                std::vector<int> gate_ops = ops;
+                gate_ops.push_back(i);
+                if (has_init) gate_ops.push_back(n.in[2]);
+                accumulate(n.in[0], backward(BOP_SCAN_DGATE, gate_ops, n.dim0, has, {}));
+                accumulate(n.in[1], backward(BOP_SCAN_DX, ops, n.dim0, has, {}));
+                if (has_init) accumulate(n.in[2], backward(BOP_SCAN_DINIT, ops, n.dim0, has, {}));
+                break;
+            }
+            case TT_OP_TOKEN_LOGPROB: case TT_OP_POLICY_LOSS: case TT_OP_PREFERENCE_LOSS: {
+                // with respect to the logits; the other operands are data (constants)
+                const int op = n.op == TT_OP_TOKEN_LOGPROB ? BOP_LOGPROB_GRAD
+                               : n.op == TT_OP_POLICY_LOSS ? BOP_POLICY_GRAD : BOP_PREFERENCE_GRAD;
+                std::vector<int> ops = n.in;
+                ops.push_back(gidx);
+                accumulate(n.in[0], backward(op, ops, 0, {}, n.attr));
                 break;
             }
             case TT_OP_REDUCE_MAX:

@@ -101,7 +101,7 @@ struct tt_program {
     std::vector<double> prof_sum;   // per launch: summed ms over profiled runs
     int64_t prof_runs = 0;
     bool prof_pending = false;
-    bool has_tc = false;
+    bool has_status = false;              // some launch can set the device status word
     std::vector<cudaEvent_t> out_events;  // caller's events, recorded when an output is complete
     std::vector<cudaEvent_t> in_events;   // caller's events, recorded after an input's last reader
     cudaStream_t side = nullptr;          // second stream for concurrent GEMM pairs
@@ -121,9 +121,16 @@ struct tt_program {
     }
 };
 
+static std::string status_text(int32_t status) {
+    if (status == TT_STATUS_BAD_TOKEN) return "a token id lies outside the vocabulary";
+    return "a kernel gave up a bounded wait (status " + std::to_string(status) + ")";
+}
+
 static int launches_of(const Plan& p, const Launch& L) {
     if (L.type == LT_REGION) return p.regions[static_cast<size_t>(L.region)].grid > 0 ? 1 : 0;
     if (L.type == LT_REDUCE) return L.rd.outer == 0 ? 0 : (L.rd.R == 0 ? 1 : (L.rd.splits > 1 ? 2 : 1));
+    if (L.type == LT_SCAN) return scan_launch_count(L.sd);
+    if (L.type == LT_TOKEN) return token_launch_count(L.td);
     return gemm_launch_count(L.gd);
 }
 
@@ -135,7 +142,7 @@ static std::string execution_plan(const tt_program& p) {
     ss << "Input Nodes (" << g.inputs.size() << "):\n";
     for (int k : g.inputs) {
         const Node& n = g.nodes[static_cast<size_t>(k)];
-        ss << "  %" << n.id << " [" << tuple_str(n.shape) << ", float32]";
+        ss << "  %" << n.id << " [" << tuple_str(n.shape) << (n.dtype == TT_INT32 ? ", int32]" : ", float32]");
         if (!n.name.empty()) ss << " name=\"" << n.name << "\"";
         ss << "\n";
     }
@@ -208,7 +215,9 @@ int tt_compile(const tt_graph* cg, const tt_compile_options* opt, tt_program** o
         verify(g);
         if (o.grad_loss >= 0) {
             std::vector<int> wrt(o.grad_wrt, o.grad_wrt + o.num_grad_wrt);
-            append_gradients(g, o.grad_loss, wrt);
+            const bool seeded = (o.flags & TT_FLAG_GRAD_SEED) != 0;
+            if (seeded && (!o.grad_wrt || o.grad_wrt[o.num_grad_wrt] < 0)) fail(TT_ERR_INVALID, "seed node out of range");
+            append_gradients(g, o.grad_loss, wrt, seeded ? o.grad_wrt[o.num_grad_wrt] : -1);
         }
         g = expand_fused(g);
         if (o.optimize) g = cse(g, &p->cse_removed);
@@ -229,7 +238,8 @@ int tt_compile(const tt_graph* cg, const tt_compile_options* opt, tt_program** o
             p->out_shapes.push_back(p->plan.g.nodes[static_cast<size_t>(k)].shape);
             p->out_bytes.push_back(numel(p->out_shapes.back()) * 4);
         }
-        for (const Launch& L : p->plan.launches) p->has_tc |= (L.type == LT_GEMM && L.gd.algo == 2);
+        for (const Launch& L : p->plan.launches)
+            p->has_status |= (L.type == LT_GEMM && L.gd.algo == 2) || L.type == LT_TOKEN;
 
         // Generated kernels: NVRTC -> cubin (cached); loaded unless host-only.
         const bool host_only = (o.flags & TT_FLAG_HOST_ONLY) != 0;
@@ -376,6 +386,17 @@ static void run_launches(tt_program* p, char* const* in_ptr, char* const* out_pt
         } else if (L.type == LT_REDUCE) {
             rc = launch_reduce(L.rd, reinterpret_cast<const float*>(resolve(L.in_ref)),
                                reinterpret_cast<float*>(resolve(L.out_ref)), resolve(L.scratch_ref), st);
+        } else if (L.type == LT_SCAN) {
+            const float* in[SI_COUNT];
+            float* out[SO_COUNT];
+            for (size_t k = 0; k < SI_COUNT; ++k) in[k] = reinterpret_cast<const float*>(resolve(L.in_refs[k]));
+            for (size_t k = 0; k < SO_COUNT; ++k) out[k] = reinterpret_cast<float*>(resolve(L.out_refs[k]));
+            rc = launch_scan(L.sd, in, out, st);
+        } else if (L.type == LT_TOKEN) {
+            const void* in[TI_COUNT];
+            for (size_t k = 0; k < TI_COUNT; ++k) in[k] = resolve(L.in_refs[k]);
+            rc = launch_token(L.td, in, reinterpret_cast<float*>(resolve(L.out_refs[0])),
+                              reinterpret_cast<float*>(resolve(L.out_refs[1])), resolve(L.scratch_ref), status, st);
         } else {
             // operands whose hi/lo copies the producing region wrote
             GemmSplitIO io;
@@ -482,7 +503,7 @@ int tt_program_run(tt_program* p, const void* const* inputs, void* const* output
                                                cudaMemcpyDeviceToHost, stream),
                                "output copy");
             int32_t status = 0;
-            if (p->has_tc)
+            if (p->has_status)
                 check_cuda(cudaMemcpyAsync(&status, p->arena + p->plan.status_offset, sizeof(status),
                                            cudaMemcpyDeviceToHost, stream),
                            "status copy");
@@ -490,7 +511,7 @@ int tt_program_run(tt_program* p, const void* const* inputs, void* const* output
             collect_profile(p);
             if (status != 0) {
                 cudaMemsetAsync(p->arena + p->plan.status_offset, 0, 4, stream);
-                fail(TT_ERR_DEVICE_STATUS, "a kernel gave up a bounded wait (status " + std::to_string(status) + ")");
+                fail(TT_ERR_DEVICE_STATUS, status_text(status));
             }
         }
     });
@@ -634,7 +655,7 @@ int tt_program_status(tt_program* p, int32_t* device_status) {
         if (device_status) *device_status = status;
         if (status != 0) {
             cudaMemset(p->arena + p->plan.status_offset, 0, 4);
-            fail(TT_ERR_DEVICE_STATUS, "a kernel gave up a bounded wait (status " + std::to_string(status) + ")");
+            fail(TT_ERR_DEVICE_STATUS, status_text(status));
         }
     });
 }

@@ -5,7 +5,9 @@
 // IRVerifier (src/ir/verifier.cpp:7-202); the IR text follows IRPrinter
 // (src/ir/printer.cpp:6-62) so that cache keys and diagnostics read the same.
 #include <algorithm>
+#include <cmath>
 #include <cstring>
+#include <iomanip>
 #include <map>
 #include <set>
 #include <sstream>
@@ -91,6 +93,17 @@ const char* op_name(int op) {
         case TT_OP_STEP: return "step";
         case TT_OP_RESHAPE: return "reshape";
         case TT_OP_EXPAND: return "expand";
+        case TT_OP_GATED_SCAN: return "gated_scan";
+        case TT_OP_SCAN_LAST: return "scan_last";
+        case TT_OP_TOKEN_LOGPROB: return "token_logprob";
+        case TT_OP_POLICY_LOSS: return "policy_loss";
+        case TT_OP_PREFERENCE_LOSS: return "preference_loss";
+        case BOP_SCAN_DX: return "gated_scan_dx";
+        case BOP_SCAN_DGATE: return "gated_scan_dgate";
+        case BOP_SCAN_DINIT: return "gated_scan_dinit";
+        case BOP_LOGPROB_GRAD: return "token_logprob_grad";
+        case BOP_POLICY_GRAD: return "policy_loss_grad";
+        case BOP_PREFERENCE_GRAD: return "preference_loss_grad";
         default: return "unknown";
     }
 }
@@ -107,13 +120,55 @@ bool is_elementwise(int op) {
 }
 bool is_view(int op) { return op == TT_OP_TRANSPOSE || op == TT_OP_RESHAPE || op == TT_OP_EXPAND; }
 bool is_reduce(int op) { return op == TT_OP_REDUCE_SUM || op == TT_OP_REDUCE_MEAN || op == TT_OP_REDUCE_MAX; }
+bool is_scan(int op) {
+    return op == TT_OP_GATED_SCAN || op == TT_OP_SCAN_LAST || op == BOP_SCAN_DX || op == BOP_SCAN_DGATE ||
+           op == BOP_SCAN_DINIT;
+}
+bool is_token_op(int op) {
+    return op == TT_OP_TOKEN_LOGPROB || op == TT_OP_POLICY_LOSS || op == TT_OP_PREFERENCE_LOSS ||
+           op == BOP_LOGPROB_GRAD || op == BOP_POLICY_GRAD || op == BOP_PREFERENCE_GRAD;
+}
 
-static int arity(int op) {
+// Operands of an op: [lo, hi].
+static std::pair<int, int> arity(int op) {
     switch (op) {
-        case TT_OP_INPUT: case TT_OP_CONSTANT: return 0;
-        case TT_OP_ADD: case TT_OP_SUB: case TT_OP_MUL: case TT_OP_DIV: case TT_OP_MATMUL: return 2;
-        case TT_OP_FUSED_ELEMENTWISE: return -1;
-        default: return 1;
+        case TT_OP_INPUT: case TT_OP_CONSTANT: return {0, 0};
+        case TT_OP_ADD: case TT_OP_SUB: case TT_OP_MUL: case TT_OP_DIV: case TT_OP_MATMUL:
+        case TT_OP_TOKEN_LOGPROB: return {2, 2};
+        case TT_OP_FUSED_ELEMENTWISE: return {0, TT_MAX_NODE_INPUTS};
+        case TT_OP_GATED_SCAN: return {2, 3};
+        case TT_OP_POLICY_LOSS: return {4, 5};
+        case TT_OP_PREFERENCE_LOSS: return {3, 3};
+        default: return {1, 1};
+    }
+}
+
+// The ops whose tt_node.data is a tt_op_attrs.
+static bool has_attrs(int op) { return op >= TT_OP_GATED_SCAN && op <= TT_OP_PREFERENCE_LOSS; }
+
+static Shape without_axis(Shape s, int64_t axis) {
+    s.erase(s.begin() + static_cast<long>(axis));
+    return s;
+}
+
+// Operand shapes of a token operator: logits [..., V], every other operand of the leading
+// shape (for the preference loss [N, 2, T], its upstream gradient [N]).
+static void check_token_shapes(const Graph& g, const Node& n) {
+    const std::string what = op_name(n.op);
+    auto shape = [&](size_t k) -> const Shape& { return g.nodes[static_cast<size_t>(n.in[k])].shape; };
+    const Shape& logits = shape(0);
+    if (logits.empty()) fail(TT_ERR_DIMENSION, what + " needs logits of rank 1 or more");
+    if (logits.back() == 0) fail(TT_ERR_SHAPE, what + " needs a vocabulary of at least one token");
+    const Shape lead(logits.begin(), logits.end() - 1);
+    const bool pref = n.op == TT_OP_PREFERENCE_LOSS || n.op == BOP_PREFERENCE_GRAD;
+    if (pref && (lead.size() != 3 || lead[1] != 2))
+        fail(TT_ERR_SHAPE, what + " needs logits [pairs, 2, tokens, vocabulary], got " + shape_str(logits));
+    for (size_t k = 1; k < n.in.size(); ++k) {
+        const bool up = n.op == BOP_PREFERENCE_GRAD && k + 1 == n.in.size();
+        const Shape want = up ? Shape{lead[0]} : lead;
+        if (shape(k) != want)
+            fail(TT_ERR_SHAPE, what + " operand " + std::to_string(k) + " must have shape " + shape_str(want) +
+                                   ", got " + shape_str(shape(k)));
     }
 }
 
@@ -183,6 +238,46 @@ void infer_shape(Graph& g, Node& n) {
             n.dtype = in(0).dtype;
             return;
         }
+        case TT_OP_GATED_SCAN: {
+            const Shape& x = in(0).shape;
+            const int64_t r = static_cast<int64_t>(x.size());
+            if (n.dim0 < 0) n.dim0 += r;
+            if (n.dim0 < 0 || n.dim0 >= r)
+                fail(TT_ERR_DIMENSION, "Invalid gated_scan axis for rank " + std::to_string(r));
+            if (in(1).shape != x)
+                fail(TT_ERR_SHAPE, "gated_scan gate " + shape_str(x) + " and x " + shape_str(in(1).shape) + " differ");
+            if (n.in.size() > 2 && in(2).shape != without_axis(x, n.dim0))
+                fail(TT_ERR_SHAPE, "gated_scan init must have shape " + shape_str(without_axis(x, n.dim0)) + ", got " +
+                                       shape_str(in(2).shape));
+            n.shape = x;
+            n.dtype = in(0).dtype;
+            return;
+        }
+        case TT_OP_SCAN_LAST:
+            if (in(0).op != TT_OP_GATED_SCAN) fail(TT_ERR_IR, "scan_last takes the result of a gated_scan");
+            n.shape = without_axis(in(0).shape, in(0).dim0);
+            n.dtype = in(0).dtype;
+            return;
+        case TT_OP_TOKEN_LOGPROB: case TT_OP_POLICY_LOSS: case TT_OP_PREFERENCE_LOSS: {
+            check_token_shapes(g, n);
+            const Shape& logits = in(0).shape;
+            n.shape = n.op == TT_OP_PREFERENCE_LOSS ? Shape{logits[0]} : Shape(logits.begin(), logits.end() - 1);
+            n.dtype = in(0).dtype;
+            return;
+        }
+        case BOP_SCAN_DX: case BOP_SCAN_DGATE:
+            n.shape = in(0).shape;
+            n.dtype = in(0).dtype;
+            return;
+        case BOP_SCAN_DINIT:
+            n.shape = without_axis(in(0).shape, n.dim0);
+            n.dtype = in(0).dtype;
+            return;
+        case BOP_LOGPROB_GRAD: case BOP_POLICY_GRAD: case BOP_PREFERENCE_GRAD:
+            check_token_shapes(g, n);
+            n.shape = in(0).shape;
+            n.dtype = in(0).dtype;
+            return;
         default:
             fail(TT_ERR_IR, std::string("Unknown op code ") + std::to_string(n.op));
     }
@@ -197,19 +292,30 @@ Graph import_graph(const tt_graph* cg) {
         Node n;
         n.op = c.op;
         n.dtype = c.dtype;
-        if (c.dtype != TT_FLOAT32 && c.dtype != TT_FLOAT64) fail(TT_ERR_TYPE, "Unknown dtype");
+        if (c.dtype != TT_FLOAT32 && c.dtype != TT_FLOAT64 && c.dtype != TT_INT32)
+            fail(TT_ERR_TYPE, "Unknown dtype");
+        if (c.op > TT_OP_PREFERENCE_LOSS) fail(TT_ERR_IR, "Unknown op code " + std::to_string(c.op));
         if (c.rank < 0 || c.rank > TT_MAX_RANK) fail(TT_ERR_DIMENSION, "rank out of range");
-        if (c.num_inputs < 0 || c.num_inputs > TT_MAX_NODE_INPUTS) fail(TT_ERR_IR, "bad input count");
-        int ar = arity(c.op);
-        if (ar >= 0 && ar != c.num_inputs)
-            fail(TT_ERR_IR, std::string("Node %") + std::to_string(c.id) + " (" + op_name(c.op) + ") requires exactly " +
-                                std::to_string(ar) + " inputs");
+        const bool attrs = has_attrs(c.op);
+        if (c.num_inputs < 0 || c.num_inputs > (attrs ? TT_MAX_OPERANDS : TT_MAX_NODE_INPUTS))
+            fail(TT_ERR_IR, "bad input count");
+        const auto ar = arity(c.op);
+        if (c.op != TT_OP_FUSED_ELEMENTWISE && (c.num_inputs < ar.first || c.num_inputs > ar.second))
+            fail(TT_ERR_IR, std::string("Node %") + std::to_string(c.id) + " (" + op_name(c.op) + ") requires " +
+                                (ar.first == ar.second ? "exactly " + std::to_string(ar.first)
+                                                       : std::to_string(ar.first) + " to " + std::to_string(ar.second)) +
+                                " inputs");
+        const tt_op_attrs* at = attrs ? static_cast<const tt_op_attrs*>(c.data) : nullptr;
+        if (!at && (c.num_inputs > TT_MAX_NODE_INPUTS || c.op == TT_OP_POLICY_LOSS || c.op == TT_OP_PREFERENCE_LOSS))
+            fail(TT_ERR_IR, std::string(op_name(c.op)) + " node without attributes");
         for (int32_t k = 0; k < c.num_inputs; ++k) {
-            if (c.inputs[k] < 0 || c.inputs[k] >= i)
+            const int32_t q = k < TT_MAX_NODE_INPUTS ? c.inputs[k] : at->more_inputs[k - TT_MAX_NODE_INPUTS];
+            if (q < 0 || q >= i)
                 fail(TT_ERR_IR, "Topological ordering violation: node %" + std::to_string(c.id) +
                                     " uses an operand defined later or not at all");
-            n.in.push_back(c.inputs[k]);
+            n.in.push_back(q);
         }
+        if (at) n.attr.assign(at->f, at->f + 4);
         n.shape.assign(c.shape, c.shape + c.rank);
         n.id = c.id;
         n.dim0 = c.dim0;
@@ -224,6 +330,7 @@ Graph import_graph(const tt_graph* cg) {
                 if (d < 0) fail(TT_ERR_IR, "Input node %" + std::to_string(c.id) + " has negative dimension");
         }
         if (c.op == TT_OP_CONSTANT) {
+            if (c.dtype == TT_INT32) fail(TT_ERR_TYPE, "int32 values are graph inputs (token ids), not constants");
             int64_t ne = numel(n.shape);
             if (ne > 0 && !c.data) fail(TT_ERR_IR, "Constant node without data");
             n.cdata.resize(static_cast<size_t>(ne));
@@ -264,10 +371,30 @@ void verify(const Graph& g) {
         for (int k : n.in)
             if (k < 0 || static_cast<size_t>(k) >= i)
                 fail(TT_ERR_IR, "Topological ordering violation at node %" + std::to_string(n.id));
-        for (int k : n.in)
-            if (g.nodes[static_cast<size_t>(k)].dtype != n.dtype)
+        for (size_t k = 0; k < n.in.size(); ++k) {
+            const int dt = g.nodes[static_cast<size_t>(n.in[k])].dtype;
+            if (is_token_op(n.op) && k == 1) {
+                if (dt != TT_INT32) fail(TT_ERR_TYPE, std::string(op_name(n.op)) + " takes int32 tokens");
+            } else if (dt != n.dtype) {
                 fail(TT_ERR_IR, std::string("Type mismatch in ") + op_name(n.op) + " %" + std::to_string(n.id));
+            }
+        }
+        if (n.dtype == TT_INT32 && n.op != TT_OP_INPUT && !is_view(n.op))
+            fail(TT_ERR_TYPE, std::string(op_name(n.op)) + " does not take int32 operands");
+        auto number = [&](bool ok, const char* what) {
+            if (!ok) fail(TT_ERR_INVALID, std::string(op_name(n.op)) + ": " + what);
+        };
         switch (n.op) {
+            case TT_OP_POLICY_LOSS:
+                number(n.attr[0] >= 0.0f && n.attr[0] <= 1.0f, "the lower clip must lie in [0, 1]");
+                number(n.attr[1] >= 0.0f && n.attr[1] < INFINITY, "the upper clip must be finite and not negative");
+                number(n.attr[2] >= 0.0f && n.attr[2] < INFINITY, "kl must be finite and not negative");
+                number((n.attr[2] > 0.0f) == (n.in.size() == 5), "a ref operand goes with kl > 0, and only with it");
+                break;
+            case TT_OP_PREFERENCE_LOSS:
+                number(n.attr[0] > 0.0f && n.attr[0] < INFINITY, "beta must be finite and positive");
+                number(n.attr[1] >= 0.0f && n.attr[1] <= 0.5f, "smoothing must lie in [0, 0.5]");
+                break;
             case TT_OP_CONSTANT:
                 if (static_cast<int64_t>(n.cdata.size()) != numel(n.shape))
                     fail(TT_ERR_IR, "Constant node %" + std::to_string(n.id) + " shape mismatch with underlying tensor");
@@ -291,9 +418,14 @@ void verify(const Graph& g) {
     for (int o : g.outputs)
         if (o < 0 || static_cast<size_t>(o) >= g.nodes.size())
             fail(TT_ERR_IR, "Graph output does not exist in graph");
+    for (int o : g.outputs)
+        if (g.nodes[static_cast<size_t>(o)].dtype == TT_INT32)
+            fail(TT_ERR_TYPE, "an int32 node cannot be a graph output");
 }
 
-static const char* dtype_name(int dt) { return dt == TT_FLOAT64 ? "float64" : "float32"; }
+static const char* dtype_name(int dt) {
+    return dt == TT_FLOAT64 ? "float64" : dt == TT_INT32 ? "int32" : "float32";
+}
 
 // IRPrinter::to_string (src/ir/printer.cpp:6-62).  Nodes are kept in creation
 // order, which is the order the reference DFS topological sort yields for graphs
@@ -319,6 +451,12 @@ std::string ir_text(const Graph& g) {
                 ss << " expr=\"" << n.expr << "\"";
             } else if (n.op == TT_OP_RESHAPE || n.op == TT_OP_EXPAND) {
                 ss << " shape=" << shape_str(n.shape);
+            } else if (is_scan(n.op) && n.op != TT_OP_SCAN_LAST) {
+                ss << " axis=" << n.dim0;
+            } else if (n.op == TT_OP_POLICY_LOSS || n.op == BOP_POLICY_GRAD) {
+                ss << std::setprecision(9) << " clip=[" << n.attr[0] << ", " << n.attr[1] << "] kl=" << n.attr[2];
+            } else if (n.op == TT_OP_PREFERENCE_LOSS || n.op == BOP_PREFERENCE_GRAD) {
+                ss << std::setprecision(9) << " beta=" << n.attr[0] << " smoothing=" << n.attr[1];
             }
         }
         ss << "\n";
@@ -455,6 +593,11 @@ Graph cse(const Graph& g, size_t* removed) {
         key << "|" << n.dim0 << "," << n.dim1 << "|" << n.keepdims << "|";
         for (int64_t a : n.axes) key << a << ",";
         key << "|" << n.expr << "|";
+        for (float f : n.attr) {
+            uint32_t u;
+            std::memcpy(&u, &f, 4);
+            key << u << ";";
+        }
         if (n.op == TT_OP_CONSTANT) {
             for (float f : n.cdata) {
                 uint32_t u;

@@ -101,6 +101,43 @@ int launch_splitk_reduce(const float* P, float* C, int64_t per, int ksplit, int6
 // bounded wait and the given clock budget; the wait records its timeout code in *status.
 int launch_bounded_wait_selftest(int* status, long long budget, void* stream);
 
+// ---- gated scans (kernels_scan.cu) ----
+// The lanes of a scan are its positions without the axis: [outer][n1][n2], n1*n2 the dims
+// behind the axis.  Operands have any strides over (outer, time, n1, n2), 0 where they are
+// broadcast; results are row-major [outer][T][n1][n2] (lane results [outer][n1][n2]).
+struct ScanStrides {
+    int64_t off = 0, so = 0, st = 0, s1 = 0, s2 = 0;
+};
+enum ScanIn { SI_GATE = 0, SI_X = 1, SI_CARRY = 2, SI_H = 3, SI_INIT = 4, SI_COUNT = 5 };
+enum ScanOut { SO_MAIN = 0, SO_LANE = 1, SO_GATE = 2, SO_COUNT = 3 };
+struct ScanDesc {
+    // forward: gate, x, carry = init -> main = h, lane = last state.
+    // backward: gate, x = upstream g (absent: 0), carry = upstream gradient of the last
+    // state (absent: 0), h, init -> main = dx, lane = dinit, gate = dgate.
+    bool backward = false;
+    int64_t outer = 1, T = 0, n1 = 1, n2 = 1;
+    ScanStrides in[SI_COUNT];
+};
+int scan_launch_count(const ScanDesc& d);
+// in[] / out[]: null where an operand is absent or a result not wanted
+int launch_scan(const ScanDesc& d, const float* const* in, float* const* out, void* stream);
+
+// ---- token log-probabilities and losses over logits (kernels_token.cu) ----
+enum TokenKind { TK_LOGPROB = 0, TK_POLICY = 1, TK_PREFERENCE = 2 };
+enum TokenIn { TI_LOGITS = 0, TI_TOKENS = 1, TI_OLD = 2, TI_ADVANTAGE = 3, TI_REF = 4, TI_GRAD = 5, TI_COUNT = 6 };
+struct TokenDesc {
+    int kind = TK_LOGPROB;
+    bool grad = false;               // the gradient of the logits is wanted too (or only)
+    int64_t n0 = 1, n1 = 1, V = 1;   // rows [n0][n1]; for the preference loss n0 pairs of n1 = 2*T tokens
+    int64_t off[TI_COUNT] = {}, s0[TI_COUNT] = {}, s1[TI_COUNT] = {};  // element strides over (n0, n1)
+    float f[4] = {};                 // tt_op_attrs.f
+};
+int64_t token_scratch_bytes(const TokenDesc& d);
+int token_launch_count(const TokenDesc& d);
+// y (values, row-major) and dlogits ([n0][n1][V]) may be null; *status takes TT_STATUS_BAD_TOKEN
+int launch_token(const TokenDesc& d, const void* const* in, float* y, float* dlogits, void* scratch, int* status,
+                 void* stream);
+
 // ---- misc kernels (kernels_misc.cu) ----
 int launch_sgd(int n, float* const* params, const float* const* grads, float* const* vel, const int64_t* numels,
                float lr, float momentum, void* stream);
@@ -139,7 +176,7 @@ struct Region {
     int64_t copy_R = 0, copy_C = 0;
 };
 
-enum LaunchType { LT_REGION = 0, LT_REDUCE = 1, LT_GEMM = 2 };
+enum LaunchType { LT_REGION = 0, LT_REDUCE = 1, LT_GEMM = 2, LT_SCAN = 3, LT_TOKEN = 4 };
 
 struct Launch {
     int type = LT_REGION;
@@ -156,6 +193,12 @@ struct Launch {
     // GEMM: for a pre-split operand, the region launch that wrote its copies and the layout read
     int a_split_src = -1, a_split_layout = 0;
     int b_split_src = -1, b_split_layout = 0;
+    // LT_SCAN / LT_TOKEN: operands by ScanIn / TokenIn and results by ScanOut / {values,
+    // gradient} (storage nodes, -1 where absent) and where they live
+    ScanDesc sd;
+    TokenDesc td;
+    std::vector<int> in_nodes, out_nodes;
+    std::vector<BufRef> in_refs, out_refs;
 };
 
 struct Slot {

@@ -4,7 +4,8 @@
 //     cycle through another launch);
 //  2. fold views (transpose / reshape / expand) into the strides their consumers
 //     read with, so no transpose is materialised for reductions, GEMMs or regions;
-//  3. order the launches (regions, reductions, GEMMs) topologically;
+//  3. order the launches (regions, reductions, GEMMs, scans, token losses)
+//     topologically; a loss and its gradient, or a scan's gradients, share a launch;
 //  4. plan memory: the reference MemoryPlanner's lifetimes and greedy first-fit slot
 //     reuse (src/optimizer/memory_planner.cpp:21-89), applied to launch steps and
 //     mapped onto ONE device arena (slot offsets = 256-B aligned prefix sums).
@@ -174,7 +175,7 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
             const auto& dq = deps[static_cast<size_t>(q)];
             d.insert(d.end(), dq.begin(), dq.end());
         }
-        if (n.dtype != TT_FLOAT32) fail(TT_ERR_COMPILE, "The CUDA backend computes in float32 only (node %" +
+        if (n.dtype == TT_FLOAT64) fail(TT_ERR_COMPILE, "The CUDA backend computes in float32 only (node %" +
                                                             std::to_string(n.id) + " is float64)");
         if ((is_elementwise(n.op) && n.fused_into < 0) || n.inline_mm) {
             int R = -1;
@@ -219,7 +220,7 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
         for (size_t i = 0; i < N0; ++i) {
             const Node& n = g.nodes[i];
             if (p.region_of[i] >= 0) unit_of[i] = p.region_of[i];
-            else if (n.op == TT_OP_MATMUL || is_reduce(n.op)) unit_of[i] = nu++;
+            else if (n.op == TT_OP_MATMUL || is_reduce(n.op) || is_scan(n.op) || is_token_op(n.op)) unit_of[i] = nu++;
             else if (is_view(n.op) || n.fused_into >= 0) unit_of[i] = unit_of[static_cast<size_t>(n.in[0])];
         }
         std::vector<int> alias(static_cast<size_t>(nu));
@@ -375,6 +376,8 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
                 if (is_elementwise(n.op)) {
                     if (stored[i]) p.st[i] = make_root(i);
                     else p.st[i].kind = SK_REG;
+                } else if (is_scan(n.op) || is_token_op(n.op)) {
+                    p.st[i] = make_root(i);
                 } else {
                     fail(TT_ERR_COMPILE, std::string("Unsupported op in CUDA backend: ") + op_name(n.op));
                 }
@@ -505,8 +508,96 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
         p.regions.push_back(r);
         return idx;
     };
-    std::vector<int> launch_nodes;  // reduce / matmul nodes, original order
-    g.nodes.reserve(N0 * 3 + 8);      // materialise() appends nodes: no reference is held across it
+    // Operands of scans and token losses.  A scalar constant becomes a one-element buffer
+    // read with zero strides; a view whose strides the kernel cannot take becomes a dense
+    // copy.  Both are made once per node, so launches that share an operand still do.
+    std::map<int, int> dense_copy;
+    auto operand = [&](int src, bool fits) {
+        auto it = dense_copy.find(src);
+        if (it != dense_copy.end()) return it->second;
+        if (p.st[static_cast<size_t>(src)].kind == SK_IMM) {
+            Node c;
+            c.op = TT_OP_CONSTANT;
+            c.shape = g.nodes[static_cast<size_t>(src)].shape;  // the operand's shape, one stored value
+            c.cdata = {p.st[static_cast<size_t>(src)].imm};
+            c.id = g.next_id;
+            const int idx = g.add(c);
+            Storage s;
+            s.kind = SK_BUF;
+            s.root = idx;
+            s.strides.assign(c.shape.size(), 0);
+            p.st.push_back(s);
+            p.region_of.push_back(-1);
+            return dense_copy[src] = idx;
+        }
+        return fits ? src : dense_copy[src] = materialise(src);
+    };
+    // Flattened stride of dims [lo, hi) of a view: dims of size 1 carry none, broadcast
+    // dims stride 0; false when the dims are not one arithmetic sequence.
+    auto flat_stride = [&](int q, size_t lo, size_t hi, int64_t& stride) {
+        const Storage& s = p.st[static_cast<size_t>(q)];
+        const Shape& sh = g.nodes[static_cast<size_t>(q)].shape;
+        stride = 0;
+        if (s.kind != SK_BUF) return true;  // a scalar constant: read with stride 0
+        int64_t inner = 1;
+        bool have = false;
+        for (size_t d = hi; d-- > lo;) {
+            if (sh[d] == 1) continue;
+            if (!have) {
+                stride = s.strides[d];
+                have = true;
+            } else if (s.strides[d] != stride * inner) {
+                return false;
+            }
+            inner *= sh[d];
+        }
+        return true;
+    };
+    // A scan's operand over (outer, time, n1, n2), the dims behind the axis split at `split`;
+    // lane operands (init, last state) have no time dim.
+    auto scan_strides = [&](int q, size_t axis, size_t split, bool lane, ScanStrides& o) {
+        const Storage& s = p.st[static_cast<size_t>(q)];
+        const size_t r = g.nodes[static_cast<size_t>(q)].shape.size(), skip = lane ? 0 : 1;
+        o.off = s.offset;
+        o.st = lane || s.kind != SK_BUF ? 0 : s.strides[axis];
+        const size_t sp = lane ? split - 1 : split;
+        return flat_stride(q, 0, axis, o.so) && flat_stride(q, axis + skip, sp, o.s1) && flat_stride(q, sp, r, o.s2);
+    };
+    // The first split at which the gate's strides fit (axis + 1, i.e. n1 = 1, when none does).
+    auto scan_split = [&](int gate, size_t axis) {
+        const size_t r = g.nodes[static_cast<size_t>(gate)].shape.size();
+        ScanStrides o;
+        for (size_t sp = axis + 1; sp < std::max(r, axis + 2); ++sp)
+            if (scan_strides(gate, axis, sp, false, o)) return sp;
+        return axis + 1;
+    };
+    // Is operand k of a scan node a lane operand?
+    auto lane_operand = [&](const Node& n, size_t k) {
+        if (n.op == TT_OP_GATED_SCAN) return k == 2;
+        if (k == 0) return false;
+        const bool has_g = n.axes[0] != 0, has_last = n.axes[1] != 0;
+        if (has_last && k == (has_g ? 2u : 1u)) return true;
+        return n.op == BOP_SCAN_DGATE && n.axes[2] != 0 && k + 1 == n.in.size();
+    };
+    // A token op's operand over the rows [n0][n1] (logits: without the vocabulary, whose
+    // values must be adjacent); the preference loss's upstream gradient is [n0].
+    auto token_strides = [&](const Node& n, size_t k, int64_t& s0, int64_t& s1) {
+        const int q = n.in[k];
+        const Storage& s = p.st[static_cast<size_t>(q)];
+        const Shape& sh = g.nodes[static_cast<size_t>(q)].shape;
+        const bool pref = n.op == TT_OP_PREFERENCE_LOSS || n.op == BOP_PREFERENCE_GRAD;
+        const size_t lead = k == 0 ? sh.size() - 1 : sh.size();
+        if (k == 0 && s.kind == SK_BUF && sh.back() != 1 && s.strides.back() != 1) return false;
+        if (n.op == BOP_PREFERENCE_GRAD && k + 1 == n.in.size()) {
+            s1 = 0;
+            return flat_stride(q, 0, 1, s0);
+        }
+        const size_t cut = pref ? 1 : lead > 0 ? lead - 1 : 0;  // n0: the dims before, n1: the rest
+        return flat_stride(q, 0, cut, s0) && flat_stride(q, cut, lead, s1);
+    };
+
+    std::vector<int> launch_nodes;  // reduce / matmul / scan / token nodes, original order
+    g.nodes.reserve(N0 * 6 + 8);      // materialise() appends nodes: no reference is held across it
     for (size_t i = 0; i < N0; ++i) {
         const int op = g.nodes[i].op;
         if (op == TT_OP_MATMUL && !g.nodes[i].inline_mm) {
@@ -526,6 +617,27 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
             if (p.st[static_cast<size_t>(src)].kind != SK_BUF) {
                 const int m = materialise(src);
                 g.nodes[i].in[0] = m;
+            }
+            launch_nodes.push_back(static_cast<int>(i));
+        } else if (is_token_op(op)) {
+            for (size_t k = 0; k < g.nodes[i].in.size(); ++k) {
+                int64_t s0, s1;
+                const bool fits = token_strides(g.nodes[i], k, s0, s1);
+                // logits are read row by row: a scalar constant is expanded, not read with stride 0
+                const int src = g.nodes[i].in[k];
+                const int m = k == 0 && p.st[static_cast<size_t>(src)].kind == SK_IMM ? materialise(src)
+                                                                                      : operand(src, fits);
+                g.nodes[i].in[k] = m;
+            }
+            launch_nodes.push_back(static_cast<int>(i));
+        } else if (is_scan(op) && op != TT_OP_SCAN_LAST) {
+            const size_t axis = static_cast<size_t>(g.nodes[i].dim0);
+            const size_t split = scan_split(g.nodes[i].in[0], axis);
+            for (size_t k = 0; k < g.nodes[i].in.size(); ++k) {
+                ScanStrides o;
+                const int src = g.nodes[i].in[k];
+                const int m = operand(src, scan_strides(src, axis, split, lane_operand(g.nodes[i], k), o));
+                g.nodes[i].in[k] = m;
             }
             launch_nodes.push_back(static_cast<int>(i));
         }
@@ -571,6 +683,7 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
     struct Unit {
         int type, idx, key;
         std::vector<int> reads, writes;  // root nodes
+        std::vector<int> nodes = {};     // scans / token losses: the nodes computed by the launch
     };
     std::vector<Unit> units;
     for (size_t R = 0; R < p.regions.size(); ++R) {
@@ -592,9 +705,85 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
     }
     for (int i : launch_nodes) {
         const Node& n = g.nodes[static_cast<size_t>(i)];
-        Unit u{n.op == TT_OP_MATMUL ? LT_GEMM : LT_REDUCE, i, i, {}, {i}};
+        const int type = n.op == TT_OP_MATMUL ? LT_GEMM : is_scan(n.op) ? LT_SCAN : is_token_op(n.op) ? LT_TOKEN : LT_REDUCE;
+        Unit u{type, i, i, {}, {i}};
         for (int q : n.in) u.reads.push_back(p.st[static_cast<size_t>(q)].root);
+        if (type == LT_SCAN || type == LT_TOKEN) u.nodes.push_back(i);
+        if (n.op == TT_OP_GATED_SCAN) {
+            // scan_last is a second result of the scan's launch; states that only scan_last
+            // reads are not stored
+            bool stored_h = out_pos[static_cast<size_t>(i)] >= 0;
+            for (int k : users[static_cast<size_t>(i)]) {
+                if (g.nodes[static_cast<size_t>(k)].op == TT_OP_SCAN_LAST) {
+                    u.nodes.push_back(k);
+                    u.writes.push_back(k);
+                } else {
+                    stored_h = true;
+                }
+            }
+            if (!stored_h) u.writes.erase(u.writes.begin());
+        }
         units.push_back(u);
+    }
+    // A loss and its gradient (the logits are read once for both), and a scan's gradients
+    // (the reverse scan runs once), share a launch unless one needs the other's result.
+    if (opt.fuse) {
+        auto same_launch = [&](const Unit& a, const Unit& b) {
+            if (a.type != b.type) return false;
+            const Node& x = g.nodes[static_cast<size_t>(a.idx)];
+            const Node& y = g.nodes[static_cast<size_t>(b.idx)];
+            if (a.type == LT_TOKEN) {  // forward a, gradient b: b's operands are a's, then g
+                const bool pair = (x.op == TT_OP_TOKEN_LOGPROB && y.op == BOP_LOGPROB_GRAD) ||
+                                  (x.op == TT_OP_POLICY_LOSS && y.op == BOP_POLICY_GRAD) ||
+                                  (x.op == TT_OP_PREFERENCE_LOSS && y.op == BOP_PREFERENCE_GRAD);
+                return pair && a.nodes.size() == 1 && b.nodes.size() == 1 && x.attr == y.attr &&
+                       std::equal(x.in.begin(), x.in.end(), y.in.begin(), y.in.end() - 1);
+            }
+            // backward scans of the same gate and upstream gradients, different results
+            if (a.type != LT_SCAN || x.op == TT_OP_GATED_SCAN || y.op == TT_OP_GATED_SCAN) return false;
+            for (int i : a.nodes)
+                for (int j : b.nodes)
+                    if (g.nodes[static_cast<size_t>(i)].op == g.nodes[static_cast<size_t>(j)].op) return false;
+            const size_t common = 1 + static_cast<size_t>(x.axes[0] != 0) + static_cast<size_t>(x.axes[1] != 0);
+            return x.dim0 == y.dim0 && x.axes == y.axes &&
+                   std::equal(x.in.begin(), x.in.begin() + static_cast<long>(common), y.in.begin());
+        };
+        auto reaches = [&](size_t from, size_t to) {
+            std::vector<char> seen(units.size(), 0);
+            std::vector<size_t> stack{from};
+            while (!stack.empty()) {
+                const size_t u = stack.back();
+                stack.pop_back();
+                for (size_t v = 0; v < units.size(); ++v) {
+                    if (seen[v]) continue;
+                    bool edge = false;
+                    for (int w : units[u].writes)
+                        edge |= std::find(units[v].reads.begin(), units[v].reads.end(), w) != units[v].reads.end();
+                    if (!edge) continue;
+                    if (v == to) return true;
+                    seen[v] = 1;
+                    stack.push_back(v);
+                }
+            }
+            return false;
+        };
+        for (size_t a = 0; a < units.size(); ++a) {
+            if (units[a].type != LT_SCAN && units[a].type != LT_TOKEN) continue;
+            for (size_t b = 0; b < units.size();) {
+                // (the later unit of a pair goes; a loss always precedes its gradient)
+                if (b <= a || !same_launch(units[a], units[b]) || reaches(a, b) || reaches(b, a)) {
+                    ++b;
+                    continue;
+                }
+                Unit& u = units[a];
+                const Unit& v = units[b];
+                u.reads.insert(u.reads.end(), v.reads.begin(), v.reads.end());
+                u.writes.insert(u.writes.end(), v.writes.begin(), v.writes.end());
+                u.nodes.insert(u.nodes.end(), v.nodes.begin(), v.nodes.end());
+                u.key = std::min(u.key, v.key);
+                units.erase(units.begin() + static_cast<long>(b));
+            }
+        }
     }
     std::map<int, int> producer;  // root -> unit
     for (size_t u = 0; u < units.size(); ++u)
@@ -728,6 +917,80 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
             std::ostringstream lb;
             lb << op_name(n.op) << (d.kind == RK_ROW ? "/row" : d.kind == RK_COL ? "/col" : "/generic")
                << shape_str(a.shape);
+            L.label = lb.str();
+        } else if (un.type == LT_SCAN) {
+            ScanDesc& d = L.sd;
+            L.in_nodes.assign(SI_COUNT, -1);
+            L.out_nodes.assign(SO_COUNT, -1);
+            const Node& first = g.nodes[static_cast<size_t>(un.idx)];
+            const Shape& sh = g.nodes[static_cast<size_t>(first.in[0])].shape;
+            const size_t axis = static_cast<size_t>(first.dim0), split = scan_split(first.in[0], axis);
+            d.backward = first.op != TT_OP_GATED_SCAN;
+            d.T = sh[axis];
+            for (size_t k = 0; k < axis; ++k) d.outer *= sh[k];
+            for (size_t k = axis + 1; k < split; ++k) d.n1 *= sh[k];
+            for (size_t k = split; k < sh.size(); ++k) d.n2 *= sh[k];
+            auto bind = [&](const Node& n, size_t k, int slot) {
+                scan_strides(n.in[k], axis, split, lane_operand(n, k), d.in[slot]);
+                L.in_nodes[static_cast<size_t>(slot)] = p.st[static_cast<size_t>(n.in[k])].root;
+            };
+            std::ostringstream lb;
+            for (int i : un.nodes) {
+                const Node& n = g.nodes[static_cast<size_t>(i)];
+                const bool written = std::find(un.writes.begin(), un.writes.end(), i) != un.writes.end();
+                lb << (i == un.idx ? "" : "+") << op_name(n.op);
+                const int slot = n.op == TT_OP_GATED_SCAN || n.op == BOP_SCAN_DX ? SO_MAIN
+                                 : n.op == BOP_SCAN_DGATE                        ? SO_GATE
+                                                                                 : SO_LANE;
+                if (written) L.out_nodes[static_cast<size_t>(slot)] = i;
+                if (n.op == TT_OP_SCAN_LAST) continue;
+                bind(n, 0, SI_GATE);
+                if (n.op == TT_OP_GATED_SCAN) {
+                    bind(n, 1, SI_X);
+                    if (n.in.size() > 2) bind(n, 2, SI_CARRY);
+                    continue;
+                }
+                size_t k = 1;
+                if (n.axes[0]) bind(n, k++, SI_X);
+                if (n.axes[1]) bind(n, k++, SI_CARRY);
+                if (n.op == BOP_SCAN_DGATE) {
+                    bind(n, k++, SI_H);
+                    if (n.axes[2]) bind(n, k++, SI_INIT);
+                }
+            }
+            lb << shape_str(sh) << " axis=" << axis;
+            L.label = lb.str();
+        } else if (un.type == LT_TOKEN) {
+            TokenDesc& d = L.td;
+            L.in_nodes.assign(TI_COUNT, -1);
+            L.out_nodes.assign(2, -1);
+            const Node& first = g.nodes[static_cast<size_t>(un.idx)];
+            const Shape& sh = g.nodes[static_cast<size_t>(first.in[0])].shape;
+            d.kind = first.op == TT_OP_TOKEN_LOGPROB || first.op == BOP_LOGPROB_GRAD ? TK_LOGPROB
+                     : first.op == TT_OP_POLICY_LOSS || first.op == BOP_POLICY_GRAD  ? TK_POLICY
+                                                                                     : TK_PREFERENCE;
+            d.V = sh.back();
+            const size_t lead = sh.size() - 1, cut = d.kind == TK_PREFERENCE ? 1 : lead > 0 ? lead - 1 : 0;
+            for (size_t k = 0; k < lead; ++k) (k < cut ? d.n0 : d.n1) *= sh[k];
+            for (size_t k = 0; k < first.attr.size() && k < 4; ++k) d.f[k] = first.attr[k];
+            std::ostringstream lb;
+            for (int i : un.nodes) {
+                const Node& n = g.nodes[static_cast<size_t>(i)];
+                const bool bw = n.op == BOP_LOGPROB_GRAD || n.op == BOP_POLICY_GRAD || n.op == BOP_PREFERENCE_GRAD;
+                lb << (i == un.idx ? "" : "+") << op_name(n.op);
+                d.grad |= bw;
+                L.out_nodes[bw ? 1 : 0] = i;
+                for (size_t k = 0; k < n.in.size(); ++k) {
+                    size_t slot = k;  // logits, tokens, old, advantage, ref
+                    if (d.kind == TK_PREFERENCE && k == 2) slot = TI_REF;
+                    if (bw && k + 1 == n.in.size()) slot = TI_GRAD;
+                    token_strides(n, k, d.s0[slot], d.s1[slot]);
+                    d.off[slot] = p.st[static_cast<size_t>(n.in[k])].offset;
+                    L.in_nodes[slot] = p.st[static_cast<size_t>(n.in[k])].root;
+                }
+            }
+            L.scratch_bytes = token_scratch_bytes(d);
+            lb << shape_str(sh);
             L.label = lb.str();
         } else {
             const Node& n = g.nodes[static_cast<size_t>(un.idx)];
@@ -871,6 +1134,8 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
                         other |= !a.imm && a.node == q;
                 } else if (U.type == LT_REDUCE) {
                     other |= U.in_node == q;
+                } else if (U.type == LT_SCAN || U.type == LT_TOKEN) {
+                    other |= std::find(U.in_nodes.begin(), U.in_nodes.end(), q) != U.in_nodes.end();
                 } else {
                     other |= (U.in_node == q && !U.gd.a_presplit) || (U.in_node2 == q && !U.gd.b_presplit);
                 }
@@ -995,7 +1260,7 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
     int64_t off = 0;
     for (size_t i = 0; i < N; ++i) {
         const Node& n = g.nodes[i];
-        if (n.op == TT_OP_CONSTANT && n.cdata.size() > 1) {
+        if (n.op == TT_OP_CONSTANT && (n.cdata.size() > 1 || (n.cdata.size() == 1 && p.st[i].kind == SK_BUF))) {
             BufRef r;
             r.kind = BK_ARENA;
             r.offset = off;
@@ -1039,6 +1304,9 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
             Region& r = p.regions[static_cast<size_t>(L.region)];
             if (r.store_ref.empty())
                 for (int s : r.stores) r.store_ref.push_back(p.root_ref[static_cast<size_t>(s)]);
+        } else if (L.type == LT_SCAN || L.type == LT_TOKEN) {
+            for (int q : L.in_nodes) L.in_refs.push_back(q < 0 ? BufRef{} : p.root_ref[static_cast<size_t>(q)]);
+            for (int q : L.out_nodes) L.out_refs.push_back(q < 0 ? BufRef{} : p.root_ref[static_cast<size_t>(q)]);
         } else {
             L.in_ref = p.root_ref[static_cast<size_t>(L.in_node)];
             if (L.in_node2 >= 0) L.in_ref2 = p.root_ref[static_cast<size_t>(L.in_node2)];
@@ -1062,6 +1330,8 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
             if (L.type == LT_REGION) {
                 for (const Access& a : p.regions[static_cast<size_t>(L.region)].ext_access)
                     if (!a.imm) mark(a.node);
+            } else if (L.type == LT_SCAN || L.type == LT_TOKEN) {
+                for (int q : L.in_nodes) mark(q);
             } else {
                 mark(L.in_node);
                 if (L.in_node2 >= 0) mark(L.in_node2);
@@ -1076,6 +1346,8 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
         };
         if (L.type == LT_REGION) {
             for (const BufRef& b : p.regions[static_cast<size_t>(L.region)].store_ref) mark(b);
+        } else if (L.type == LT_SCAN || L.type == LT_TOKEN) {
+            for (const BufRef& b : L.out_refs) mark(b);
         } else {
             mark(L.out_ref);
         }
@@ -1109,6 +1381,11 @@ std::string plan_text(const Plan& p) {
             if (r.copy_store >= 0)
                 ss << " copies=" << split_copies_bytes(r.copy_R, r.copy_C, r.copy_rows, r.copy_t) << "@"
                    << L.split_ref.offset;
+        } else if (L.type == LT_SCAN || L.type == LT_TOKEN) {
+            ss << " ->";
+            for (const BufRef& b : L.out_refs)
+                if (b.kind != BK_NONE) ss << " " << kind_name(b.kind) << ":" << (b.kind == BK_ARENA ? b.offset : b.index);
+            if (L.scratch_bytes) ss << " scratch=" << L.scratch_bytes << "@" << L.scratch_ref.offset;
         } else {
             ss << " ->" << " " << kind_name(L.out_ref.kind) << ":"
                << (L.out_ref.kind == BK_ARENA ? L.out_ref.offset : L.out_ref.index);

@@ -33,6 +33,7 @@ struct Node {
     bool keepdims = false;
     std::vector<float> cdata;  // Constant payload (float32)
     std::string name, expr;
+    std::vector<float> attr;   // sequence operators: tt_op_attrs.f
     // Set by the scheduler only: a matmul's epilogue activation (program.hpp Epilogue),
     // and on that activation node the index of the matmul that computes it.
     int epilogue = 0;
@@ -60,6 +61,20 @@ bool is_elementwise(int op);
 bool is_view(int op);
 bool is_reduce(int op);
 
+// Backward nodes of the sequence operators, made by append_gradients only (import refuses
+// them).  axes of the scan's: {has g, has g_last, has init}, saying which optional operands
+// follow; dim0 is the scan's axis.
+enum BackwardOp {
+    BOP_SCAN_DX = 64,     // (gate[, g][, g_last])            gradient of x
+    BOP_SCAN_DGATE = 65,  // (gate[, g][, g_last], h[, init])  gradient of gate
+    BOP_SCAN_DINIT = 66,  // (gate[, g][, g_last])            gradient of init
+    BOP_LOGPROB_GRAD = 67,     // the forward's operands, then g: gradient of the logits
+    BOP_POLICY_GRAD = 68,
+    BOP_PREFERENCE_GRAD = 69
+};
+bool is_scan(int op);      // GatedScan, ScanLast and the scan's backward nodes
+bool is_token_op(int op);  // the three token operators and their backward nodes
+
 // graph.cpp
 Graph import_graph(const tt_graph* g);
 void infer_shape(Graph& g, Node& n);  // sets n.shape from inputs/attrs, throws on bad shapes
@@ -69,8 +84,9 @@ Graph expand_fused(const Graph& g);   // FusedElementwise -> primitive nodes
 Graph dce(const Graph& g, size_t* removed);
 Graph cse(const Graph& g, size_t* removed);
 
-// autodiff.cpp: appends the backward graph and the gradient outputs
-void append_gradients(Graph& g, int loss, const std::vector<int>& wrt);
+// autodiff.cpp: appends the backward graph and the gradient outputs.  seed: the node that
+// stands for the loss's own gradient (-1: ones)
+void append_gradients(Graph& g, int loss, const std::vector<int>& wrt, int seed = -1);
 
 // sha256.cpp
 std::string sha256_hex(const std::string& data);

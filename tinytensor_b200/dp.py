@@ -155,7 +155,7 @@ class DataParallelSGD:
         from .compiler import DeviceBuffer, Event, Stream
 
         if getattr(self, "_slots", None) is None:
-            self._slots = [[DeviceBuffer(h.shape) for h in host_inputs] for _ in range(2)]
+            self._slots = [[DeviceBuffer(h.shape, dtype=h.dtype) for h in host_inputs] for _ in range(2)]
             self._copy_stream = Stream()
             self._copied = [Event(), Event()]
             self._consumed = [Event(), Event()]

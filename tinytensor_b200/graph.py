@@ -4,7 +4,8 @@ node table the C ABI compiles (tt_graph in include/tt_cuda.h).
 Shape rules and the exceptions they raise follow the reference builders
 (src/graph/graph.cpp:51-200): NumPy broadcasting for binary ops, the batched matmul
 rule, transpose axis normalisation, and reductions with optional keepdims.
-Additional builders for ops the reference lacks: exp, neg, tanh, reduce_max.
+Additional builders for ops the reference lacks: exp, neg, tanh, reduce_max, and the
+sequence operators gated_scan, scan_last, token_logprob, policy_loss, preference_loss.
 """
 
 import builtins
@@ -18,11 +19,13 @@ from ._lib import BroadcastError, DimensionError, IRError, ShapeError, TypeError
 
 float32 = "float32"
 float64 = "float64"
-_DTYPE_CODE = {float32: 0, float64: 1}
+int32 = "int32"  # token ids: graph inputs read by the token operators
+_DTYPE_CODE = {float32: 0, float64: 1, int32: 2}
 
 __all__ = [
-    "Graph", "Node", "float32", "float64", "add", "sub", "mul", "div", "relu", "sigmoid",
+    "Graph", "Node", "float32", "float64", "int32", "add", "sub", "mul", "div", "relu", "sigmoid",
     "matmul", "sum", "mean", "max", "transpose", "exp", "neg", "tanh",
+    "gated_scan", "scan_last", "token_logprob", "policy_loss", "preference_loss",
 ]
 
 
@@ -43,7 +46,7 @@ class Node:
     """A graph node (the Python face of tinytensor::Node)."""
 
     __slots__ = ("_graph", "index", "op", "shape", "dtype", "inputs", "id", "name", "dim0", "dim1",
-                 "axes", "keepdims", "data", "expr")
+                 "axes", "keepdims", "data", "expr", "attrs")
 
     def __init__(self, graph, op, shape, dtype, inputs=(), name=""):
         self._graph = graph
@@ -59,6 +62,7 @@ class Node:
         self.keepdims = False
         self.data = None
         self.expr = None
+        self.attrs = None  # sequence operators: their numbers (tt_op_attrs.f)
 
     def __add__(self, other):
         return self._graph.add(self, other)
@@ -240,6 +244,124 @@ class Graph:
     def reduce_max(self, a, axes=None, keepdims: bool = False) -> Node:
         return self._reduce(_lib.OP_REDUCE_MAX, a, axes, keepdims)
 
+    def _expand(self, a, shape):
+        a = self._ensure(a)
+        if a.shape == shape:
+            return a
+        if broadcast_shapes(a.shape, shape) != shape:
+            raise BroadcastError(f"Shape {a.shape} does not broadcast to {shape}")
+        return self._add(Node(self, _lib.OP_EXPAND, shape, a.dtype, [a]))
+
+    def _float32(self, what, *nodes):
+        for n in nodes:
+            if n.dtype != float32:
+                raise TypeError(f"{what} takes float32 operands, got {n.dtype}")
+
+    def gated_scan(self, gate, x, init=None, axis: int = -2) -> Node:
+        """Gated linear recurrence h[t] = gate[t] * h[t-1] + x[t] along `axis`, from h[-1] = init
+        (zeros when None).  gate and x broadcast together; init broadcasts to their shape
+        without the axis.  The gradient reaches all three.  One step (an axis of size 1)
+        with the last state as init is the form for serving one token at a time; a gate
+        of 0 starts anew there, e.g. at a document's first token.  A NaN or infinite state
+        stays until a gate of 0 meets it, where it is NaN (0 * inf), as in the recurrence."""
+        gate, x = self._ensure(gate), self._ensure(x)
+        self._float32("gated_scan", gate, x)
+        shape = broadcast_shapes(gate.shape, x.shape)
+        r = len(shape)
+        ax = axis + r if axis < 0 else axis
+        if not 0 <= ax < r:
+            raise DimensionError(f"Invalid gated_scan axis {axis} for rank {r}")
+        ins = [self._expand(gate, shape), self._expand(x, shape)]
+        if init is not None:
+            init = self._ensure(init)
+            self._float32("gated_scan", init)
+            ins.append(self._expand(init, shape[:ax] + shape[ax + 1:]))
+        n = Node(self, _lib.OP_GATED_SCAN, shape, float32, ins)
+        n.dim0 = ax
+        n.attrs = ()
+        return self._add(n)
+
+    def scan_last(self, h) -> Node:
+        """The state after the last step of gated_scan's result `h` (init, or zeros, when there
+        are no steps): the next window's init.  When only it is used, the states in between
+        are not stored."""
+        h = self._ensure(h)
+        if h.op != _lib.OP_GATED_SCAN:
+            raise IRError("scan_last takes the result of a gated_scan")
+        return self._add(Node(self, _lib.OP_SCAN_LAST, h.shape[:h.dim0] + h.shape[h.dim0 + 1:], h.dtype, [h]))
+
+    def _token_operands(self, what, logits, tokens, rank=None):
+        logits, tokens = self._ensure(logits), self._ensure(tokens)
+        self._float32(what, logits)
+        if tokens.dtype != int32:
+            raise TypeError(f"{what} takes int32 tokens, got {tokens.dtype}")
+        if not logits.shape:
+            raise DimensionError(f"{what} needs logits of rank 1 or more")
+        if logits.shape[-1] == 0:
+            raise ShapeError(f"{what} needs a vocabulary of at least one token")
+        if rank is not None and (len(logits.shape) != rank or logits.shape[-3] != 2):
+            raise ShapeError(f"{what} needs logits [pairs, 2, tokens, vocabulary], got {logits.shape}")
+        if tokens.shape != logits.shape[:-1]:
+            raise ShapeError(f"{what}: tokens {tokens.shape} do not go with logits {logits.shape}")
+        return logits, tokens
+
+    def _token_node(self, op, shape, ins, attrs):
+        n = Node(self, op, shape, float32, ins)
+        n.attrs = tuple(float(a) for a in attrs)
+        return self._add(n)
+
+    def token_logprob(self, logits, tokens) -> Node:
+        """log softmax(logits)[token] for logits [..., V] and int32 tokens [...].
+
+        Padding is a negative token: its logits are not read (whatever they hold), its value
+        and its gradient are 0.  A token of V or more gives NaN and DeviceStatusError.  With
+        seed = -weights it is the cross-entropy's gradient."""
+        logits, tokens = self._token_operands("token_logprob", logits, tokens)
+        return self._token_node(_lib.OP_TOKEN_LOGPROB, tokens.shape, [logits, tokens], ())
+
+    def policy_loss(self, logits, tokens, old_logp, advantage, ref_logp=None, clip=(0.2, 0.2), kl: float = 0.0) -> Node:
+        """Clipped policy loss of every token, with a KL term to a reference policy:
+
+            r = exp(p - old_logp),  p = token_logprob(logits, tokens)
+            -min(r * advantage, clamp(r, 1 - clip[0], 1 + clip[1]) * advantage)
+              + kl * (exp(ref_logp - p) - (ref_logp - p) - 1)
+
+        old_logp, advantage and ref_logp broadcast to the tokens' shape and count as data:
+        the gradient reaches the logits only.  kl > 0 takes ref_logp, kl = 0 does not.
+        Padding as in token_logprob, whatever the other operands hold there."""
+        logits, tokens = self._token_operands("policy_loss", logits, tokens)
+        if len(clip) != 2 or not 0.0 <= clip[0] <= 1.0 or not 0.0 <= clip[1] < float("inf"):
+            raise ValueError("clip must be (lower in [0, 1], upper >= 0)")
+        if not 0.0 <= kl < float("inf"):
+            raise ValueError("kl must be finite and not negative")
+        if (ctypes.c_float(kl).value > 0.0) != (ref_logp is not None):
+            raise ValueError("ref_logp goes with kl > 0, and only with it")
+        data = [old_logp, advantage] + ([] if ref_logp is None else [ref_logp])
+        data = [self._ensure(d) for d in data]
+        self._float32("policy_loss", *data)
+        ins = [logits, tokens] + [self._expand(d, tokens.shape) for d in data]
+        return self._token_node(_lib.OP_POLICY_LOSS, tokens.shape, ins, (clip[0], clip[1], kl))
+
+    def preference_loss(self, logits, tokens, ref_logp, beta: float = 0.1, smoothing: float = 0.0) -> Node:
+        """Preference loss of answer pairs: logits [N, 2, T, V] and tokens [N, 2, T] of the chosen
+        (0) and the rejected (1) answer, ref_logp (broadcast to the tokens' shape) the tokens'
+        log-probabilities under the reference.  Per pair, with S(j) the sum of token_logprob -
+        ref_logp over answer j's tokens and z = beta * (S(0) - S(1)):
+
+            -(1 - smoothing) * log sigmoid(z) - smoothing * log sigmoid(-z)
+
+        The gradient reaches the logits only.  Padding as in token_logprob; an answer of
+        padding alone has S = 0."""
+        logits, tokens = self._token_operands("preference_loss", logits, tokens, rank=4)
+        if not 0.0 < beta < float("inf"):
+            raise ValueError("beta must be finite and positive")
+        if not 0.0 <= smoothing <= 0.5:
+            raise ValueError("smoothing must lie in [0, 0.5]")
+        ref = self._ensure(ref_logp)
+        self._float32("preference_loss", ref)
+        ins = [logits, tokens, self._expand(ref, tokens.shape)]
+        return self._token_node(_lib.OP_PREFERENCE_LOSS, tokens.shape[:1], ins, (beta, smoothing))
+
     def mark_output(self, node: Node) -> None:
         if node is None:
             raise IRError("Cannot mark null node as output")
@@ -269,8 +391,16 @@ class Graph:
             c.op = n.op
             c.dtype = _DTYPE_CODE[n.dtype]
             c.num_inputs = len(n.inputs)
-            for k, q in enumerate(n.inputs):
+            for k, q in enumerate(n.inputs[:_lib.TT_MAX_NODE_INPUTS]):
                 c.inputs[k] = q.index
+            if n.attrs is not None:
+                at = _lib.TTOpAttrs()
+                for k, q in enumerate(n.inputs[_lib.TT_MAX_NODE_INPUTS:]):
+                    at.more_inputs[k] = q.index
+                for k, f in enumerate(n.attrs):
+                    at.f[k] = f
+                keep.append(at)
+                c.data = ctypes.addressof(at)
             if len(n.shape) > _lib.TT_MAX_RANK:
                 raise DimensionError(f"rank {len(n.shape)} exceeds {_lib.TT_MAX_RANK}")
             c.rank = len(n.shape)
@@ -380,3 +510,23 @@ def max(a, axes=None, keepdims=False):  # noqa: A001 - mirrors sum/mean
 
 def transpose(a, dim0, dim1):
     return _unary_node(a).transpose(a, dim0, dim1)
+
+
+def gated_scan(gate, x, init=None, axis=-2):
+    return _graph_of(gate, x).gated_scan(gate, x, init, axis)
+
+
+def scan_last(h):
+    return _unary_node(h).scan_last(h)
+
+
+def token_logprob(logits, tokens):
+    return _graph_of(logits, tokens).token_logprob(logits, tokens)
+
+
+def policy_loss(logits, tokens, old_logp, advantage, ref_logp=None, clip=(0.2, 0.2), kl=0.0):
+    return _graph_of(logits, tokens).policy_loss(logits, tokens, old_logp, advantage, ref_logp, clip, kl)
+
+
+def preference_loss(logits, tokens, ref_logp, beta=0.1, smoothing=0.0):
+    return _graph_of(logits, tokens).preference_loss(logits, tokens, ref_logp, beta, smoothing)

@@ -12,6 +12,7 @@ import ctypes
 from . import _lib
 from ._lib import TypeError
 from .compiler import DeviceBuffer, Stream
+from .graph import float32
 
 __all__ = ["SGD"]
 
@@ -21,6 +22,8 @@ class SGD:
         for p in params:
             if not isinstance(p, DeviceBuffer):
                 raise TypeError("SGD on the CUDA backend updates DeviceBuffer parameters")
+            if p.dtype != float32:
+                raise TypeError("SGD updates float32 parameters")
         self.params = list(params)
         self.lr = float(lr)
         self.momentum = float(momentum)
