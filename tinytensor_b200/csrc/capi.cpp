@@ -391,7 +391,7 @@ static void run_launches(tt_program* p, char* const* in_ptr, char* const* out_pt
             float* out[SO_COUNT];
             for (size_t k = 0; k < SI_COUNT; ++k) in[k] = reinterpret_cast<const float*>(resolve(L.in_refs[k]));
             for (size_t k = 0; k < SO_COUNT; ++k) out[k] = reinterpret_cast<float*>(resolve(L.out_refs[k]));
-            rc = launch_scan(L.sd, in, out, st);
+            rc = launch_scan(L.sd, in, out, resolve(L.scratch_ref), st);
         } else if (L.type == LT_TOKEN) {
             const void* in[TI_COUNT];
             for (size_t k = 0; k < TI_COUNT; ++k) in[k] = resolve(L.in_refs[k]);

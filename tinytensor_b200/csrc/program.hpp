@@ -118,9 +118,10 @@ struct ScanDesc {
     int64_t outer = 1, T = 0, n1 = 1, n2 = 1;
     ScanStrides in[SI_COUNT];
 };
+int64_t scan_scratch_bytes(const ScanDesc& d);
 int scan_launch_count(const ScanDesc& d);
 // in[] / out[]: null where an operand is absent or a result not wanted
-int launch_scan(const ScanDesc& d, const float* const* in, float* const* out, void* stream);
+int launch_scan(const ScanDesc& d, const float* const* in, float* const* out, void* scratch, void* stream);
 
 // ---- token log-probabilities and losses over logits (kernels_token.cu) ----
 enum TokenKind { TK_LOGPROB = 0, TK_POLICY = 1, TK_PREFERENCE = 2 };

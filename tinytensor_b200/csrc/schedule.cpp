@@ -959,6 +959,7 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
                 }
             }
             lb << shape_str(sh) << " axis=" << axis;
+            L.scratch_bytes = scan_scratch_bytes(d);
             L.label = lb.str();
         } else if (un.type == LT_TOKEN) {
             TokenDesc& d = L.td;
