@@ -5,12 +5,14 @@
 //              last state;  dx[t] = u[t],  dgate[t] = u[t]*h[t-1],  dinit = c[0]
 //
 // Both are a chain of maps c -> A*c + H, and maps compose: a run of steps is one map, found
-// without knowing the state it starts from.  Every warp holds a tile of the time axis in
-// registers, finds its tile's map, learns its first state by joining the maps of the tiles
-// before it, and only then writes its states: one pass over the data, each value read once
-// and written once, which is what bounds these kernels (forward 12 bytes a value, backward
-// 20 with all gradients).  Tiles are joined in time order at three levels, so results do not
-// depend on how CTAs are scheduled:
+// without knowing the state it starts from.  Every warp takes a tile of the time axis, finds
+// its map, learns its first state by joining the maps of the tiles before it, and only then
+// writes its states: one pass over the data, each value read once and written once, which is
+// what bounds these kernels (forward 12 bytes a value, backward 20 with all gradients).
+// Tiles come through a two-stage ring in shared memory filled by cp.async: a stage is refilled
+// as soon as its values are in registers, so the loads of the next tiles are in flight while
+// the tiles of this step wait for one another's maps.  Tiles are joined in time order, so
+// results do not depend on how CTAs are scheduled, at three levels:
 //   warps of a CTA        through shared memory, one block barrier a step;
 //   CTAs of a cluster     through distributed shared memory, one cluster barrier a step,
 //                         where there are too few lanes to fill the card;
@@ -20,6 +22,7 @@
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 #include "program.hpp"
@@ -29,6 +32,8 @@ namespace cg = cooperative_groups;
 namespace ttb {
 
 namespace {
+
+constexpr int NW = 8;  // warps of a CTA
 
 struct Operand {
     const float* p;  // null: absent
@@ -43,7 +48,7 @@ struct ScanArgs {
     int64_t seg_len;  // steps of a segment
     int segments;
     int W;            // warps of a CTA along time; the others take further lanes
-    int vec;          // line kernel: bit k = operand k can be read as float4
+    int vec;          // bit k: operand k moves as vectors
 };
 
 enum Pass { ONLY = 0, MAPS = 1, JOINED = 2 };  // the whole scan; its segments' maps; the scan from them
@@ -63,50 +68,63 @@ __device__ __forceinline__ float join_gates(float a, float b) {
 // First m, then n.
 __device__ __forceinline__ float2 join(float2 m, float2 n) { return make_float2(join_gates(m.x, n.x), apply(n, m.y)); }
 
-// The maps of a CTA's warps and of a cluster's CTAs, double-buffered: a buffer is written
-// again two steps later, after a barrier that every reader passes behind its reads.
-template <int NW, int LW>
-struct Exchange {
-    float2 warp[2][NW][LW];
-    float2 cta[2][8][LW];  // [buffer][rank in the cluster]; clusters are cut with W = NW, one lane group a CTA
-};
-
-// Gives this warp the state its tile starts from and advances `c` (the state before the
-// step's first tile, the same in all warps) past the step.  m: the map of the warp's tile.
-template <int NW, int LW>
-__device__ __forceinline__ float tile_state(Exchange<NW, LW>& ex, int buf, float2 m, float& c, int W, int warp, int l,
-                                            int cluster_size, int rank) {
-    const int wt = warp % W, wr = warp / W;
-    ex.warp[buf][warp][l] = m;
-    __syncthreads();
-    float first = c;
-    if (cluster_size > 1) {
-        cg::cluster_group cl = cg::this_cluster();
-        if (wt == 0) {
-            float2 all = ex.warp[buf][warp][l];
-            for (int w = 1; w < W; ++w) all = join(all, ex.warp[buf][wr * W + w][l]);
-            for (int q = 0; q < cluster_size; ++q) cl.map_shared_rank(&ex, q)->cta[buf][rank][l] = all;
-        }
-        cl.sync();
-        float s = c;
-        for (int q = 0; q < cluster_size; ++q) {
-            if (q == rank) first = s;
-            s = apply(ex.cta[buf][q][l], s);
-        }
-        c = s;
-        for (int w = 0; w < wt; ++w) first = apply(ex.warp[buf][wr * W + w][l], first);
-    } else {
-        float s = c;
-        for (int w = 0; w < W; ++w) {
-            if (w == wt) first = s;
-            s = apply(ex.warp[buf][wr * W + w][l], s);
-        }
-        c = s;
+// The map of N steps in scan order.  Gates are multiplied plainly; where that gave NaN, a zero
+// gate among them settles it (after an overflow 0 * inf).
+template <bool BACKWARD, int N, class G, class X>
+__device__ __forceinline__ float2 tile_map(G gate, X x) {
+    float2 m = make_float2(gate(0), BACKWARD ? gate(0) * x(0) : x(0));
+#pragma unroll
+    for (int j = 1; j < N; ++j) {
+        m.x *= gate(j);
+        m.y = BACKWARD ? gate(j) * (x(j) + m.y) : fmaf(gate(j), m.y, x(j));
     }
-    return first;
+    if (m.x != m.x) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (gate(j) == 0.0f) m.x = 0.0f;
+    }
+    return m;
 }
 
-// The state before segment `seg` and what it starts from otherwise.
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// Asynchronous copy of BYTES (4, 8 or 16).
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const float* src) {
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_wait_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+__device__ __forceinline__ void copies_wait_all() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+// Maps and states that the tiles of a step exchange.  Double-buffered: a buffer is written
+// again two steps later, after a barrier that every reader passes behind its reads.
+template <int LW>  // lanes of a warp's tile
+struct Exchange {
+    float2 warp[2][NW][LW];
+    // only where W = NW (otherwise one step covers the axis):
+    float2 cta[2][8][LW];  // by rank in the cluster
+    float state[2][LW];    // the last warp's state behind a step, for the next one
+};
+
+// Where a CTA works: its block of lanes, segment of the axis and place in its cluster.
+struct Place {
+    int64_t block;
+    int seg, rank, size;
+};
+__device__ __forceinline__ Place place(const ScanArgs& a) {
+    Place p;
+    cg::cluster_group cl = cg::this_cluster();
+    p.size = static_cast<int>(cl.num_blocks());
+    p.rank = static_cast<int>(cl.block_rank());
+    const unsigned unit = blockIdx.x / p.size;
+    p.seg = static_cast<int>(unit % a.segments);
+    p.block = unit / a.segments;
+    return p;
+}
+
+// The state before a segment.
 template <int PASS>
 __device__ __forceinline__ float segment_state(const ScanArgs& a, int seg, int64_t lane, const float* carry) {
     float c = 0.0f;
@@ -116,246 +134,526 @@ __device__ __forceinline__ float segment_state(const ScanArgs& a, int seg, int64
     return c;
 }
 
-struct Place {
-    int64_t block;  // of lanes
-    int seg, rank, size;
-};
-__device__ __forceinline__ Place place(const ScanArgs& a) {
-    Place p;
-    cg::cluster_group cl = cg::this_cluster();
-    p.size = static_cast<int>(cl.num_blocks());
-    p.rank = static_cast<int>(cl.block_rank());
-    const int64_t unit = blockIdx.x / p.size;
-    p.seg = static_cast<int>(unit % a.segments);
-    p.block = unit / a.segments;
-    return p;
-}
-
-// ---- lanes side by side in memory ([.., T, lanes]): a warp takes 32 lanes and TS steps, a lane
-// per thread, every step of it one coalesced 128-byte row per operand.
-template <bool BACKWARD, int PASS, int TS, int NW>
-__global__ void __launch_bounds__(NW * 32, 2) scan_cols_kernel(ScanArgs a) {
-    __shared__ Exchange<NW, 32> ex;
-    const Place at = place(a);
-    const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, W = a.W;
-    const int wt = warp % W, wr = warp / W;
-    const int64_t lane = (at.block * (NW / W) + wr) * 32 + l;
-    const bool live = lane < a.lanes;
-    const int64_t o = live ? lane / a.inner : 0, i = live ? lane % a.inner : 0, i1 = i / a.n2, i2 = i % a.n2;
-    const float* p[SI_COUNT];
-#pragma unroll
-    for (int k = 0; k < SI_COUNT; ++k)
-        p[k] = a.in[k].p ? a.in[k].p + o * a.in[k].so + i1 * a.in[k].s1 + i2 * a.in[k].s2 : nullptr;
-    const int64_t dst = o * a.T * a.inner + i;
-    float c = live ? segment_state<PASS>(a, at.seg, lane, p[SI_CARRY]) : 0.0f;
-    float gates = 1.0f;  // MAPS: the segment's product of gates
-    const int64_t begin = at.seg * a.seg_len, end = min(a.T, begin + a.seg_len);
-    const bool want_gate = BACKWARD && PASS != MAPS && a.out[SO_GATE];
+// A CTA's part in the exchange, one lane per thread: thread l of a warp handles lane l of its
+// tile (LW = 32), or all threads the tile's one row (LW = 1; `writer` is one of them).
+template <int LW>
+struct Joiner {
+    Exchange<LW>& ex;
+    const Place& at;
+    int W, wt, wr, warp, l;
     int buf = 0;
-    for (int64_t base = begin; base < end; base += static_cast<int64_t>(at.size) * W * TS, buf ^= 1) {
-        const int64_t r0 = base + (static_cast<int64_t>(at.rank) * W + wt) * TS;
-        const int n = live ? static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(TS), end - r0))) : 0;
-        const int64_t t0 = BACKWARD ? a.T - 1 - r0 : r0, dt = BACKWARD ? -1 : 1;
-        float ga[TS], xv[TS], hv[BACKWARD ? TS : 1];
-        {
-            const float* q = p[SI_GATE] + t0 * a.in[SI_GATE].st;
-            const int64_t step = dt * a.in[SI_GATE].st;
-#pragma unroll
-            for (int j = 0; j < TS; ++j, q += step) ga[j] = j < n ? __ldg(q) : 1.0f;
-        }
-        {
-            const float* q = p[SI_X] + t0 * a.in[SI_X].st;
-            const int64_t step = dt * a.in[SI_X].st;
-            const int nx = p[SI_X] ? n : 0;
-#pragma unroll
-            for (int j = 0; j < TS; ++j, q += step) xv[j] = j < nx ? __ldcs(q) : 0.0f;
-        }
-        if (BACKWARD) {
-            const float* q = p[SI_H] + (t0 - 1) * a.in[SI_H].st;
-            const int64_t step = dt * a.in[SI_H].st;
-            const int nh = want_gate ? static_cast<int>(min(static_cast<int64_t>(n), t0)) : 0;  // t = 0 has init before it
-#pragma unroll
-            for (int j = 0; j < TS; ++j, q += step) hv[j] = j < nh ? __ldcs(q) : 0.0f;
-            if (want_gate && nh < n && p[SI_INIT]) {
-                const float first = __ldg(p[SI_INIT]);
-#pragma unroll
-                for (int j = 0; j < TS; ++j)
-                    if (j == nh) hv[j] = first;
-            }
-        }
-        float2 m = make_float2(ga[0], BACKWARD ? ga[0] * xv[0] : xv[0]);
-#pragma unroll
-        for (int j = 1; j < TS; ++j) {
-            m.x = ga[j] == 0.0f ? 0.0f : m.x * ga[j];
-            m.y = BACKWARD ? ga[j] * (xv[j] + m.y) : fmaf(ga[j], m.y, xv[j]);
-        }
-        float s = tile_state<NW, 32>(ex, buf, m, c, W, warp, l, at.size, at.rank);
-        if constexpr (PASS == MAPS) {
-            for (int w = 0; w < W; ++w) gates = join_gates(gates, ex.warp[buf][wr * W + w][l].x);
-            continue;
-        }
-        int64_t y = dst + t0 * a.inner;
-        const int64_t step = dt * a.inner;
-        const int nm = a.out[SO_MAIN] ? n : 0, ng = want_gate ? n : 0;
-#pragma unroll
-        for (int j = 0; j < TS; ++j, y += step) {  // (past the end: gate 1, x 0, the state stays)
-            if (BACKWARD) {
-                const float u = xv[j] + s;
-                if (j < nm) __stcs(a.out[SO_MAIN] + y, u);
-                if (j < ng) __stcs(a.out[SO_GATE] + y, u * hv[j]);
-                s = ga[j] * u;
-            } else {
-                s = fmaf(ga[j], s, xv[j]);
-                if (j < nm) a.out[SO_MAIN][y] = s;
-            }
-        }
-        // the thread of the last step has the last state as it was stored
-        if (n > 0 && r0 + n == a.T && a.out[SO_LANE]) a.out[SO_LANE][lane] = s;
-    }
-    if (!live || wt != 0 || at.rank != 0) return;
-    if (PASS == MAPS) a.maps[at.seg * a.lanes + lane] = make_float2(gates, c);
-    else if (a.T == 0 && a.out[SO_LANE]) a.out[SO_LANE][lane] = c;
-}
 
-// ---- time adjacent in memory ([.., T]): a warp takes one row and K*128 steps, four adjacent
-// steps per thread and chunk of 128; the threads' maps are joined by shuffles.  Rows need
-// not start on 16 bytes: vectors are cut at the row's own 16-byte boundaries (`shift` steps
-// before its first one), so whole vectors move as float4 and only ragged ends as scalars.
-__device__ __forceinline__ void load4(const Operand& q, const float* p, bool vec, int64_t t, int64_t T, float none, float* v) {
-    if (vec && t >= 0 && t + 3 < T) {
-        const float4 f = __ldcs(reinterpret_cast<const float4*>(p + t));
+    // m: the map of this warp's tile.  Returns the state before the tile; c is the state before
+    // the first step (later steps find theirs in the exchange).
+    __device__ __forceinline__ float first(float2 m, float c, bool first_step, bool writer) {
+        if (writer) ex.warp[buf][warp][l] = m;
+        __syncthreads();
+        if (at.size > 1) {
+            cg::cluster_group cl = cg::this_cluster();
+            if (wt == 0 && writer) {
+                float2 all = m;
+#pragma unroll
+                for (int w = 1; w < NW; ++w) all = join(all, ex.warp[buf][w][l]);
+                for (int q = 0; q < at.size; ++q) cl.map_shared_rank(&ex, q)->cta[buf][at.rank][l] = all;
+            }
+            cl.sync();
+        }
+        float s = first_step ? c : ex.state[buf][l];
+        if (at.size > 1) {
+#pragma unroll
+            for (int q = 0; q < 7; ++q)
+                if (q < at.rank) s = apply(ex.cta[buf][q][l], s);
+        }
+#pragma unroll
+        for (int w = 0; w < NW - 1; ++w)
+            if (w < wt) s = apply(ex.warp[buf][wr * W + w][l], s);
+        return s;
+    }
+    // s: the state behind this warp's tile.  The step's last tile hands it to the next step
+    // (not behind the last step: another CTA of the cluster may have left).
+    __device__ __forceinline__ void hand_on(float s, bool last_step, bool writer) {
+        if (wt == W - 1 && at.rank == at.size - 1 && !last_step && writer) {
+            if (at.size > 1) {
+                cg::cluster_group cl = cg::this_cluster();
+                for (int q = 0; q < at.size; ++q) cl.map_shared_rank(&ex, q)->state[buf ^ 1][l] = s;
+            } else {
+                ex.state[buf ^ 1][l] = s;
+            }
+        }
+        buf ^= 1;
+    }
+    // The product of all gates of a step (for a segment's map; one lane group a CTA).
+    __device__ __forceinline__ void gates_of_step(float& gates) const {
+#pragma unroll
+        for (int w = 0; w < NW; ++w) gates = join_gates(gates, ex.warp[buf][w][l].x);
+    }
+};
+
+template <int V>
+__device__ __forceinline__ void load_shared(const float* p, float* v) {
+    if constexpr (V == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(p);
         v[0] = f.x;
         v[1] = f.y;
         v[2] = f.z;
         v[3] = f.w;
+    } else if constexpr (V == 2) {
+        const float2 f = *reinterpret_cast<const float2*>(p);
+        v[0] = f.x;
+        v[1] = f.y;
     } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = t + j >= 0 && t + j < T ? __ldg(p + (t + j) * q.st) : none;
+        v[0] = *p;
+    }
+}
+template <int V>
+__device__ __forceinline__ void store_vec(float* p, const float* v, bool stream) {
+    if constexpr (V == 4) {
+        const float4 f = make_float4(v[0], v[1], v[2], v[3]);
+        if (stream) __stcs(reinterpret_cast<float4*>(p), f);
+        else *reinterpret_cast<float4*>(p) = f;
+    } else if constexpr (V == 2) {
+        const float2 f = make_float2(v[0], v[1]);
+        if (stream) __stcs(reinterpret_cast<float2*>(p), f);
+        else *reinterpret_cast<float2*>(p) = f;
+    } else {
+        if (stream) __stcs(p, v[0]);
+        else *p = v[0];
     }
 }
 
-__device__ __forceinline__ void store4(float* p, int64_t t, int64_t T, const float* v) {
-    if (t >= 0 && t + 3 < T) {
-        *reinterpret_cast<float4*>(p + t) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (t + j >= 0 && t + j < T) p[t + j] = v[j];
-    }
+// ---- lanes side by side in memory ([.., T, lanes]): a warp's tile is 16 steps of 32 adjacent
+// lanes.  A thread takes V adjacent lanes and 16/V adjacent steps (32/V threads lie across the
+// lanes, V behind one another in time), so that operands move in 4*V bytes a thread and 128
+// bytes a row whatever V is; the V threads of a lane join their maps by shuffles.  Operands
+// whose lanes are adjacent move as V-vectors, operands broadcast over the lanes behind n1 as one
+// value (V > 1 is only cut where each operand is one or the other); V = 1 takes any strides.
+// A thread reads back only what it copied itself, so the ring needs no barrier.
+constexpr int kTileSteps = 16;
+
+template <bool BACKWARD>
+constexpr int kArrays = BACKWARD ? 3 : 2;
+
+template <bool BACKWARD>
+constexpr size_t cols_smem() {
+    return sizeof(Exchange<32>) + 2 * kArrays<BACKWARD> * NW * kTileSteps * 32 * sizeof(float);
 }
 
-template <bool BACKWARD, int PASS, int K, int NW>
-__global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
-    __shared__ Exchange<NW, 1> ex;
+template <bool BACKWARD, int PASS, int V>
+__global__ void __launch_bounds__(NW * 32, BACKWARD ? 2 : 3) scan_cols_kernel(ScanArgs a) {
+    constexpr int TS = kTileSteps / V, COLS = 32 / V, NA = kArrays<BACKWARD>;
+    extern __shared__ __align__(16) unsigned char raw[];
+    float* ring = reinterpret_cast<float*>(raw);  // [stage][operand][warp][step][thread][V]
+    Exchange<32>& ex = *reinterpret_cast<Exchange<32>*>(raw + 2 * NA * NW * kTileSteps * 32 * sizeof(float));
     const Place at = place(a);
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, W = a.W;
     const int wt = warp % W, wr = warp / W;
+    const int col = l % COLS, sub = l / COLS;
+    const int64_t lane0 = (at.block * (NW / W) + wr) * 32, lane = lane0 + col * V;
+    const bool live = lane < a.lanes;
+    int64_t o = 0, i = 0;
+    if (live) {
+        if (a.lanes <= 0x7fffffff) {
+            const unsigned q = static_cast<unsigned>(lane), n = static_cast<unsigned>(a.inner);
+            o = q / n;
+            i = q % n;
+        } else {
+            o = lane / a.inner;
+            i = lane % a.inner;
+        }
+    }
+    const int64_t i1 = a.n2 == a.inner ? 0 : i / a.n2, i2 = i - i1 * a.n2;
+    const float* p[SI_COUNT];
+#pragma unroll
+    for (int k = 0; k < SI_COUNT; ++k)
+        p[k] = a.in[k].p ? a.in[k].p + o * a.in[k].so + i1 * a.in[k].s1 + i2 * a.in[k].s2 : nullptr;
+    const bool want_gate = BACKWARD && PASS != MAPS && a.out[SO_GATE];
+    const int64_t begin = at.seg * a.seg_len, end = min(a.T, begin + a.seg_len);
+    const int64_t stride = static_cast<int64_t>(at.size) * W * kTileSteps;  // of this warp's tiles
+    const int64_t own = begin + (static_cast<int64_t>(at.rank) * W + wt) * kTileSteps + sub * TS;
+    auto run_len = [&](int64_t r0) {
+        return live ? static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(TS), end - r0))) : 0;
+    };
+    auto slot = [&](int stage, int k) { return ring + (((stage * NA + k) * NW + warp) * kTileSteps * 32 + l * V); };
+    // copies of one operand: n steps in scan order from time t on
+    auto fetch = [&](int k, int stage, int arr, int64_t t, int n) {
+        const int64_t step = BACKWARD ? -a.in[k].st : a.in[k].st;
+        const float* q = p[k] + t * a.in[k].st;
+        const uint32_t dst = smem_addr(slot(stage, arr));
+        if (V > 1 && (a.vec >> k & 1)) {
+#pragma unroll
+            for (int j = 0; j < TS; ++j, q += step)
+                if (j < n) copy_async<4 * V>(dst + j * 128 * V, q);
+        } else {
+#pragma unroll
+            for (int j = 0; j < TS; ++j, q += step)
+                if (j < n) copy_async<4>(dst + j * 128 * V, q);
+        }
+    };
+    auto issue = [&](int64_t r0, int stage) {
+        const int n = run_len(r0);
+        const int64_t t = BACKWARD ? a.T - 1 - r0 : r0;
+        if (n > 0) {
+            fetch(SI_GATE, stage, 0, t, n);
+            if (p[SI_X]) fetch(SI_X, stage, 1, t, n);
+            // the states before each step; before t = 0 there is init
+            if (want_gate) fetch(SI_H, stage, NA - 1, t - 1, static_cast<int>(min(static_cast<int64_t>(n), t)));
+        }
+        copies_commit();
+    };
+    issue(own, 0);
+    issue(own + stride, 1);
+    if (at.size > 1) cg::this_cluster().sync();  // every CTA runs before another writes to it
+
+    // the exchange takes lane lane0 + l: its state before the segment
+    float c = 0.0f;
+    if (lane0 + l < a.lanes) {
+        const float* q = nullptr;
+        if (p[SI_CARRY]) {
+            const int64_t ol = (lane0 + l) / a.inner, il = (lane0 + l) % a.inner;
+            q = a.in[SI_CARRY].p + ol * a.in[SI_CARRY].so + il / a.n2 * a.in[SI_CARRY].s1 + il % a.n2 * a.in[SI_CARRY].s2;
+        }
+        c = segment_state<PASS>(a, at.seg, lane0 + l, q);
+    }
+    if (a.T == 0) {  // no steps: the last state is the first
+        copies_wait_all();
+        if (lane0 + l < a.lanes && wt == 0 && a.out[SO_LANE]) a.out[SO_LANE][lane0 + l] = c;
+        return;
+    }
+    Joiner<32> joiner{ex, at, W, wt, wr, warp, l};
+    float gates = 1.0f;
+    const bool splat_gate = V > 1 && !(a.vec >> SI_GATE & 1), splat_x = V > 1 && !(a.vec >> SI_X & 1);
+    const bool splat_h = V > 1 && !(a.vec >> SI_H & 1);
+    int stage = 0;
+    for (int64_t base = begin; base < end; base += stride, stage ^= 1) {
+        const int64_t r0 = own + (base - begin);
+        const int n = run_len(r0);
+        float ga[TS][V], xv[TS][V], hv[BACKWARD ? TS : 1][V];
+        copies_wait_one();
+        auto read = [&](const float* q, bool splat, int count, float none, float (*dst)[V]) {
+#pragma unroll
+            for (int j = 0; j < TS; ++j) {
+                if (splat) {
+                    const float f = q[j * 32 * V];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) dst[j][v] = f;
+                } else {
+                    load_shared<V>(q + j * 32 * V, dst[j]);
+                }
+            }
+            if (count < TS) {
+#pragma unroll
+                for (int j = 0; j < TS; ++j)
+#pragma unroll
+                    for (int v = 0; v < V; ++v)
+                        if (j >= count) dst[j][v] = none;
+            }
+        };
+        read(slot(stage, 0), splat_gate, n, 1.0f, ga);
+        read(slot(stage, 1), splat_x, p[SI_X] ? n : 0, 0.0f, xv);
+        if constexpr (BACKWARD) {
+            const int64_t t0 = a.T - 1 - r0;
+            const int nh = want_gate ? static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(n), t0))) : 0;
+            read(slot(stage, NA - 1), splat_h, nh, 0.0f, hv);
+            if (want_gate && nh < n && p[SI_INIT]) {
+#pragma unroll
+                for (int j = 0; j < TS; ++j)
+                    if (j == nh)
+#pragma unroll
+                        for (int v = 0; v < V; ++v) hv[j][v] = __ldg(p[SI_INIT] + v * a.in[SI_INIT].s2);
+            }
+        }
+        issue(r0 + 2 * stride, stage);
+        // this thread's maps, those of the threads before it in time, and the tile's
+        float2 m[V], before[V];
+        float2 tile = make_float2(1.0f, 0.0f);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            m[v] = tile_map<BACKWARD, TS>([&](int j) { return ga[j][v]; }, [&](int j) { return xv[j][v]; });
+            before[v] = make_float2(1.0f, 0.0f);
+#pragma unroll
+            for (int d = COLS; d < 32; d *= 2) {
+                const float2 b = make_float2(__shfl_up_sync(0xffffffffu, m[v].x, d), __shfl_up_sync(0xffffffffu, m[v].y, d));
+                if (l >= d) m[v] = join(b, m[v]);
+            }
+            if (V > 1) {
+                const float2 b = make_float2(__shfl_up_sync(0xffffffffu, m[v].x, COLS), __shfl_up_sync(0xffffffffu, m[v].y, COLS));
+                if (sub > 0) before[v] = b;
+                // lane l's map lies with the last of its threads, 32 - COLS + l / V, at v = l % V
+                const float2 w = make_float2(__shfl_sync(0xffffffffu, m[v].x, 32 - COLS + l / V),
+                                             __shfl_sync(0xffffffffu, m[v].y, 32 - COLS + l / V));
+                if (l % V == v) tile = w;
+            } else {
+                tile = m[v];
+            }
+        }
+        const float first = joiner.first(tile, c, base == begin, true);
+        const bool last_step = base + stride >= end;
+        if constexpr (PASS == MAPS) {
+            joiner.gates_of_step(gates);
+            const float s = apply(tile, first);
+            if (last_step && lane0 + l < a.lanes && wt == W - 1) a.maps[at.seg * a.lanes + lane0 + l] = make_float2(gates, s);
+            joiner.hand_on(s, last_step, true);
+        } else {
+            float s[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                s[v] = V > 1 ? __shfl_sync(0xffffffffu, first, col * V + v) : first;
+                if (V > 1 && sub > 0) s[v] = apply(before[v], s[v]);
+            }
+            const int64_t step = BACKWARD ? -a.inner : a.inner;
+            const int64_t y = (o * a.T + (BACKWARD ? a.T - 1 - r0 : r0)) * a.inner + i;
+            float* ym = a.out[SO_MAIN] + y;
+            float* yg = a.out[SO_GATE] + y;
+            const int nm = a.out[SO_MAIN] ? n : 0, ng = want_gate ? n : 0;
+#pragma unroll
+            for (int j = 0; j < TS; ++j, ym += step, yg += step) {  // (past the end: gate 1, x 0, the state stays)
+                float main[V], dg[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if (BACKWARD) {
+                        main[v] = xv[j][v] + s[v];
+                        dg[v] = main[v] * hv[BACKWARD ? j : 0][v];
+                        s[v] = ga[j][v] * main[v];
+                    } else {
+                        main[v] = s[v] = fmaf(ga[j][v], s[v], xv[j][v]);
+                    }
+                }
+                if (j < nm) store_vec<V>(ym, main, BACKWARD);
+                if (j < ng) store_vec<V>(yg, dg, true);
+            }
+            // the thread of the last step has the last state as it was stored
+            if (n > 0 && r0 + n == a.T && a.out[SO_LANE]) store_vec<V>(a.out[SO_LANE] + lane, s, false);
+            float behind = s[0];  // the state behind the tile, of lane l
+            if (V > 1) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const float w = __shfl_sync(0xffffffffu, s[v], 32 - COLS + l / V);
+                    if (l % V == v) behind = w;
+                }
+            }
+            joiner.hand_on(behind, last_step, true);
+        }
+    }
+    copies_wait_all();
+}
+
+// ---- time adjacent in memory ([.., T]): a warp's tile is 384 steps of one row, a run of 12
+// adjacent steps per thread (an odd number of 16-byte vectors, so that the threads' runs lie
+// in different banks), the runs' maps joined by shuffles.  Tiles move between global and
+// shared memory in coalesced vectors, in and out.  Rows need not start on 16 bytes: vectors are
+// cut at the row's own 16-byte boundaries (`shift` steps before its first one), so whole
+// vectors move as 16 bytes and only ragged ends value by value.
+constexpr int kRun = 12, kTile = 32 * kRun, kVectors = kTile / 4;
+
+template <bool BACKWARD>
+struct RowTile {
+    float in[2][kArrays<BACKWARD>][kTile];
+    float out[kTile];
+    float before[2];  // backward: the state before the tile's first step in memory
+    float pad[2];
+};
+template <bool BACKWARD>
+constexpr size_t rows_smem() {
+    return NW * sizeof(RowTile<BACKWARD>) + sizeof(Exchange<1>);
+}
+
+template <bool BACKWARD, int PASS>
+__global__ void __launch_bounds__(NW * 32, BACKWARD ? 2 : 3) scan_rows_kernel(ScanArgs a) {
+    constexpr int NA = kArrays<BACKWARD>;
+    extern __shared__ __align__(16) unsigned char raw[];
+    const Place at = place(a);
+    const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, W = a.W;
+    const int wt = warp % W, wr = warp / W;
+    RowTile<BACKWARD>& tile = reinterpret_cast<RowTile<BACKWARD>*>(raw)[warp];
+    Exchange<1>& ex = *reinterpret_cast<Exchange<1>*>(raw + NW * sizeof(RowTile<BACKWARD>));
     const int64_t row = at.block * (NW / W) + wr;
     const bool live = row < a.lanes;
     const float* p[SI_COUNT];
 #pragma unroll
     for (int k = 0; k < SI_COUNT; ++k) p[k] = a.in[k].p ? a.in[k].p + (live ? row : 0) * a.in[k].so : nullptr;
     const int64_t dst = (live ? row : 0) * a.T;
-    const int64_t shift = dst & 3, vectors = (a.T + shift + 3) / 4;
-    float c = live ? segment_state<PASS>(a, at.seg, row, p[SI_CARRY]) : 0.0f;
-    float gates = 1.0f;
-    // segments and steps are counted in vectors of four
-    const int64_t begin = at.seg * a.seg_len, end = live ? min(vectors, begin + a.seg_len) : begin;
-    const int64_t steps = (min((a.T + 6) / 4, begin + a.seg_len) - begin);  // the longest row's: all warps loop alike
+    const int shift = static_cast<int>(dst & 3);
+    const int64_t vectors = (a.T + shift + 3) / 4;
     const bool want_gate = BACKWARD && PASS != MAPS && a.out[SO_GATE];
-    int buf = 0;
-    for (int64_t base = 0; base < steps; base += static_cast<int64_t>(at.size) * W * K * 32, buf ^= 1) {
-        const int64_t v0 = begin + base + (static_cast<int64_t>(at.rank) * W + wt) * K * 32 + l;
-        float ga[K][4], xv[K][4];
+    // segments and tiles are counted in vectors of four; scan order r
+    const int64_t begin = at.seg * a.seg_len, end = live ? min(vectors, begin + a.seg_len) : begin;
+    const int64_t all_end = min((a.T + 6) / 4, begin + a.seg_len);  // the longest row's: all warps loop alike
+    const int64_t stride = static_cast<int64_t>(at.size) * W * kVectors;
+    const int64_t own = begin + (static_cast<int64_t>(at.rank) * W + wt) * kVectors;
+    // the tile at r0: its first vector in memory and how many vectors it has; backward a tile that is
+    // cut short keeps its high end
+    auto tile_place = [&](int64_t r0, int64_t& v0) {
+        const int n = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(kVectors), end - r0)));
+        v0 = BACKWARD ? vectors - r0 - kVectors : r0;  // may be negative where n < kVectors
+        return n;
+    };
+    auto issue = [&](int64_t r0, int stage) {
+        int64_t v0;
+        const int n = tile_place(r0, v0);
+        if (n > 0) {
+            const int lo = BACKWARD ? kVectors - n : 0;  // the vectors of the tile that exist: [lo, lo + n)
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int64_t v = v0 + k * 32;
-            const int64_t t = 4 * (BACKWARD ? vectors - 1 - v : v) - shift;
-            const int64_t T = v < end ? a.T : 0;  // 0: nothing of this vector is read
-            load4(a.in[SI_GATE], p[SI_GATE], a.vec >> SI_GATE & 1, t, T, 1.0f, ga[k]);
-            if (p[SI_X]) load4(a.in[SI_X], p[SI_X], a.vec >> SI_X & 1, t, T, 0.0f, xv[k]);
-            else xv[k][0] = xv[k][1] = xv[k][2] = xv[k][3] = 0.0f;
-        }
-        // per chunk: this thread's map, the map of the threads before it, the chunk's map
-        float2 before[K], m = make_float2(1.0f, 0.0f);
-        float2 chunk[K];
+            for (int arr = 0; arr < NA; ++arr) {
+                const int k = arr == 0 ? SI_GATE : arr == 1 ? SI_X : SI_H;
+                if (arr == 1 && !p[SI_X]) continue;
+                if (arr == 2 && !want_gate) continue;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            float2 q;
+                for (int q = 0; q < kVectors / 32; ++q) {
+                    const int v = l + 32 * q;
+                    if (v < lo || v >= lo + n) continue;
+                    const int64_t t = 4 * (v0 + v) - shift;
+                    const uint32_t to = smem_addr(&tile.in[stage][arr][4 * v]);
+                    if ((a.vec >> k & 1) && t >= 0 && t + 3 < a.T) {
+                        copy_async<16>(to, p[k] + t);
+                    } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float g = ga[k][BACKWARD ? 3 - j : j], x = xv[k][BACKWARD ? 3 - j : j];
-                if (j == 0) {
-                    q = make_float2(g, BACKWARD ? g * x : x);
-                } else {
-                    q.x = g == 0.0f ? 0.0f : q.x * g;
-                    q.y = BACKWARD ? g * (x + q.y) : fmaf(g, q.y, x);
+                        for (int j = 0; j < 4; ++j)
+                            if (t + j >= 0 && t + j < a.T) copy_async<4>(to + 4 * j, p[k] + (t + j) * a.in[k].st);
+                    }
                 }
             }
-#pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const float2 b = make_float2(__shfl_up_sync(0xffffffffu, q.x, d), __shfl_up_sync(0xffffffffu, q.y, d));
-                if (l >= d) q = join(b, q);
+            if (want_gate && l == 0) {
+                const int64_t t = 4 * (v0 + lo) - shift - 1;  // before the tile's first step in memory
+                if (t >= 0) copy_async<4>(smem_addr(&tile.before[stage]), p[SI_H] + t * a.in[SI_H].st);
             }
-            chunk[k] = make_float2(__shfl_sync(0xffffffffu, q.x, 31), __shfl_sync(0xffffffffu, q.y, 31));
-            const float2 b = make_float2(__shfl_up_sync(0xffffffffu, q.x, 1), __shfl_up_sync(0xffffffffu, q.y, 1));
-            before[k] = l > 0 ? b : make_float2(1.0f, 0.0f);
-            m = k == 0 ? chunk[0] : join(m, chunk[k]);
         }
-        float s = tile_state<NW, 1>(ex, buf, m, c, W, warp, 0, at.size, at.rank);
+        copies_commit();
+    };
+    issue(own, 0);
+    issue(own + stride, 1);
+    if (at.size > 1) cg::this_cluster().sync();  // every CTA runs before another writes to it
+    float c = live ? segment_state<PASS>(a, at.seg, row, p[SI_CARRY]) : 0.0f;
+    if (a.T == 0) {
+        copies_wait_all();
+        if (live && wt == 0 && l == 0 && a.out[SO_LANE]) a.out[SO_LANE][row] = c;
+        return;
+    }
+    Joiner<1> joiner{ex, at, W, wt, wr, warp, 0};
+    float gates = 1.0f;
+    const float init = want_gate && live && p[SI_INIT] ? __ldg(p[SI_INIT]) : 0.0f;
+    const int run = (BACKWARD ? 31 - l : l) * kRun;  // this thread's run within the tile
+    int stage = 0;
+    for (int64_t base = begin; base < all_end; base += stride, stage ^= 1) {
+        const int64_t r0 = own + (base - begin);
+        int64_t v0;
+        const int n = tile_place(r0, v0);
+        const int lo = BACKWARD ? kVectors - n : 0;
+        const int64_t t0 = 4 * v0 - shift + run;  // the run's first step in memory
+        copies_wait_one();
+        __syncwarp();
+        float ga[kRun], xv[kRun], hv[BACKWARD ? kRun : 1];
+#pragma unroll
+        for (int j = 0; j < kRun; j += 4) {
+            load_shared<4>(&tile.in[stage][0][run + j], ga + j);
+            load_shared<4>(&tile.in[stage][1][run + j], xv + j);
+        }
+        if constexpr (BACKWARD) {
+            if (want_gate) {  // the state before each step
+                float h[kRun];
+#pragma unroll
+                for (int j = 0; j < kRun; j += 4) load_shared<4>(&tile.in[stage][2][run + j], h + j);
+                hv[0] = run > 4 * lo ? tile.in[stage][2][run > 0 ? run - 1 : 0] : tile.before[stage];
+#pragma unroll
+                for (int j = 1; j < kRun; ++j) hv[j] = h[j - 1];
+            }
+        }
+        // the row's ends: steps outside it leave the state as it is
+        const bool whole = n == kVectors && t0 >= (BACKWARD ? 1 : 0) && t0 + kRun <= a.T && p[SI_X];
+        if (!whole) {
+#pragma unroll
+            for (int j = 0; j < kRun; ++j) {
+                const int v = (run + j) / 4;
+                const bool inside = v >= lo && v < lo + n && t0 + j >= 0 && t0 + j < a.T;
+                if (!inside) ga[j] = 1.0f;
+                if (!inside || !p[SI_X]) xv[j] = 0.0f;
+                if (BACKWARD && want_gate && run + j == 4 * lo) hv[BACKWARD ? j : 0] = tile.before[stage];
+                if (BACKWARD && t0 + j == 0) hv[BACKWARD ? j : 0] = init;
+            }
+        }
+        __syncwarp();
+        issue(r0 + 2 * stride, stage);
+        float2 q = tile_map<BACKWARD, kRun>([&](int j) { return ga[BACKWARD ? kRun - 1 - j : j]; },
+                                            [&](int j) { return xv[BACKWARD ? kRun - 1 - j : j]; });
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const float2 b = make_float2(__shfl_up_sync(0xffffffffu, q.x, d), __shfl_up_sync(0xffffffffu, q.y, d));
+            if (l >= d) q = join(b, q);
+        }
+        const float2 m = make_float2(__shfl_sync(0xffffffffu, q.x, 31), __shfl_sync(0xffffffffu, q.y, 31));
+        float2 b = make_float2(__shfl_up_sync(0xffffffffu, q.x, 1), __shfl_up_sync(0xffffffffu, q.y, 1));
+        float s = joiner.first(m, c, base == begin, l == 0);
+        const bool last_step = base + stride >= all_end;
+        float y = l > 0 ? apply(b, s) : s;
         if constexpr (PASS == MAPS) {
-            for (int w = 0; w < W; ++w) gates = join_gates(gates, ex.warp[buf][wr * W + w][0].x);
-            continue;
-        }
+            joiner.gates_of_step(gates);
+            s = apply(m, s);
+            if (last_step && live && wt == W - 1 && l == 0) a.maps[at.seg * a.lanes + row] = make_float2(gates, s);
+        } else {
+            // results over the inputs' registers: x becomes h or dx, h becomes dgate
+            if constexpr (BACKWARD) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int64_t v = v0 + k * 32;
-            const int64_t t = 4 * (BACKWARD ? vectors - 1 - v : v) - shift;
-            const int64_t T = v < end ? a.T : 0;
-            float y = apply(before[k], s);
-            s = apply(chunk[k], s);
-            float main[4], dg[4];
-            if (BACKWARD) {
-                float hv[4];
-                if (want_gate) {
-                    // h[t-1 .. t+2]: the vector at t, moved by one, and its predecessor
-                    load4(a.in[SI_H], p[SI_H], a.vec >> SI_H & 1, t, T, 0.0f, hv);
-                    hv[3] = hv[2];
-                    hv[2] = hv[1];
-                    hv[1] = hv[0];
-                    hv[0] = t > 0 && t - 1 < T ? __ldg(p[SI_H] + (t - 1) * a.in[SI_H].st) : 0.0f;
-                    const float first = t <= 0 && t > -4 && T > 0 && p[SI_INIT] ? __ldg(p[SI_INIT]) : 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (t + j == 0) hv[j] = first;
+                for (int j = kRun - 1; j >= 0; --j) {
+                    xv[j] += y;
+                    y = ga[j] * xv[j];
+                    if (want_gate) hv[j] *= xv[j];
                 }
-#pragma unroll
-                for (int j = 3; j >= 0; --j) {
-                    main[j] = xv[k][j] + y;
-                    if (want_gate) dg[j] = main[j] * hv[j];
-                    y = ga[k][j] * main[j];
-                }
-                if (a.out[SO_MAIN]) store4(a.out[SO_MAIN] + dst, t, T, main);
-                if (want_gate) store4(a.out[SO_GATE] + dst, t, T, dg);
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) main[j] = y = fmaf(ga[k][j], y, xv[k][j]);
-                if (a.out[SO_MAIN]) store4(a.out[SO_MAIN] + dst, t, T, main);
+                for (int j = 0; j < kRun; ++j) xv[j] = y = fmaf(ga[j], y, xv[j]);
             }
-            if (v == vectors - 1 && v < end && a.out[SO_LANE]) a.out[SO_LANE][row] = y;  // the last step's thread
+            auto write = [&](float* out, const float* v) {
+#pragma unroll
+                for (int j = 0; j < kRun; j += 4)
+                    *reinterpret_cast<float4*>(&tile.out[run + j]) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                __syncwarp();
+#pragma unroll
+                for (int u = 0; u < kVectors / 32; ++u) {
+                    const int k = l + 32 * u;
+                    if (k < lo || k >= lo + n) continue;
+                    const int64_t t = 4 * (v0 + k) - shift;
+                    float f[4];
+                    load_shared<4>(&tile.out[4 * k], f);
+                    if (t >= 0 && t + 3 < a.T) {
+                        store_vec<4>(out + dst + t, f, BACKWARD);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (t + j >= 0 && t + j < a.T) out[dst + t + j] = f[j];
+                    }
+                }
+                __syncwarp();
+            };
+            if (a.out[SO_MAIN]) write(a.out[SO_MAIN], xv);
+            if constexpr (BACKWARD) {
+                if (want_gate) write(a.out[SO_GATE], hv);
+            }
+            s = __shfl_sync(0xffffffffu, y, 31);  // behind the tile's last run
+            if (n > 0 && r0 + n == vectors && l == 0 && a.out[SO_LANE]) a.out[SO_LANE][row] = s;
         }
+        joiner.hand_on(s, last_step, l == 0);
     }
-    if (!live || wt != 0 || at.rank != 0 || l != 0) return;
-    if (PASS == MAPS) a.maps[at.seg * a.lanes + row] = make_float2(gates, c);
-    else if (a.T == 0 && a.out[SO_LANE]) a.out[SO_LANE][row] = c;
+    copies_wait_all();
 }
 
-constexpr int kWarps = 16, kSteps = 16, kStepsBack = 8, kChunks = 4, kChunksBack = 2;
+// The widest vectors of lanes: every operand has adjacent lanes behind n1 whose vectors are
+// aligned wherever they start (buffers start on 16 bytes), or is broadcast over them.
+int widest(const ScanDesc& d) {
+    for (int v = 4; v > 1; v /= 2) {
+        bool ok = d.n2 % v == 0;
+        for (int k = 0; k < SI_COUNT && ok; ++k) {
+            const ScanStrides& s = d.in[k];  // (all 0 where absent)
+            if (s.s2 == 0) continue;
+            ok = s.s2 == 1 && s.so % v == 0 && s.st % v == 0 && s.s1 % v == 0 && s.off % v == 0;
+        }
+        if (ok) return v;
+    }
+    return 1;
+}
 
-// How a scan is cut: warps along time, CTAs of a cluster along time, segments.
+// How a scan is cut: lanes per thread, warps along time, CTAs of a cluster along time, segments.
 struct Cut {
     bool rows;
-    int W = 1, cluster = 1, segments = 1;
+    int V = 1, W = 1, cluster = 1, segments = 1;
     int64_t seg_len = 0, blocks = 0;
 };
 
@@ -363,18 +661,16 @@ Cut cut(const ScanDesc& d) {
     Cut c;
     const int64_t inner = d.n1 * d.n2, lanes = d.outer * inner;
     c.rows = inner == 1;
-    // time in units of what one warp holds
-    const int64_t len = c.rows ? (d.T + 6) / 4 : d.T;
-    const int64_t tile = c.rows ? 32 * (d.backward ? kChunksBack : kChunks) : d.backward ? kStepsBack : kSteps;
-    const int64_t tiles = (len + tile - 1) / tile;
-    while (c.W < kWarps && c.W < tiles) c.W *= 2;
+    if (!c.rows) c.V = widest(d);
+    const int64_t len = c.rows ? (d.T + 6) / 4 : d.T;  // rows count time in vectors of four
+    const int64_t tile = c.rows ? kVectors : kTileSteps, tiles = (len + tile - 1) / tile;
+    while (c.W < NW && c.W < tiles) c.W *= 2;
     const int64_t groups = c.rows ? lanes : (lanes + 31) / 32;
-    c.blocks = (groups + kWarps / c.W - 1) / (kWarps / c.W);
-    // two CTAs fit an SM: more of them along time while the card is not full and every CTA
-    // still has a step of its own
-    while (c.W == kWarps && c.cluster < 8 && c.blocks * c.cluster < 192 && c.cluster * c.W * tile * 2 <= len) c.cluster *= 2;
+    c.blocks = (groups + NW / c.W - 1) / (NW / c.W);
+    // more CTAs along time while the card is not full and every CTA has a step of its own
+    while (c.W == NW && c.cluster < 8 && c.blocks * c.cluster < 256 && c.cluster * c.W * tile * 2 <= len) c.cluster *= 2;
     c.seg_len = len > 0 ? len : 1;
-    if (c.blocks * c.cluster < 96 && len > static_cast<int64_t>(c.cluster) * c.W * tile) {
+    if (c.blocks * c.cluster < 128 && len > static_cast<int64_t>(c.cluster) * c.W * tile) {
         c.cluster = 1;
         const int64_t step = c.W * tile, most = (len + step - 1) / step;
         int64_t want = (296 + c.blocks - 1) / c.blocks;
@@ -385,20 +681,38 @@ Cut cut(const ScanDesc& d) {
     return c;
 }
 
-template <bool BACKWARD, int PASS>
-cudaError_t launch_pass(const Cut& c, const ScanArgs& a, cudaStream_t stream) {
+template <auto Kernel>
+cudaError_t launch_kernel(size_t smem, const Cut& c, const ScanArgs& a, cudaStream_t stream) {
+    static std::atomic<uint64_t> ready{0};  // devices on which the kernel's shared memory limit is raised
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (!(ready.load() & bit)) {
+        e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+        ready |= bit;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(c.blocks * c.segments * c.cluster));
-    cfg.blockDim = dim3(kWarps * 32);
+    cfg.blockDim = dim3(NW * 32);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = static_cast<unsigned>(c.cluster);
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    if (c.rows) return cudaLaunchKernelEx(&cfg, scan_rows_kernel<BACKWARD, PASS, BACKWARD ? kChunksBack : kChunks, kWarps>, a);
-    return cudaLaunchKernelEx(&cfg, scan_cols_kernel<BACKWARD, PASS, BACKWARD ? kStepsBack : kSteps, kWarps>, a);
+    cfg.numAttrs = c.cluster > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, Kernel, a);
+}
+
+template <bool BACKWARD, int PASS>
+cudaError_t launch_pass(const Cut& c, const ScanArgs& a, cudaStream_t stream) {
+    if (c.rows) return launch_kernel<scan_rows_kernel<BACKWARD, PASS>>(rows_smem<BACKWARD>(), c, a, stream);
+    if (c.V == 4) return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 4>>(cols_smem<BACKWARD>(), c, a, stream);
+    if (c.V == 2) return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 2>>(cols_smem<BACKWARD>(), c, a, stream);
+    return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 1>>(cols_smem<BACKWARD>(), c, a, stream);
 }
 
 template <bool BACKWARD>
@@ -429,9 +743,8 @@ int launch_scan(const ScanDesc& d, const float* const* in, float* const* out, vo
     for (int k = 0; k < SI_COUNT; ++k) {
         const ScanStrides& s = d.in[k];
         a.in[k] = Operand{in[k] ? in[k] + s.off : nullptr, s.so, s.st, s.s1, s.s2};
-        // float4 where every row starts at the same place within 16 bytes as the result's
-        if (a.in[k].p && s.st == 1 && reinterpret_cast<uintptr_t>(a.in[k].p) % 16 == 0 && (s.so - d.T) % 4 == 0)
-            a.vec |= 1 << k;
+        // rows: every row starts at the same place within 16 bytes as the result's
+        if (c.rows ? s.st == 1 && s.off % 4 == 0 && (s.so - d.T) % 4 == 0 : s.s2 == 1) a.vec |= 1 << k;
     }
     for (int k = 0; k < SO_COUNT; ++k) a.out[k] = out[k];
     a.maps = static_cast<float2*>(scratch);
