@@ -1,14 +1,16 @@
 """The sequence operators in 64 bits, and how far a float32 result may be from them.
 
 Every bound is first-order rounding analysis with u = 2^-24 (half a step of float32):
-each float32 operation multiplies its result by (1 + d), |d| <= u; expf is documented to
-2 ulp, that is 4u relative, on top of its argument's rounding.
+each float32 operation multiplies its result by (1 + d), |d| <= u.  An exponential is
+formed as 2^(d * log2 e): ex2.approx is documented to 2^-22.5, that is 2.83u relative, and
+its argument is off by u |d| each for the difference d = x - m and the product, and by
+0.23u |d| for the constant in float32 (1.3e-8 relative), all in units of the exponent.
 """
 
 import numpy as np
 
 U = 2.0 ** -24
-EXP = 4 * U  # expf, 2 ulp
+EXP, ARG = 4 * U, 2.25 * U  # of the exponential itself, and per |d|
 TINY = 2.0 ** -120  # results so small that float32 holds them as subnormals or zero
 
 
@@ -76,11 +78,11 @@ def _rows(logits, tokens):
         dist = np.where(soft > 0, np.abs(d), 0.0)
         V = x.shape[-1]
         # a sum of V terms in which no term passes more than V/256 + 48 additions
-        rel = EXP + U * (V / 256 + 48) + U * (soft * dist).sum(-1, keepdims=True)
+        rel = EXP + U * (V / 256 + 48) + ARG * (soft * dist).sum(-1, keepdims=True)
         k = np.maximum(tokens, 0)[..., None]
         p = np.take_along_axis(d, k, -1)[..., 0] - np.log(s)[..., 0]
         ptol = rel[..., 0] + U * np.abs(p)
-        soft_rel = EXP + U * dist + rel + 8 * U
+        soft_rel = EXP + ARG * dist + rel + 8 * U
     return p, ptol, soft, soft_rel
 
 

@@ -159,6 +159,7 @@ static void check_token_shapes(const Graph& g, const Node& n) {
     const Shape& logits = shape(0);
     if (logits.empty()) fail(TT_ERR_DIMENSION, what + " needs logits of rank 1 or more");
     if (logits.back() == 0) fail(TT_ERR_SHAPE, what + " needs a vocabulary of at least one token");
+    if (logits.back() > (1 << 30)) fail(TT_ERR_SHAPE, what + " takes a vocabulary of at most 2^30 tokens");
     const Shape lead(logits.begin(), logits.end() - 1);
     const bool pref = n.op == TT_OP_PREFERENCE_LOSS || n.op == BOP_PREFERENCE_GRAD;
     if (pref && (lead.size() != 3 || lead[1] != 2))

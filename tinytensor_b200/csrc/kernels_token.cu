@@ -17,6 +17,7 @@
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 
@@ -47,7 +48,8 @@ struct TokenArgs {
     float* stats;   // preference loss: per row {m, 1/s, p - ref}; null otherwise
     float* slopes;  // preference loss: per pair, upstream gradient * d loss / d S(0)
     int* status;
-    int64_t rows, n1, V;
+    int64_t rows, n1;
+    int V;  // at most 2^30
     int kind;
     float f0, f1, f2;
 };
@@ -63,6 +65,16 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN propagates
 struct Part {
     float m, s;
 };
+
+// exp(d), d <= 0, as 2^(d log2 e): two instructions instead of a library exp, which made these
+// kernels issue-bound (37 instructions a value; now about 10).  Relative error 2^-22.5 from ex2
+// and at most 2.25 |d| 2^-24 from rounding d, the product and the constant; results below the
+// normal range become 0.
+__device__ __forceinline__ float exp_part(float d) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * 1.44269504f));
+    return e;
+}
 
 // exp(a - b) for the maxima of a part and a whole: 0 for a part of -inf alone, whose sum is 0 too
 __device__ __forceinline__ float part_weight(float m, float whole) { return m == -INFINITY ? 0.0f : expf(m - whole); }
@@ -106,9 +118,10 @@ struct Row {
     }
 };
 
-// `once`: the value is not read again soon (evict it first).
-__device__ __forceinline__ void load_vec(const float* x, int64_t j, int64_t V, bool once, float* v) {
-    if (j >= 0 && j + 3 < V) {
+// Values j .. j+3 of a row, -inf outside it.  `once`: they are not read again soon (evict them
+// first).
+__device__ __forceinline__ void load_vec(const float* x, int j, int V, bool once, float* v) {
+    if (j >= 0 && j <= V - 4) {
         const float4* p = reinterpret_cast<const float4*>(x + j);
         const float4 f = once ? __ldcs(p) : __ldg(p);
         v[0] = f.x;
@@ -120,8 +133,8 @@ __device__ __forceinline__ void load_vec(const float* x, int64_t j, int64_t V, b
         for (int u = 0; u < 4; ++u) v[u] = j + u >= 0 && j + u < V ? __ldg(x + j + u) : -INFINITY;
     }
 }
-__device__ __forceinline__ void store_vec(float* x, int64_t j, int64_t V, bool vec, const float* v) {
-    if (vec && j >= 0 && j + 3 < V) {
+__device__ __forceinline__ void store_vec(float* x, int j, int V, bool vec, const float* v) {
+    if (vec && j >= 0 && j <= V - 4) {
         __stcs(reinterpret_cast<float4*>(x + j), make_float4(v[0], v[1], v[2], v[3]));
     } else {
 #pragma unroll
@@ -129,10 +142,21 @@ __device__ __forceinline__ void store_vec(float* x, int64_t j, int64_t V, bool v
             if (j + u >= 0 && j + u < V) x[j + u] = v[u];
     }
 }
+// The gradient of values j .. j+3 from their exponentials, over them.
+__device__ __forceinline__ void grad_vec(float* v, int j, int token, float scale, float c) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] *= scale;
+    const int k = token - j;
+    if (k >= 0 && k < 4) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (u == k) v[u] += c;
+    }
+}
 
 // A row that is not computed: padding is 0, a token outside the vocabulary is NaN.  `first`:
 // this thread writes the row's scalars; part / parts and tid / G share out the gradient.
-__device__ void fill_row(const TokenArgs& a, const Row& r, bool first, int64_t from, int64_t step) {
+__device__ void fill_row(const TokenArgs& a, const Row& r, bool first, int from, int step) {
     const float v = r.token < 0 ? 0.0f : __int_as_float(0x7fc00000);
     if (first) {
         if (r.token >= 0) *a.status = TT_STATUS_BAD_TOKEN;
@@ -142,7 +166,7 @@ __device__ void fill_row(const TokenArgs& a, const Row& r, bool first, int64_t f
     if (!r.dx || a.stats) return;
     const int out = static_cast<int>(reinterpret_cast<uintptr_t>(r.dx) / 4 % 4);
     const float f[4] = {v, v, v, v};
-    for (int64_t q = from; 4 * q - out < a.V; q += step) store_vec(r.dx, 4 * q - out, a.V, true, f);
+    for (int q = from; 4 * q - out < a.V; q += step) store_vec(r.dx, 4 * q - out, a.V, true, f);
 }
 
 // The row's outputs besides the gradient, and the gradient's factor c, by one thread.
@@ -163,123 +187,115 @@ __device__ __forceinline__ float row_scalars(const TokenArgs& a, const Row& r, f
     return r.dx ? static_cast<float>(slope * static_cast<double>(a.g.at(r.i0, r.i1))) : 0.0f;
 }
 
-// Sum / maximum over a CTA's threads (G a multiple of 32), the same in every thread.  sh: G/32
-// floats that no other reduction of the kernel uses.
-template <int G, bool MAX>
-__device__ __forceinline__ float all_threads(float v, float* sh) {
+template <bool MAX>
+__device__ __forceinline__ float warp_all(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         const float w = __shfl_xor_sync(0xffffffffu, v, o);
         v = MAX ? max_nan(v, w) : v + w;
     }
-    if (G == 32) return v;
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = sh[0];
-#pragma unroll
-    for (int w = 1; w < G / 32; ++w) v = MAX ? max_nan(v, sh[w]) : v + sh[w];
     return v;
 }
 
-// ---- rows held in registers: G threads (a warp, or a CTA of a cluster) hold up to 4*NV values
-// each.  G = 32: 8 rows a CTA, a warp each.
-template <int G, int NV, bool GRAD>
-__global__ void __launch_bounds__(G == 32 ? 256 : G, G == 512 ? 2 : 4) token_held_kernel(TokenArgs a) {
-    __shared__ float sh_max[G / 32], sh_sum[G / 32];
-    __shared__ Part parts[kMaxCluster];
-    __shared__ float sh_c;
-    cg::cluster_group cl = cg::this_cluster();
-    const int size = G == 32 ? 1 : static_cast<int>(cl.num_blocks()), rank = G == 32 ? 0 : static_cast<int>(cl.block_rank());
-    const int tid = G == 32 ? threadIdx.x & 31 : threadIdx.x;
-    const int64_t index = G == 32 ? static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5) : blockIdx.x / size;
-    if (G == 32 && index >= a.rows) return;
+// The part of a warp from its threads' values: v becomes exp(v - maximum).
+template <int NV>
+__device__ __forceinline__ Part warp_part(float (*v)[4]) {
+    float m = v[0][0];
+#pragma unroll
+    for (int q = 0; q < NV; ++q)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) m = max_nan(m, v[q][u]);
+    m = warp_all<true>(m);
+    const float from = m == -INFINITY ? 0.0f : m;
+    float s = 0.0f;
+#pragma unroll
+    for (int q = 0; q < NV; ++q)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s += v[q][u] = exp_part(v[q][u] - from);
+    return Part{m, warp_all<false>(s)};
+}
+
+// Joins N parts (a multiple of 32 or less than 32), the same in every thread of the warp.
+__device__ __forceinline__ Part join_parts(const Part* parts, int n, int l) {
+    Part all{-INFINITY, 0.0f};
+    for (int q = l; q < n; q += 32) all.m = max_nan(all.m, parts[q].m);
+    all.m = warp_all<true>(all.m);
+    for (int q = l; q < n; q += 32) all.s += parts[q].s * part_weight(parts[q].m, all.m);
+    all.s = warp_all<false>(all.s);
+    return all;
+}
+
+// Parts of a CTA's warps or a cluster's: lane q < size hands this warp's part to CTA q.
+struct Parts {
+    Part of[2][kMaxCluster * 16];
+};
+__device__ __forceinline__ void hand_part(Parts& sh, int buf, int size, int slot, int l, Part part) {
+    if (size == 1) {
+        if (l == 0) sh.of[buf][slot] = part;
+        __syncthreads();
+    } else {
+        cg::cluster_group cl = cg::this_cluster();
+        if (l < size) cl.map_shared_rank(&sh, l)->of[buf][slot] = part;
+        cl.sync();
+    }
+}
+
+// ---- short rows: a warp holds a row of at most 128*NV values, 8 rows a CTA.
+template <int NV, bool GRAD>
+__global__ void __launch_bounds__(256, 4) token_warp_kernel(TokenArgs a) {
+    const int l = threadIdx.x & 31;
+    const int64_t index = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (index >= a.rows) return;
     const Row r(a, index);
-    if (r.token < 0 || r.token >= a.V) {  // (the whole cluster leaves)
-        fill_row(a, r, tid == 0 && rank == 0, rank * G + tid, size * G);
+    if (r.token < 0 || r.token >= a.V) {
+        fill_row(a, r, l == 0, l, 32);
         return;
     }
-    if (size > 1) cl.barrier_arrive();  // every CTA runs before another writes to it
     const float xk = __ldg(r.x + r.token);
-    // this CTA's vectors: NV runs of G adjacent ones
-    const int64_t j0 = 4 * (static_cast<int64_t>(rank) * NV * G + tid) - r.shift;
     float v[NV][4];
 #pragma unroll
-    for (int q = 0; q < NV; ++q) load_vec(r.x, j0 + 4 * q * G, a.V, GRAD, v[q]);
-    Part all;
-    all.m = v[0][0];
-#pragma unroll
-    for (int q = 0; q < NV; ++q)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) all.m = max_nan(all.m, v[q][u]);
-    all.m = all_threads<G, true>(all.m, sh_max);
-    const float own = all.m, from = own == -INFINITY ? 0.0f : own;
-    all.s = 0.0f;
-#pragma unroll
-    for (int q = 0; q < NV; ++q)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) all.s += v[q][u] = expf(v[q][u] - from);
-    all.s = all_threads<G, false>(all.s, sh_sum);
-    if (size > 1) {
-        cl.barrier_wait();
-        if (tid < size) *cl.map_shared_rank(&parts[rank], tid) = all;
-        cl.sync();
-        float whole = -INFINITY, sum = 0.0f;
-        for (int q = 0; q < size; ++q) whole = max_nan(whole, parts[q].m);
-        for (int q = 0; q < size; ++q) sum += parts[q].s * part_weight(parts[q].m, whole);
-        all.m = whole;
-        all.s = sum;
-    }
-    if (!GRAD) {
-        if (tid == 0 && rank == 0) row_scalars(a, r, xk, all, true);
-        return;
-    }
-    float c;
-    if (a.kind == TK_LOGPROB) {  // the gradient does not need p
-        c = a.g.at(r.i0, r.i1);
-        if (tid == 0 && rank == 0) row_scalars(a, r, xk, all, true);
-    } else if (G == 32) {
-        c = __shfl_sync(0xffffffffu, tid == 0 ? row_scalars(a, r, xk, all, true) : 0.0f, 0);
-    } else {
-        if (tid == 0) sh_c = row_scalars(a, r, xk, all, rank == 0);
-        __syncthreads();
-        c = sh_c;
-    }
-    // (all.m = NaN or -inf: the sum is NaN or 0 and makes the row NaN)
-    const float scale = -c * (size > 1 ? part_weight(own, all.m) : 1.0f) / all.s;
+    for (int q = 0; q < NV; ++q) load_vec(r.x, 4 * (l + 32 * q) - r.shift, a.V, GRAD, v[q]);
+    const Part all = warp_part<NV>(v);
+    float c = l == 0 ? row_scalars(a, r, xk, all, true) : 0.0f;
+    if (!GRAD) return;
+    c = __shfl_sync(0xffffffffu, c, 0);
+    const float scale = -c / all.s;  // (a NaN row: the sum is NaN; one of -inf: 0)
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
-        const int64_t j = j0 + 4 * q * G;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) v[q][u] = v[q][u] * scale + (j + u == r.token ? c : 0.0f);
+        const int j = 4 * (l + 32 * q) - r.shift;
+        grad_vec(v[q], j, r.token, scale, c);
         store_vec(r.dx, j, a.V, r.dx_vec, v[q]);
     }
 }
 
-// ---- rows longer than a cluster can hold: every CTA reads its share twice, joining maximum and
-// sum as it goes the first time (the second time most of it comes from L2).
-constexpr int kStream = 512, kStreamVec = 4;
+// ---- values without a gradient, and rows longer than a cluster can hold: every CTA walks its
+// share of a row once, joining maximum and sum as it goes; for the gradient it reads it a second
+// time (mostly from L2, latest first).  Few rows are shared by a cluster.
+constexpr int kStream = 256, kStreamVec = 8;
 
 template <bool GRAD>
-__global__ void __launch_bounds__(kStream, 2) token_stream_kernel(TokenArgs a) {
-    __shared__ float sh_max[kStream / 32], sh_sum[kStream / 32];
-    __shared__ Part parts[kMaxCluster];
-    __shared__ float sh_c;
+__global__ void __launch_bounds__(kStream, 4) token_stream_kernel(TokenArgs a) {
+    __shared__ Parts sh;
+    const int tid = threadIdx.x, l = tid & 31, warp = tid >> 5;
     cg::cluster_group cl = cg::this_cluster();
-    const int size = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank()), tid = threadIdx.x;
+    const int size = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
     const Row r(a, blockIdx.x / size);
-    if (r.token < 0 || r.token >= a.V) {
+    if (r.token < 0 || r.token >= a.V) {  // (the whole cluster leaves)
         fill_row(a, r, tid == 0 && rank == 0, rank * kStream + tid, size * kStream);
         return;
     }
-    cl.barrier_arrive();
+    if (size > 1) cl.barrier_arrive();  // every CTA runs before another writes to it
     const float xk = __ldg(r.x + r.token);
-    const int64_t vectors = (a.V + r.shift + 3) / 4, share = (vectors + size - 1) / size;
-    const int64_t begin = min(vectors, rank * share), end = min(vectors, begin + share);
+    const int vectors = (a.V + r.shift + 3) / 4, share = (vectors + size - 1) / size;
+    const int begin = min(vectors, rank * share), end = min(vectors, begin + share);
     Part t{-INFINITY, 0.0f};
-    for (int64_t q0 = begin + tid; q0 < end; q0 += kStreamVec * kStream) {
+    for (int q0 = begin + tid; q0 < end; q0 += kStreamVec * kStream) {
         float v[kStreamVec][4];
 #pragma unroll
-        for (int q = 0; q < kStreamVec; ++q) load_vec(r.x, 4 * (q0 + q * kStream) - r.shift, q0 + q * kStream < end ? a.V : 0, false, v[q]);
+        for (int q = 0; q < kStreamVec; ++q) {
+            const bool in = q0 + q * kStream < end;
+            load_vec(r.x, in ? 4 * (q0 + q * kStream) - r.shift : 0, in ? a.V : 0, false, v[q]);
+        }
         float m = t.m;
 #pragma unroll
         for (int q = 0; q < kStreamVec; ++q)
@@ -290,30 +306,156 @@ __global__ void __launch_bounds__(kStream, 2) token_stream_kernel(TokenArgs a) {
 #pragma unroll
         for (int q = 0; q < kStreamVec; ++q)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) t.s += expf(v[q][u] - from);
+            for (int u = 0; u < 4; ++u) t.s += exp_part(v[q][u] - from);
         t.m = m;
     }
-    Part all;
-    all.m = all_threads<kStream, true>(t.m, sh_max);
-    all.s = all_threads<kStream, false>(t.s * part_weight(t.m, all.m), sh_sum);
-    cl.barrier_wait();
-    if (tid < size) *cl.map_shared_rank(&parts[rank], tid) = all;
-    cl.sync();
-    float whole = -INFINITY, sum = 0.0f;
-    for (int q = 0; q < size; ++q) whole = max_nan(whole, parts[q].m);
-    for (int q = 0; q < size; ++q) sum += parts[q].s * part_weight(parts[q].m, whole);
-    if (tid == 0) sh_c = row_scalars(a, r, xk, Part{whole, sum}, rank == 0);
+    Part w;
+    w.m = warp_all<true>(t.m);
+    w.s = warp_all<false>(t.s * part_weight(t.m, w.m));
+    if (size > 1) cl.barrier_wait();
+    hand_part(sh, 0, size, rank * (kStream / 32) + warp, l, w);
+    if (!GRAD && (warp > 0 || rank > 0)) return;
+    const Part all = join_parts(sh.of[0], size * (kStream / 32), l);
+    float c = l == 0 ? row_scalars(a, r, xk, all, rank == 0 && warp == 0) : 0.0f;
     if (!GRAD) return;
-    __syncthreads();
-    const float c = sh_c, scale = -c / sum;
-    for (int64_t q = end - 1 - tid; q >= begin; q -= kStream) {
+    c = __shfl_sync(0xffffffffu, c, 0);
+    const float scale = -c / all.s;
+    for (int q = end - 1 - tid; q >= begin; q -= kStream) {
         float v[4];
-        const int64_t j = 4 * q - r.shift;
+        const int j = 4 * q - r.shift;
         load_vec(r.x, j, a.V, true, v);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[u] = expf(v[u] - whole) * scale + (j + u == r.token ? c : 0.0f);
+        for (int u = 0; u < 4; ++u) v[u] = exp_part(v[u] - all.m);
+        grad_vec(v, j, r.token, scale, c);
         store_vec(r.dx, j, a.V, r.dx_vec, v);
     }
+}
+
+// ---- loss and gradient of rows that a cluster holds: clusters walk the rows, the next rows
+// coming through a two-stage ring in shared memory (cp.async) while this one's parts are joined.
+// A thread holds NV vectors of its CTA's share and reads back only what it copied itself.  A row
+// costs one cluster barrier (a block barrier where one CTA holds it) for the parts and a block
+// barrier for the row's scalars, which one warp forms.  What bounds it besides the bytes is the
+// instructions a row costs on top of its values (an earlier form spent 30 a value, 20 of them
+// on that), so warps whose vectors all lie inside the row move them without checks.
+template <int G, int NV>
+__global__ void __launch_bounds__(G, G == 512 ? 1 : 3) token_grad_kernel(TokenArgs a, int clusters) {
+    extern __shared__ __align__(16) float ring[];  // [stage][vector][thread][4]
+    __shared__ Parts sh;
+    __shared__ float3 sh_row[2];  // m, -c/s, c
+    cg::cluster_group cl = cg::this_cluster();
+    const int size = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
+    const int tid = threadIdx.x, l = tid & 31, warp = tid >> 5;
+    const int v0 = 4 * (rank * NV * G + tid);           // this thread's first value, its vectors 4*G apart
+    const int lo = v0 - 4 * l, hi = v0 + 4 * (31 - l) + 4 * (NV - 1) * G;  // the warp's first and last vector
+    auto computed = [&](const Row& r) { return r.token >= 0 && r.token < a.V; };
+    auto inside = [&](const Row& r) { return lo >= r.shift && hi - r.shift <= a.V - 4; };
+    auto fetch = [&](const Row& r, bool real, int stage) {
+        if (real && computed(r)) {
+            const int j0 = v0 - r.shift;
+            const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + (stage * NV * G + tid) * 16;
+            const float* x = r.x + j0;
+            if (inside(r)) {
+#pragma unroll
+                for (int q = 0; q < NV; ++q)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + q * G * 16), "l"(x + 4 * q * G) : "memory");
+            } else {
+                for (int q = 0; q < NV; ++q) {
+                    const int j = j0 + 4 * q * G;
+                    if (j >= 0 && j <= a.V - 4) {
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + q * G * 16), "l"(r.x + j) : "memory");
+                    } else {
+                        for (int u = 0; u < 4; ++u)
+                            if (j + u >= 0 && j + u < a.V)
+                                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + q * G * 16 + 4 * u), "l"(r.x + j + u) : "memory");
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    const int64_t first = blockIdx.x / size;
+    Row r0(a, first), r1(a, min(first + clusters, a.rows - 1));
+    fetch(r0, true, 0);
+    fetch(r1, first + clusters < a.rows, 1);
+    float xk = computed(r0) ? __ldg(r0.x + r0.token) : 0.0f;
+    if (size > 1) cl.sync();  // every CTA runs before another writes to it
+    int stage = 0, buf = 0;
+    for (int64_t row = first; row < a.rows; row += clusters, stage ^= 1) {
+        const Row r2(a, min(row + 2 * clusters, a.rows - 1));
+        const float xk1 = computed(r1) ? __ldg(r1.x + r1.token) : 0.0f;
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        const bool real2 = row + 2 * clusters < a.rows;
+        if (!computed(r0)) {  // (the same for the whole cluster)
+            fetch(r2, real2, stage);
+            fill_row(a, r0, tid == 0 && rank == 0, rank * G + tid, size * G);
+        } else {
+            const bool in = inside(r0);
+            const int j0 = v0 - r0.shift;
+            float v[NV][4];
+#pragma unroll
+            for (int q = 0; q < NV; ++q) {
+                const float4 f = *reinterpret_cast<const float4*>(ring + ((stage * NV + q) * G + tid) * 4);
+                v[q][0] = f.x;
+                v[q][1] = f.y;
+                v[q][2] = f.z;
+                v[q][3] = f.w;
+            }
+            if (!in) {
+#pragma unroll
+                for (int q = 0; q < NV; ++q)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (j0 + 4 * q * G + u < 0 || j0 + 4 * q * G + u >= a.V) v[q][u] = -INFINITY;
+            }
+            fetch(r2, real2, stage);
+            const Part own = warp_part<NV>(v);
+            hand_part(sh, buf, size, rank * (G / 32) + warp, l, own);
+            if (warp == 0) {
+                const Part all = join_parts(sh.of[buf], size * (G / 32), l);
+                if (l == 0) {
+                    const bool write = rank == 0;
+                    float c;
+                    if (a.kind == TK_LOGPROB) {  // the gradient does not need p
+                        c = a.g.at(r0.i0, r0.i1);
+                        if (write) row_scalars(a, r0, xk, all, true);
+                    } else {
+                        c = row_scalars(a, r0, xk, all, write);
+                    }
+                    sh_row[buf] = make_float3(all.m, -c / all.s, c);
+                }
+            }
+            __syncthreads();
+            const float3 f = sh_row[buf];
+            buf ^= 1;
+            const float scale = f.y * part_weight(own.m, f.x);  // (a NaN row: the sum is NaN; one of -inf: 0)
+#pragma unroll
+            for (int q = 0; q < NV; ++q)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[q][u] *= scale;
+            const int k = r0.token - j0;  // the token's place among this thread's vectors
+            if (k >= 0 && k < 4 * NV * G && k / 4 % G == 0) {
+#pragma unroll
+                for (int q = 0; q < NV; ++q)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (k == 4 * q * G + u) v[q][u] += f.z;
+            }
+            float* dx = r0.dx + j0;
+            if (in && r0.dx_vec) {
+#pragma unroll
+                for (int q = 0; q < NV; ++q)
+                    __stcs(reinterpret_cast<float4*>(dx + 4 * q * G), make_float4(v[q][0], v[q][1], v[q][2], v[q][3]));
+            } else {
+#pragma unroll
+                for (int q = 0; q < NV; ++q) store_vec(r0.dx, j0 + 4 * q * G, a.V, r0.dx_vec, v[q]);
+            }
+        }
+        r0 = r1;
+        r1 = r2;
+        xk = xk1;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // ---- preference loss: one CTA per pair: z = beta*(S(0) - S(1)), the loss and its slope.
@@ -347,7 +489,7 @@ __global__ void __launch_bounds__(kPair) preference_pair_kernel(TokenArgs a) {
 constexpr int kGrad = 256, kGradVec = 4;
 __global__ void __launch_bounds__(kGrad) preference_grad_kernel(TokenArgs a, int per_row) {
     const Row r(a, a.rows - 1 - blockIdx.x / per_row);
-    const int64_t q0 = static_cast<int64_t>(blockIdx.x % per_row) * kGradVec * kGrad + threadIdx.x;
+    const int q0 = static_cast<int>(blockIdx.x % per_row) * kGradVec * kGrad + threadIdx.x;
     if (r.token < 0 || r.token >= a.V) {
         const float f = r.token < 0 ? 0.0f : __int_as_float(0x7fc00000), v[4] = {f, f, f, f};
 #pragma unroll
@@ -361,54 +503,96 @@ __global__ void __launch_bounds__(kGrad) preference_grad_kernel(TokenArgs a, int
     const float scale = -c * __ldg(a.stats + 3 * r.row + 1);
 #pragma unroll
     for (int q = 0; q < kGradVec; ++q) {
-        const int64_t j = 4 * (q0 + q * kGrad) - r.shift;
+        const int j = 4 * (q0 + q * kGrad) - r.shift;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) v[q][u] = expf(v[q][u] - m) * scale + (j + u == r.token ? c : 0.0f);
+        for (int u = 0; u < 4; ++u) v[q][u] = exp_part(v[q][u] - m);
+        grad_vec(v[q], j, r.token, scale, c);
         store_vec(r.dx, j, a.V, r.dx_vec, v[q]);
     }
 }
 
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
-template <class Kernel>
-cudaError_t launch_rows(Kernel kernel, int64_t blocks, int threads, int cluster, const TokenArgs& a, cudaStream_t stream) {
-    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+// Launch configuration of `blocks` CTAs in clusters.
+struct Launcher {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-    cfg.blockDim = dim3(static_cast<unsigned>(threads));
-    cfg.stream = stream;
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, a);
-}
+    Launcher(int64_t blocks, int threads, size_t smem, int cluster, cudaStream_t stream) {
+        cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+        cfg.blockDim = dim3(static_cast<unsigned>(threads));
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = stream;
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = cluster > 1 ? 1 : 0;
+    }
+};
 
-template <int G, bool GRAD>
-cudaError_t launch_held(int nv, int64_t blocks, int cluster, const TokenArgs& a, cudaStream_t stream) {
-    const int threads = G == 32 ? 256 : G;
-    if (nv <= 1) return launch_rows(token_held_kernel<G, 1, GRAD>, blocks, threads, cluster, a, stream);
-    if (nv <= 2) return launch_rows(token_held_kernel<G, 2, GRAD>, blocks, threads, cluster, a, stream);
-    if (nv <= 4) return launch_rows(token_held_kernel<G, 4, GRAD>, blocks, threads, cluster, a, stream);
-    return launch_rows(token_held_kernel<G, 8, GRAD>, blocks, threads, cluster, a, stream);
+template <int G, int NV>
+cudaError_t launch_grad(const TokenArgs& a, int cluster, cudaStream_t stream) {
+    constexpr size_t smem = 2 * NV * G * 16;
+    // clusters that run at the same time, per device and cluster size (found once: the query
+    // costs more than a small launch)
+    static std::atomic<int> resident[64][kMaxCluster + 1];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    int n = dev < 64 ? resident[dev][cluster].load() : 0;
+    if (n == 0) {
+        e = cudaFuncSetAttribute(token_grad_kernel<G, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        if (e != cudaSuccess) return e;
+        Launcher probe(cluster, G, smem, cluster, stream);
+        if (cluster > 1) {
+            e = cudaOccupancyMaxActiveClusters(&n, token_grad_kernel<G, NV>, &probe.cfg);
+        } else {
+            int per_sm = 0, sms = 0;
+            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, token_grad_kernel<G, NV>, G, smem);
+            if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+            n = per_sm * sms;
+        }
+        if (e != cudaSuccess) return e;
+        if (n < 1) return cudaErrorInvalidConfiguration;
+        if (dev < 64) resident[dev][cluster] = n;
+    }
+    const int clusters = static_cast<int>(a.rows < n ? a.rows : n);
+    Launcher l(static_cast<int64_t>(clusters) * cluster, G, smem, cluster, stream);
+    return cudaLaunchKernelEx(&l.cfg, token_grad_kernel<G, NV>, a, clusters);
 }
 
 template <bool GRAD>
 cudaError_t launch_row_kernel(const TokenArgs& a, cudaStream_t stream) {
-    const int64_t vectors = (a.V + 6) / 4;  // at most, wherever a row starts
-    if (vectors <= 32 * 8)
-        return launch_held<32, GRAD>(static_cast<int>((vectors + 31) / 32), (a.rows + 7) / 8, 1, a, stream);
-    if (vectors > static_cast<int64_t>(kMaxCluster) * 512 * 8)
-        return launch_rows(token_stream_kernel<GRAD>, a.rows * kMaxCluster, kStream, kMaxCluster, a, stream);
-    const int G = vectors > kMaxCluster * 256 * 8 ? 512 : 256;
-    // as many CTAs as hold the row, and more while rows do not fill the card
-    int cluster = static_cast<int>((vectors + G * 8 - 1) / (G * 8));
+    const int vectors = (a.V + 6) / 4;  // at most, wherever a row starts
+    if (vectors <= 32 * 8) {
+        const int nv = (vectors + 31) / 32;
+        const int64_t blocks = (a.rows + 7) / 8;
+        if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+        const dim3 grid(static_cast<unsigned>(blocks));
+        if (nv <= 1) token_warp_kernel<1, GRAD><<<grid, 256, 0, stream>>>(a);
+        else if (nv <= 2) token_warp_kernel<2, GRAD><<<grid, 256, 0, stream>>>(a);
+        else if (nv <= 4) token_warp_kernel<4, GRAD><<<grid, 256, 0, stream>>>(a);
+        else token_warp_kernel<8, GRAD><<<grid, 256, 0, stream>>>(a);
+        return cudaGetLastError();
+    }
+    // as many CTAs a row as hold it, and more while the rows do not fill the card
+    const bool held = GRAD && vectors <= kMaxCluster * 512 * 8;
+    const int G = held && vectors > kMaxCluster * 256 * 8 ? 512 : 256;
+    int cluster = held ? (vectors + G * 8 - 1) / (G * 8) : GRAD ? kMaxCluster : 1;
     while (cluster < kMaxCluster && a.rows * cluster < 296 && cluster * G < vectors) ++cluster;
-    const int nv = static_cast<int>((vectors + cluster * G - 1) / (cluster * G));
-    return G == 512 ? launch_held<512, GRAD>(nv, a.rows * cluster, cluster, a, stream)
-                    : launch_held<256, GRAD>(nv, a.rows * cluster, cluster, a, stream);
+    if constexpr (GRAD) {
+        if (held) {
+            const int nv = (vectors + cluster * G - 1) / (cluster * G);
+            if (G == 512) return launch_grad<512, 8>(a, cluster, stream);
+            if (nv <= 1) return launch_grad<256, 1>(a, cluster, stream);
+            if (nv <= 2) return launch_grad<256, 2>(a, cluster, stream);
+            if (nv <= 4) return launch_grad<256, 4>(a, cluster, stream);
+            return launch_grad<256, 8>(a, cluster, stream);
+        }
+    }
+    if (a.rows * cluster > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    Launcher l(a.rows * cluster, kStream, 0, cluster, stream);
+    return cudaLaunchKernelEx(&l.cfg, token_stream_kernel<GRAD>, a);
 }
 
 }  // namespace
@@ -445,7 +629,7 @@ int launch_token(const TokenDesc& d, const void* const* in, float* y, float* dlo
     a.status = status;
     a.rows = d.n0 * d.n1;
     a.n1 = d.n1;
-    a.V = d.V;
+    a.V = static_cast<int>(d.V);
     a.kind = d.kind;
     a.f0 = d.f[0];
     a.f1 = d.f[1];

@@ -299,6 +299,8 @@ class Graph:
             raise DimensionError(f"{what} needs logits of rank 1 or more")
         if logits.shape[-1] == 0:
             raise ShapeError(f"{what} needs a vocabulary of at least one token")
+        if logits.shape[-1] > 2**30:
+            raise ShapeError(f"{what} takes a vocabulary of at most 2^30 tokens")
         if rank is not None and (len(logits.shape) != rank or logits.shape[-3] != 2):
             raise ShapeError(f"{what} needs logits [pairs, 2, tokens, vocabulary], got {logits.shape}")
         if tokens.shape != logits.shape[:-1]:
