@@ -79,23 +79,10 @@ __device__ __forceinline__ float exp_part(float d) {
 // exp(a - b) for the maxima of a part and a whole: 0 for a part of -inf alone, whose sum is 0 too
 __device__ __forceinline__ float part_weight(float m, float whole) { return m == -INFINITY ? 0.0f : expf(m - whole); }
 
-// Value and slope (d value / d p) of a row from its token's log-probability.
-__device__ void row_value(const TokenArgs& a, int64_t i0, int64_t i1, double p, double& value, double& slope) {
-    value = p;
-    slope = 1.0;
-    if (a.kind != TK_POLICY) return;
-    const double adv = a.adv.at(i0, i1), r = exp(p - static_cast<double>(a.old.at(i0, i1)));
-    const double lo = 1.0 - static_cast<double>(a.f0), hi = 1.0 + static_cast<double>(a.f1);
-    const double plain = r * adv, held = (r < lo ? lo : r > hi ? hi : r) * adv;
-    value = plain <= held ? -plain : -held;
-    slope = plain <= held ? -plain : 0.0;
-    if (plain != plain) value = slope = plain;  // NaN in the row or its numbers
-    if (a.ref.p) {
-        const double k = static_cast<double>(a.ref.at(i0, i1)) - p, e = exp(k), kl = a.f2;
-        value += kl * (e - k - 1.0);
-        slope += kl * (1.0 - e);
-    }
-}
+// What a row's scalars are formed from: the token's logit and the row's operands.
+struct RowNumbers {
+    float xk, old, adv, ref, g;
+};
 
 // A row: its token, where its logits and its gradient lie, and how they lie within 16 bytes.
 // Vectors are cut at the logits' 16-byte boundaries, `shift` values before the row's first.
@@ -155,36 +142,52 @@ __device__ __forceinline__ void grad_vec(float* v, int j, int token, float scale
 }
 
 // A row that is not computed: padding is 0, a token outside the vocabulary is NaN.  `first`:
-// this thread writes the row's scalars; part / parts and tid / G share out the gradient.
-__device__ void fill_row(const TokenArgs& a, const Row& r, bool first, int from, int step) {
-    const float v = r.token < 0 ? 0.0f : __int_as_float(0x7fc00000);
+// this thread writes the row's scalars; vectors from, from + step, ... of the gradient are its.
+__device__ void fill_row(const TokenArgs& a, int64_t row, int token, float* dx, bool first, int from, int step) {
+    const float v = token < 0 ? 0.0f : __int_as_float(0x7fc00000);
     if (first) {
-        if (r.token >= 0) *a.status = TT_STATUS_BAD_TOKEN;
-        if (a.stats) a.stats[3 * r.row + 2] = v;
-        else if (a.y) a.y[r.row] = v;
+        if (token >= 0) *a.status = TT_STATUS_BAD_TOKEN;
+        if (a.stats) a.stats[3 * row + 2] = v;
+        else if (a.y) a.y[row] = v;
     }
-    if (!r.dx || a.stats) return;
-    const int out = static_cast<int>(reinterpret_cast<uintptr_t>(r.dx) / 4 % 4);
+    if (!dx || a.stats) return;
+    const int out = static_cast<int>(reinterpret_cast<uintptr_t>(dx) / 4 % 4);
     const float f[4] = {v, v, v, v};
-    for (int q = from; 4 * q - out < a.V; q += step) store_vec(r.dx, 4 * q - out, a.V, true, f);
+    for (int q = from; 4 * q - out < a.V; q += step) store_vec(dx, 4 * q - out, a.V, true, f);
 }
 
-// The row's outputs besides the gradient, and the gradient's factor c, by one thread.
-__device__ __forceinline__ float row_scalars(const TokenArgs& a, const Row& r, float xk, Part all, bool write) {
+__device__ __forceinline__ RowNumbers row_numbers(const TokenArgs& a, const Row& r) {
+    auto at = [&](const RowOperand& o) { return o.p ? o.at(r.i0, r.i1) : 0.0f; };
+    return RowNumbers{__ldg(r.x + r.token), at(a.old), at(a.adv), at(a.ref), a.kind == TK_PREFERENCE ? 0.0f : at(a.g)};
+}
+
+// The row's value (written where `write`) and the gradient's factor c, by one thread.
+__device__ __forceinline__ float row_scalars(const TokenArgs& a, int64_t row, const RowNumbers& k, Part all, bool write) {
+    const double p = static_cast<double>(k.xk) - static_cast<double>(all.m) - log(static_cast<double>(all.s));
     if (a.stats) {
         if (write) {
-            const double p = static_cast<double>(xk) - static_cast<double>(all.m) - log(static_cast<double>(all.s));
-            a.stats[3 * r.row] = all.m;
-            a.stats[3 * r.row + 1] = 1.0f / all.s;
-            a.stats[3 * r.row + 2] = static_cast<float>(p - static_cast<double>(a.ref.at(r.i0, r.i1)));
+            a.stats[3 * row] = all.m;
+            a.stats[3 * row + 1] = 1.0f / all.s;
+            a.stats[3 * row + 2] = static_cast<float>(p - static_cast<double>(k.ref));
         }
         return 0.0f;
     }
-    const double p = static_cast<double>(xk) - static_cast<double>(all.m) - log(static_cast<double>(all.s));
-    double value, slope;
-    row_value(a, r.i0, r.i1, p, value, slope);
-    if (write && a.y) a.y[r.row] = static_cast<float>(value);
-    return r.dx ? static_cast<float>(slope * static_cast<double>(a.g.at(r.i0, r.i1))) : 0.0f;
+    double value = p, slope = 1.0;  // slope: d value / d p
+    if (a.kind == TK_POLICY) {
+        const double adv = k.adv, r = exp(p - static_cast<double>(k.old));
+        const double lo = 1.0 - static_cast<double>(a.f0), hi = 1.0 + static_cast<double>(a.f1);
+        const double plain = r * adv, held = (r < lo ? lo : r > hi ? hi : r) * adv;
+        value = plain <= held ? -plain : -held;
+        slope = plain <= held ? -plain : 0.0;
+        if (plain != plain) value = slope = plain;  // NaN in the row or its numbers
+        if (a.ref.p) {
+            const double d = static_cast<double>(k.ref) - p, e = exp(d), kl = a.f2;
+            value += kl * (e - d - 1.0);
+            slope += kl * (1.0 - e);
+        }
+    }
+    if (write && a.y) a.y[row] = static_cast<float>(value);
+    return static_cast<float>(slope * static_cast<double>(k.g));
 }
 
 template <bool MAX>
@@ -225,17 +228,17 @@ __device__ __forceinline__ Part join_parts(const Part* parts, int n, int l) {
     return all;
 }
 
-// Parts of a CTA's warps or a cluster's: lane q < size hands this warp's part to CTA q.
+// Hands a warp's part to every CTA of a cluster (lane q < size to CTA q), or to its own CTA.
 struct Parts {
-    Part of[2][kMaxCluster * 16];
+    Part of[kMaxCluster * 8];
 };
-__device__ __forceinline__ void hand_part(Parts& sh, int buf, int size, int slot, int l, Part part) {
+__device__ __forceinline__ void hand_part(Parts& sh, int size, int slot, int l, Part part) {
     if (size == 1) {
-        if (l == 0) sh.of[buf][slot] = part;
+        if (l == 0) sh.of[slot] = part;
         __syncthreads();
     } else {
         cg::cluster_group cl = cg::this_cluster();
-        if (l < size) cl.map_shared_rank(&sh, l)->of[buf][slot] = part;
+        if (l < size) cl.map_shared_rank(&sh, l)->of[slot] = part;
         cl.sync();
     }
 }
@@ -248,15 +251,15 @@ __global__ void __launch_bounds__(256, 4) token_warp_kernel(TokenArgs a) {
     if (index >= a.rows) return;
     const Row r(a, index);
     if (r.token < 0 || r.token >= a.V) {
-        fill_row(a, r, l == 0, l, 32);
+        fill_row(a, r.row, r.token, r.dx, l == 0, l, 32);
         return;
     }
-    const float xk = __ldg(r.x + r.token);
+    const RowNumbers k = row_numbers(a, r);
     float v[NV][4];
 #pragma unroll
     for (int q = 0; q < NV; ++q) load_vec(r.x, 4 * (l + 32 * q) - r.shift, a.V, GRAD, v[q]);
     const Part all = warp_part<NV>(v);
-    float c = l == 0 ? row_scalars(a, r, xk, all, true) : 0.0f;
+    float c = l == 0 ? row_scalars(a, r.row, k, all, true) : 0.0f;
     if (!GRAD) return;
     c = __shfl_sync(0xffffffffu, c, 0);
     const float scale = -c / all.s;  // (a NaN row: the sum is NaN; one of -inf: 0)
@@ -281,11 +284,11 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(TokenArgs a) {
     const int size = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
     const Row r(a, blockIdx.x / size);
     if (r.token < 0 || r.token >= a.V) {  // (the whole cluster leaves)
-        fill_row(a, r, tid == 0 && rank == 0, rank * kStream + tid, size * kStream);
+        fill_row(a, r.row, r.token, r.dx, tid == 0 && rank == 0, rank * kStream + tid, size * kStream);
         return;
     }
     if (size > 1) cl.barrier_arrive();  // every CTA runs before another writes to it
-    const float xk = __ldg(r.x + r.token);
+    const RowNumbers k = row_numbers(a, r);
     const int vectors = (a.V + r.shift + 3) / 4, share = (vectors + size - 1) / size;
     const int begin = min(vectors, rank * share), end = min(vectors, begin + share);
     Part t{-INFINITY, 0.0f};
@@ -313,10 +316,10 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(TokenArgs a) {
     w.m = warp_all<true>(t.m);
     w.s = warp_all<false>(t.s * part_weight(t.m, w.m));
     if (size > 1) cl.barrier_wait();
-    hand_part(sh, 0, size, rank * (kStream / 32) + warp, l, w);
+    hand_part(sh, size, rank * (kStream / 32) + warp, l, w);
     if (!GRAD && (warp > 0 || rank > 0)) return;
-    const Part all = join_parts(sh.of[0], size * (kStream / 32), l);
-    float c = l == 0 ? row_scalars(a, r, xk, all, rank == 0 && warp == 0) : 0.0f;
+    const Part all = join_parts(sh.of, size * (kStream / 32), l);
+    float c = l == 0 ? row_scalars(a, r.row, k, all, rank == 0 && warp == 0) : 0.0f;
     if (!GRAD) return;
     c = __shfl_sync(0xffffffffu, c, 0);
     const float scale = -c / all.s;
@@ -331,29 +334,112 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(TokenArgs a) {
     }
 }
 
-// ---- loss and gradient of rows that a cluster holds: clusters walk the rows, the next rows
-// coming through a two-stage ring in shared memory (cp.async) while this one's parts are joined.
-// A thread holds NV vectors of its CTA's share and reads back only what it copied itself.  A row
-// costs one cluster barrier (a block barrier where one CTA holds it) for the parts and a block
-// barrier for the row's scalars, which one warp forms.  What bounds it besides the bytes is the
-// instructions a row costs on top of its values (an earlier form spent 30 a value, 20 of them
-// on that), so warps whose vectors all lie inside the row move them without checks.
+// ---- loss and gradient of rows that a cluster holds.  Clusters walk the rows.  In each CTA G data
+// threads hold NV vectors of its share of a row in shared memory (they come by cp.async; a thread
+// reads back only what it copied itself) and one more warp joins the parts of the CTA's warps
+// and of the cluster's CTAs and forms the row's scalars.  The data threads work on two rows at a
+// time: while the scalars of row n are formed they find the maximum and the exponentials of row
+// n + 1, and row n + 2 is on its way; then they scale row n and write it.  So neither the
+// cluster barrier nor the scalars' latency is waited for (a form that waited took 5 us a row
+// where the bytes take 3), and the data threads' earlier global stores, which a release waits
+// for, are behind none: only the joining warp releases.
+//   data:  part(n + 1) -> parts full(n + 1) | scalars full(n) -> scale and write row n, fetch n + 3
+//   join:  info(n + 4), parts full(n) -> cluster barrier -> scalars(n) -> scalars full(n)
+// What bounds it besides the bytes is the instructions a row costs on top of its values, so warps
+// whose vectors all lie inside the row move them without checks.
+struct RowInfo {
+    const float* x;
+    float* dx;
+    int64_t row;
+    int token, shift;
+    bool dx_vec;
+};
+constexpr int kStages = 3, kInfos = 8;
+
+// Barriers between the data threads and the joining warp, one id per parity of the row: a fast
+// warp may be one row ahead of a slow one, never two.
+template <int N>
+__device__ __forceinline__ void named_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(N) : "memory"); }
+template <int N>
+__device__ __forceinline__ void named_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory"); }
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive_release() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
 template <int G, int NV>
-__global__ void __launch_bounds__(G, G == 512 ? 1 : 3) token_grad_kernel(TokenArgs a, int clusters) {
-    extern __shared__ __align__(16) float ring[];  // [stage][vector][thread][4]
-    __shared__ Parts sh;
-    __shared__ float3 sh_row[2];  // m, -c/s, c
+__global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(TokenArgs a, int clusters) {
+    constexpr int N = G + 32, FULL = 1, SCALARS = 3;  // barrier ids (+ parity)
+    extern __shared__ __align__(16) float ring[];     // [stage][vector][thread][4]
+    __shared__ Part warp_parts[2][G / 32], cta_parts[2][kMaxCluster];
+    __shared__ float3 scalars[2];  // m, -c/s, c
+    __shared__ RowInfo infos[kInfos];
     cg::cluster_group cl = cg::this_cluster();
     const int size = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
     const int tid = threadIdx.x, l = tid & 31, warp = tid >> 5;
-    const int v0 = 4 * (rank * NV * G + tid);           // this thread's first value, its vectors 4*G apart
+    const int64_t first = blockIdx.x / size;
+    const int count = static_cast<int>((a.rows - first + clusters - 1) / clusters);  // this cluster's rows
+    auto computed = [&](const RowInfo& r) { return r.token >= 0 && r.token < a.V; };
+
+    if (warp == G / 32) {  // ---- the joining warp
+        // lane q keeps operand q of the rows ahead: the token's logit, old, advantage, ref, g
+        auto look = [&](int n) {
+            if (n >= count) return 0.0f;
+            const Row r(a, first + static_cast<int64_t>(n) * clusters);
+            if (l == 0) infos[n % kInfos] = RowInfo{r.x, r.dx, r.row, r.token, r.shift, r.dx_vec};
+            const RowOperand o = l == 1 ? a.old : l == 2 ? a.adv : l == 3 ? a.ref : l == 4 ? a.g : RowOperand{nullptr, 0, 0};
+            if (r.token < 0 || r.token >= a.V) return 0.0f;
+            return l == 0 ? __ldg(r.x + r.token) : o.p ? o.at(r.i0, r.i1) : 0.0f;
+        };
+        float ahead[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) ahead[q] = look(q);
+        __syncthreads();
+        if (size > 1) cl.sync();  // every CTA runs before another writes to it
+        for (int n = 0; n < count; ++n) {
+            const int p = n & 1;
+            const RowInfo r = infos[n % kInfos];
+            const float mine = ahead[0];
+            ahead[0] = ahead[1];
+            ahead[1] = ahead[2];
+            ahead[2] = ahead[3];
+            ahead[3] = look(n + 4);
+            named_sync<N>(FULL + p);
+            if (computed(r)) {  // (the same for the whole cluster)
+                Part all = join_parts(warp_parts[p], G / 32, l);
+                if (size > 1) {
+                    if (l < size) *cl.map_shared_rank(&cta_parts[p][rank], l) = all;
+                    cluster_arrive_release();
+                    cluster_wait();
+                    all = join_parts(cta_parts[p], size, l);
+                }
+                RowNumbers k;
+                k.xk = __shfl_sync(0xffffffffu, mine, 0);
+                k.old = __shfl_sync(0xffffffffu, mine, 1);
+                k.adv = __shfl_sync(0xffffffffu, mine, 2);
+                k.ref = __shfl_sync(0xffffffffu, mine, 3);
+                k.g = __shfl_sync(0xffffffffu, mine, 4);
+                if (l == 0) {
+                    float c = k.g;
+                    if (a.kind != TK_LOGPROB || rank == 0) c = row_scalars(a, r.row, k, all, rank == 0);
+                    scalars[p] = make_float3(all.m, -c / all.s, c);
+                }
+            }
+            __syncwarp();
+            named_arrive<N>(SCALARS + p);
+        }
+        return;
+    }
+
+    // ---- the data threads
+    const int v0 = 4 * (rank * NV * G + tid);  // this thread's first value, its vectors 4*G apart
     const int lo = v0 - 4 * l, hi = v0 + 4 * (31 - l) + 4 * (NV - 1) * G;  // the warp's first and last vector
-    auto computed = [&](const Row& r) { return r.token >= 0 && r.token < a.V; };
-    auto inside = [&](const Row& r) { return lo >= r.shift && hi - r.shift <= a.V - 4; };
-    auto fetch = [&](const Row& r, bool real, int stage) {
-        if (real && computed(r)) {
+    const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + tid * 16;
+    auto inside = [&](const RowInfo& r) { return lo >= r.shift && hi - r.shift <= a.V - 4; };
+    auto fetch = [&](int n) {
+        const RowInfo r = infos[n % kInfos];
+        if (n < count && computed(r)) {
             const int j0 = v0 - r.shift;
-            const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + (stage * NV * G + tid) * 16;
+            const uint32_t to = mine + (n % kStages) * NV * G * 16;
             const float* x = r.x + j0;
             if (inside(r)) {
 #pragma unroll
@@ -374,86 +460,88 @@ __global__ void __launch_bounds__(G, G == 512 ? 1 : 3) token_grad_kernel(TokenAr
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    const int64_t first = blockIdx.x / size;
-    Row r0(a, first), r1(a, min(first + clusters, a.rows - 1));
-    fetch(r0, true, 0);
-    fetch(r1, first + clusters < a.rows, 1);
-    float xk = computed(r0) ? __ldg(r0.x + r0.token) : 0.0f;
-    if (size > 1) cl.sync();  // every CTA runs before another writes to it
-    int stage = 0, buf = 0;
-    for (int64_t row = first; row < a.rows; row += clusters, stage ^= 1) {
-        const Row r2(a, min(row + 2 * clusters, a.rows - 1));
-        const float xk1 = computed(r1) ? __ldg(r1.x + r1.token) : 0.0f;
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-        const bool real2 = row + 2 * clusters < a.rows;
-        if (!computed(r0)) {  // (the same for the whole cluster)
-            fetch(r2, real2, stage);
-            fill_row(a, r0, tid == 0 && rank == 0, rank * G + tid, size * G);
-        } else {
-            const bool in = inside(r0);
-            const int j0 = v0 - r0.shift;
+    auto slot = [&](int n, int q) { return reinterpret_cast<float4*>(ring + (((n % kStages) * NV + q) * G + tid) * 4); };
+    // the row's exponentials over its values, this warp's part of the row; returns the warp's maximum
+    auto part = [&](int n) {
+        const RowInfo r = infos[n % kInfos];
+        float m = 0.0f;
+        if (computed(r)) {
             float v[NV][4];
 #pragma unroll
             for (int q = 0; q < NV; ++q) {
-                const float4 f = *reinterpret_cast<const float4*>(ring + ((stage * NV + q) * G + tid) * 4);
+                const float4 f = *slot(n, q);
                 v[q][0] = f.x;
                 v[q][1] = f.y;
                 v[q][2] = f.z;
                 v[q][3] = f.w;
             }
-            if (!in) {
+            if (!inside(r)) {
+                const int j0 = v0 - r.shift;
 #pragma unroll
                 for (int q = 0; q < NV; ++q)
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
                         if (j0 + 4 * q * G + u < 0 || j0 + 4 * q * G + u >= a.V) v[q][u] = -INFINITY;
             }
-            fetch(r2, real2, stage);
             const Part own = warp_part<NV>(v);
-            hand_part(sh, buf, size, rank * (G / 32) + warp, l, own);
-            if (warp == 0) {
-                const Part all = join_parts(sh.of[buf], size * (G / 32), l);
-                if (l == 0) {
-                    const bool write = rank == 0;
-                    float c;
-                    if (a.kind == TK_LOGPROB) {  // the gradient does not need p
-                        c = a.g.at(r0.i0, r0.i1);
-                        if (write) row_scalars(a, r0, xk, all, true);
-                    } else {
-                        c = row_scalars(a, r0, xk, all, write);
-                    }
-                    sh_row[buf] = make_float3(all.m, -c / all.s, c);
+#pragma unroll
+            for (int q = 0; q < NV; ++q) *slot(n, q) = make_float4(v[q][0], v[q][1], v[q][2], v[q][3]);
+            if (l == 0) warp_parts[n & 1][warp] = own;
+            m = own.m;
+        }
+        __syncwarp();
+        named_arrive<N>(FULL + (n & 1));
+        return m;
+    };
+    __syncthreads();  // the first rows' infos
+    fetch(0);
+    fetch(1);
+    fetch(2);
+    if (size > 1) cl.sync();
+    asm volatile("cp.async.wait_group 2;" ::: "memory");
+    float own = part(0);
+    if (size > 1 && computed(infos[0])) cluster_arrive_relaxed();
+    for (int n = 0; n < count; ++n) {
+        float next = 0.0f;
+        if (n + 1 < count) {
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            next = part(n + 1);
+        }
+        named_sync<N>(SCALARS + (n & 1));
+        const RowInfo r = infos[n % kInfos];
+        const bool real = computed(r);
+        if (size > 1) {
+            if (real) cluster_wait();
+            if (n + 1 < count && computed(infos[(n + 1) % kInfos])) cluster_arrive_relaxed();
+        }
+        if (real) {
+            const float3 f = scalars[n & 1];
+            const float scale = f.y * part_weight(own, f.x);  // (a NaN row: the sum is NaN; one of -inf: 0)
+            const int j0 = v0 - r.shift;
+            const int k = r.token - j0;  // the token's place among this thread's vectors
+            const bool here = k >= 0 && k < 4 * NV * G && k / 4 % G == 0;
+            const bool plain = inside(r) && r.dx_vec;
+            float* dx = r.dx + j0;
+#pragma unroll
+            for (int q = 0; q < NV; ++q) {
+                float4 e = *slot(n, q);
+                e.x *= scale;
+                e.y *= scale;
+                e.z *= scale;
+                e.w *= scale;
+                if (here && k / 4 == q * G) (k % 4 == 0 ? e.x : k % 4 == 1 ? e.y : k % 4 == 2 ? e.z : e.w) += f.z;
+                if (plain) {
+                    __stcs(reinterpret_cast<float4*>(dx + 4 * q * G), e);
+                } else {
+                    const float v[4] = {e.x, e.y, e.z, e.w};
+                    store_vec(r.dx, j0 + 4 * q * G, a.V, r.dx_vec, v);
                 }
             }
-            __syncthreads();
-            const float3 f = sh_row[buf];
-            buf ^= 1;
-            const float scale = f.y * part_weight(own.m, f.x);  // (a NaN row: the sum is NaN; one of -inf: 0)
-#pragma unroll
-            for (int q = 0; q < NV; ++q)
-#pragma unroll
-                for (int u = 0; u < 4; ++u) v[q][u] *= scale;
-            const int k = r0.token - j0;  // the token's place among this thread's vectors
-            if (k >= 0 && k < 4 * NV * G && k / 4 % G == 0) {
-#pragma unroll
-                for (int q = 0; q < NV; ++q)
-#pragma unroll
-                    for (int u = 0; u < 4; ++u)
-                        if (k == 4 * q * G + u) v[q][u] += f.z;
-            }
-            float* dx = r0.dx + j0;
-            if (in && r0.dx_vec) {
-#pragma unroll
-                for (int q = 0; q < NV; ++q)
-                    __stcs(reinterpret_cast<float4*>(dx + 4 * q * G), make_float4(v[q][0], v[q][1], v[q][2], v[q][3]));
-            } else {
-#pragma unroll
-                for (int q = 0; q < NV; ++q) store_vec(r0.dx, j0 + 4 * q * G, a.V, r0.dx_vec, v[q]);
-            }
+        } else {
+            fill_row(a, r.row, r.token, r.dx, tid == 0 && rank == 0, rank * G + tid, size * G);
         }
-        r0 = r1;
-        r1 = r2;
-        xk = xk1;
+        own = next;
+        fetch(n + 3);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
@@ -532,7 +620,7 @@ struct Launcher {
 
 template <int G, int NV>
 cudaError_t launch_grad(const TokenArgs& a, int cluster, cudaStream_t stream) {
-    constexpr size_t smem = 2 * NV * G * 16;
+    constexpr size_t smem = kStages * NV * G * 16;
     // clusters that run at the same time, per device and cluster size (found once: the query
     // costs more than a small launch)
     static std::atomic<int> resident[64][kMaxCluster + 1];
@@ -543,12 +631,12 @@ cudaError_t launch_grad(const TokenArgs& a, int cluster, cudaStream_t stream) {
     if (n == 0) {
         e = cudaFuncSetAttribute(token_grad_kernel<G, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
         if (e != cudaSuccess) return e;
-        Launcher probe(cluster, G, smem, cluster, stream);
+        Launcher probe(cluster, G + 32, smem, cluster, stream);
         if (cluster > 1) {
             e = cudaOccupancyMaxActiveClusters(&n, token_grad_kernel<G, NV>, &probe.cfg);
         } else {
             int per_sm = 0, sms = 0;
-            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, token_grad_kernel<G, NV>, G, smem);
+            e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, token_grad_kernel<G, NV>, G + 32, smem);
             if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
             n = per_sm * sms;
         }
@@ -557,7 +645,7 @@ cudaError_t launch_grad(const TokenArgs& a, int cluster, cudaStream_t stream) {
         if (dev < 64) resident[dev][cluster] = n;
     }
     const int clusters = static_cast<int>(a.rows < n ? a.rows : n);
-    Launcher l(static_cast<int64_t>(clusters) * cluster, G, smem, cluster, stream);
+    Launcher l(static_cast<int64_t>(clusters) * cluster, G + 32, smem, cluster, stream);
     return cudaLaunchKernelEx(&l.cfg, token_grad_kernel<G, NV>, a, clusters);
 }
 
