@@ -12,11 +12,12 @@
 // distributed shared memory, one barrier a row; so are rows that are too few to fill the card.
 // The preference loss's slope depends on all rows of its pair, so its gradient is a second
 // pass, from the rows' m and s, in reverse order: the rows read last are still in L2.
-// Row scalars (p, ratios, losses, c) are formed in double: one thread per row does it, and
-// differences of log-probabilities decide on which side of a clip border a ratio lies.
+// Differences of log-probabilities are formed in double: they decide on which side of a clip border
+// a ratio lies, and a float of p's size is off by more than the ratio should be.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
+#include <cstdlib>
 #include <atomic>
 #include <cmath>
 #include <cstdint>
@@ -70,11 +71,12 @@ struct Part {
 // kernels issue-bound (37 instructions a value; now about 10).  Relative error 2^-22.5 from ex2
 // and at most 2.25 |d| 2^-24 from rounding d, the product and the constant; results below the
 // normal range become 0.
-__device__ __forceinline__ float exp_part(float d) {
+__device__ __forceinline__ float exp2_part(float d) {
     float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * 1.44269504f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d));
     return e;
 }
+__device__ __forceinline__ float exp_part(float d) { return exp2_part(d * 1.44269504f); }
 
 // exp(a - b) for the maxima of a part and a whole: 0 for a part of -inf alone, whose sum is 0 too
 __device__ __forceinline__ float part_weight(float m, float whole) { return m == -INFINITY ? 0.0f : expf(m - whole); }
@@ -161,70 +163,125 @@ __device__ __forceinline__ RowNumbers row_numbers(const TokenArgs& a, const Row&
     return RowNumbers{__ldg(r.x + r.token), at(a.old), at(a.adv), at(a.ref), a.kind == TK_PREFERENCE ? 0.0f : at(a.g)};
 }
 
-// The row's value (written where `write`) and the gradient's factor c, by one thread.
-__device__ __forceinline__ float row_scalars(const TokenArgs& a, int64_t row, const RowNumbers& k, Part all, bool write) {
-    const double p = static_cast<double>(k.xk) - static_cast<double>(all.m) - log(static_cast<double>(all.s));
-    if (a.stats) {
-        if (write) {
-            a.stats[3 * row] = all.m;
-            a.stats[3 * row + 1] = 1.0f / all.s;
-            a.stats[3 * row + 2] = static_cast<float>(p - static_cast<double>(k.ref));
-        }
-        return 0.0f;
-    }
-    double value = p, slope = 1.0;  // slope: d value / d p
-    if (a.kind == TK_POLICY) {
-        const double adv = k.adv, r = exp(p - static_cast<double>(k.old));
-        const double lo = 1.0 - static_cast<double>(a.f0), hi = 1.0 + static_cast<double>(a.f1);
-        const double plain = r * adv, held = (r < lo ? lo : r > hi ? hi : r) * adv;
-        value = plain <= held ? -plain : -held;
-        slope = plain <= held ? -plain : 0.0;
-        if (plain != plain) value = slope = plain;  // NaN in the row or its numbers
-        if (a.ref.p) {
-            const double d = static_cast<double>(k.ref) - p, e = exp(d), kl = a.f2;
-            value += kl * (e - d - 1.0);
-            slope += kl * (1.0 - e);
-        }
-    }
-    if (write && a.y) a.y[row] = static_cast<float>(value);
-    return static_cast<float>(slope * static_cast<double>(k.g));
+// The token's log-probability.  log s of s = 2^k f, 0.75 <= f < 1.5, is k log 2 (in double) + logf(f):
+// |log f| < 0.41, so that float is off by 3e-8 at most, where logf(s) would be by 1e-6.
+__device__ __forceinline__ double token_logp(float xk, Part all) {
+    const int bits = __float_as_int(all.s), k = (bits - 0x3f400000) >> 23;
+    const double log_s = bits >= 0x00800000 && bits < 0x7f800000
+                             ? k * 0.69314718055994530942 + static_cast<double>(logf(__int_as_float(bits - (k << 23))))
+                             : static_cast<double>(logf(all.s));  // 0 (a row of -inf), inf, NaN
+    return static_cast<double>(xk) - static_cast<double>(all.m) - log_s;
 }
 
-template <bool MAX>
-__device__ __forceinline__ float warp_all(float v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float w = __shfl_xor_sync(0xffffffffu, v, o);
-        v = MAX ? max_nan(v, w) : v + w;
+// The gradient's factor c = g * d value / d p.  Ratios are expf of differences formed in double
+// (2 ulp on the slope): the row's data threads wait for this, and two double exponentials in
+// a row took longer than the cluster's exchange.
+__device__ __forceinline__ float row_slope(const TokenArgs& a, const RowNumbers& k, double p) {
+    if (a.kind != TK_POLICY) return k.g;
+    const float r = expf(static_cast<float>(p - static_cast<double>(k.old)));
+    const float lo = 1.0f - a.f0, hi = 1.0f + a.f1;
+    const float plain = r * k.adv, held = (r < lo ? lo : r > hi ? hi : r) * k.adv;
+    float slope = plain <= held ? -plain : 0.0f;
+    if (plain != plain) slope = plain;  // NaN in the row or its numbers
+    if (a.ref.p) slope -= a.f2 * expm1f(static_cast<float>(static_cast<double>(k.ref) - p));
+    return slope * k.g;
+}
+
+// The row's value, or its stats for the preference loss.
+__device__ __forceinline__ void write_value(const TokenArgs& a, int64_t row, const RowNumbers& k, Part all, double p) {
+    if (a.stats) {
+        a.stats[3 * row] = all.m;
+        a.stats[3 * row + 1] = 1.0f / all.s;
+        a.stats[3 * row + 2] = static_cast<float>(p - static_cast<double>(k.ref));
+        return;
     }
+    if (!a.y) return;
+    if (a.kind != TK_POLICY) {
+        a.y[row] = static_cast<float>(p);
+        return;
+    }
+    const float r = expf(static_cast<float>(p - static_cast<double>(k.old)));
+    const float lo = 1.0f - a.f0, hi = 1.0f + a.f1;
+    const float plain = r * k.adv, held = (r < lo ? lo : r > hi ? hi : r) * k.adv;
+    float value = plain <= held ? -plain : -held;
+    if (plain != plain) value = plain;
+    if (a.ref.p) {
+        const float d = static_cast<float>(static_cast<double>(k.ref) - p);
+        value += a.f2 * (expm1f(d) - d);
+    }
+    a.y[row] = value;
+}
+
+__device__ __forceinline__ float warp_max(float v) {  // NaN propagates
+    float d;
+    asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
+    return d;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
-// The part of a warp from its threads' values: v becomes exp(v - maximum).
+// Two float32 operations in one instruction, each rounded as the scalar one.
+struct Pair {
+    uint64_t v;
+};
+__device__ __forceinline__ Pair pair(float x, float y) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(x), "f"(y));
+    return p;
+}
+__device__ __forceinline__ float2 halves(Pair p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+    return f;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+
+// The part of a warp from its threads' values: v becomes exp(v - maximum).  Maxima and sums
+// run in four chains a thread: one chain of 32 dependent operations cost more than their number.
 template <int NV>
 __device__ __forceinline__ Part warp_part(float (*v)[4]) {
-    float m = v[0][0];
+    float m4[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
 #pragma unroll
-    for (int q = 0; q < NV; ++q)
+    for (int q = 1; q < NV; ++q)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) m = max_nan(m, v[q][u]);
-    m = warp_all<true>(m);
+        for (int u = 0; u < 4; ++u) m4[u] = max_nan(m4[u], v[q][u]);
+    const float m = warp_max(max_nan(max_nan(m4[0], m4[1]), max_nan(m4[2], m4[3])));
     const float from = m == -INFINITY ? 0.0f : m;
-    float s = 0.0f;
+    const Pair shift = pair(-from, -from), log2e = pair(1.44269504f, 1.44269504f);
+    Pair s0 = pair(0.0f, 0.0f), s1 = s0;
 #pragma unroll
-    for (int q = 0; q < NV; ++q)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) s += v[q][u] = exp_part(v[q][u] - from);
-    return Part{m, warp_all<false>(s)};
+    for (int q = 0; q < NV; ++q) {
+        const float2 a = halves((pair(v[q][0], v[q][1]) + shift) * log2e), b = halves((pair(v[q][2], v[q][3]) + shift) * log2e);
+        v[q][0] = exp2_part(a.x);
+        v[q][1] = exp2_part(a.y);
+        v[q][2] = exp2_part(b.x);
+        v[q][3] = exp2_part(b.y);
+        s0 = s0 + pair(v[q][0], v[q][1]);
+        s1 = s1 + pair(v[q][2], v[q][3]);
+    }
+    const float2 s = halves(s0 + s1);
+    return Part{m, warp_sum(s.x + s.y)};
 }
 
 // Joins N parts (a multiple of 32 or less than 32), the same in every thread of the warp.
 __device__ __forceinline__ Part join_parts(const Part* parts, int n, int l) {
     Part all{-INFINITY, 0.0f};
     for (int q = l; q < n; q += 32) all.m = max_nan(all.m, parts[q].m);
-    all.m = warp_all<true>(all.m);
+    all.m = warp_max(all.m);
     for (int q = l; q < n; q += 32) all.s += parts[q].s * part_weight(parts[q].m, all.m);
-    all.s = warp_all<false>(all.s);
+    all.s = warp_sum(all.s);
     return all;
 }
 
@@ -259,9 +316,10 @@ __global__ void __launch_bounds__(256, 4) token_warp_kernel(TokenArgs a) {
 #pragma unroll
     for (int q = 0; q < NV; ++q) load_vec(r.x, 4 * (l + 32 * q) - r.shift, a.V, GRAD, v[q]);
     const Part all = warp_part<NV>(v);
-    float c = l == 0 ? row_scalars(a, r.row, k, all, true) : 0.0f;
+    const double p = token_logp(k.xk, all);
+    if (l == 0) write_value(a, r.row, k, all, p);
     if (!GRAD) return;
-    c = __shfl_sync(0xffffffffu, c, 0);
+    const float c = row_slope(a, k, p);
     const float scale = -c / all.s;  // (a NaN row: the sum is NaN; one of -inf: 0)
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
@@ -313,15 +371,16 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(TokenArgs a) {
         t.m = m;
     }
     Part w;
-    w.m = warp_all<true>(t.m);
-    w.s = warp_all<false>(t.s * part_weight(t.m, w.m));
+    w.m = warp_max(t.m);
+    w.s = warp_sum(t.s * part_weight(t.m, w.m));
     if (size > 1) cl.barrier_wait();
     hand_part(sh, size, rank * (kStream / 32) + warp, l, w);
     if (!GRAD && (warp > 0 || rank > 0)) return;
     const Part all = join_parts(sh.of, size * (kStream / 32), l);
-    float c = l == 0 ? row_scalars(a, r.row, k, all, rank == 0 && warp == 0) : 0.0f;
+    const double p = token_logp(k.xk, all);
+    if (l == 0 && rank == 0 && warp == 0) write_value(a, r.row, k, all, p);
     if (!GRAD) return;
-    c = __shfl_sync(0xffffffffu, c, 0);
+    const float c = row_slope(a, k, p);
     const float scale = -c / all.s;
     for (int q = end - 1 - tid; q >= begin; q -= kStream) {
         float v[4];
@@ -367,7 +426,7 @@ __device__ __forceinline__ void cluster_arrive_release() { asm volatile("barrier
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 template <int G, int NV>
-__global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(TokenArgs a, int clusters) {
+__global__ void __launch_bounds__(G + 32, G * NV > 2048 ? 1 : 2) token_grad_kernel(TokenArgs a, int clusters) {
     constexpr int N = G + 32, FULL = 1, SCALARS = 3;  // barrier ids (+ parity)
     extern __shared__ __align__(16) float ring[];     // [stage][vector][thread][4]
     __shared__ Part warp_parts[2][G / 32], cta_parts[2][kMaxCluster];
@@ -404,28 +463,29 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
             ahead[2] = ahead[3];
             ahead[3] = look(n + 4);
             named_sync<N>(FULL + p);
+            Part all;
+            RowNumbers k;
+            double logp = 0.0;
             if (computed(r)) {  // (the same for the whole cluster)
-                Part all = join_parts(warp_parts[p], G / 32, l);
+                all = join_parts(warp_parts[p], G / 32, l);
                 if (size > 1) {
                     if (l < size) *cl.map_shared_rank(&cta_parts[p][rank], l) = all;
                     cluster_arrive_release();
                     cluster_wait();
                     all = join_parts(cta_parts[p], size, l);
                 }
-                RowNumbers k;
                 k.xk = __shfl_sync(0xffffffffu, mine, 0);
                 k.old = __shfl_sync(0xffffffffu, mine, 1);
                 k.adv = __shfl_sync(0xffffffffu, mine, 2);
                 k.ref = __shfl_sync(0xffffffffu, mine, 3);
                 k.g = __shfl_sync(0xffffffffu, mine, 4);
-                if (l == 0) {
-                    float c = k.g;
-                    if (a.kind != TK_LOGPROB || rank == 0) c = row_scalars(a, r.row, k, all, rank == 0);
-                    scalars[p] = make_float3(all.m, -c / all.s, c);
-                }
+                logp = token_logp(k.xk, all);
+                const float c = row_slope(a, k, logp);
+                if (l == 0) scalars[p] = make_float3(all.m, -c / all.s, c);
             }
             __syncwarp();
             named_arrive<N>(SCALARS + p);
+            if (l == 0 && rank == 0 && computed(r)) write_value(a, r.row, k, all, logp);  // nobody waits for it
         }
         return;
     }
@@ -525,10 +585,8 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
 #pragma unroll
             for (int q = 0; q < NV; ++q) {
                 float4 e = *slot(n, q);
-                e.x *= scale;
-                e.y *= scale;
-                e.z *= scale;
-                e.w *= scale;
+                const float2 ex = halves(pair(e.x, e.y) * pair(scale, scale)), ez = halves(pair(e.z, e.w) * pair(scale, scale));
+                e = make_float4(ex.x, ex.y, ez.x, ez.y);
                 if (here && k / 4 == q * G) (k % 4 == 0 ? e.x : k % 4 == 1 ? e.y : k % 4 == 2 ? e.z : e.w) += f.z;
                 if (plain) {
                     __stcs(reinterpret_cast<float4*>(dx + 4 * q * G), e);
@@ -672,6 +730,7 @@ cudaError_t launch_row_kernel(const TokenArgs& a, cudaStream_t stream) {
         if (held) {
             const int nv = (vectors + cluster * G - 1) / (cluster * G);
             if (G == 512) return launch_grad<512, 8>(a, cluster, stream);
+            if (getenv("TG") && vectors > 2048) return launch_grad<512, 8>(a, (vectors + 4095) / 4096, stream);
             if (nv <= 1) return launch_grad<256, 1>(a, cluster, stream);
             if (nv <= 2) return launch_grad<256, 2>(a, cluster, stream);
             if (nv <= 4) return launch_grad<256, 4>(a, cluster, stream);
