@@ -211,7 +211,7 @@ int tt_program_run(tt_program* p, const void* const* inputs, void* const* output
  * (0 = fine; TT_STATUS_BAD_TOKEN = a token id outside the vocabulary, whose position's
  * value and gradient are NaN; anything else = a bounded wait gave up).  Returns
  * TT_ERR_DEVICE_STATUS when it is nonzero and clears it. */
-#define TT_STATUS_BAD_TOKEN 0x400
+#define TT_STATUS_BAD_TOKEN 0x800
 int tt_program_status(tt_program* p, int32_t* device_status);
 /* Per-launch profiling (Profiler::record_node for compiled mode): when enabled, each
  * run records CUDA events around every launch on the run's stream; enabling resets the

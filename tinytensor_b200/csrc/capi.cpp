@@ -121,6 +121,8 @@ struct tt_program {
     }
 };
 
+// The program's status words: [0] a bounded wait that gave up (kernels that wait look at it and
+// stop too), [1] TT_STATUS_BAD_TOKEN (nothing stops for it).
 static std::string status_text(int32_t status) {
     if (status == TT_STATUS_BAD_TOKEN) return "a token id lies outside the vocabulary";
     return "a kernel gave up a bounded wait (status " + std::to_string(status) + ")";
@@ -502,15 +504,16 @@ int tt_program_run(tt_program* p, const void* const* inputs, void* const* output
                     check_cuda(cudaMemcpyAsync(outputs[k], out_ptr[k], static_cast<size_t>(p->out_bytes[k]),
                                                cudaMemcpyDeviceToHost, stream),
                                "output copy");
-            int32_t status = 0;
+            int32_t words[2] = {0, 0};
             if (p->has_status)
-                check_cuda(cudaMemcpyAsync(&status, p->arena + p->plan.status_offset, sizeof(status),
+                check_cuda(cudaMemcpyAsync(words, p->arena + p->plan.status_offset, sizeof(words),
                                            cudaMemcpyDeviceToHost, stream),
                            "status copy");
             check_cuda(cudaStreamSynchronize(stream), "kernel execution");
             collect_profile(p);
+            const int32_t status = words[0] ? words[0] : words[1];
             if (status != 0) {
-                cudaMemsetAsync(p->arena + p->plan.status_offset, 0, 4, stream);
+                cudaMemsetAsync(p->arena + p->plan.status_offset, 0, sizeof(words), stream);
                 fail(TT_ERR_DEVICE_STATUS, status_text(status));
             }
         }
@@ -646,15 +649,16 @@ int tt_program_status(tt_program* p, int32_t* device_status) {
         if (!p) fail(TT_ERR_INVALID, "null program");
         if (p->device < 0) fail(TT_ERR_NO_DEVICE, "program was compiled host-only (TT_FLAG_HOST_ONLY)");
         check_cuda(cudaSetDevice(p->device), "cudaSetDevice");
-        int32_t status = 0;
-        check_cuda(cudaMemcpyAsync(&status, p->arena + p->plan.status_offset, sizeof(status), cudaMemcpyDeviceToHost,
+        int32_t words[2] = {0, 0};
+        check_cuda(cudaMemcpyAsync(words, p->arena + p->plan.status_offset, sizeof(words), cudaMemcpyDeviceToHost,
                                    p->last_stream),
                    "status copy");
         check_cuda(cudaStreamSynchronize(p->last_stream), "kernel execution");
         collect_profile(p);
+        const int32_t status = words[0] ? words[0] : words[1];
         if (device_status) *device_status = status;
         if (status != 0) {
-            cudaMemset(p->arena + p->plan.status_offset, 0, 4);
+            cudaMemset(p->arena + p->plan.status_offset, 0, sizeof(words));
             fail(TT_ERR_DEVICE_STATUS, status_text(status));
         }
     });

@@ -9,7 +9,7 @@
 // wanted.  A loss and its gradient are one kernel that reads a row once: its values stay in
 // registers between the row's maximum and sum and the gradient's write.  A row that no CTA
 // can hold is held by a cluster of up to 8, whose parts' (maximum, sum) are joined through
-// distributed shared memory, one barrier a row; so are rows that are too few to fill the card.
+// distributed shared memory; so are rows that are too few to fill the card.
 // The preference loss's slope depends on all rows of its pair, so its gradient is a second
 // pass, from the rows' m and s, in reverse order: the rows read last are still in L2.
 // Differences of log-probabilities are formed in double: they decide on which side of a clip border
@@ -17,7 +17,6 @@
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
-#include <cstdlib>
 #include <atomic>
 #include <cmath>
 #include <cstdint>
@@ -148,7 +147,7 @@ __device__ __forceinline__ void grad_vec(float* v, int j, int token, float scale
 __device__ void fill_row(const TokenArgs& a, int64_t row, int token, float* dx, bool first, int from, int step) {
     const float v = token < 0 ? 0.0f : __int_as_float(0x7fc00000);
     if (first) {
-        if (token >= 0) *a.status = TT_STATUS_BAD_TOKEN;
+        if (token >= 0) a.status[1] = TT_STATUS_BAD_TOKEN;
         if (a.stats) a.stats[3 * row + 2] = v;
         else if (a.y) a.y[row] = v;
     }
@@ -300,9 +299,10 @@ __device__ __forceinline__ void hand_part(Parts& sh, int size, int slot, int l, 
     }
 }
 
-// ---- short rows: a warp holds a row of at most 128*NV values, 8 rows a CTA.
+// ---- short rows: a warp holds a row of at most 128*NV values, 8 rows a CTA.  Without a gradient a
+// row may be longer: the warp walks it, joining maximum and sum as it goes.
 template <int NV, bool GRAD>
-__global__ void __launch_bounds__(256, 4) token_warp_kernel(TokenArgs a) {
+__global__ void __launch_bounds__(256, NV == 16 ? 2 : GRAD ? 4 : 5) token_warp_kernel(TokenArgs a) {
     const int l = threadIdx.x & 31;
     const int64_t index = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
     if (index >= a.rows) return;
@@ -315,7 +315,17 @@ __global__ void __launch_bounds__(256, 4) token_warp_kernel(TokenArgs a) {
     float v[NV][4];
 #pragma unroll
     for (int q = 0; q < NV; ++q) load_vec(r.x, 4 * (l + 32 * q) - r.shift, a.V, GRAD, v[q]);
-    const Part all = warp_part<NV>(v);
+    Part all = warp_part<NV>(v);
+    if constexpr (!GRAD) {
+        for (int j = 128 * NV - r.shift; j < a.V; j += 128 * NV) {
+#pragma unroll
+            for (int q = 0; q < NV; ++q) load_vec(r.x, j + 4 * (l + 32 * q), a.V, false, v[q]);
+            const Part next = warp_part<NV>(v);
+            const float m = max_nan(all.m, next.m);
+            all.s = all.s * part_weight(all.m, m) + next.s * part_weight(next.m, m);
+            all.m = m;
+        }
+    }
     const double p = token_logp(k.xk, all);
     if (l == 0) write_value(a, r.row, k, all, p);
     if (!GRAD) return;
@@ -333,6 +343,7 @@ __global__ void __launch_bounds__(256, 4) token_warp_kernel(TokenArgs a) {
 // share of a row once, joining maximum and sum as it goes; for the gradient it reads it a second
 // time (mostly from L2, latest first).  Few rows are shared by a cluster.
 constexpr int kStream = 256, kStreamVec = 8;
+constexpr int kWalk = 4096;  // vectors of the longest row that one warp walks
 
 template <bool GRAD>
 __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(TokenArgs a) {
@@ -399,11 +410,10 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(TokenArgs a) {
 // and of the cluster's CTAs and forms the row's scalars.  The data threads work on two rows at a
 // time: while the scalars of row n are formed they find the maximum and the exponentials of row
 // n + 1, and row n + 2 is on its way; then they scale row n and write it.  So neither the
-// cluster barrier nor the scalars' latency is waited for (a form that waited took 5 us a row
-// where the bytes take 3), and the data threads' earlier global stores, which a release waits
-// for, are behind none: only the joining warp releases.
+// cluster's exchange nor the scalars' latency is waited for (a form that waited took 5 us a
+// row where the bytes take 3).
 //   data:  part(n + 1) -> parts full(n + 1) | scalars full(n) -> scale and write row n, fetch n + 3
-//   join:  info(n + 4), parts full(n) -> cluster barrier -> scalars(n) -> scalars full(n)
+//   join:  info(n + 4), parts full(n) -> exchange -> scalars(n) -> scalars full(n)
 // What bounds it besides the bytes is the instructions a row costs on top of its values, so warps
 // whose vectors all lie inside the row move them without checks.
 struct RowInfo {
@@ -421,17 +431,54 @@ template <int N>
 __device__ __forceinline__ void named_arrive(int id) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "n"(N) : "memory"); }
 template <int N>
 __device__ __forceinline__ void named_sync(int id) { asm volatile("bar.sync %0, %1;" ::"r"(id), "n"(N) : "memory"); }
-__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
-__device__ __forceinline__ void cluster_arrive_release() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+
+// The exchange of a cluster's parts: each CTA's joining warp writes its part into every CTA's
+// shared memory with st.async, which also counts the bytes on that CTA's mbarrier, and waits for
+// its own to have all of them.  (A cluster barrier instead held every warp of the cluster to the
+// slowest: 3.4 us a row and SM where the bytes take 3.0.)  The wait is bounded: about 2 s, or
+// until another kernel of the program gave up; then status word 0 has a code and the rows' results
+// are wrong.  Nobody writes to a CTA that has left: it leaves after it received the last row's
+// parts of all the others.
+constexpr int kTimeout = 0x500;
+constexpr long long kWaitBudget = 4000000000LL;  // SM cycles
+__device__ __forceinline__ void exchange_expect(uint32_t bar, int bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void exchange_send(uint32_t dst, uint32_t bar, int cta, Part part) {
+    const uint64_t v = static_cast<uint64_t>(__float_as_uint(part.s)) << 32 | __float_as_uint(part.m);
+    asm volatile(
+        "{\n\t.reg .b32 d, b;\n\t"
+        "mapa.shared::cluster.u32 d, %0, %2;\n\t"
+        "mapa.shared::cluster.u32 b, %1, %2;\n\t"
+        "st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [d], %3, [b];\n\t}"
+        ::"r"(dst), "r"(bar), "r"(cta), "l"(v) : "memory");
+}
+__device__ __forceinline__ bool exchange_wait(uint32_t bar, uint32_t parity, int* status) {
+    const long long t0 = clock64();
+    for (uint32_t polls = 1;; ++polls) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+        if (done) return true;
+        if ((polls & 255) == 0 && *reinterpret_cast<volatile int*>(status) != 0) return false;
+        if (clock64() - t0 > kWaitBudget) {
+            atomicCAS(status, 0, kTimeout);
+            return false;
+        }
+    }
+}
 
 template <int G, int NV>
-__global__ void __launch_bounds__(G + 32, G * NV > 2048 ? 1 : 2) token_grad_kernel(TokenArgs a, int clusters) {
+__global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(TokenArgs a, int clusters) {
     constexpr int N = G + 32, FULL = 1, SCALARS = 3;  // barrier ids (+ parity)
     extern __shared__ __align__(16) float ring[];     // [stage][vector][thread][4]
     __shared__ Part warp_parts[2][G / 32], cta_parts[2][kMaxCluster];
     __shared__ float3 scalars[2];  // m, -c/s, c
     __shared__ RowInfo infos[kInfos];
+    __shared__ __align__(8) uint64_t bars[2];  // the exchange's mbarriers, by parity of the computed rows
     cg::cluster_group cl = cg::this_cluster();
     const int size = static_cast<int>(cl.num_blocks()), rank = static_cast<int>(cl.block_rank());
     const int tid = threadIdx.x, l = tid & 31, warp = tid >> 5;
@@ -452,8 +499,15 @@ __global__ void __launch_bounds__(G + 32, G * NV > 2048 ? 1 : 2) token_grad_kern
         float ahead[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) ahead[q] = look(q);
+        if (l == 0 && size > 1) {
+            for (uint64_t& b : bars)
+                asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(&b))) : "memory");
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
         __syncthreads();
-        if (size > 1) cl.sync();  // every CTA runs before another writes to it
+        if (size > 1) cl.sync();  // every CTA runs, with its mbarriers, before another writes to it
+        unsigned rows_done = 0;   // computed rows so far
+        bool failed = false;
         for (int n = 0; n < count; ++n) {
             const int p = n & 1;
             const RowInfo r = infos[n % kInfos];
@@ -469,10 +523,14 @@ __global__ void __launch_bounds__(G + 32, G * NV > 2048 ? 1 : 2) token_grad_kern
             if (computed(r)) {  // (the same for the whole cluster)
                 all = join_parts(warp_parts[p], G / 32, l);
                 if (size > 1) {
-                    if (l < size) *cl.map_shared_rank(&cta_parts[p][rank], l) = all;
-                    cluster_arrive_release();
-                    cluster_wait();
-                    all = join_parts(cta_parts[p], size, l);
+                    const int x = rows_done & 1;
+                    const uint32_t bar = static_cast<uint32_t>(__cvta_generic_to_shared(&bars[x]));
+                    if (l == 0) exchange_expect(bar, size * static_cast<int>(sizeof(Part)));
+                    if (l < size) exchange_send(static_cast<uint32_t>(__cvta_generic_to_shared(&cta_parts[x][rank])), bar, l, all);
+                    if (!failed) failed = !exchange_wait(bar, rows_done >> 1 & 1, a.status);
+                    failed = __any_sync(0xffffffffu, failed);
+                    all = join_parts(cta_parts[x], size, l);
+                    ++rows_done;
                 }
                 k.xk = __shfl_sync(0xffffffffu, mine, 0);
                 k.old = __shfl_sync(0xffffffffu, mine, 1);
@@ -487,6 +545,8 @@ __global__ void __launch_bounds__(G + 32, G * NV > 2048 ? 1 : 2) token_grad_kern
             named_arrive<N>(SCALARS + p);
             if (l == 0 && rank == 0 && computed(r)) write_value(a, r.row, k, all, logp);  // nobody waits for it
         }
+        __syncwarp();
+        if (size > 1) cl.sync();
         return;
     }
 
@@ -560,7 +620,6 @@ __global__ void __launch_bounds__(G + 32, G * NV > 2048 ? 1 : 2) token_grad_kern
     if (size > 1) cl.sync();
     asm volatile("cp.async.wait_group 2;" ::: "memory");
     float own = part(0);
-    if (size > 1 && computed(infos[0])) cluster_arrive_relaxed();
     for (int n = 0; n < count; ++n) {
         float next = 0.0f;
         if (n + 1 < count) {
@@ -570,10 +629,6 @@ __global__ void __launch_bounds__(G + 32, G * NV > 2048 ? 1 : 2) token_grad_kern
         named_sync<N>(SCALARS + (n & 1));
         const RowInfo r = infos[n % kInfos];
         const bool real = computed(r);
-        if (size > 1) {
-            if (real) cluster_wait();
-            if (n + 1 < count && computed(infos[(n + 1) % kInfos])) cluster_arrive_relaxed();
-        }
         if (real) {
             const float3 f = scalars[n & 1];
             const float scale = f.y * part_weight(own, f.x);  // (a NaN row: the sum is NaN; one of -inf: 0)
@@ -602,6 +657,8 @@ __global__ void __launch_bounds__(G + 32, G * NV > 2048 ? 1 : 2) token_grad_kern
         fetch(n + 3);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+    if (size > 1) cl.sync();  // nobody writes to a CTA that has left
 }
 
 // ---- preference loss: one CTA per pair: z = beta*(S(0) - S(1)), the loss and its slope.
@@ -710,7 +767,9 @@ cudaError_t launch_grad(const TokenArgs& a, int cluster, cudaStream_t stream) {
 template <bool GRAD>
 cudaError_t launch_row_kernel(const TokenArgs& a, cudaStream_t stream) {
     const int vectors = (a.V + 6) / 4;  // at most, wherever a row starts
-    if (vectors <= 32 * 8) {
+    // Values alone: a warp a row while the rows are enough to fill the card with warps (V = 4000:
+    // 2.5 TB/s with a CTA a row), a CTA or a cluster a row otherwise.
+    if (vectors <= 32 * (GRAD ? 16 : 8) || (!GRAD && vectors <= kWalk && a.rows >= 148 * 16)) {
         const int nv = (vectors + 31) / 32;
         const int64_t blocks = (a.rows + 7) / 8;
         if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
@@ -718,7 +777,8 @@ cudaError_t launch_row_kernel(const TokenArgs& a, cudaStream_t stream) {
         if (nv <= 1) token_warp_kernel<1, GRAD><<<grid, 256, 0, stream>>>(a);
         else if (nv <= 2) token_warp_kernel<2, GRAD><<<grid, 256, 0, stream>>>(a);
         else if (nv <= 4) token_warp_kernel<4, GRAD><<<grid, 256, 0, stream>>>(a);
-        else token_warp_kernel<8, GRAD><<<grid, 256, 0, stream>>>(a);
+        else if (nv <= 8 || !GRAD) token_warp_kernel<8, GRAD><<<grid, 256, 0, stream>>>(a);
+        else token_warp_kernel<GRAD ? 16 : 8, GRAD><<<grid, 256, 0, stream>>>(a);
         return cudaGetLastError();
     }
     // as many CTAs a row as hold it, and more while the rows do not fill the card
@@ -730,8 +790,6 @@ cudaError_t launch_row_kernel(const TokenArgs& a, cudaStream_t stream) {
         if (held) {
             const int nv = (vectors + cluster * G - 1) / (cluster * G);
             if (G == 512) return launch_grad<512, 8>(a, cluster, stream);
-            if (getenv("TG") && vectors > 2048) return launch_grad<512, 8>(a, (vectors + 4095) / 4096, stream);
-            if (nv <= 1) return launch_grad<256, 1>(a, cluster, stream);
             if (nv <= 2) return launch_grad<256, 2>(a, cluster, stream);
             if (nv <= 4) return launch_grad<256, 4>(a, cluster, stream);
             return launch_grad<256, 8>(a, cluster, stream);

@@ -135,7 +135,8 @@ struct TokenDesc {
 };
 int64_t token_scratch_bytes(const TokenDesc& d);
 int token_launch_count(const TokenDesc& d);
-// y (values, row-major) and dlogits ([n0][n1][V]) may be null; *status takes TT_STATUS_BAD_TOKEN
+// y (values, row-major) and dlogits ([n0][n1][V]) may be null.  status: the program's status words,
+// [0] takes a bounded wait's code, [1] TT_STATUS_BAD_TOKEN
 int launch_token(const TokenDesc& d, const void* const* in, float* y, float* dlogits, void* scratch, int* status,
                  void* stream);
 
