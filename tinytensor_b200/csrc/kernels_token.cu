@@ -78,7 +78,7 @@ __device__ __forceinline__ float exp2_part(float d) {
 __device__ __forceinline__ float exp_part(float d) { return exp2_part(d * 1.44269504f); }
 
 // exp(a - b) for the maxima of a part and a whole: 0 for a part of -inf alone, whose sum is 0 too
-__device__ __forceinline__ float part_weight(float m, float whole) { return m == -INFINITY ? 0.0f : expf(m - whole); }
+__device__ __forceinline__ float part_weight(float m, float whole) { return m == -INFINITY ? 0.0f : exp_part(m - whole); }
 
 // What a row's scalars are formed from: the token's logit and the row's operands.
 struct RowNumbers {
@@ -93,12 +93,23 @@ struct Row {
     float* dx;
     int token, shift;
     bool dx_vec;  // the gradient lies alike
-    __device__ Row(const TokenArgs& a, int64_t r) : row(r), i0(r / a.n1), i1(r % a.n1) {
+    static __device__ void split(const TokenArgs& a, int64_t r, int64_t& i0, int64_t& i1) {
         if (a.rows <= 0x7fffffff) {
             i0 = static_cast<unsigned>(r) / static_cast<unsigned>(a.n1);
             i1 = static_cast<unsigned>(r) % static_cast<unsigned>(a.n1);
+        } else {
+            i0 = r / a.n1;
+            i1 = r % a.n1;
         }
-        token = __ldg(a.tokens + i0 * a.ts0 + i1 * a.ts1);
+    }
+    static __device__ int token_of(const TokenArgs& a, int64_t r) {
+        int64_t i0, i1;
+        split(a, r, i0, i1);
+        return __ldg(a.tokens + i0 * a.ts0 + i1 * a.ts1);
+    }
+    __device__ Row(const TokenArgs& a, int64_t r) : Row(a, r, token_of(a, r)) {}
+    __device__ Row(const TokenArgs& a, int64_t r, int t) : row(r), token(t) {
+        split(a, r, i0, i1);
         x = a.logits + i0 * a.ls0 + i1 * a.ls1;
         dx = a.dlogits ? a.dlogits + r * a.V : nullptr;
         shift = static_cast<int>(reinterpret_cast<uintptr_t>(x) / 4 % 4);
@@ -487,10 +498,12 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
     auto computed = [&](const RowInfo& r) { return r.token >= 0 && r.token < a.V; };
 
     if (warp == G / 32) {  // ---- the joining warp
-        // lane q keeps operand q of the rows ahead: the token's logit, old, advantage, ref, g
-        auto look = [&](int n) {
+        // lane q keeps operand q of the rows ahead: the token's logit, old, advantage, ref, g.  Tokens are
+        // loaded a row earlier still: waiting for them here made this warp the slowest part.
+        auto token = [&](int n) { return n < count ? Row::token_of(a, first + static_cast<int64_t>(n) * clusters) : -1; };
+        auto look = [&](int n, int tok) {
             if (n >= count) return 0.0f;
-            const Row r(a, first + static_cast<int64_t>(n) * clusters);
+            const Row r(a, first + static_cast<int64_t>(n) * clusters, tok);
             if (l == 0) infos[n % kInfos] = RowInfo{r.x, r.dx, r.row, r.token, r.shift, r.dx_vec};
             const RowOperand o = l == 1 ? a.old : l == 2 ? a.adv : l == 3 ? a.ref : l == 4 ? a.g : RowOperand{nullptr, 0, 0};
             if (r.token < 0 || r.token >= a.V) return 0.0f;
@@ -498,7 +511,8 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
         };
         float ahead[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) ahead[q] = look(q);
+        for (int q = 0; q < 4; ++q) ahead[q] = look(q, token(q));
+        int tok = token(4);
         if (l == 0 && size > 1) {
             for (uint64_t& b : bars)
                 asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(&b))) : "memory");
@@ -515,7 +529,8 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
             ahead[0] = ahead[1];
             ahead[1] = ahead[2];
             ahead[2] = ahead[3];
-            ahead[3] = look(n + 4);
+            ahead[3] = look(n + 4, tok);
+            tok = token(n + 5);
             named_sync<N>(FULL + p);
             Part all;
             RowNumbers k;
@@ -537,13 +552,14 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
                 k.adv = __shfl_sync(0xffffffffu, mine, 2);
                 k.ref = __shfl_sync(0xffffffffu, mine, 3);
                 k.g = __shfl_sync(0xffffffffu, mine, 4);
-                logp = token_logp(k.xk, all);
+                if (a.kind == TK_POLICY) logp = token_logp(k.xk, all);
                 const float c = row_slope(a, k, logp);
                 if (l == 0) scalars[p] = make_float3(all.m, -c / all.s, c);
             }
             __syncwarp();
             named_arrive<N>(SCALARS + p);
-            if (l == 0 && rank == 0 && computed(r)) write_value(a, r.row, k, all, logp);  // nobody waits for it
+            if (l == 0 && rank == 0 && computed(r))  // nobody waits for it
+                write_value(a, r.row, k, all, a.kind == TK_POLICY ? logp : token_logp(k.xk, all));
         }
         __syncwarp();
         if (size > 1) cl.sync();
@@ -555,6 +571,17 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
     const int lo = v0 - 4 * l, hi = v0 + 4 * (31 - l) + 4 * (NV - 1) * G;  // the warp's first and last vector
     const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + tid * 16;
     auto inside = [&](const RowInfo& r) { return lo >= r.shift && hi - r.shift <= a.V - 4; };
+    // A row has two vectors at most that it does not fill, its first and its last: calls f(q, u) for
+    // the values of those that are this thread's.
+    auto ends = [&](const RowInfo& r, int j0, auto f) {
+        if (j0 < 0) {
+            for (int u = -j0; u < 4; ++u) f(0, u);
+        }
+        const int left = (a.V + r.shift) & 3, k = a.V - left - j0;  // the last vector's values, its place
+        if (left != 0 && k >= 0 && k / 4 % G == 0 && k / 4 / G < NV) {
+            for (int u = 0; u < left; ++u) f(k / 4 / G, u);
+        }
+    };
     auto fetch = [&](int n) {
         const RowInfo r = infos[n % kInfos];
         if (n < count && computed(r)) {
@@ -566,16 +593,13 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
                 for (int q = 0; q < NV; ++q)
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + q * G * 16), "l"(x + 4 * q * G) : "memory");
             } else {
-                for (int q = 0; q < NV; ++q) {
-                    const int j = j0 + 4 * q * G;
-                    if (j >= 0 && j <= a.V - 4) {
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + q * G * 16), "l"(r.x + j) : "memory");
-                    } else {
-                        for (int u = 0; u < 4; ++u)
-                            if (j + u >= 0 && j + u < a.V)
-                                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + q * G * 16 + 4 * u), "l"(r.x + j + u) : "memory");
-                    }
-                }
+#pragma unroll
+                for (int q = 0; q < NV; ++q)
+                    if (j0 + 4 * q * G >= 0 && j0 + 4 * q * G <= a.V - 4)
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + q * G * 16), "l"(x + 4 * q * G) : "memory");
+                ends(r, j0, [&](int q, int u) {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to + q * G * 16 + 4 * u), "l"(x + 4 * q * G + u) : "memory");
+                });
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -601,7 +625,7 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
                 for (int q = 0; q < NV; ++q)
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
-                        if (j0 + 4 * q * G + u < 0 || j0 + 4 * q * G + u >= a.V) v[q][u] = -INFINITY;
+                        if (static_cast<unsigned>(j0 + 4 * q * G + u) >= static_cast<unsigned>(a.V)) v[q][u] = -INFINITY;
             }
             const Part own = warp_part<NV>(v);
 #pragma unroll
@@ -635,7 +659,7 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
             const int j0 = v0 - r.shift;
             const int k = r.token - j0;  // the token's place among this thread's vectors
             const bool here = k >= 0 && k < 4 * NV * G && k / 4 % G == 0;
-            const bool plain = inside(r) && r.dx_vec;
+            const bool in = inside(r);
             float* dx = r.dx + j0;
 #pragma unroll
             for (int q = 0; q < NV; ++q) {
@@ -643,13 +667,17 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
                 const float2 ex = halves(pair(e.x, e.y) * pair(scale, scale)), ez = halves(pair(e.z, e.w) * pair(scale, scale));
                 e = make_float4(ex.x, ex.y, ez.x, ez.y);
                 if (here && k / 4 == q * G) (k % 4 == 0 ? e.x : k % 4 == 1 ? e.y : k % 4 == 2 ? e.z : e.w) += f.z;
-                if (plain) {
+                const int j = j0 + 4 * q * G;
+                if (!r.dx_vec) {  // the logits are a view that lies differently: value by value
+                    const float v[4] = {e.x, e.y, e.z, e.w};
+                    store_vec(r.dx, j, a.V, false, v);
+                } else if (in || (j >= 0 && j <= a.V - 4)) {
                     __stcs(reinterpret_cast<float4*>(dx + 4 * q * G), e);
                 } else {
-                    const float v[4] = {e.x, e.y, e.z, e.w};
-                    store_vec(r.dx, j0 + 4 * q * G, a.V, r.dx_vec, v);
+                    *slot(n, q) = e;
                 }
             }
+            if (!in && r.dx_vec) ends(r, j0, [&](int q, int u) { dx[4 * q * G + u] = reinterpret_cast<const float*>(slot(n, q))[u]; });
         } else {
             fill_row(a, r.row, r.token, r.dx, tid == 0 && rank == 0, rank * G + tid, size * G);
         }
@@ -766,7 +794,9 @@ cudaError_t launch_grad(const TokenArgs& a, int cluster, cudaStream_t stream) {
 
 template <bool GRAD>
 cudaError_t launch_row_kernel(const TokenArgs& a, cudaStream_t stream) {
-    const int vectors = (a.V + 6) / 4;  // at most, wherever a row starts
+    // vectors of a row at most: all rows start on 16 bytes, or one starts up to 3 values behind it
+    const bool aligned = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.ls0 % 4 == 0 && a.ls1 % 4 == 0;
+    const int vectors = aligned ? (a.V + 3) / 4 : (a.V + 6) / 4;
     // Values alone: a warp a row while the rows are enough to fill the card with warps (V = 4000:
     // 2.5 TB/s with a CTA a row), a CTA or a cluster a row otherwise.
     if (vectors <= 32 * (GRAD ? 16 : 8) || (!GRAD && vectors <= kWalk && a.rows >= 148 * 16)) {
@@ -788,11 +818,18 @@ cudaError_t launch_row_kernel(const TokenArgs& a, cudaStream_t stream) {
     while (cluster < kMaxCluster && a.rows * cluster < 296 && cluster * G < vectors) ++cluster;
     if constexpr (GRAD) {
         if (held) {
-            const int nv = (vectors + cluster * G - 1) / (cluster * G);
+            // no more vectors a thread than it takes: rows of 33000 are 7 a thread of 5 CTAs (8 left the
+            // fifth nearly empty and its ring as large as the others')
             if (G == 512) return launch_grad<512, 8>(a, cluster, stream);
-            if (nv <= 2) return launch_grad<256, 2>(a, cluster, stream);
-            if (nv <= 4) return launch_grad<256, 4>(a, cluster, stream);
-            return launch_grad<256, 8>(a, cluster, stream);
+            switch ((vectors + cluster * G - 1) / (cluster * G)) {
+                case 1: case 2: return launch_grad<256, 2>(a, cluster, stream);
+                case 3: return launch_grad<256, 3>(a, cluster, stream);
+                case 4: return launch_grad<256, 4>(a, cluster, stream);
+                case 5: return launch_grad<256, 5>(a, cluster, stream);
+                case 6: return launch_grad<256, 6>(a, cluster, stream);
+                case 7: return launch_grad<256, 7>(a, cluster, stream);
+                default: return launch_grad<256, 8>(a, cluster, stream);
+            }
         }
     }
     if (a.rows * cluster > 0x7fffffff) return cudaErrorInvalidConfiguration;
