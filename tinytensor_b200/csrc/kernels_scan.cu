@@ -11,8 +11,10 @@
 // what bounds these kernels (forward 12 bytes a value, backward 20 with all gradients).
 // Tiles come through a two-stage ring in shared memory filled by cp.async: a stage is refilled
 // as soon as its values are in registers, so the loads of the next tiles are in flight while
-// the tiles of this step wait for one another's maps.  Tiles are joined in time order, so
-// results do not depend on how CTAs are scheduled, at three levels:
+// the tiles of this step wait for one another's maps.  CTAs stay and walk the blocks of lanes,
+// the ring running on from one block to the next (a CTA per block spent most of a short scan
+// on starting and draining).  Tiles are joined in time order, so results do not depend on how
+// CTAs are scheduled, at three levels:
 //   warps of a CTA        through shared memory, one block barrier a step;
 //   CTAs of a cluster     through distributed shared memory, one cluster barrier a step,
 //                         where there are too few lanes to fill the card;
@@ -47,6 +49,8 @@ struct ScanArgs {
     int64_t lanes, inner, n2, T;
     int64_t seg_len;  // steps of a segment
     int segments;
+    int64_t units;    // blocks of lanes * segments, walked by the clusters of the grid
+    int steps;        // of a unit
     int W;            // warps of a CTA along time; the others take further lanes
     int vec;          // bit k: operand k moves as vectors
 };
@@ -108,29 +112,55 @@ struct Exchange {
     float state[2][LW];    // the last warp's state behind a step, for the next one
 };
 
-// Where a CTA works: its block of lanes, segment of the axis and place in its cluster.
+// A CTA's place: its rank in its cluster, the cluster's first unit and how many clusters walk them.
 struct Place {
-    int64_t block;
-    int seg, rank, size;
+    int rank, size;
+    int64_t first, clusters;
 };
-__device__ __forceinline__ Place place(const ScanArgs& a) {
+__device__ __forceinline__ Place place() {
     Place p;
     cg::cluster_group cl = cg::this_cluster();
     p.size = static_cast<int>(cl.num_blocks());
     p.rank = static_cast<int>(cl.block_rank());
-    const unsigned unit = blockIdx.x / p.size;
-    p.seg = static_cast<int>(unit % a.segments);
-    p.block = unit / a.segments;
+    p.first = blockIdx.x / p.size;
+    p.clusters = gridDim.x / p.size;
     return p;
 }
 
-// The state before a segment.
-template <int PASS>
-__device__ __forceinline__ float segment_state(const ScanArgs& a, int seg, int64_t lane, const float* carry) {
-    float c = 0.0f;
-    if (PASS != MAPS && carry) c = __ldg(carry);
-    if constexpr (PASS == JOINED)
-        for (int s = 0; s < seg; ++s) c = apply(a.maps[s * a.lanes + lane], c);
+// Lane -> (outer, inner) index.
+__device__ __forceinline__ void split_lane(const ScanArgs& a, int64_t lane, int64_t& o, int64_t& i) {
+    if (a.lanes <= 0x7fffffff) {
+        const unsigned q = static_cast<unsigned>(lane), n = static_cast<unsigned>(a.inner);
+        o = q / n;
+        i = q % n;
+    } else {
+        o = lane / a.inner;
+        i = lane % a.inner;
+    }
+}
+
+// The state before segment `seg` of a lane, from the maps of the segments before it and the lane's
+// first state.  The warps of the CTA (all on the same lanes) join a share of the maps each,
+// loading 8 at a time; LW lanes a warp, `writer` one thread of a lane.
+template <int LW>
+__device__ __forceinline__ float segment_state(const ScanArgs& a, Exchange<LW>& ex, int seg, int64_t lane, bool live,
+                                               float c, int warp, int l, bool writer) {
+    const int share = (seg + NW - 1) / NW, begin = min(seg, warp * share), end = min(seg, begin + share);
+    float2 m = make_float2(1.0f, 0.0f);
+    for (int s0 = begin; s0 < end; s0 += 8) {
+        float2 q[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            q[u] = live && s0 + u < end ? __ldcg(a.maps + (s0 + u) * a.lanes + lane) : make_float2(1.0f, 0.0f);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) m = join(m, q[u]);
+    }
+    __syncthreads();  // (the unit before may still be reading)
+    if (writer) ex.warp[0][warp][l] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) c = apply(ex.warp[0][w][l], c);
+    __syncthreads();
     return c;
 }
 
@@ -221,63 +251,71 @@ __device__ __forceinline__ void store_vec(float* p, const float* v, bool stream)
     }
 }
 
-// ---- lanes side by side in memory ([.., T, lanes]): a warp's tile is 16 steps of 32 adjacent
-// lanes.  A thread takes V adjacent lanes and 16/V adjacent steps (32/V threads lie across the
-// lanes, V behind one another in time), so that operands move in 4*V bytes a thread and 128
-// bytes a row whatever V is; the V threads of a lane join their maps by shuffles.  Operands
-// whose lanes are adjacent move as V-vectors, operands broadcast over the lanes behind n1 as one
-// value (V > 1 is only cut where each operand is one or the other); V = 1 takes any strides.
-// A thread reads back only what it copied itself, so the ring needs no barrier.
-constexpr int kTileSteps = 16;
-
+// ---- lanes side by side in memory ([.., T, lanes]): a warp's tile is TILE steps of 32 adjacent
+// lanes, 16 or, forward, 24.  A thread takes V adjacent lanes and a V-th of the
+// steps (32/V threads lie across the lanes, V behind one another in time), so that operands move
+// in 4*V bytes a thread and 128 bytes a row whatever V is; the V threads of a lane join their
+// maps by shuffles.  Operands whose lanes are adjacent move as V-vectors, operands broadcast over
+// the lanes behind n1 as one value (V > 1 is only cut where each operand is one or the other);
+// V = 1 takes any strides.  A thread reads back only what it copied itself, so the ring needs
+// no barrier.
 template <bool BACKWARD>
 constexpr int kArrays = BACKWARD ? 3 : 2;
 
-template <bool BACKWARD>
-constexpr size_t cols_smem() {
-    return sizeof(Exchange<32>) + 2 * kArrays<BACKWARD> * NW * kTileSteps * 32 * sizeof(float);
-}
+template <bool BACKWARD, int TILE>
+struct ColTile {
+    float in[2][kArrays<BACKWARD>][NW][TILE * 32];  // [stage][operand][warp][step][thread][V]
+    float carry[2][NW][32];                         // [stage][warp][lane]: a unit's first states
+    Exchange<32> ex;
+};
 
-template <bool BACKWARD, int PASS, int V>
-__global__ void __launch_bounds__(NW * 32, BACKWARD ? 2 : 3) scan_cols_kernel(ScanArgs a) {
-    constexpr int TS = kTileSteps / V, COLS = 32 / V, NA = kArrays<BACKWARD>;
+template <bool BACKWARD, int PASS, int V, int TILE>
+__global__ void __launch_bounds__(NW * 32, 2) scan_cols_kernel(ScanArgs a) {
+    constexpr int TS = TILE / V, COLS = 32 / V, NA = kArrays<BACKWARD>;
     extern __shared__ __align__(16) unsigned char raw[];
-    float* ring = reinterpret_cast<float*>(raw);  // [stage][operand][warp][step][thread][V]
-    Exchange<32>& ex = *reinterpret_cast<Exchange<32>*>(raw + 2 * NA * NW * kTileSteps * 32 * sizeof(float));
-    const Place at = place(a);
+    ColTile<BACKWARD, TILE>& sh = *reinterpret_cast<ColTile<BACKWARD, TILE>*>(raw);
+    const Place at = place();
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, W = a.W;
     const int wt = warp % W, wr = warp / W;
     const int col = l % COLS, sub = l / COLS;
-    const int64_t lane0 = (at.block * (NW / W) + wr) * 32, lane = lane0 + col * V;
-    const bool live = lane < a.lanes;
-    int64_t o = 0, i = 0;
-    if (live) {
-        if (a.lanes <= 0x7fffffff) {
-            const unsigned q = static_cast<unsigned>(lane), n = static_cast<unsigned>(a.inner);
-            o = q / n;
-            i = q % n;
-        } else {
-            o = lane / a.inner;
-            i = lane % a.inner;
-        }
-    }
-    const int64_t i1 = a.n2 == a.inner ? 0 : i / a.n2, i2 = i - i1 * a.n2;
-    const float* p[SI_COUNT];
-#pragma unroll
-    for (int k = 0; k < SI_COUNT; ++k)
-        p[k] = a.in[k].p ? a.in[k].p + o * a.in[k].so + i1 * a.in[k].s1 + i2 * a.in[k].s2 : nullptr;
     const bool want_gate = BACKWARD && PASS != MAPS && a.out[SO_GATE];
-    const int64_t begin = at.seg * a.seg_len, end = min(a.T, begin + a.seg_len);
-    const int64_t stride = static_cast<int64_t>(at.size) * W * kTileSteps;  // of this warp's tiles
-    const int64_t own = begin + (static_cast<int64_t>(at.rank) * W + wt) * kTileSteps + sub * TS;
-    auto run_len = [&](int64_t r0) {
+    const int64_t stride = static_cast<int64_t>(at.size) * W * TILE;  // of this warp's tiles
+    const int64_t own = (static_cast<int64_t>(at.rank) * W + wt) * TILE + sub * TS;
+    auto first_lane = [&](int64_t unit) { return (unit / a.segments * (NW / W) + wr) * 32; };
+    // this thread's steps from r0 on
+    auto run_len = [&](bool live, int64_t r0, int64_t end) {
         return live ? static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(TS), end - r0))) : 0;
     };
-    auto slot = [&](int stage, int k) { return ring + (((stage * NA + k) * NW + warp) * kTileSteps * 32 + l * V); };
+    auto slot = [&](int stage, int k) { return &sh.in[stage][k][warp][l * V]; };
+
+    // ---- the ring: a place ahead of the computation
+    struct {
+        int64_t unit, r0, end;
+        int step;
+        bool live;
+        const float *gate, *x, *h, *init;
+    } ahead;
+    auto aim = [&](int64_t unit) {
+        ahead.unit = unit;
+        ahead.step = 0;
+        if (unit >= a.units) return;
+        const int64_t lane = first_lane(unit) + col * V, begin = unit % a.segments * a.seg_len;
+        ahead.live = lane < a.lanes;
+        ahead.r0 = begin + own;
+        ahead.end = min(a.T, begin + a.seg_len);
+        int64_t o = 0, i = 0;
+        if (ahead.live) split_lane(a, lane, o, i);
+        const int64_t i1 = a.n2 == a.inner ? 0 : i / a.n2, i2 = i - i1 * a.n2;
+        auto ptr = [&](int k) { return a.in[k].p ? a.in[k].p + o * a.in[k].so + i1 * a.in[k].s1 + i2 * a.in[k].s2 : nullptr; };
+        ahead.gate = ptr(SI_GATE);
+        ahead.x = ptr(SI_X);
+        ahead.h = ptr(SI_H);
+        ahead.init = ptr(SI_INIT);
+    };
     // copies of one operand: n steps in scan order from time t on
-    auto fetch = [&](int k, int stage, int arr, int64_t t, int n) {
+    auto fetch = [&](const float* p, int k, int stage, int arr, int64_t t, int n) {
         const int64_t step = BACKWARD ? -a.in[k].st : a.in[k].st;
-        const float* q = p[k] + t * a.in[k].st;
+        const float* q = p + t * a.in[k].st;
         const uint32_t dst = smem_addr(slot(stage, arr));
         if (V > 1 && (a.vec >> k & 1)) {
 #pragma unroll
@@ -289,149 +327,171 @@ __global__ void __launch_bounds__(NW * 32, BACKWARD ? 2 : 3) scan_cols_kernel(Sc
                 if (j < n) copy_async<4>(dst + j * 128 * V, q);
         }
     };
-    auto issue = [&](int64_t r0, int stage) {
-        const int n = run_len(r0);
-        const int64_t t = BACKWARD ? a.T - 1 - r0 : r0;
-        if (n > 0) {
-            fetch(SI_GATE, stage, 0, t, n);
-            if (p[SI_X]) fetch(SI_X, stage, 1, t, n);
-            // the states before each step; before t = 0 there is init
-            if (want_gate) fetch(SI_H, stage, NA - 1, t - 1, static_cast<int>(min(static_cast<int64_t>(n), t)));
+    auto issue = [&](int stage) {
+        if (ahead.unit < a.units) {
+            const int n = run_len(ahead.live, ahead.r0, ahead.end);
+            const int64_t t = BACKWARD ? a.T - 1 - ahead.r0 : ahead.r0;
+            if (n > 0) {
+                fetch(ahead.gate, SI_GATE, stage, 0, t, n);
+                if (ahead.x) fetch(ahead.x, SI_X, stage, 1, t, n);
+                if (want_gate) {  // the states before each step; before t = 0 there is init
+                    fetch(ahead.h, SI_H, stage, NA - 1, t - 1, static_cast<int>(min(static_cast<int64_t>(n), t)));
+                    if (t < n && ahead.init) {
+                        const uint32_t dst = smem_addr(slot(stage, NA - 1)) + static_cast<int>(t) * 128 * V;
+#pragma unroll
+                        for (int v = 0; v < V; ++v) copy_async<4>(dst + 4 * v, ahead.init + v * a.in[SI_INIT].s2);
+                    }
+                }
+            }
+            if (PASS == ONLY && ahead.step == 0 && a.in[SI_CARRY].p) {  // the unit's first states, lane by lane
+                const int64_t lane = first_lane(ahead.unit) + l;
+                if (lane < a.lanes) {
+                    int64_t o, i;
+                    split_lane(a, lane, o, i);
+                    const int64_t i1 = a.n2 == a.inner ? 0 : i / a.n2, i2 = i - i1 * a.n2;
+                    copy_async<4>(smem_addr(&sh.carry[stage][warp][l]),
+                                  a.in[SI_CARRY].p + o * a.in[SI_CARRY].so + i1 * a.in[SI_CARRY].s1 + i2 * a.in[SI_CARRY].s2);
+                }
+            }
+            ahead.r0 += stride;
+            if (++ahead.step == a.steps) aim(ahead.unit + at.clusters);
         }
         copies_commit();
     };
-    issue(own, 0);
-    issue(own + stride, 1);
+    aim(at.first);
+    issue(0);
+    issue(1);
     if (at.size > 1) cg::this_cluster().sync();  // every CTA runs before another writes to it
 
-    // the exchange takes lane lane0 + l: its state before the segment
-    float c = 0.0f;
-    if (lane0 + l < a.lanes) {
-        const float* q = nullptr;
-        if (p[SI_CARRY]) {
-            const int64_t ol = (lane0 + l) / a.inner, il = (lane0 + l) % a.inner;
-            q = a.in[SI_CARRY].p + ol * a.in[SI_CARRY].so + il / a.n2 * a.in[SI_CARRY].s1 + il % a.n2 * a.in[SI_CARRY].s2;
-        }
-        c = segment_state<PASS>(a, at.seg, lane0 + l, q);
-    }
-    if (a.T == 0) {  // no steps: the last state is the first
-        copies_wait_all();
-        if (lane0 + l < a.lanes && wt == 0 && a.out[SO_LANE]) a.out[SO_LANE][lane0 + l] = c;
-        return;
-    }
-    Joiner<32> joiner{ex, at, W, wt, wr, warp, l};
-    float gates = 1.0f;
+    Joiner<32> joiner{sh.ex, at, W, wt, wr, warp, l};
     const bool splat_gate = V > 1 && !(a.vec >> SI_GATE & 1), splat_x = V > 1 && !(a.vec >> SI_X & 1);
     const bool splat_h = V > 1 && !(a.vec >> SI_H & 1);
     int stage = 0;
-    for (int64_t base = begin; base < end; base += stride, stage ^= 1) {
-        const int64_t r0 = own + (base - begin);
-        const int n = run_len(r0);
-        float ga[TS][V], xv[TS][V], hv[BACKWARD ? TS : 1][V];
-        copies_wait_one();
-        auto read = [&](const float* q, bool splat, int count, float none, float (*dst)[V]) {
-#pragma unroll
-            for (int j = 0; j < TS; ++j) {
-                if (splat) {
-                    const float f = q[j * 32 * V];
-#pragma unroll
-                    for (int v = 0; v < V; ++v) dst[j][v] = f;
-                } else {
-                    load_shared<V>(q + j * 32 * V, dst[j]);
-                }
+    for (int64_t unit = at.first; unit < a.units; unit += at.clusters) {
+        const int seg = static_cast<int>(unit % a.segments);
+        const int64_t lane0 = first_lane(unit), lane = lane0 + col * V;
+        const bool live = lane < a.lanes;
+        const int64_t begin = seg * a.seg_len, end = min(a.T, begin + a.seg_len);
+        int64_t o = 0, i = 0;
+        if (live) split_lane(a, lane, o, i);
+        float c = 0.0f, gates = 1.0f;
+        if constexpr (PASS == JOINED) {
+            const bool in = lane0 + l < a.lanes;
+            if (in && a.in[SI_CARRY].p) {
+                int64_t oc, ic;
+                split_lane(a, lane0 + l, oc, ic);
+                c = __ldg(a.in[SI_CARRY].p + oc * a.in[SI_CARRY].so + ic / a.n2 * a.in[SI_CARRY].s1 + ic % a.n2 * a.in[SI_CARRY].s2);
             }
-            if (count < TS) {
-#pragma unroll
-                for (int j = 0; j < TS; ++j)
-#pragma unroll
-                    for (int v = 0; v < V; ++v)
-                        if (j >= count) dst[j][v] = none;
-            }
-        };
-        read(slot(stage, 0), splat_gate, n, 1.0f, ga);
-        read(slot(stage, 1), splat_x, p[SI_X] ? n : 0, 0.0f, xv);
-        if constexpr (BACKWARD) {
-            const int64_t t0 = a.T - 1 - r0;
-            const int nh = want_gate ? static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(n), t0))) : 0;
-            read(slot(stage, NA - 1), splat_h, nh, 0.0f, hv);
-            if (want_gate && nh < n && p[SI_INIT]) {
-#pragma unroll
-                for (int j = 0; j < TS; ++j)
-                    if (j == nh)
-#pragma unroll
-                        for (int v = 0; v < V; ++v) hv[j][v] = __ldg(p[SI_INIT] + v * a.in[SI_INIT].s2);
-            }
+            c = segment_state<32>(a, sh.ex, seg, lane0 + l, in, c, warp, l, true);
         }
-        issue(r0 + 2 * stride, stage);
-        // this thread's maps, those of the threads before it in time, and the tile's
-        float2 m[V], before[V];
-        float2 tile = make_float2(1.0f, 0.0f);
+        int64_t r0 = begin + own;
+        for (int k = 0; k < a.steps; ++k, r0 += stride, stage ^= 1) {
+            const int n = run_len(live, r0, end);
+            float ga[TS][V], xv[TS][V], hv[BACKWARD ? TS : 1][V];
+            copies_wait_one();
+            auto read = [&](const float* q, bool splat, int count, float none, float (*dst)[V]) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            m[v] = tile_map<BACKWARD, TS>([&](int j) { return ga[j][v]; }, [&](int j) { return xv[j][v]; });
-            before[v] = make_float2(1.0f, 0.0f);
+                for (int j = 0; j < TS; ++j) {
+                    if (splat) {
+                        const float f = q[j * 32 * V];
 #pragma unroll
-            for (int d = COLS; d < 32; d *= 2) {
-                const float2 b = make_float2(__shfl_up_sync(0xffffffffu, m[v].x, d), __shfl_up_sync(0xffffffffu, m[v].y, d));
-                if (l >= d) m[v] = join(b, m[v]);
-            }
-            if (V > 1) {
-                const float2 b = make_float2(__shfl_up_sync(0xffffffffu, m[v].x, COLS), __shfl_up_sync(0xffffffffu, m[v].y, COLS));
-                if (sub > 0) before[v] = b;
-                // lane l's map lies with the last of its threads, 32 - COLS + l / V, at v = l % V
-                const float2 w = make_float2(__shfl_sync(0xffffffffu, m[v].x, 32 - COLS + l / V),
-                                             __shfl_sync(0xffffffffu, m[v].y, 32 - COLS + l / V));
-                if (l % V == v) tile = w;
-            } else {
-                tile = m[v];
-            }
-        }
-        const float first = joiner.first(tile, c, base == begin, true);
-        const bool last_step = base + stride >= end;
-        if constexpr (PASS == MAPS) {
-            joiner.gates_of_step(gates);
-            const float s = apply(tile, first);
-            if (last_step && lane0 + l < a.lanes && wt == W - 1) a.maps[at.seg * a.lanes + lane0 + l] = make_float2(gates, s);
-            joiner.hand_on(s, last_step, true);
-        } else {
-            float s[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                s[v] = V > 1 ? __shfl_sync(0xffffffffu, first, col * V + v) : first;
-                if (V > 1 && sub > 0) s[v] = apply(before[v], s[v]);
-            }
-            const int64_t step = BACKWARD ? -a.inner : a.inner;
-            const int64_t y = (o * a.T + (BACKWARD ? a.T - 1 - r0 : r0)) * a.inner + i;
-            float* ym = a.out[SO_MAIN] + y;
-            float* yg = a.out[SO_GATE] + y;
-            const int nm = a.out[SO_MAIN] ? n : 0, ng = want_gate ? n : 0;
-#pragma unroll
-            for (int j = 0; j < TS; ++j, ym += step, yg += step) {  // (past the end: gate 1, x 0, the state stays)
-                float main[V], dg[V];
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    if (BACKWARD) {
-                        main[v] = xv[j][v] + s[v];
-                        dg[v] = main[v] * hv[BACKWARD ? j : 0][v];
-                        s[v] = ga[j][v] * main[v];
+                        for (int v = 0; v < V; ++v) dst[j][v] = f;
                     } else {
-                        main[v] = s[v] = fmaf(ga[j][v], s[v], xv[j][v]);
+                        load_shared<V>(q + j * 32 * V, dst[j]);
                     }
                 }
-                if (j < nm) store_vec<V>(ym, main, BACKWARD);
-                if (j < ng) store_vec<V>(yg, dg, true);
-            }
-            // the thread of the last step has the last state as it was stored
-            if (n > 0 && r0 + n == a.T && a.out[SO_LANE]) store_vec<V>(a.out[SO_LANE] + lane, s, false);
-            float behind = s[0];  // the state behind the tile, of lane l
-            if (V > 1) {
+                if (count < TS) {
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    const float w = __shfl_sync(0xffffffffu, s[v], 32 - COLS + l / V);
-                    if (l % V == v) behind = w;
+                    for (int j = 0; j < TS; ++j)
+#pragma unroll
+                        for (int v = 0; v < V; ++v)
+                            if (j >= count) dst[j][v] = none;
+                }
+            };
+            read(slot(stage, 0), splat_gate, n, 1.0f, ga);
+            read(slot(stage, 1), splat_x, a.in[SI_X].p ? n : 0, 0.0f, xv);
+            if constexpr (BACKWARD) {
+                const int64_t t0 = a.T - 1 - r0;
+                const int nh = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(n), t0)));
+                read(slot(stage, NA - 1), splat_h, want_gate ? (a.in[SI_INIT].p ? n : nh) : 0, 0.0f, hv);
+                if (splat_h && want_gate && a.in[SI_INIT].p && nh < n) {  // init need not be broadcast where h is
+#pragma unroll
+                    for (int j = 0; j < TS; ++j)
+                        if (j == nh) load_shared<V>(slot(stage, NA - 1) + j * 32 * V, hv[j]);
                 }
             }
-            joiner.hand_on(behind, last_step, true);
+            if (PASS == ONLY && k == 0) c = a.in[SI_CARRY].p && lane0 + l < a.lanes ? sh.carry[stage][warp][l] : 0.0f;
+            issue(stage);
+            // this thread's maps, those of the threads before it in time, and the tile's
+            float2 m[V], before[V];
+            float2 tile = make_float2(1.0f, 0.0f);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                m[v] = tile_map<BACKWARD, TS>([&](int j) { return ga[j][v]; }, [&](int j) { return xv[j][v]; });
+                before[v] = make_float2(1.0f, 0.0f);
+#pragma unroll
+                for (int d = COLS; d < 32; d *= 2) {
+                    const float2 b = make_float2(__shfl_up_sync(0xffffffffu, m[v].x, d), __shfl_up_sync(0xffffffffu, m[v].y, d));
+                    if (l >= d) m[v] = join(b, m[v]);
+                }
+                if (V > 1) {
+                    const float2 b = make_float2(__shfl_up_sync(0xffffffffu, m[v].x, COLS), __shfl_up_sync(0xffffffffu, m[v].y, COLS));
+                    if (sub > 0) before[v] = b;
+                    // lane l's map lies with the last of its threads, 32 - COLS + l / V, at v = l % V
+                    const float2 w = make_float2(__shfl_sync(0xffffffffu, m[v].x, 32 - COLS + l / V),
+                                                 __shfl_sync(0xffffffffu, m[v].y, 32 - COLS + l / V));
+                    if (l % V == v) tile = w;
+                } else {
+                    tile = m[v];
+                }
+            }
+            const bool last = k + 1 == a.steps;
+            const float first = joiner.first(tile, c, k == 0, true);
+            if constexpr (PASS == MAPS) {
+                joiner.gates_of_step(gates);
+                const float s = apply(tile, first);
+                if (last && lane0 + l < a.lanes && wt == W - 1) a.maps[seg * a.lanes + lane0 + l] = make_float2(gates, s);
+                joiner.hand_on(s, last, true);
+            } else {
+                float s[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    s[v] = V > 1 ? __shfl_sync(0xffffffffu, first, col * V + v) : first;
+                    if (V > 1 && sub > 0) s[v] = apply(before[v], s[v]);
+                }
+                const int64_t step = BACKWARD ? -a.inner : a.inner;
+                const int64_t y = (o * a.T + (BACKWARD ? a.T - 1 - r0 : r0)) * a.inner + i;
+                float* ym = a.out[SO_MAIN] + y;
+                float* yg = a.out[SO_GATE] + y;
+                const int nm = a.out[SO_MAIN] ? n : 0, ng = want_gate ? n : 0;
+#pragma unroll
+                for (int j = 0; j < TS; ++j, ym += step, yg += step) {  // (past the end: gate 1, x 0, the state stays)
+                    float main[V], dg[V];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        if (BACKWARD) {
+                            main[v] = xv[j][v] + s[v];
+                            dg[v] = main[v] * hv[BACKWARD ? j : 0][v];
+                            s[v] = ga[j][v] * main[v];
+                        } else {
+                            main[v] = s[v] = fmaf(ga[j][v], s[v], xv[j][v]);
+                        }
+                    }
+                    if (j < nm) store_vec<V>(ym, main, BACKWARD);
+                    if (j < ng) store_vec<V>(yg, dg, true);
+                }
+                // the thread of the last step has the last state as it was stored
+                if (n > 0 && r0 + n == a.T && a.out[SO_LANE]) store_vec<V>(a.out[SO_LANE] + lane, s, false);
+                float behind = s[0];  // the state behind the tile, of lane l
+                if (V > 1) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        const float w = __shfl_sync(0xffffffffu, s[v], 32 - COLS + l / V);
+                        if (l % V == v) behind = w;
+                    }
+                }
+                joiner.hand_on(behind, last, true);
+            }
         }
     }
     copies_wait_all();
@@ -439,156 +499,200 @@ __global__ void __launch_bounds__(NW * 32, BACKWARD ? 2 : 3) scan_cols_kernel(Sc
 
 // ---- time adjacent in memory ([.., T]): a warp's tile is 384 steps of one row, a run of 12
 // adjacent steps per thread (an odd number of 16-byte vectors, so that the threads' runs lie
-// in different banks), the runs' maps joined by shuffles.  Tiles move between global and
-// shared memory in coalesced vectors, in and out.  Rows need not start on 16 bytes: vectors are
-// cut at the row's own 16-byte boundaries (`shift` steps before its first one), so whole
-// vectors move as 16 bytes and only ragged ends value by value.
+// in different banks), the runs' maps joined by shuffles.  Rows of up to SUB*12 - 3 steps take
+// SUB threads, 32/SUB rows a warp.  Tiles move between global and shared memory in coalesced
+// vectors, in and out.  Rows need not start on 16 bytes: vectors are cut at the row's own 16-byte
+// boundaries (`shift` steps before its first one), so whole vectors move as 16 bytes and only
+// ragged ends value by value.
 constexpr int kRun = 12, kTile = 32 * kRun, kVectors = kTile / 4;
 
 template <bool BACKWARD>
 struct RowTile {
     float in[2][kArrays<BACKWARD>][kTile];
     float out[kTile];
-    float before[2];  // backward: the state before the tile's first step in memory
-    float pad[2];
+    float before[2][8];  // [stage][row]: backward, the state before the tile's first step in memory
+    float carry[2][8], init[2][8];
 };
 template <bool BACKWARD>
 constexpr size_t rows_smem() {
     return NW * sizeof(RowTile<BACKWARD>) + sizeof(Exchange<1>);
 }
 
-template <bool BACKWARD, int PASS>
-__global__ void __launch_bounds__(NW * 32, BACKWARD ? 2 : 3) scan_rows_kernel(ScanArgs a) {
-    constexpr int NA = kArrays<BACKWARD>;
+template <bool BACKWARD, int PASS, int SUB>
+__global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
+    constexpr int NA = kArrays<BACKWARD>, R = 32 / SUB, VR = SUB * kRun / 4;  // rows a warp, vectors of a row's tile
     extern __shared__ __align__(16) unsigned char raw[];
-    const Place at = place(a);
+    const Place at = place();
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, W = a.W;
-    const int wt = warp % W, wr = warp / W;
+    const int wt = warp % W, wr = warp / W, sr = l / SUB, ls = l % SUB;  // ls: the thread's place in its row
     RowTile<BACKWARD>& tile = reinterpret_cast<RowTile<BACKWARD>*>(raw)[warp];
     Exchange<1>& ex = *reinterpret_cast<Exchange<1>*>(raw + NW * sizeof(RowTile<BACKWARD>));
-    const int64_t row = at.block * (NW / W) + wr;
-    const bool live = row < a.lanes;
-    const float* p[SI_COUNT];
-#pragma unroll
-    for (int k = 0; k < SI_COUNT; ++k) p[k] = a.in[k].p ? a.in[k].p + (live ? row : 0) * a.in[k].so : nullptr;
-    const int64_t dst = (live ? row : 0) * a.T;
-    const int shift = static_cast<int>(dst & 3);
-    const int64_t vectors = (a.T + shift + 3) / 4;
     const bool want_gate = BACKWARD && PASS != MAPS && a.out[SO_GATE];
-    // segments and tiles are counted in vectors of four; scan order r
-    const int64_t begin = at.seg * a.seg_len, end = live ? min(vectors, begin + a.seg_len) : begin;
-    const int64_t all_end = min((a.T + 6) / 4, begin + a.seg_len);  // the longest row's: all warps loop alike
-    const int64_t stride = static_cast<int64_t>(at.size) * W * kVectors;
-    const int64_t own = begin + (static_cast<int64_t>(at.rank) * W + wt) * kVectors;
-    // the tile at r0: its first vector in memory and how many vectors it has; backward a tile that is
-    // cut short keeps its high end
-    auto tile_place = [&](int64_t r0, int64_t& v0) {
-        const int n = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(kVectors), end - r0)));
-        v0 = BACKWARD ? vectors - r0 - kVectors : r0;  // may be negative where n < kVectors
-        return n;
+    const int64_t stride = static_cast<int64_t>(at.size) * W * VR;  // of this warp's tiles, in vectors of four
+    const int64_t own = (static_cast<int64_t>(at.rank) * W + wt) * VR;
+    auto first_row = [&](int64_t unit) { return (unit / a.segments * (NW / W) + wr) * R; };
+    // A row's tile at r0 (vectors, scan order): where it lies.  A tile that is cut short keeps, backward, its
+    // high end; vectors [lo, lo + n) of it exist, the first at v0 of the row.
+    struct Cutout {
+        int64_t v0, vectors;
+        int lo, n, shift;
     };
-    auto issue = [&](int64_t r0, int stage) {
-        int64_t v0;
-        const int n = tile_place(r0, v0);
-        if (n > 0) {
-            const int lo = BACKWARD ? kVectors - n : 0;  // the vectors of the tile that exist: [lo, lo + n)
+    auto cutout = [&](int64_t row, int seg, int64_t r0) {
+        Cutout q;
+        q.shift = static_cast<int>(row * a.T & 3);
+        q.vectors = (a.T + q.shift + 3) / 4;
+        const int64_t end = row < a.lanes ? min(q.vectors, (seg + 1) * a.seg_len) : r0;
+        q.n = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(VR), end - r0)));
+        q.v0 = BACKWARD ? q.vectors - r0 - VR : r0;  // may be negative where n < VR
+        q.lo = BACKWARD ? VR - q.n : 0;
+        return q;
+    };
+    auto whole_tile = [&](const Cutout& q) {
+        return q.n == VR && 4 * q.v0 >= q.shift && 4 * (q.v0 + VR) - q.shift <= a.T;
+    };
+    const int need = 1 << SI_GATE | (a.in[SI_X].p ? 1 << SI_X : 0) | (want_gate ? 1 << SI_H : 0);
+    int64_t ahead_unit = at.first, ahead_r0 = 0;
+    int ahead_step = 0;
+    auto issue = [&](int stage) {
+        if (ahead_unit < a.units) {
+            const int seg = static_cast<int>(ahead_unit % a.segments);
+            const int64_t row0 = first_row(ahead_unit), r0 = seg * a.seg_len + own + ahead_r0;
+            const Cutout first = cutout(row0, seg, r0);
+            const int64_t at_t = 4 * first.v0 - first.shift;
+            if (SUB == 32 && whole_tile(first) && (a.vec & need) == need) {  // nothing to check vector by vector
+                auto copy = [&](int op, int arr) {
+                    const float* p = a.in[op].p + row0 * a.in[op].so + at_t + 4 * l;
+                    const uint32_t to = smem_addr(&tile.in[stage][arr][4 * l]);
 #pragma unroll
-            for (int arr = 0; arr < NA; ++arr) {
-                const int k = arr == 0 ? SI_GATE : arr == 1 ? SI_X : SI_H;
-                if (arr == 1 && !p[SI_X]) continue;
-                if (arr == 2 && !want_gate) continue;
+                    for (int q = 0; q < kVectors / 32; ++q) copy_async<16>(to + 512 * q, p + 128 * q);
+                };
+                copy(SI_GATE, 0);
+                if (a.in[SI_X].p) copy(SI_X, 1);
+                if (want_gate) copy(SI_H, NA - 1);
+            } else {
 #pragma unroll
                 for (int q = 0; q < kVectors / 32; ++q) {
-                    const int v = l + 32 * q;
-                    if (v < lo || v >= lo + n) continue;
-                    const int64_t t = 4 * (v0 + v) - shift;
-                    const uint32_t to = smem_addr(&tile.in[stage][arr][4 * v]);
-                    if ((a.vec >> k & 1) && t >= 0 && t + 3 < a.T) {
-                        copy_async<16>(to, p[k] + t);
-                    } else {
+                    const int at_v = l + 32 * q, v = at_v % VR;
+                    const int64_t row = row0 + at_v / VR;
+                    const Cutout k = cutout(row, seg, r0);
+                    if (v < k.lo || v >= k.lo + k.n) continue;
+                    const int64_t t = 4 * (k.v0 + v) - k.shift;
+                    const bool whole = t >= 0 && t + 3 < a.T;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (t + j >= 0 && t + j < a.T) copy_async<4>(to + 4 * j, p[k] + (t + j) * a.in[k].st);
+                    for (int arr = 0; arr < NA; ++arr) {
+                        const int op = arr == 0 ? SI_GATE : arr == 1 ? SI_X : SI_H;
+                        if (arr == 1 && !a.in[SI_X].p) continue;
+                        if (arr == 2 && !want_gate) continue;
+                        const float* p = a.in[op].p + row * a.in[op].so;
+                        const uint32_t to = smem_addr(&tile.in[stage][arr][4 * at_v]);
+                        if ((a.vec >> op & 1) && whole) {
+                            copy_async<16>(to, p + t);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                if (t + j >= 0 && t + j < a.T) copy_async<4>(to + 4 * j, p + (t + j) * a.in[op].st);
+                        }
                     }
                 }
             }
-            if (want_gate && l == 0) {
-                const int64_t t = 4 * (v0 + lo) - shift - 1;  // before the tile's first step in memory
-                if (t >= 0) copy_async<4>(smem_addr(&tile.before[stage]), p[SI_H] + t * a.in[SI_H].st);
+            const int64_t row = row0 + sr;
+            if (ls == 0 && row < a.lanes) {
+                if (PASS == ONLY && ahead_step == 0 && a.in[SI_CARRY].p)
+                    copy_async<4>(smem_addr(&tile.carry[stage][sr]), a.in[SI_CARRY].p + row * a.in[SI_CARRY].so);
+                if (want_gate) {
+                    const Cutout k = SUB == 32 ? first : cutout(row, seg, r0);
+                    const int64_t t = 4 * (k.v0 + k.lo) - k.shift - 1;  // before the tile's first step in memory
+                    if (k.n > 0 && t >= 0) copy_async<4>(smem_addr(&tile.before[stage][sr]), a.in[SI_H].p + row * a.in[SI_H].so + t * a.in[SI_H].st);
+                    if (k.n > 0 && t < 0 && a.in[SI_INIT].p)
+                        copy_async<4>(smem_addr(&tile.init[stage][sr]), a.in[SI_INIT].p + row * a.in[SI_INIT].so);
+                }
+            }
+            ahead_r0 += stride;
+            if (++ahead_step == a.steps) {
+                ahead_step = 0;
+                ahead_r0 = 0;
+                ahead_unit += at.clusters;
             }
         }
         copies_commit();
     };
-    issue(own, 0);
-    issue(own + stride, 1);
+    issue(0);
+    issue(1);
     if (at.size > 1) cg::this_cluster().sync();  // every CTA runs before another writes to it
-    float c = live ? segment_state<PASS>(a, at.seg, row, p[SI_CARRY]) : 0.0f;
-    if (a.T == 0) {
-        copies_wait_all();
-        if (live && wt == 0 && l == 0 && a.out[SO_LANE]) a.out[SO_LANE][row] = c;
-        return;
-    }
     Joiner<1> joiner{ex, at, W, wt, wr, warp, 0};
-    float gates = 1.0f;
-    const float init = want_gate && live && p[SI_INIT] ? __ldg(p[SI_INIT]) : 0.0f;
-    const int run = (BACKWARD ? 31 - l : l) * kRun;  // this thread's run within the tile
+    const int run = (BACKWARD ? SUB - 1 - ls : ls) * kRun;  // this thread's run within its row's tile
     int stage = 0;
-    for (int64_t base = begin; base < all_end; base += stride, stage ^= 1) {
-        const int64_t r0 = own + (base - begin);
-        int64_t v0;
-        const int n = tile_place(r0, v0);
-        const int lo = BACKWARD ? kVectors - n : 0;
-        const int64_t t0 = 4 * v0 - shift + run;  // the run's first step in memory
-        copies_wait_one();
-        __syncwarp();
-        float ga[kRun], xv[kRun], hv[BACKWARD ? kRun : 1];
-#pragma unroll
-        for (int j = 0; j < kRun; j += 4) {
-            load_shared<4>(&tile.in[stage][0][run + j], ga + j);
-            load_shared<4>(&tile.in[stage][1][run + j], xv + j);
+    for (int64_t unit = at.first; unit < a.units; unit += at.clusters) {
+        const int seg = static_cast<int>(unit % a.segments);
+        const int64_t row0 = first_row(unit), row = row0 + sr;
+        const bool live = row < a.lanes;
+        float c = 0.0f, gates = 1.0f;
+        if constexpr (PASS == JOINED) {
+            if (live && a.in[SI_CARRY].p) c = __ldg(a.in[SI_CARRY].p + row * a.in[SI_CARRY].so);
+            c = segment_state<1>(a, ex, seg, row, live, c, warp, 0, l == 0);
         }
-        if constexpr (BACKWARD) {
-            if (want_gate) {  // the state before each step
-                float h[kRun];
+        for (int k = 0; k < a.steps; ++k, stage ^= 1) {
+            const int64_t r0 = seg * a.seg_len + own + k * stride;
+            const Cutout cut = cutout(row, seg, r0);
+            const int64_t t0 = 4 * cut.v0 - cut.shift + run;  // the run's first step in memory
+            copies_wait_one();
+            __syncwarp();
+            const float* in = &tile.in[stage][0][sr * SUB * kRun + run];
+            float ga[kRun], xv[kRun], hv[BACKWARD ? kRun : 1];
 #pragma unroll
-                for (int j = 0; j < kRun; j += 4) load_shared<4>(&tile.in[stage][2][run + j], h + j);
-                hv[0] = run > 4 * lo ? tile.in[stage][2][run > 0 ? run - 1 : 0] : tile.before[stage];
-#pragma unroll
-                for (int j = 1; j < kRun; ++j) hv[j] = h[j - 1];
+            for (int j = 0; j < kRun; j += 4) {
+                load_shared<4>(in + j, ga + j);
+                load_shared<4>(in + kTile + j, xv + j);
             }
-        }
-        // the row's ends: steps outside it leave the state as it is
-        const bool whole = n == kVectors && t0 >= (BACKWARD ? 1 : 0) && t0 + kRun <= a.T && p[SI_X];
-        if (!whole) {
+            if constexpr (BACKWARD) {
+                if (want_gate) {  // the state before each step
+                    float h[kRun];
 #pragma unroll
-            for (int j = 0; j < kRun; ++j) {
-                const int v = (run + j) / 4;
-                const bool inside = v >= lo && v < lo + n && t0 + j >= 0 && t0 + j < a.T;
-                if (!inside) ga[j] = 1.0f;
-                if (!inside || !p[SI_X]) xv[j] = 0.0f;
-                if (BACKWARD && want_gate && run + j == 4 * lo) hv[BACKWARD ? j : 0] = tile.before[stage];
-                if (BACKWARD && t0 + j == 0) hv[BACKWARD ? j : 0] = init;
+                    for (int j = 0; j < kRun; j += 4) load_shared<4>(in + 2 * kTile + j, h + j);
+                    hv[0] = run > 4 * cut.lo ? in[2 * kTile - 1] : tile.before[stage][sr];
+#pragma unroll
+                    for (int j = 1; j < kRun; ++j) hv[j] = h[j - 1];
+                }
             }
-        }
-        __syncwarp();
-        issue(r0 + 2 * stride, stage);
-        float2 q = tile_map<BACKWARD, kRun>([&](int j) { return ga[BACKWARD ? kRun - 1 - j : j]; },
-                                            [&](int j) { return xv[BACKWARD ? kRun - 1 - j : j]; });
+            // the row's ends: steps outside it leave the state as it is
+            const bool whole = cut.n == VR && t0 >= (BACKWARD ? 1 : 0) && t0 + kRun <= a.T && a.in[SI_X].p;
+            if (!whole) {
+                const float init = want_gate && a.in[SI_INIT].p ? tile.init[stage][sr] : 0.0f;
 #pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const float2 b = make_float2(__shfl_up_sync(0xffffffffu, q.x, d), __shfl_up_sync(0xffffffffu, q.y, d));
-            if (l >= d) q = join(b, q);
-        }
-        const float2 m = make_float2(__shfl_sync(0xffffffffu, q.x, 31), __shfl_sync(0xffffffffu, q.y, 31));
-        float2 b = make_float2(__shfl_up_sync(0xffffffffu, q.x, 1), __shfl_up_sync(0xffffffffu, q.y, 1));
-        float s = joiner.first(m, c, base == begin, l == 0);
-        const bool last_step = base + stride >= all_end;
-        float y = l > 0 ? apply(b, s) : s;
-        if constexpr (PASS == MAPS) {
-            joiner.gates_of_step(gates);
-            s = apply(m, s);
-            if (last_step && live && wt == W - 1 && l == 0) a.maps[at.seg * a.lanes + row] = make_float2(gates, s);
-        } else {
+                for (int j = 0; j < kRun; ++j) {
+                    const int v = (run + j) / 4;
+                    const bool inside = v >= cut.lo && v < cut.lo + cut.n && t0 + j >= 0 && t0 + j < a.T;
+                    if (!inside) ga[j] = 1.0f;
+                    if (!inside || !a.in[SI_X].p) xv[j] = 0.0f;
+                    if (BACKWARD && want_gate && run + j == 4 * cut.lo) hv[BACKWARD ? j : 0] = tile.before[stage][sr];
+                    if (BACKWARD && t0 + j == 0) hv[BACKWARD ? j : 0] = init;
+                }
+            }
+            if (PASS == ONLY && k == 0) c = a.in[SI_CARRY].p && live ? tile.carry[stage][sr] : 0.0f;
+            __syncwarp();
+            issue(stage);
+            float2 q = tile_map<BACKWARD, kRun>([&](int j) { return ga[BACKWARD ? kRun - 1 - j : j]; },
+                                                [&](int j) { return xv[BACKWARD ? kRun - 1 - j : j]; });
+#pragma unroll
+            for (int d = 1; d < SUB; d *= 2) {
+                const float2 b = make_float2(__shfl_up_sync(0xffffffffu, q.x, d), __shfl_up_sync(0xffffffffu, q.y, d));
+                if (ls >= d) q = join(b, q);
+            }
+            const float2 b = make_float2(__shfl_up_sync(0xffffffffu, q.x, 1), __shfl_up_sync(0xffffffffu, q.y, 1));
+            const bool last = k + 1 == a.steps;
+            float s = c;
+            if constexpr (SUB == 32) {
+                const float2 m = make_float2(__shfl_sync(0xffffffffu, q.x, 31), __shfl_sync(0xffffffffu, q.y, 31));
+                s = joiner.first(m, c, k == 0, l == 0);
+                if constexpr (PASS == MAPS) {
+                    joiner.gates_of_step(gates);
+                    s = apply(m, s);
+                    if (last && live && wt == W - 1 && l == 0) a.maps[seg * a.lanes + row] = make_float2(gates, s);
+                    joiner.hand_on(s, last, l == 0);
+                    continue;
+                }
+            }
+            float y = ls > 0 ? apply(b, s) : s;
             // results over the inputs' registers: x becomes h or dx, h becomes dgate
             if constexpr (BACKWARD) {
 #pragma unroll
@@ -602,23 +706,36 @@ __global__ void __launch_bounds__(NW * 32, BACKWARD ? 2 : 3) scan_rows_kernel(Sc
                 for (int j = 0; j < kRun; ++j) xv[j] = y = fmaf(ga[j], y, xv[j]);
             }
             auto write = [&](float* out, const float* v) {
+                float* to = &tile.out[sr * SUB * kRun + run];
 #pragma unroll
-                for (int j = 0; j < kRun; j += 4)
-                    *reinterpret_cast<float4*>(&tile.out[run + j]) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                for (int j = 0; j < kRun; j += 4) *reinterpret_cast<float4*>(to + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                 __syncwarp();
+                if (SUB == 32 && whole_tile(cut)) {
+                    float* to_g = out + row * a.T + 4 * cut.v0 - cut.shift + 4 * l;
+#pragma unroll
+                    for (int u = 0; u < kVectors / 32; ++u) {
+                        float f[4];
+                        load_shared<4>(&tile.out[4 * l + 128 * u], f);
+                        store_vec<4>(to_g + 128 * u, f, BACKWARD);
+                    }
+                    __syncwarp();
+                    return;
+                }
 #pragma unroll
                 for (int u = 0; u < kVectors / 32; ++u) {
-                    const int k = l + 32 * u;
-                    if (k < lo || k >= lo + n) continue;
-                    const int64_t t = 4 * (v0 + k) - shift;
+                    const int at_v = l + 32 * u, v = at_v % VR;
+                    const int64_t r = row0 + at_v / VR;
+                    const Cutout e = SUB == 32 ? cut : cutout(r, seg, r0);
+                    if (v < e.lo || v >= e.lo + e.n) continue;
+                    const int64_t t = 4 * (e.v0 + v) - e.shift;
                     float f[4];
-                    load_shared<4>(&tile.out[4 * k], f);
+                    load_shared<4>(&tile.out[4 * at_v], f);
                     if (t >= 0 && t + 3 < a.T) {
-                        store_vec<4>(out + dst + t, f, BACKWARD);
+                        store_vec<4>(out + r * a.T + t, f, BACKWARD);
                     } else {
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            if (t + j >= 0 && t + j < a.T) out[dst + t + j] = f[j];
+                            if (t + j >= 0 && t + j < a.T) out[r * a.T + t + j] = f[j];
                     }
                 }
                 __syncwarp();
@@ -627,12 +744,80 @@ __global__ void __launch_bounds__(NW * 32, BACKWARD ? 2 : 3) scan_rows_kernel(Sc
             if constexpr (BACKWARD) {
                 if (want_gate) write(a.out[SO_GATE], hv);
             }
-            s = __shfl_sync(0xffffffffu, y, 31);  // behind the tile's last run
-            if (n > 0 && r0 + n == vectors && l == 0 && a.out[SO_LANE]) a.out[SO_LANE][row] = s;
+            // behind the tile's last run
+            if (SUB == 32) s = __shfl_sync(0xffffffffu, y, 31);
+            if (live && cut.n > 0 && r0 + cut.n == cut.vectors && ls == SUB - 1 && a.out[SO_LANE]) a.out[SO_LANE][row] = y;
+            if constexpr (SUB == 32) joiner.hand_on(s, last, l == 0);
         }
-        joiner.hand_on(s, last_step, l == 0);
     }
     copies_wait_all();
+}
+
+// ---- a few steps (a token for each of many sequences): a thread walks V lanes, nothing to join.
+constexpr int kShort = 16;
+
+template <bool BACKWARD, int V>
+__global__ void __launch_bounds__(256) scan_short_kernel(ScanArgs a) {
+    const int64_t lane = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * V;
+    if (lane >= a.lanes) return;
+    int64_t o, i;
+    split_lane(a, lane, o, i);
+    const int64_t i1 = a.n2 == a.inner ? 0 : i / a.n2, i2 = i - i1 * a.n2;
+    auto ptr = [&](int k) { return a.in[k].p ? a.in[k].p + o * a.in[k].so + i1 * a.in[k].s1 + i2 * a.in[k].s2 : nullptr; };
+    const float *gate = ptr(SI_GATE), *x = ptr(SI_X), *carry = ptr(SI_CARRY), *h = ptr(SI_H), *init = ptr(SI_INIT);
+    auto load = [&](const float* p, int k, float* v) {
+        if (V > 1 && (a.vec >> k & 1)) {
+            load_shared<V>(p, v);
+        } else {
+#pragma unroll
+            for (int u = 0; u < V; ++u) v[u] = p[u * a.in[k].s2];
+        }
+    };
+    float s[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[v] = 0.0f;
+    if (carry) load(carry, SI_CARRY, s);
+    const int T = static_cast<int>(a.T);
+    const int64_t y0 = o * a.T * a.inner + i;
+    for (int r0 = 0; r0 < T; r0 += 4) {
+        float ga[4][V], xv[4][V], hv[BACKWARD ? 4 : 1][V];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int t = BACKWARD ? T - 1 - r0 - j : r0 + j;
+            if (r0 + j >= T) continue;
+            load(gate + t * a.in[SI_GATE].st, SI_GATE, ga[j]);
+#pragma unroll
+            for (int v = 0; v < V; ++v) xv[j][v] = 0.0f;
+            if (x) load(x + t * a.in[SI_X].st, SI_X, xv[j]);
+            if (BACKWARD) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) hv[j][v] = 0.0f;
+                if (a.out[SO_GATE]) {
+                    if (t > 0) load(h + (t - 1) * a.in[SI_H].st, SI_H, hv[j]);
+                    else if (init) load(init, SI_INIT, hv[j]);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (r0 + j >= T) continue;
+            const int64_t y = y0 + (BACKWARD ? T - 1 - r0 - j : r0 + j) * a.inner;
+            float main[V], dg[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                if (BACKWARD) {
+                    main[v] = xv[j][v] + s[v];
+                    dg[v] = main[v] * hv[BACKWARD ? j : 0][v];
+                    s[v] = ga[j][v] * main[v];
+                } else {
+                    main[v] = s[v] = fmaf(ga[j][v], s[v], xv[j][v]);
+                }
+            }
+            if (a.out[SO_MAIN]) store_vec<V>(a.out[SO_MAIN] + y, main, false);
+            if (BACKWARD && a.out[SO_GATE]) store_vec<V>(a.out[SO_GATE] + y, dg, false);
+        }
+    }
+    if (a.out[SO_LANE]) store_vec<V>(a.out[SO_LANE] + lane, s, false);
 }
 
 // The widest vectors of lanes: every operand has adjacent lanes behind n1 whose vectors are
@@ -650,27 +835,46 @@ int widest(const ScanDesc& d) {
     return 1;
 }
 
-// How a scan is cut: lanes per thread, warps along time, CTAs of a cluster along time, segments.
+// How a scan is cut: threads of a row, lanes per thread, warps along time, CTAs of a cluster along
+// time, segments.
 struct Cut {
-    bool rows;
-    int V = 1, W = 1, cluster = 1, segments = 1;
-    int64_t seg_len = 0, blocks = 0;
+    bool rows, direct;
+    int sub = 32, V = 1, tile = 16, W = 1, cluster = 1, segments = 1;
+    int64_t seg_len = 1, blocks = 0, steps = 0;
 };
 
 Cut cut(const ScanDesc& d) {
     Cut c;
     const int64_t inner = d.n1 * d.n2, lanes = d.outer * inner;
-    c.rows = inner == 1;
-    if (!c.rows) c.V = widest(d);
+    c.direct = d.T <= kShort;
+    c.rows = inner == 1 && !c.direct;
+    if (inner > 1) c.V = widest(d);
+    if (c.direct) {
+        // (a few lanes only: one each, for more threads)
+        if (lanes < 148 * 256 * c.V) c.V = 1;
+        c.blocks = (lanes + 256 * c.V - 1) / (256 * c.V);
+        return c;
+    }
     const int64_t len = c.rows ? (d.T + 6) / 4 : d.T;  // rows count time in vectors of four
-    const int64_t tile = c.rows ? kVectors : kTileSteps, tiles = (len + tile - 1) / tile;
-    while (c.W < NW && c.W < tiles) c.W *= 2;
-    const int64_t groups = c.rows ? lanes : (lanes + 31) / 32;
+    while (c.rows && c.sub > 4 && len <= c.sub / 2 * kRun / 4) c.sub /= 2;
+    if (c.rows) c.tile = c.sub * kRun / 4;
+    auto warps = [&](int64_t t) {  // along time
+        int w = 1;
+        while (w < NW && w * t < len) w *= 2;
+        return w;
+    };
+    auto padded = [&](int64_t t) { return (len + warps(t) * t - 1) / (warps(t) * t) * warps(t) * t; };
+    // 24 steps a tile are faster than 16 (fewer exchanges: 39 against 49 us for 8 x 2048 x 1024), unless
+    // they pad the axis by a tenth more
+    if (!c.rows && !d.backward && 10 * padded(24) <= 11 * padded(16)) c.tile = 24;
+    const int64_t tile = c.tile;
+    c.W = warps(tile);
+    const int64_t groups = c.rows ? (lanes + 32 / c.sub - 1) / (32 / c.sub) : (lanes + 31) / 32;
     c.blocks = (groups + NW / c.W - 1) / (NW / c.W);
     // more CTAs along time while the card is not full and every CTA has a step of its own
     while (c.W == NW && c.cluster < 8 && c.blocks * c.cluster < 256 && c.cluster * c.W * tile * 2 <= len) c.cluster *= 2;
-    c.seg_len = len > 0 ? len : 1;
-    if (c.blocks * c.cluster < 128 && len > static_cast<int64_t>(c.cluster) * c.W * tile) {
+    c.seg_len = len;
+    if (c.blocks * c.cluster < 128 && len > c.cluster * c.W * tile) {
         c.cluster = 1;
         const int64_t step = c.W * tile, most = (len + step - 1) / step;
         int64_t want = (296 + c.blocks - 1) / c.blocks;
@@ -678,23 +882,31 @@ Cut cut(const ScanDesc& d) {
         c.seg_len = ((len + want - 1) / want + step - 1) / step * step;
         c.segments = static_cast<int>((len + c.seg_len - 1) / c.seg_len);
     }
+    const int64_t span = c.cluster * c.W * tile;
+    c.steps = (c.seg_len + span - 1) / span;
     return c;
 }
 
 template <auto Kernel>
 cudaError_t launch_kernel(size_t smem, const Cut& c, const ScanArgs& a, cudaStream_t stream) {
-    static std::atomic<uint64_t> ready{0};  // devices on which the kernel's shared memory limit is raised
+    static std::atomic<int> resident[64];  // CTAs that run at the same time, by device; 0: not found yet
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-    if (!(ready.load() & bit)) {
+    int slots = dev < 64 ? resident[dev].load() : 0;
+    if (slots == 0) {
         e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        int sms = 0;
+        if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&slots, Kernel, NW * 32, smem);
+        if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
         if (e != cudaSuccess) return e;
-        ready |= bit;
+        slots *= sms;
+        if (slots < 1) return cudaErrorInvalidConfiguration;
+        if (dev < 64) resident[dev] = slots;
     }
+    const int64_t clusters = c.cluster > 1 || a.units < slots ? a.units : slots;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(c.blocks * c.segments * c.cluster));
+    cfg.gridDim = dim3(static_cast<unsigned>(clusters * c.cluster));
     cfg.blockDim = dim3(NW * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -707,16 +919,39 @@ cudaError_t launch_kernel(size_t smem, const Cut& c, const ScanArgs& a, cudaStre
     return cudaLaunchKernelEx(&cfg, Kernel, a);
 }
 
+template <bool BACKWARD, int PASS, int TILE>
+cudaError_t launch_cols(const Cut& c, const ScanArgs& a, cudaStream_t stream) {
+    constexpr size_t smem = sizeof(ColTile<BACKWARD, TILE>);
+    if (c.V == 4) return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 4, TILE>>(smem, c, a, stream);
+    if (c.V == 2) return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 2, TILE>>(smem, c, a, stream);
+    return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 1, TILE>>(smem, c, a, stream);
+}
+
 template <bool BACKWARD, int PASS>
 cudaError_t launch_pass(const Cut& c, const ScanArgs& a, cudaStream_t stream) {
-    if (c.rows) return launch_kernel<scan_rows_kernel<BACKWARD, PASS>>(rows_smem<BACKWARD>(), c, a, stream);
-    if (c.V == 4) return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 4>>(cols_smem<BACKWARD>(), c, a, stream);
-    if (c.V == 2) return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 2>>(cols_smem<BACKWARD>(), c, a, stream);
-    return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 1>>(cols_smem<BACKWARD>(), c, a, stream);
+    if (c.rows) {
+        if constexpr (PASS == ONLY) {
+            if (c.sub == 4) return launch_kernel<scan_rows_kernel<BACKWARD, PASS, 4>>(rows_smem<BACKWARD>(), c, a, stream);
+            if (c.sub == 8) return launch_kernel<scan_rows_kernel<BACKWARD, PASS, 8>>(rows_smem<BACKWARD>(), c, a, stream);
+            if (c.sub == 16) return launch_kernel<scan_rows_kernel<BACKWARD, PASS, 16>>(rows_smem<BACKWARD>(), c, a, stream);
+        }
+        return launch_kernel<scan_rows_kernel<BACKWARD, PASS, 32>>(rows_smem<BACKWARD>(), c, a, stream);
+    }
+    if constexpr (!BACKWARD) {
+        if (c.tile == 24) return launch_cols<BACKWARD, PASS, 24>(c, a, stream);
+    }
+    return launch_cols<BACKWARD, PASS, 16>(c, a, stream);
 }
 
 template <bool BACKWARD>
 cudaError_t launch_cut(const Cut& c, const ScanArgs& a, cudaStream_t stream) {
+    if (c.direct) {
+        const dim3 grid(static_cast<unsigned>(c.blocks));
+        if (c.V == 4) scan_short_kernel<BACKWARD, 4><<<grid, 256, 0, stream>>>(a);
+        else if (c.V == 2) scan_short_kernel<BACKWARD, 2><<<grid, 256, 0, stream>>>(a);
+        else scan_short_kernel<BACKWARD, 1><<<grid, 256, 0, stream>>>(a);
+        return cudaGetLastError();
+    }
     if (c.segments == 1) return launch_pass<BACKWARD, ONLY>(c, a, stream);
     const cudaError_t e = launch_pass<BACKWARD, MAPS>(c, a, stream);
     return e != cudaSuccess ? e : launch_pass<BACKWARD, JOINED>(c, a, stream);
@@ -737,7 +972,7 @@ int launch_scan(const ScanDesc& d, const float* const* in, float* const* out, vo
     const int64_t lanes = d.outer * d.n1 * d.n2;
     if (lanes == 0) return 0;
     const Cut c = cut(d);
-    if (c.blocks * c.segments * c.cluster > 0x7fffffff) return static_cast<int>(cudaErrorInvalidConfiguration);
+    if (c.blocks * c.segments > 0x7fffffff / 8 || c.steps > 0x7fffffff) return static_cast<int>(cudaErrorInvalidConfiguration);
     ScanArgs a;
     a.vec = 0;
     for (int k = 0; k < SI_COUNT; ++k) {
@@ -754,6 +989,8 @@ int launch_scan(const ScanDesc& d, const float* const* in, float* const* out, vo
     a.T = d.T;
     a.seg_len = c.seg_len;
     a.segments = c.segments;
+    a.units = c.blocks * c.segments;
+    a.steps = static_cast<int>(c.steps);
     a.W = c.W;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return static_cast<int>(d.backward ? launch_cut<true>(c, a, st) : launch_cut<false>(c, a, st));
