@@ -194,9 +194,15 @@ struct Joiner {
             for (int q = 0; q < 7; ++q)
                 if (q < at.rank) s = apply(ex.cta[buf][q][l], s);
         }
+        if (W == NW) {
+            float2 q[NW - 1];  // (all loaded, so that the loads do not wait for one another)
 #pragma unroll
-        for (int w = 0; w < NW - 1; ++w)
-            if (w < wt) s = apply(ex.warp[buf][wr * W + w][l], s);
+            for (int w = 0; w < NW - 1; ++w) q[w] = ex.warp[buf][w][l];
+#pragma unroll
+            for (int w = 0; w < NW - 1; ++w) s = w < wt ? apply(q[w], s) : s;
+        } else {
+            for (int w = 0; w < wt; ++w) s = apply(ex.warp[buf][wr * W + w][l], s);
+        }
         return s;
     }
     // s: the state behind this warp's tile.  The step's last tile hands it to the next step
@@ -281,7 +287,8 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_cols_kernel(ScanArgs a) {
     const bool want_gate = BACKWARD && PASS != MAPS && a.out[SO_GATE];
     const int64_t stride = static_cast<int64_t>(at.size) * W * TILE;  // of this warp's tiles
     const int64_t own = (static_cast<int64_t>(at.rank) * W + wt) * TILE + sub * TS;
-    auto first_lane = [&](int64_t unit) { return (unit / a.segments * (NW / W) + wr) * 32; };
+    auto block_of = [&](int64_t unit) { return a.segments == 1 ? unit : unit / a.segments; };
+    auto first_lane = [&](int64_t unit) { return (block_of(unit) * (NW / W) + wr) * 32; };
     // this thread's steps from r0 on
     auto run_len = [&](bool live, int64_t r0, int64_t end) {
         return live ? static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(TS), end - r0))) : 0;
@@ -299,7 +306,7 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_cols_kernel(ScanArgs a) {
         ahead.unit = unit;
         ahead.step = 0;
         if (unit >= a.units) return;
-        const int64_t lane = first_lane(unit) + col * V, begin = unit % a.segments * a.seg_len;
+        const int64_t lane = first_lane(unit) + col * V, begin = (unit - block_of(unit) * a.segments) * a.seg_len;
         ahead.live = lane < a.lanes;
         ahead.r0 = begin + own;
         ahead.end = min(a.T, begin + a.seg_len);
@@ -368,7 +375,7 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_cols_kernel(ScanArgs a) {
     const bool splat_h = V > 1 && !(a.vec >> SI_H & 1);
     int stage = 0;
     for (int64_t unit = at.first; unit < a.units; unit += at.clusters) {
-        const int seg = static_cast<int>(unit % a.segments);
+        const int seg = static_cast<int>(unit - block_of(unit) * a.segments);
         const int64_t lane0 = first_lane(unit), lane = lane0 + col * V;
         const bool live = lane < a.lanes;
         const int64_t begin = seg * a.seg_len, end = min(a.T, begin + a.seg_len);
@@ -497,19 +504,20 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_cols_kernel(ScanArgs a) {
     copies_wait_all();
 }
 
-// ---- time adjacent in memory ([.., T]): a warp's tile is 384 steps of one row, a run of 12
-// adjacent steps per thread (an odd number of 16-byte vectors, so that the threads' runs lie
-// in different banks), the runs' maps joined by shuffles.  Rows of up to SUB*12 - 3 steps take
-// SUB threads, 32/SUB rows a warp.  Tiles move between global and shared memory in coalesced
+// ---- time adjacent in memory ([.., T]): a warp's tile is 640 (backward 384) steps of one row, a
+// run of 20 (12) adjacent steps per thread (an odd number of 16-byte vectors, so that the
+// threads' runs lie in different banks), the runs' maps joined by shuffles.  Rows of up to
+// SUB runs less 3 steps take SUB threads, 32/SUB rows a warp.  Tiles move between global and shared memory in coalesced
 // vectors, in and out.  Rows need not start on 16 bytes: vectors are cut at the row's own 16-byte
 // boundaries (`shift` steps before its first one), so whole vectors move as 16 bytes and only
 // ragged ends value by value.
-constexpr int kRun = 12, kTile = 32 * kRun, kVectors = kTile / 4;
+template <bool BACKWARD>
+constexpr int kRowRun = BACKWARD ? 12 : 20;
 
 template <bool BACKWARD>
 struct RowTile {
-    float in[2][kArrays<BACKWARD>][kTile];
-    float out[kTile];
+    float in[2][kArrays<BACKWARD>][32 * kRowRun<BACKWARD>];
+    float out[32 * kRowRun<BACKWARD>];
     float before[2][8];  // [stage][row]: backward, the state before the tile's first step in memory
     float carry[2][8], init[2][8];
 };
@@ -518,9 +526,19 @@ constexpr size_t rows_smem() {
     return NW * sizeof(RowTile<BACKWARD>) + sizeof(Exchange<1>);
 }
 
+template <bool FIRST, class A, class B>
+struct Select {
+    using type = A;
+};
+template <class A, class B>
+struct Select<false, A, B> {
+    using type = B;
+};
+
 template <bool BACKWARD, int PASS, int SUB>
 __global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
-    constexpr int NA = kArrays<BACKWARD>, R = 32 / SUB, VR = SUB * kRun / 4;  // rows a warp, vectors of a row's tile
+    constexpr int NA = kArrays<BACKWARD>, kRun = kRowRun<BACKWARD>, kTile = 32 * kRun, kVectors = kTile / 4;
+    constexpr int R = 32 / SUB, VR = SUB * kRun / 4;  // rows a warp, vectors of a row's tile
     extern __shared__ __align__(16) unsigned char raw[];
     const Place at = place();
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, W = a.W;
@@ -530,38 +548,53 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
     const bool want_gate = BACKWARD && PASS != MAPS && a.out[SO_GATE];
     const int64_t stride = static_cast<int64_t>(at.size) * W * VR;  // of this warp's tiles, in vectors of four
     const int64_t own = (static_cast<int64_t>(at.rank) * W + wt) * VR;
-    auto first_row = [&](int64_t unit) { return (unit / a.segments * (NW / W) + wr) * R; };
+    // A unit's rows for this warp and its segment (without a division where there is one segment).
+    struct Rows {
+        int64_t row0, begin, end;  // segment in vectors of four, scan order
+        int seg;
+    };
+    auto rows_of = [&](int64_t unit) {
+        Rows r;
+        const int64_t block = a.segments == 1 ? unit : unit / a.segments;
+        r.seg = static_cast<int>(unit - block * a.segments);
+        r.row0 = (block * (NW / W) + wr) * R;
+        r.begin = r.seg * a.seg_len;
+        r.end = r.begin + a.seg_len;
+        return r;
+    };
     // A row's tile at r0 (vectors, scan order): where it lies.  A tile that is cut short keeps, backward, its
-    // high end; vectors [lo, lo + n) of it exist, the first at v0 of the row.
+    // high end; vectors [lo, lo + n) of it exist, the tile's first is v0 of the row.
+    using Count = typename Select<SUB == 32, int64_t, int>::type;  // rows of a few threads are short
     struct Cutout {
-        int64_t v0, vectors;
+        Count v0, vectors;
         int lo, n, shift;
     };
-    auto cutout = [&](int64_t row, int seg, int64_t r0) {
+    auto cutout = [&](int64_t row, Count end, Count r0) {
         Cutout q;
-        q.shift = static_cast<int>(row * a.T & 3);
-        q.vectors = (a.T + q.shift + 3) / 4;
-        const int64_t end = row < a.lanes ? min(q.vectors, (seg + 1) * a.seg_len) : r0;
-        q.n = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(VR), end - r0)));
+        q.shift = static_cast<int>(static_cast<unsigned>(row) * static_cast<unsigned>(a.T) & 3);
+        q.vectors = (static_cast<Count>(a.T) + q.shift + 3) / 4;
+        const Count last = row < a.lanes ? min(q.vectors, end) : r0;
+        q.n = static_cast<int>(max(static_cast<Count>(0), min(static_cast<Count>(VR), last - r0)));
         q.v0 = BACKWARD ? q.vectors - r0 - VR : r0;  // may be negative where n < VR
         q.lo = BACKWARD ? VR - q.n : 0;
         return q;
     };
+    // all of the tile is inside the row: nothing to check vector by vector
     auto whole_tile = [&](const Cutout& q) {
         return q.n == VR && 4 * q.v0 >= q.shift && 4 * (q.v0 + VR) - q.shift <= a.T;
     };
     const int need = 1 << SI_GATE | (a.in[SI_X].p ? 1 << SI_X : 0) | (want_gate ? 1 << SI_H : 0);
-    int64_t ahead_unit = at.first, ahead_r0 = 0;
+    int64_t ahead_unit = at.first;
+    Rows ahead = rows_of(ahead_unit);
+    Count ahead_r0 = static_cast<Count>(ahead.begin + own);
     int ahead_step = 0;
     auto issue = [&](int stage) {
         if (ahead_unit < a.units) {
-            const int seg = static_cast<int>(ahead_unit % a.segments);
-            const int64_t row0 = first_row(ahead_unit), r0 = seg * a.seg_len + own + ahead_r0;
-            const Cutout first = cutout(row0, seg, r0);
-            const int64_t at_t = 4 * first.v0 - first.shift;
-            if (SUB == 32 && whole_tile(first) && (a.vec & need) == need) {  // nothing to check vector by vector
+            const Cutout mine = cutout(ahead.row0 + sr, static_cast<Count>(ahead.end), ahead_r0);
+            const int64_t at_t = 4 * static_cast<int64_t>(mine.v0) - mine.shift;
+            if (SUB == 32 && whole_tile(mine) && (a.vec & need) == need) {
                 auto copy = [&](int op, int arr) {
-                    const float* p = a.in[op].p + row0 * a.in[op].so + at_t + 4 * l;
+                    const float* p = a.in[op].p + ahead.row0 * a.in[op].so + at_t + 4 * l;
                     const uint32_t to = smem_addr(&tile.in[stage][arr][4 * l]);
 #pragma unroll
                     for (int q = 0; q < kVectors / 32; ++q) copy_async<16>(to + 512 * q, p + 128 * q);
@@ -573,10 +606,10 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
 #pragma unroll
                 for (int q = 0; q < kVectors / 32; ++q) {
                     const int at_v = l + 32 * q, v = at_v % VR;
-                    const int64_t row = row0 + at_v / VR;
-                    const Cutout k = cutout(row, seg, r0);
+                    const int64_t row = ahead.row0 + at_v / VR;
+                    const Cutout k = SUB == 32 ? mine : cutout(row, static_cast<Count>(ahead.end), ahead_r0);
                     if (v < k.lo || v >= k.lo + k.n) continue;
-                    const int64_t t = 4 * (k.v0 + v) - k.shift;
+                    const Count t = 4 * (k.v0 + v) - k.shift;
                     const bool whole = t >= 0 && t + 3 < a.T;
 #pragma unroll
                     for (int arr = 0; arr < NA; ++arr) {
@@ -595,23 +628,22 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
                     }
                 }
             }
-            const int64_t row = row0 + sr;
+            const int64_t row = ahead.row0 + sr;
             if (ls == 0 && row < a.lanes) {
                 if (PASS == ONLY && ahead_step == 0 && a.in[SI_CARRY].p)
                     copy_async<4>(smem_addr(&tile.carry[stage][sr]), a.in[SI_CARRY].p + row * a.in[SI_CARRY].so);
-                if (want_gate) {
-                    const Cutout k = SUB == 32 ? first : cutout(row, seg, r0);
-                    const int64_t t = 4 * (k.v0 + k.lo) - k.shift - 1;  // before the tile's first step in memory
-                    if (k.n > 0 && t >= 0) copy_async<4>(smem_addr(&tile.before[stage][sr]), a.in[SI_H].p + row * a.in[SI_H].so + t * a.in[SI_H].st);
-                    if (k.n > 0 && t < 0 && a.in[SI_INIT].p)
-                        copy_async<4>(smem_addr(&tile.init[stage][sr]), a.in[SI_INIT].p + row * a.in[SI_INIT].so);
+                if (want_gate && mine.n > 0) {
+                    const int64_t t = at_t + 4 * mine.lo - 1;  // before the tile's first step in memory
+                    if (t >= 0) copy_async<4>(smem_addr(&tile.before[stage][sr]), a.in[SI_H].p + row * a.in[SI_H].so + t * a.in[SI_H].st);
+                    else if (a.in[SI_INIT].p) copy_async<4>(smem_addr(&tile.init[stage][sr]), a.in[SI_INIT].p + row * a.in[SI_INIT].so);
                 }
             }
-            ahead_r0 += stride;
+            ahead_r0 += static_cast<Count>(stride);
             if (++ahead_step == a.steps) {
                 ahead_step = 0;
-                ahead_r0 = 0;
                 ahead_unit += at.clusters;
+                ahead = rows_of(ahead_unit);
+                ahead_r0 = static_cast<Count>(ahead.begin + own);
             }
         }
         copies_commit();
@@ -623,18 +655,19 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
     const int run = (BACKWARD ? SUB - 1 - ls : ls) * kRun;  // this thread's run within its row's tile
     int stage = 0;
     for (int64_t unit = at.first; unit < a.units; unit += at.clusters) {
-        const int seg = static_cast<int>(unit % a.segments);
-        const int64_t row0 = first_row(unit), row = row0 + sr;
+        const Rows here = rows_of(unit);
+        const int seg = here.seg;
+        const int64_t row0 = here.row0, row = row0 + sr;
         const bool live = row < a.lanes;
         float c = 0.0f, gates = 1.0f;
         if constexpr (PASS == JOINED) {
             if (live && a.in[SI_CARRY].p) c = __ldg(a.in[SI_CARRY].p + row * a.in[SI_CARRY].so);
             c = segment_state<1>(a, ex, seg, row, live, c, warp, 0, l == 0);
         }
-        for (int k = 0; k < a.steps; ++k, stage ^= 1) {
-            const int64_t r0 = seg * a.seg_len + own + k * stride;
-            const Cutout cut = cutout(row, seg, r0);
-            const int64_t t0 = 4 * cut.v0 - cut.shift + run;  // the run's first step in memory
+        Count r0 = static_cast<Count>(here.begin + own);
+        for (int k = 0; k < a.steps; ++k, stage ^= 1, r0 += static_cast<Count>(stride)) {
+            const Cutout cut = cutout(row, static_cast<Count>(here.end), r0);
+            const Count t0 = 4 * cut.v0 - cut.shift + run;  // the run's first step in memory
             copies_wait_one();
             __syncwarp();
             const float* in = &tile.in[stage][0][sr * SUB * kRun + run];
@@ -725,9 +758,9 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
                 for (int u = 0; u < kVectors / 32; ++u) {
                     const int at_v = l + 32 * u, v = at_v % VR;
                     const int64_t r = row0 + at_v / VR;
-                    const Cutout e = SUB == 32 ? cut : cutout(r, seg, r0);
+                    const Cutout e = SUB == 32 ? cut : cutout(r, static_cast<Count>(here.end), r0);
                     if (v < e.lo || v >= e.lo + e.n) continue;
-                    const int64_t t = 4 * (e.v0 + v) - e.shift;
+                    const Count t = 4 * (e.v0 + v) - e.shift;
                     float f[4];
                     load_shared<4>(&tile.out[4 * at_v], f);
                     if (t >= 0 && t + 3 < a.T) {
@@ -856,8 +889,9 @@ Cut cut(const ScanDesc& d) {
         return c;
     }
     const int64_t len = c.rows ? (d.T + 6) / 4 : d.T;  // rows count time in vectors of four
-    while (c.rows && c.sub > 4 && len <= c.sub / 2 * kRun / 4) c.sub /= 2;
-    if (c.rows) c.tile = c.sub * kRun / 4;
+    const int run = d.backward ? kRowRun<true> : kRowRun<false>;
+    while (c.rows && c.sub > 4 && len <= c.sub / 2 * run / 4) c.sub /= 2;
+    if (c.rows) c.tile = c.sub * run / 4;
     auto warps = [&](int64_t t) {  // along time
         int w = 1;
         while (w < NW && w * t < len) w *= 2;
