@@ -516,10 +516,10 @@ constexpr int kRowRun = BACKWARD ? 12 : 20;
 
 template <bool BACKWARD>
 struct RowTile {
-    float in[2][kArrays<BACKWARD>][32 * kRowRun<BACKWARD>];
+    float in[2][2][32 * kRowRun<BACKWARD>];                     // gate, x
+    float h[BACKWARD ? 2 : 1][BACKWARD ? 32 * (kRowRun<BACKWARD> + 4) : 4];  // [stage]: rows apart by 4, for [-1]
     float out[32 * kRowRun<BACKWARD>];
-    float before[2][8];  // [stage][row]: backward, the state before the tile's first step in memory
-    float carry[2][8], init[2][8];
+    float carry[2][8];
 };
 template <bool BACKWARD>
 constexpr size_t rows_smem() {
@@ -583,6 +583,7 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
     auto whole_tile = [&](const Cutout& q) {
         return q.n == VR && 4 * q.v0 >= q.shift && 4 * (q.v0 + VR) - q.shift <= a.T;
     };
+    auto h_row = [&](int stage, int r) { return &tile.h[BACKWARD ? stage : 0][BACKWARD ? 4 + r * (SUB * kRun + 4) : 0]; };
     const int need = 1 << SI_GATE | (a.in[SI_X].p ? 1 << SI_X : 0) | (want_gate ? 1 << SI_H : 0);
     int64_t ahead_unit = at.first;
     Rows ahead = rows_of(ahead_unit);
@@ -593,17 +594,17 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
             const Cutout mine = cutout(ahead.row0 + sr, static_cast<Count>(ahead.end), ahead_r0);
             const int64_t at_t = 4 * static_cast<int64_t>(mine.v0) - mine.shift;
             if (SUB == 32 && whole_tile(mine) && (a.vec & need) == need) {
-                auto copy = [&](int op, int arr) {
+                auto copy = [&](int op, float* dst) {
                     const float* p = a.in[op].p + ahead.row0 * a.in[op].so + at_t + 4 * l;
-                    const uint32_t to = smem_addr(&tile.in[stage][arr][4 * l]);
+                    const uint32_t to = smem_addr(dst + 4 * l);
 #pragma unroll
                     for (int q = 0; q < kVectors / 32; ++q) copy_async<16>(to + 512 * q, p + 128 * q);
                 };
-                copy(SI_GATE, 0);
-                if (a.in[SI_X].p) copy(SI_X, 1);
-                if (want_gate) copy(SI_H, NA - 1);
+                copy(SI_GATE, tile.in[stage][0]);
+                if (a.in[SI_X].p) copy(SI_X, tile.in[stage][1]);
+                if (want_gate) copy(SI_H, h_row(stage, 0));
             } else {
-#pragma unroll
+#pragma unroll 1
                 for (int q = 0; q < kVectors / 32; ++q) {
                     const int at_v = l + 32 * q, v = at_v % VR;
                     const int64_t row = ahead.row0 + at_v / VR;
@@ -617,7 +618,7 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
                         if (arr == 1 && !a.in[SI_X].p) continue;
                         if (arr == 2 && !want_gate) continue;
                         const float* p = a.in[op].p + row * a.in[op].so;
-                        const uint32_t to = smem_addr(&tile.in[stage][arr][4 * at_v]);
+                        const uint32_t to = smem_addr(arr == 2 ? h_row(stage, at_v / VR) + 4 * v : &tile.in[stage][arr & 1][4 * at_v]);
                         if ((a.vec >> op & 1) && whole) {
                             copy_async<16>(to, p + t);
                         } else {
@@ -633,9 +634,12 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
                 if (PASS == ONLY && ahead_step == 0 && a.in[SI_CARRY].p)
                     copy_async<4>(smem_addr(&tile.carry[stage][sr]), a.in[SI_CARRY].p + row * a.in[SI_CARRY].so);
                 if (want_gate && mine.n > 0) {
-                    const int64_t t = at_t + 4 * mine.lo - 1;  // before the tile's first step in memory
-                    if (t >= 0) copy_async<4>(smem_addr(&tile.before[stage][sr]), a.in[SI_H].p + row * a.in[SI_H].so + t * a.in[SI_H].st);
-                    else if (a.in[SI_INIT].p) copy_async<4>(smem_addr(&tile.init[stage][sr]), a.in[SI_INIT].p + row * a.in[SI_INIT].so);
+                    // the state before the tile's first step in memory, in front of it: init before t = 0
+                    const int64_t t = at_t + 4 * mine.lo;
+                    float* dst = h_row(stage, sr) + 4 * mine.lo + (t < 0 ? -static_cast<int>(t) : 0) - 1;
+                    if (t > 0) copy_async<4>(smem_addr(dst), a.in[SI_H].p + row * a.in[SI_H].so + (t - 1) * a.in[SI_H].st);
+                    else if (a.in[SI_INIT].p) copy_async<4>(smem_addr(dst), a.in[SI_INIT].p + row * a.in[SI_INIT].so);
+                    else *dst = 0.0f;
                 }
             }
             ahead_r0 += static_cast<Count>(stride);
@@ -670,36 +674,50 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
             const Count t0 = 4 * cut.v0 - cut.shift + run;  // the run's first step in memory
             copies_wait_one();
             __syncwarp();
-            const float* in = &tile.in[stage][0][sr * SUB * kRun + run];
+            if (SUB == 32 && cut.n == 0) {  // the axis ended before this warp's tile
+                if (PASS == ONLY && k == 0) c = a.in[SI_CARRY].p && live ? tile.carry[stage][0] : 0.0f;
+                __syncwarp();
+                issue(stage);
+                const float s = joiner.first(make_float2(1.0f, 0.0f), c, k == 0, l == 0);
+                if constexpr (PASS == MAPS) {
+                    joiner.gates_of_step(gates);
+                    if (k + 1 == a.steps && live && wt == W - 1 && l == 0) a.maps[seg * a.lanes + row] = make_float2(gates, s);
+                }
+                joiner.hand_on(s, k + 1 == a.steps, l == 0);
+                continue;
+            }
+            const int at_run = sr * SUB * kRun + run;
             float ga[kRun], xv[kRun], hv[BACKWARD ? kRun : 1];
 #pragma unroll
             for (int j = 0; j < kRun; j += 4) {
-                load_shared<4>(in + j, ga + j);
-                load_shared<4>(in + kTile + j, xv + j);
+                load_shared<4>(&tile.in[stage][0][at_run + j], ga + j);
+                load_shared<4>(&tile.in[stage][1][at_run + j], xv + j);
             }
             if constexpr (BACKWARD) {
                 if (want_gate) {  // the state before each step
+                    const float* q = h_row(stage, sr) + run;
                     float h[kRun];
 #pragma unroll
-                    for (int j = 0; j < kRun; j += 4) load_shared<4>(in + 2 * kTile + j, h + j);
-                    hv[0] = run > 4 * cut.lo ? in[2 * kTile - 1] : tile.before[stage][sr];
+                    for (int j = 0; j < kRun; j += 4) load_shared<4>(q + j, h + j);
+                    hv[0] = q[-1];
 #pragma unroll
                     for (int j = 1; j < kRun; ++j) hv[j] = h[j - 1];
                 }
             }
-            // the row's ends: steps outside it leave the state as it is
-            const bool whole = cut.n == VR && t0 >= (BACKWARD ? 1 : 0) && t0 + kRun <= a.T && a.in[SI_X].p;
-            if (!whole) {
-                const float init = want_gate && a.in[SI_INIT].p ? tile.init[stage][sr] : 0.0f;
+            // steps [in0, in1) of the run are inside the tile and the row: the others leave the state as it is
+            const int in0 = max(4 * cut.lo - run, t0 < 0 ? static_cast<int>(max(t0, static_cast<Count>(-kRun))) * -1 : 0);
+            const int in1 = min(4 * (cut.lo + cut.n) - run, static_cast<int>(min(static_cast<Count>(a.T) - t0, static_cast<Count>(kRun))));
+            if (in0 > 0 || in1 < kRun) {
 #pragma unroll
                 for (int j = 0; j < kRun; ++j) {
-                    const int v = (run + j) / 4;
-                    const bool inside = v >= cut.lo && v < cut.lo + cut.n && t0 + j >= 0 && t0 + j < a.T;
-                    if (!inside) ga[j] = 1.0f;
-                    if (!inside || !a.in[SI_X].p) xv[j] = 0.0f;
-                    if (BACKWARD && want_gate && run + j == 4 * cut.lo) hv[BACKWARD ? j : 0] = tile.before[stage][sr];
-                    if (BACKWARD && t0 + j == 0) hv[BACKWARD ? j : 0] = init;
+                    const bool inside = j >= in0 && j < in1;
+                    ga[j] = inside ? ga[j] : 1.0f;
+                    xv[j] = inside ? xv[j] : 0.0f;
                 }
+            }
+            if (!a.in[SI_X].p) {
+#pragma unroll
+                for (int j = 0; j < kRun; ++j) xv[j] = 0.0f;
             }
             if (PASS == ONLY && k == 0) c = a.in[SI_CARRY].p && live ? tile.carry[stage][sr] : 0.0f;
             __syncwarp();
@@ -754,7 +772,7 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
                     __syncwarp();
                     return;
                 }
-#pragma unroll
+#pragma unroll 1
                 for (int u = 0; u < kVectors / 32; ++u) {
                     const int at_v = l + 32 * u, v = at_v % VR;
                     const int64_t r = row0 + at_v / VR;
