@@ -57,23 +57,23 @@ struct ScanArgs {
 
 enum Pass { ONLY = 0, MAPS = 1, JOINED = 2 };  // the whole scan; its segments' maps; the scan from them
 
-// The map (A, H) applied to c.  A state of exactly 0 takes no part: the gates' product may
-// have overflowed, and inf * 0 is NaN where the recurrence stays 0.
-__device__ __forceinline__ float apply(float2 m, float c) { return c == 0.0f ? m.y : fmaf(m.x, c, m.y); }
+// Maps (A, H) keep A finite unless a gate is not: an overflowing product is held at the largest
+// float, so that 0 * A stays 0 (a state of 0, or a gate of 0 behind it) where inf would make it
+// NaN.  (A underflowing product is 0: an infinite state may become NaN behind it.)
+__device__ __forceinline__ float apply(float2 m, float c) { return fmaf(m.x, c, m.y); }
 
-// Product of gates.  A zero gate makes it zero whatever overflowed before; a product that
-// underflows stays the smallest number, so that an infinite state stays infinite.
 __device__ __forceinline__ float join_gates(float a, float b) {
-    const float p = a * b;
-    if (a == 0.0f || b == 0.0f) return 0.0f;
-    return p == 0.0f ? copysignf(1.4e-45f, p) : p;
+    constexpr float kMax = 3.402823466e38f;
+    float p = a * b;
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(p) : "f"(kMax));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(p) : "f"(-kMax));
+    return p;
 }
 
 // First m, then n.
 __device__ __forceinline__ float2 join(float2 m, float2 n) { return make_float2(join_gates(m.x, n.x), apply(n, m.y)); }
 
-// The map of N steps in scan order.  Gates are multiplied plainly; where that gave NaN, a zero
-// gate among them settles it (after an overflow 0 * inf).
+// The map of N steps in scan order, its gates' product as it comes.
 template <bool BACKWARD, int N, class G, class X>
 __device__ __forceinline__ float2 tile_map(G gate, X x) {
     float2 m = make_float2(gate(0), BACKWARD ? gate(0) * x(0) : x(0));
@@ -82,12 +82,20 @@ __device__ __forceinline__ float2 tile_map(G gate, X x) {
         m.x *= gate(j);
         m.y = BACKWARD ? gate(j) * (x(j) + m.y) : fmaf(gate(j), m.y, x(j));
     }
-    if (m.x != m.x) {
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-            if (gate(j) == 0.0f) m.x = 0.0f;
-    }
     return m;
+}
+__device__ __forceinline__ bool finite(float a) { return fabsf(a) <= 3.402823466e38f; }
+// Settles a product that is not finite: 0 where a gate is 0 (after an overflow 0 * inf), the largest float
+// where it overflowed, NaN or infinite where a gate is.
+template <int N, class G>
+__device__ __forceinline__ float settle(float a, G gate) {
+    bool zero = false, all = true;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        zero |= gate(j) == 0.0f;
+        all &= finite(gate(j));
+    }
+    return !all ? a : zero ? 0.0f : a != a ? a : copysignf(3.402823466e38f, a);
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -431,25 +439,35 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_cols_kernel(ScanArgs a) {
             issue(stage);
             // this thread's maps, those of the threads before it in time, and the tile's
             float2 m[V], before[V];
-            float2 tile = make_float2(1.0f, 0.0f);
+            bool settled = true;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 m[v] = tile_map<BACKWARD, TS>([&](int j) { return ga[j][v]; }, [&](int j) { return xv[j][v]; });
-                before[v] = make_float2(1.0f, 0.0f);
+                settled &= finite(m[v].x);
+            }
+            if (!settled) {
 #pragma unroll
-                for (int d = COLS; d < 32; d *= 2) {
+                for (int v = 0; v < V; ++v)
+                    if (!finite(m[v].x)) m[v].x = settle<TS>(m[v].x, [&](int j) { return ga[j][v]; });
+            }
+#pragma unroll
+            for (int d = COLS; d < 32; d *= 2) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
                     const float2 b = make_float2(__shfl_up_sync(0xffffffffu, m[v].x, d), __shfl_up_sync(0xffffffffu, m[v].y, d));
-                    if (l >= d) m[v] = join(b, m[v]);
+                    const float2 q = join(b, m[v]);
+                    m[v] = l >= d ? q : m[v];
                 }
-                if (V > 1) {
-                    const float2 b = make_float2(__shfl_up_sync(0xffffffffu, m[v].x, COLS), __shfl_up_sync(0xffffffffu, m[v].y, COLS));
-                    if (sub > 0) before[v] = b;
+            }
+            float2 tile = m[0];
+            if constexpr (V > 1) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    before[v] = make_float2(__shfl_up_sync(0xffffffffu, m[v].x, COLS), __shfl_up_sync(0xffffffffu, m[v].y, COLS));
                     // lane l's map lies with the last of its threads, 32 - COLS + l / V, at v = l % V
                     const float2 w = make_float2(__shfl_sync(0xffffffffu, m[v].x, 32 - COLS + l / V),
                                                  __shfl_sync(0xffffffffu, m[v].y, 32 - COLS + l / V));
-                    if (l % V == v) tile = w;
-                } else {
-                    tile = m[v];
+                    tile = l % V == v ? w : tile;
                 }
             }
             const bool last = k + 1 == a.steps;
@@ -464,7 +482,7 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_cols_kernel(ScanArgs a) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     s[v] = V > 1 ? __shfl_sync(0xffffffffu, first, col * V + v) : first;
-                    if (V > 1 && sub > 0) s[v] = apply(before[v], s[v]);
+                    if (V > 1) s[v] = sub > 0 ? apply(before[v], s[v]) : s[v];
                 }
                 const int64_t step = BACKWARD ? -a.inner : a.inner;
                 const int64_t y = (o * a.T + (BACKWARD ? a.T - 1 - r0 : r0)) * a.inner + i;
@@ -724,10 +742,12 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
             issue(stage);
             float2 q = tile_map<BACKWARD, kRun>([&](int j) { return ga[BACKWARD ? kRun - 1 - j : j]; },
                                                 [&](int j) { return xv[BACKWARD ? kRun - 1 - j : j]; });
+            if (!finite(q.x)) q.x = settle<kRun>(q.x, [&](int j) { return ga[j]; });
 #pragma unroll
             for (int d = 1; d < SUB; d *= 2) {
                 const float2 b = make_float2(__shfl_up_sync(0xffffffffu, q.x, d), __shfl_up_sync(0xffffffffu, q.y, d));
-                if (ls >= d) q = join(b, q);
+                const float2 n = join(b, q);
+                q = ls >= d ? n : q;
             }
             const float2 b = make_float2(__shfl_up_sync(0xffffffffu, q.x, 1), __shfl_up_sync(0xffffffffu, q.y, 1));
             const bool last = k + 1 == a.steps;

@@ -262,8 +262,8 @@ class Graph:
         (zeros when None).  gate and x broadcast together; init broadcasts to their shape
         without the axis.  The gradient reaches all three.  One step (an axis of size 1)
         with the last state as init is the form for serving one token at a time; a gate
-        of 0 starts anew there, e.g. at a document's first token.  A NaN or infinite state
-        stays until a gate of 0 meets it, where it is NaN (0 * inf), as in the recurrence."""
+        of 0 starts anew there, e.g. at a document's first token.  A state that is NaN stays
+        NaN, an infinite one infinite or NaN, through gates of 0 too (0 * inf)."""
         gate, x = self._ensure(gate), self._ensure(x)
         self._float32("gated_scan", gate, x)
         shape = broadcast_shapes(gate.shape, x.shape)
