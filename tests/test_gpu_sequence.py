@@ -49,11 +49,12 @@ def _check_scan(cache_dir, shape, axis, init=True, seed=0, gate_shape=None, flag
     R.assert_within(out[1], rlast)
     if gate_shape is None:
         R.assert_within(out[2], rg[0])
-    else:  # summed over the axes the gate was broadcast along, in double, rounded once
+    else:  # summed over the axes the gate was broadcast along: adjacent lanes 32 at a time by a tree (five
+        # additions deep), the rest in double, each rounded to float32 once: at most 7 roundings a term
         v, tol = rg[0]
         ax = tuple(i for i in range(len(shape)) if gate_shape[i] != shape[i])
         sv = v.sum(ax, keepdims=True)
-        R.assert_within(out[2], (sv, tol.sum(ax, keepdims=True) + 2 * R.U * np.abs(v).sum(ax, keepdims=True)))
+        R.assert_within(out[2], (sv, tol.sum(ax, keepdims=True) + 7 * R.U * np.abs(v).sum(ax, keepdims=True)))
     R.assert_within(out[3], rg[1])
     if init:
         R.assert_within(out[4], rg[2])
@@ -81,6 +82,15 @@ def test_scan_shapes(cache_dir, shape, axis):
 @pytest.mark.parametrize("gate_shape", [[3, 50, 4, 1], [1, 1, 4, 8], [3, 50, 1, 8], [1, 1, 1, 1], [3, 1, 4, 1], [1, 50, 1, 1]])
 def test_scan_broadcast_gates(cache_dir, gate_shape):
     _check_scan(cache_dir, [3, 50, 4, 8], 1, gate_shape=gate_shape, seed=5)
+
+
+@pytest.mark.parametrize("shape,gate_shape,axis", [
+    ([2, 40, 3, 32], [2, 40, 3, 1], 1), ([2, 300, 2, 64], [2, 300, 2, 1], 1), ([1, 17, 5, 96], [1, 17, 5, 1], 1),
+    ([2, 33, 3, 2], [2, 33, 3, 1], 1), ([2, 33, 3, 4], [2, 33, 3, 1], 1), ([3, 33, 1, 16], [3, 33, 1, 1], 1),
+    ([2, 50, 128], [2, 50, 1], 1), ([2, 50, 2, 2, 16], [2, 50, 2, 1, 1], 1), ([2, 50, 3, 5], [2, 50, 3, 1], 1),
+    ([50, 3, 64], [50, 3, 1], 0), ([2, 5, 3, 64], [2, 5, 3, 1], 1), ([1, 9000, 64], [1, 9000, 1], 1)])
+def test_scan_shared_gates(cache_dir, shape, gate_shape, axis):
+    _check_scan(cache_dir, shape, axis, gate_shape=gate_shape, seed=sum(shape))
 
 
 def test_scan_without_fusion(cache_dir):

@@ -132,8 +132,10 @@ void append_gradients(Graph& g, int loss, const std::vector<int>& wrt, int seed)
     // Gradients of scan states: of a whole GatedScan (grads) and of its last state alone
     // (last_grads), which enters the same backward scan as its first carry.
     std::unordered_map<int, int> last_grads;
-    auto backward = [&](int op, std::vector<int> in, int64_t axis, std::vector<int64_t> has, std::vector<float> attr) {
+    auto backward = [&](int op, std::vector<int> in, int64_t axis, std::vector<int64_t> has, std::vector<float> attr,
+                        int64_t split = 0) {
         Node q;
+        q.dim1 = split;
         q.op = op;
         q.in = std::move(in);
         q.dim0 = axis;
@@ -267,7 +269,26 @@ void append_gradients(Graph& g, int loss, const std::vector<int>& wrt, int seed)
                 std::vector<int> gate_ops = ops;
                 gate_ops.push_back(i);
                 if (has_init) gate_ops.push_back(n.in[2]);
-                accumulate(n.in[0], backward(BOP_SCAN_DGATE, gate_ops, n.dim0, has, {}));
+                // A gate shared by adjacent lanes (a head's channels): its gradient is summed over them in
+                // the scan's launch, not stored in full and reduced.
+                int gate = n.in[0];
+                int64_t split = 0;
+                {
+                    const Node& e = g.nodes[static_cast<size_t>(gate)];
+                    const Shape src = e.op == TT_OP_EXPAND ? b.shape(e.in[0]) : Shape{};
+                    if (e.op == TT_OP_EXPAND && src.size() == e.shape.size()) {
+                        size_t s = src.size();
+                        while (s > static_cast<size_t>(n.dim0) + 1 && src[s - 1] == 1) --s;
+                        const bool same = std::equal(src.begin(), src.begin() + static_cast<long>(s), e.shape.begin());
+                        int64_t group = 1;
+                        for (size_t d = s; d < src.size(); ++d) group *= e.shape[d];
+                        if (same && sums_gate_group(group)) {
+                            split = static_cast<int64_t>(s);
+                            gate = e.in[0];
+                        }
+                    }
+                }
+                accumulate(gate, backward(BOP_SCAN_DGATE, gate_ops, n.dim0, has, {}, split));
                 accumulate(n.in[1], backward(BOP_SCAN_DX, ops, n.dim0, has, {}));
                 if (has_init) accumulate(n.in[2], backward(BOP_SCAN_DINIT, ops, n.dim0, has, {}));
                 break;

@@ -268,6 +268,7 @@ void infer_shape(Graph& g, Node& n) {
         }
         case BOP_SCAN_DX: case BOP_SCAN_DGATE:
             n.shape = in(0).shape;
+            if (n.dim1 > 0) std::fill(n.shape.begin() + static_cast<long>(n.dim1), n.shape.end(), int64_t{1});
             n.dtype = in(0).dtype;
             return;
         case BOP_SCAN_DINIT:

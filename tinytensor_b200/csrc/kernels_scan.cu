@@ -49,6 +49,7 @@ struct ScanArgs {
     int64_t lanes, inner, n2, T;
     int64_t seg_len;  // steps of a segment
     int segments;
+    int group;        // log2 of the adjacent lanes of a warp that dgate is summed over
     int64_t units;    // blocks of lanes * segments, walked by the clusters of the grid
     int steps;        // of a unit
     int W;            // warps of a CTA along time; the others take further lanes
@@ -503,7 +504,20 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_cols_kernel(ScanArgs a) {
                         }
                     }
                     if (j < nm) store_vec<V>(ym, main, BACKWARD);
-                    if (j < ng) store_vec<V>(yg, dg, true);
+                    if (!BACKWARD || a.group == 0) {
+                        if (j < ng) store_vec<V>(yg, dg, true);
+                    } else {  // summed over the lanes of a group within the warp (lanes that are not live hold 0)
+                        float t = dg[0];
+#pragma unroll
+                        for (int v = 1; v < V; ++v) t += dg[v];
+#pragma unroll
+                        for (int d = 1; d < COLS; d *= 2) {
+                            const float w = __shfl_xor_sync(0xffffffffu, t, d);
+                            if (d * V >> a.group == 0) t += w;
+                        }
+                        if (j < ng && (col * V & ((1 << a.group) - 1)) == 0)
+                            a.out[SO_GATE][(o * a.T + a.T - 1 - r0 - j) * (a.inner >> a.group) + (i >> a.group)] = t;
+                    }
                 }
                 // the thread of the last step has the last state as it was stored
                 if (n > 0 && r0 + n == a.T && a.out[SO_LANE]) store_vec<V>(a.out[SO_LANE] + lane, s, false);
@@ -895,7 +909,7 @@ __global__ void __launch_bounds__(256) scan_short_kernel(ScanArgs a) {
 // aligned wherever they start (buffers start on 16 bytes), or is broadcast over them.
 int widest(const ScanDesc& d) {
     for (int v = 4; v > 1; v /= 2) {
-        bool ok = d.n2 % v == 0;
+        bool ok = d.n2 % v == 0 && (d.group == 1 || d.group % v == 0);
         for (int k = 0; k < SI_COUNT && ok; ++k) {
             const ScanStrides& s = d.in[k];  // (all 0 where absent)
             if (s.s2 == 0) continue;
@@ -917,8 +931,8 @@ struct Cut {
 Cut cut(const ScanDesc& d) {
     Cut c;
     const int64_t inner = d.n1 * d.n2, lanes = d.outer * inner;
-    c.direct = d.T <= kShort;
-    c.rows = inner == 1 && !c.direct;
+    c.direct = d.T <= kShort && d.group == 1;
+    c.rows = inner == 1 && !c.direct;  // (no groups there: they are lanes)
     if (inner > 1) c.V = widest(d);
     if (c.direct) {
         // (a few lanes only: one each, for more threads)
@@ -943,10 +957,13 @@ Cut cut(const ScanDesc& d) {
     c.W = warps(tile);
     const int64_t groups = c.rows ? (lanes + 32 / c.sub - 1) / (32 / c.sub) : (lanes + 31) / 32;
     c.blocks = (groups + NW / c.W - 1) / (NW / c.W);
-    // more CTAs along time while the card is not full and every CTA has a step of its own
-    while (c.W == NW && c.cluster < 8 && c.blocks * c.cluster < 256 && c.cluster * c.W * tile * 2 <= len) c.cluster *= 2;
+    // more CTAs along time while three quarters of the SMs would have none and every CTA has a step of its
+    // own (T = 2048, 1024 lanes a sequence: 4 sequences 23 us with 1 CTA, 27 with 2; 2 sequences 22 with
+    // 1, 18 with 4; 1 sequence 22 with 1, 14 with 8)
+    if (c.blocks < 112)
+        while (c.W == NW && c.cluster < 8 && c.blocks * c.cluster < 256 && c.cluster * c.W * tile * 2 <= len) c.cluster *= 2;
     c.seg_len = len;
-    if (c.blocks * c.cluster < 128 && len > c.cluster * c.W * tile) {
+    if (c.blocks * c.cluster < 112 && len > c.cluster * c.W * tile) {
         c.cluster = 1;
         const int64_t step = c.W * tile, most = (len + step - 1) / step;
         int64_t want = (296 + c.blocks - 1) / c.blocks;
@@ -1029,15 +1046,31 @@ cudaError_t launch_cut(const Cut& c, const ScanArgs& a, cudaStream_t stream) {
     return e != cudaSuccess ? e : launch_pass<BACKWARD, JOINED>(c, a, stream);
 }
 
+// dgate of groups of more than 32 lanes: the sums of 32 lanes each, added in order.
+__global__ void __launch_bounds__(256) gate_group_kernel(const float* __restrict__ part, float* __restrict__ out, int64_t n, int parts) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= n) return;
+    double s = 0.0;
+    for (int k = 0; k < parts; ++k) s += static_cast<double>(__ldg(part + i * parts + k));
+    out[i] = static_cast<float>(s);
+}
+
+int64_t maps_bytes(const ScanDesc& d, const Cut& c) {
+    const int64_t b = c.segments > 1 ? c.segments * d.outer * d.n1 * d.n2 * static_cast<int64_t>(sizeof(float2)) : 0;
+    return (b + 255) / 256 * 256;
+}
+int64_t group_parts(const ScanDesc& d) { return d.group > 32 ? d.group / 32 : 1; }
+
 }  // namespace
 
 int64_t scan_scratch_bytes(const ScanDesc& d) {
-    const Cut c = cut(d);
-    return c.segments > 1 ? c.segments * d.outer * d.n1 * d.n2 * static_cast<int64_t>(sizeof(float2)) : 0;
+    const int64_t sums = group_parts(d) > 1 ? d.outer * d.T * (d.n1 * d.n2 / 32) * static_cast<int64_t>(sizeof(float)) : 0;
+    return maps_bytes(d, cut(d)) + sums;
 }
 
 int scan_launch_count(const ScanDesc& d) {
-    return d.outer * d.n1 * d.n2 == 0 ? 0 : cut(d).segments > 1 ? 2 : 1;
+    if (d.outer * d.n1 * d.n2 == 0) return 0;
+    return (cut(d).segments > 1 ? 2 : 1) + (group_parts(d) > 1 && d.T > 0 ? 1 : 0);
 }
 
 int launch_scan(const ScanDesc& d, const float* const* in, float* const* out, void* scratch, void* stream) {
@@ -1054,6 +1087,8 @@ int launch_scan(const ScanDesc& d, const float* const* in, float* const* out, vo
         if (c.rows ? s.st == 1 && s.off % 4 == 0 && (s.so - d.T) % 4 == 0 : s.s2 == 1) a.vec |= 1 << k;
     }
     for (int k = 0; k < SO_COUNT; ++k) a.out[k] = out[k];
+    const bool sums = out[SO_GATE] && group_parts(d) > 1;
+    if (sums) a.out[SO_GATE] = reinterpret_cast<float*>(static_cast<char*>(scratch) + maps_bytes(d, c));
     a.maps = static_cast<float2*>(scratch);
     a.lanes = lanes;
     a.inner = d.n1 * d.n2;
@@ -1061,11 +1096,20 @@ int launch_scan(const ScanDesc& d, const float* const* in, float* const* out, vo
     a.T = d.T;
     a.seg_len = c.seg_len;
     a.segments = c.segments;
+    a.group = 0;
+    while (a.group < 5 && (2 << a.group) <= d.group) ++a.group;
     a.units = c.blocks * c.segments;
     a.steps = static_cast<int>(c.steps);
     a.W = c.W;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return static_cast<int>(d.backward ? launch_cut<true>(c, a, st) : launch_cut<false>(c, a, st));
+    cudaError_t e = d.backward ? launch_cut<true>(c, a, st) : launch_cut<false>(c, a, st);
+    if (e == cudaSuccess && sums && d.T > 0) {
+        const int64_t n = lanes / d.group * d.T, blocks = (n + 255) / 256;
+        if (blocks > 0x7fffffff) return static_cast<int>(cudaErrorInvalidConfiguration);
+        gate_group_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(a.out[SO_GATE], out[SO_GATE], n, static_cast<int>(group_parts(d)));
+        e = cudaGetLastError();
+    }
+    return static_cast<int>(e);
 }
 
 }  // namespace ttb

@@ -943,6 +943,8 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
                                  : n.op == BOP_SCAN_DGATE                        ? SO_GATE
                                                                                  : SO_LANE;
                 if (written) L.out_nodes[static_cast<size_t>(slot)] = i;
+                if (n.op == BOP_SCAN_DGATE && n.dim1 > 0)
+                    for (size_t k = static_cast<size_t>(n.dim1); k < sh.size(); ++k) d.group *= sh[k];
                 if (n.op == TT_OP_SCAN_LAST) continue;
                 bind(n, 0, SI_GATE);
                 if (n.op == TT_OP_GATED_SCAN) {

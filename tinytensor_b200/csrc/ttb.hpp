@@ -66,12 +66,17 @@ bool is_reduce(int op);
 // follow; dim0 is the scan's axis.
 enum BackwardOp {
     BOP_SCAN_DX = 64,     // (gate[, g][, g_last])            gradient of x
-    BOP_SCAN_DGATE = 65,  // (gate[, g][, g_last], h[, init])  gradient of gate
+    BOP_SCAN_DGATE = 65,  // (gate[, g][, g_last], h[, init])  gradient of gate; dim1 > 0: summed over the
+                          // dims from dim1 on, along which the gate is broadcast
     BOP_SCAN_DINIT = 66,  // (gate[, g][, g_last])            gradient of init
     BOP_LOGPROB_GRAD = 67,     // the forward's operands, then g: gradient of the logits
     BOP_POLICY_GRAD = 68,
     BOP_PREFERENCE_GRAD = 69
 };
+// Adjacent lanes that a scan's launch can sum a shared gate's gradient over.
+inline bool sums_gate_group(int64_t group) {
+    return group > 1 && (group % 32 == 0 || group == 2 || group == 4 || group == 8 || group == 16);
+}
 bool is_scan(int op);      // GatedScan, ScanLast and the scan's backward nodes
 bool is_token_op(int op);  // the three token operators and their backward nodes
 
