@@ -11,7 +11,8 @@
 // can hold is held by a cluster of up to 8, whose parts' (maximum, sum) are joined through
 // distributed shared memory; so are rows that are too few to fill the card.
 // The preference loss's slope depends on all rows of its pair, so its gradient is a second
-// pass, from the rows' m and s, in reverse order: the rows read last are still in L2.
+// pass, from the rows' m and s, in reverse order: the rows read last are still in L2.  Small
+// pairs do both passes in one cluster each.
 // Differences of log-probabilities are formed in double: they decide on which side of a clip border
 // a ratio lies, and a float of p's size is off by more than the ratio should be.
 #include <cooperative_groups.h>
@@ -689,7 +690,19 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
     if (size > 1) cl.sync();  // nobody writes to a CTA that has left
 }
 
-// ---- preference loss: one CTA per pair: z = beta*(S(0) - S(1)), the loss and its slope.
+// ---- preference loss.  A pair's loss and slope from S(0) - S(1), by one thread.
+__device__ __forceinline__ float pair_value(const TokenArgs& a, int64_t n, double diff, bool write) {
+    const double beta = a.f0, eps = a.f1, z = beta * diff;
+    const double e = exp(-fabs(z)), soft = log1p(e);  // soft = -log sigmoid(|z|)
+    // (eps = 0 drops its term: an impossible rejected answer has z = inf and loss 0)
+    if (write && a.y) a.y[n] = static_cast<float>(soft + (z < 0.0 ? -z * (1.0 - eps) : z == z && eps == 0.0 ? 0.0 : z * eps));
+    if (!a.dlogits) return 0.0f;
+    const double up = 1.0 / (1.0 + e), down = e / (1.0 + e);  // sigmoid(|z|), sigmoid(-|z|)
+    const double pos = z < 0.0 ? down : up, neg = z < 0.0 ? up : down;
+    return static_cast<float>(static_cast<double>(a.g.at(n, 0)) * beta * (eps * pos - (1.0 - eps) * neg));
+}
+
+// One CTA per pair, from the rows' stats.
 constexpr int kPair = 256;
 __global__ void __launch_bounds__(kPair) preference_pair_kernel(TokenArgs a) {
     __shared__ double sh[kPair / 32];
@@ -705,14 +718,86 @@ __global__ void __launch_bounds__(kPair) preference_pair_kernel(TokenArgs a) {
     __syncthreads();
     if (threadIdx.x != 0) return;
     for (int w = 1; w < kPair / 32; ++w) v += sh[w];
-    const double beta = a.f0, eps = a.f1, z = beta * v;
-    const double e = exp(-fabs(z)), soft = log1p(e);  // soft = -log sigmoid(|z|)
-    // (eps = 0 drops its term: an impossible rejected answer has z = inf and loss 0)
-    if (a.y) a.y[n] = static_cast<float>(soft + (z < 0.0 ? -z * (1.0 - eps) : z == z && eps == 0.0 ? 0.0 : z * eps));
-    if (a.slopes) {
-        const double up = 1.0 / (1.0 + e), down = e / (1.0 + e);  // sigmoid(|z|), sigmoid(-|z|)
-        const double pos = z < 0.0 ? down : up, neg = z < 0.0 ? up : down;
-        a.slopes[n] = static_cast<float>(static_cast<double>(a.g.at(n, 0)) * beta * (eps * pos - (1.0 - eps) * neg));
+    const float slope = pair_value(a, n, v, true);
+    if (a.slopes) a.slopes[n] = slope;
+}
+
+// A pair in one cluster and one launch: its warps walk the pair's rows, the CTAs' sums of p - ref are
+// joined, and each warp walks its rows again, latest first, for the gradient.
+constexpr int kPairCluster = 8;
+template <int NV>
+__global__ void __launch_bounds__(256, 4) preference_cluster_kernel(TokenArgs a) {
+    __shared__ double warp_sums[8], cta_sums[kPairCluster];
+    __shared__ float sh_slope;
+    cg::cluster_group cl = cg::this_cluster();
+    cl.barrier_arrive();  // every CTA runs before another writes to it
+    const int rank = static_cast<int>(cl.block_rank()), l = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t n = blockIdx.x / kPairCluster, T = a.n1 / 2;
+    const int first = rank * 8 + warp, step = kPairCluster * 8;
+    double sum = 0.0;
+    int64_t i = first;
+    for (; i < a.n1; i += step) {
+        const Row r(a, n * a.n1 + i);
+        if (r.token < 0 || r.token >= a.V) {
+            fill_row(a, r.row, r.token, r.dx, l == 0, l, 32);
+            if (r.token >= 0) sum = __longlong_as_double(0x7ff8000000000000ll);
+            continue;
+        }
+        const RowNumbers k = row_numbers(a, r);
+        Part all{-INFINITY, 0.0f};
+        for (int j = -r.shift; j < a.V; j += 128 * NV) {
+            float v[NV][4];
+#pragma unroll
+            for (int q = 0; q < NV; ++q) load_vec(r.x, j + 4 * (l + 32 * q), a.V, false, v[q]);
+            const Part next = warp_part<NV>(v);
+            const float m = max_nan(all.m, next.m);
+            all.s = all.s * part_weight(all.m, m) + next.s * part_weight(next.m, m);
+            all.m = m;
+        }
+        const double diff = token_logp(k.xk, all) - static_cast<double>(k.ref);
+        sum += i < T ? diff : -diff;
+        if (l == 0 && a.dlogits) write_value(a, r.row, k, all, diff + static_cast<double>(k.ref));
+    }
+    if (l == 0) warp_sums[warp] = sum;
+    __syncthreads();
+    cl.barrier_wait();
+    if (threadIdx.x < kPairCluster) {
+        double v = 0.0;
+        for (int w = 0; w < 8; ++w) v += warp_sums[w];
+        *cl.map_shared_rank(&cta_sums[rank], static_cast<int>(threadIdx.x)) = v;
+    }
+    cl.sync();
+    if (threadIdx.x == 0) {
+        double v = 0.0;
+        for (int q = 0; q < kPairCluster; ++q) v += cta_sums[q];
+        sh_slope = pair_value(a, n, v, rank == 0);
+    }
+    if (!a.dlogits) return;
+    __syncthreads();
+    const float slope = sh_slope;
+    for (i -= step; i >= 0; i -= step) {
+        const Row r(a, n * a.n1 + i);
+        if (r.token < 0 || r.token >= a.V) {
+            const float f = r.token < 0 ? 0.0f : __int_as_float(0x7fc00000), v[4] = {f, f, f, f};
+            const int out = static_cast<int>(reinterpret_cast<uintptr_t>(r.dx) / 4 % 4);
+            for (int j = 4 * l - out; j < a.V; j += 128) store_vec(r.dx, j, a.V, true, v);
+            continue;
+        }
+        // (the warp's own stats: written by lane 0 above)
+        const float m = __ldcg(a.stats + 3 * r.row), c = i < T ? slope : -slope, scale = -c * __ldcg(a.stats + 3 * r.row + 1);
+        for (int j = -r.shift; j < a.V; j += 128 * NV) {
+            float v[NV][4];
+#pragma unroll
+            for (int q = 0; q < NV; ++q) load_vec(r.x, j + 4 * (l + 32 * q), a.V, true, v[q]);
+#pragma unroll
+            for (int q = 0; q < NV; ++q) {
+                const int at = j + 4 * (l + 32 * q);
+#pragma unroll
+                for (int u = 0; u < 4; ++u) v[q][u] = exp_part(v[q][u] - m);
+                grad_vec(v[q], at, r.token, scale, c);
+                store_vec(r.dx, at, a.V, r.dx_vec, v[q]);
+            }
+        }
     }
 }
 
@@ -743,6 +828,18 @@ __global__ void __launch_bounds__(kGrad) preference_grad_kernel(TokenArgs a, int
 }
 
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
+
+// A pair in one cluster (one launch) or all rows, then all pairs, then all rows again (three).
+bool pairs_in_clusters(const TokenDesc& d) {
+    if (d.n0 == 0 || d.n1 == 0 || d.n0 > 0x7fffffff / kPairCluster) return false;
+    // Clusters save two launches where the pairs are small, and a read from memory where the pairs that
+    // run at the same time stay in L2: 64 pairs of 2x64x4096 65 us against 93, 1000 of 2x16x1000 113
+    // against 149; but 8 clusters do not fill the card, and a warp per row is slow on long rows:
+    // 8 of 2x512x16384 669 against 262, 24 of 2x3x41309 109 against 26.
+    const int64_t pair = d.n1 * d.V;
+    if (d.n0 * pair <= 1 << 20) return d.V <= 4096;
+    return d.n0 >= 16 && d.n1 >= 16 && d.V <= 8192 && pair * (d.n0 < 74 ? d.n0 : 74) <= 40000000;
+}
 
 // Launch configuration of `blocks` CTAs in clusters.
 struct Launcher {
@@ -845,7 +942,8 @@ int64_t token_scratch_bytes(const TokenDesc& d) {
 
 int token_launch_count(const TokenDesc& d) {
     const int rows = d.n0 * d.n1 > 0 ? 1 : 0;
-    return d.kind == TK_PREFERENCE ? rows * (d.grad ? 2 : 1) + (d.n0 > 0 ? 1 : 0) : rows;
+    if (d.kind != TK_PREFERENCE) return rows;
+    return pairs_in_clusters(d) ? 1 : rows * (d.grad ? 2 : 1) + (d.n0 > 0 ? 1 : 0);
 }
 
 int launch_token(const TokenDesc& d, const void* const* in, float* y, float* dlogits, void* scratch, int* status,
@@ -877,19 +975,24 @@ int launch_token(const TokenDesc& d, const void* const* in, float* y, float* dlo
     a.f1 = d.f[1];
     a.f2 = d.f[2];
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (pref && pairs_in_clusters(d)) {
+        Launcher l(d.n0 * kPairCluster, 256, 0, kPairCluster, st);
+        if (d.V <= 512) return static_cast<int>(cudaLaunchKernelEx(&l.cfg, preference_cluster_kernel<4>, a));
+        return static_cast<int>(cudaLaunchKernelEx(&l.cfg, preference_cluster_kernel<8>, a));
+    }
+    if (!pref) return a.rows == 0 ? 0 : static_cast<int>(dlogits ? launch_row_kernel<true>(a, st) : launch_row_kernel<false>(a, st));
+    // (rounds of as many pairs as stay in L2 between their two reads were slower: 360 against 257 us for
+    // 8 pairs of 2x512x16384, the launches' ends costing more than the reads)
+    const int64_t per_row = ((a.V + 6) / 4 + kGradVec * kGrad - 1) / (kGradVec * kGrad);
+    if (d.n0 > 0x7fffffff || a.rows * per_row > 0x7fffffff) return static_cast<int>(cudaErrorInvalidConfiguration);
+    if (d.n0 == 0) return 0;
     if (a.rows > 0) {
-        const cudaError_t e = dlogits && !pref ? launch_row_kernel<true>(a, st) : launch_row_kernel<false>(a, st);
+        const cudaError_t e = launch_row_kernel<false>(a, st);
         if (e != cudaSuccess) return static_cast<int>(e);
     }
-    if (pref && d.n0 > 0) {
-        if (d.n0 > 0x7fffffff) return static_cast<int>(cudaErrorInvalidConfiguration);
-        preference_pair_kernel<<<static_cast<unsigned>(d.n0), kPair, 0, st>>>(a);
-        if (dlogits && a.rows > 0) {
-            const int64_t per_row = ((a.V + 6) / 4 + kGradVec * kGrad - 1) / (kGradVec * kGrad);
-            if (a.rows * per_row > 0x7fffffff) return static_cast<int>(cudaErrorInvalidConfiguration);
-            preference_grad_kernel<<<static_cast<unsigned>(a.rows * per_row), kGrad, 0, st>>>(a, static_cast<int>(per_row));
-        }
-    }
+    preference_pair_kernel<<<static_cast<unsigned>(d.n0), kPair, 0, st>>>(a);
+    if (dlogits && a.rows > 0)
+        preference_grad_kernel<<<static_cast<unsigned>(a.rows * per_row), kGrad, 0, st>>>(a, static_cast<int>(per_row));
     return static_cast<int>(cudaGetLastError());
 }
 
