@@ -35,7 +35,7 @@ namespace ttb {
 
 namespace {
 
-constexpr int NW = 8;  // warps of a CTA
+constexpr int kWarps = 8;  // warps of a CTA (16 where lanes are adjacent and few enough for a CTA an SM)
 
 struct Operand {
     const float* p;  // null: absent
@@ -113,7 +113,7 @@ __device__ __forceinline__ void copies_wait_all() { asm volatile("cp.async.wait_
 
 // Maps and states that the tiles of a step exchange.  Double-buffered: a buffer is written
 // again two steps later, after a barrier that every reader passes behind its reads.
-template <int LW>  // lanes of a warp's tile
+template <int NW, int LW>  // warps of the CTA, lanes of a warp's tile
 struct Exchange {
     float2 warp[2][NW][LW];
     // only where W = NW (otherwise one step covers the axis):
@@ -151,8 +151,8 @@ __device__ __forceinline__ void split_lane(const ScanArgs& a, int64_t lane, int6
 // The state before segment `seg` of a lane, from the maps of the segments before it and the lane's
 // first state.  The warps of the CTA (all on the same lanes) join a share of the maps each,
 // loading 8 at a time; LW lanes a warp, `writer` one thread of a lane.
-template <int LW>
-__device__ __forceinline__ float segment_state(const ScanArgs& a, Exchange<LW>& ex, int seg, int64_t lane, bool live,
+template <int NW, int LW>
+__device__ __forceinline__ float segment_state(const ScanArgs& a, Exchange<NW, LW>& ex, int seg, int64_t lane, bool live,
                                                float c, int warp, int l, bool writer) {
     const int share = (seg + NW - 1) / NW, begin = min(seg, warp * share), end = min(seg, begin + share);
     float2 m = make_float2(1.0f, 0.0f);
@@ -175,9 +175,9 @@ __device__ __forceinline__ float segment_state(const ScanArgs& a, Exchange<LW>& 
 
 // A CTA's part in the exchange, one lane per thread: thread l of a warp handles lane l of its
 // tile (LW = 32), or all threads the tile's one row (LW = 1; `writer` is one of them).
-template <int LW>
+template <int NW, int LW>
 struct Joiner {
-    Exchange<LW>& ex;
+    Exchange<NW, LW>& ex;
     const Place& at;
     int W, wt, wr, warp, l;
     int buf = 0;
@@ -277,18 +277,18 @@ __device__ __forceinline__ void store_vec(float* p, const float* v, bool stream)
 template <bool BACKWARD>
 constexpr int kArrays = BACKWARD ? 3 : 2;
 
-template <bool BACKWARD, int TILE>
+template <bool BACKWARD, int TILE, int NW>
 struct ColTile {
     float in[2][kArrays<BACKWARD>][NW][TILE * 32];  // [stage][operand][warp][step][thread][V]
     float carry[2][NW][32];                         // [stage][warp][lane]: a unit's first states
-    Exchange<32> ex;
+    Exchange<NW, 32> ex;
 };
 
-template <bool BACKWARD, int PASS, int V, int TILE>
-__global__ void __launch_bounds__(NW * 32, 2) scan_cols_kernel(ScanArgs a) {
+template <bool BACKWARD, int PASS, int V, int TILE, int NW>
+__global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a) {
     constexpr int TS = TILE / V, COLS = 32 / V, NA = kArrays<BACKWARD>;
     extern __shared__ __align__(16) unsigned char raw[];
-    ColTile<BACKWARD, TILE>& sh = *reinterpret_cast<ColTile<BACKWARD, TILE>*>(raw);
+    ColTile<BACKWARD, TILE, NW>& sh = *reinterpret_cast<ColTile<BACKWARD, TILE, NW>*>(raw);
     const Place at = place();
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, W = a.W;
     const int wt = warp % W, wr = warp / W;
@@ -379,7 +379,7 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_cols_kernel(ScanArgs a) {
     issue(1);
     if (at.size > 1) cg::this_cluster().sync();  // every CTA runs before another writes to it
 
-    Joiner<32> joiner{sh.ex, at, W, wt, wr, warp, l};
+    Joiner<NW, 32> joiner{sh.ex, at, W, wt, wr, warp, l};
     const bool splat_gate = V > 1 && !(a.vec >> SI_GATE & 1), splat_x = V > 1 && !(a.vec >> SI_X & 1);
     const bool splat_h = V > 1 && !(a.vec >> SI_H & 1);
     int stage = 0;
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_cols_kernel(ScanArgs a) {
                 split_lane(a, lane0 + l, oc, ic);
                 c = __ldg(a.in[SI_CARRY].p + oc * a.in[SI_CARRY].so + ic / a.n2 * a.in[SI_CARRY].s1 + ic % a.n2 * a.in[SI_CARRY].s2);
             }
-            c = segment_state<32>(a, sh.ex, seg, lane0 + l, in, c, warp, l, true);
+            c = segment_state<NW, 32>(a, sh.ex, seg, lane0 + l, in, c, warp, l, true);
         }
         int64_t r0 = begin + own;
         for (int k = 0; k < a.steps; ++k, r0 += stride, stage ^= 1) {
@@ -555,7 +555,7 @@ struct RowTile {
 };
 template <bool BACKWARD>
 constexpr size_t rows_smem() {
-    return NW * sizeof(RowTile<BACKWARD>) + sizeof(Exchange<1>);
+    return kWarps * sizeof(RowTile<BACKWARD>) + sizeof(Exchange<kWarps, 1>);
 }
 
 template <bool FIRST, class A, class B>
@@ -568,15 +568,15 @@ struct Select<false, A, B> {
 };
 
 template <bool BACKWARD, int PASS, int SUB>
-__global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
-    constexpr int NA = kArrays<BACKWARD>, kRun = kRowRun<BACKWARD>, kTile = 32 * kRun, kVectors = kTile / 4;
+__global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(ScanArgs a) {
+    constexpr int NW = kWarps, NA = kArrays<BACKWARD>, kRun = kRowRun<BACKWARD>, kTile = 32 * kRun, kVectors = kTile / 4;
     constexpr int R = 32 / SUB, VR = SUB * kRun / 4;  // rows a warp, vectors of a row's tile
     extern __shared__ __align__(16) unsigned char raw[];
     const Place at = place();
     const int warp = threadIdx.x >> 5, l = threadIdx.x & 31, W = a.W;
     const int wt = warp % W, wr = warp / W, sr = l / SUB, ls = l % SUB;  // ls: the thread's place in its row
     RowTile<BACKWARD>& tile = reinterpret_cast<RowTile<BACKWARD>*>(raw)[warp];
-    Exchange<1>& ex = *reinterpret_cast<Exchange<1>*>(raw + NW * sizeof(RowTile<BACKWARD>));
+    Exchange<NW, 1>& ex = *reinterpret_cast<Exchange<NW, 1>*>(raw + NW * sizeof(RowTile<BACKWARD>));
     const bool want_gate = BACKWARD && PASS != MAPS && a.out[SO_GATE];
     const int64_t stride = static_cast<int64_t>(at.size) * W * VR;  // of this warp's tiles, in vectors of four
     const int64_t own = (static_cast<int64_t>(at.rank) * W + wt) * VR;
@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
     issue(0);
     issue(1);
     if (at.size > 1) cg::this_cluster().sync();  // every CTA runs before another writes to it
-    Joiner<1> joiner{ex, at, W, wt, wr, warp, 0};
+    Joiner<NW, 1> joiner{ex, at, W, wt, wr, warp, 0};
     const int run = (BACKWARD ? SUB - 1 - ls : ls) * kRun;  // this thread's run within its row's tile
     int stage = 0;
     for (int64_t unit = at.first; unit < a.units; unit += at.clusters) {
@@ -698,7 +698,7 @@ __global__ void __launch_bounds__(NW * 32, 2) scan_rows_kernel(ScanArgs a) {
         float c = 0.0f, gates = 1.0f;
         if constexpr (PASS == JOINED) {
             if (live && a.in[SI_CARRY].p) c = __ldg(a.in[SI_CARRY].p + row * a.in[SI_CARRY].so);
-            c = segment_state<1>(a, ex, seg, row, live, c, warp, 0, l == 0);
+            c = segment_state<NW, 1>(a, ex, seg, row, live, c, warp, 0, l == 0);
         }
         Count r0 = static_cast<Count>(here.begin + own);
         for (int k = 0; k < a.steps; ++k, stage ^= 1, r0 += static_cast<Count>(stride)) {
@@ -924,7 +924,7 @@ int widest(const ScanDesc& d) {
 // time, segments.
 struct Cut {
     bool rows, direct;
-    int sub = 32, V = 1, tile = 16, W = 1, cluster = 1, segments = 1;
+    int sub = 32, V = 1, tile = 16, warps = kWarps, W = 1, cluster = 1, segments = 1;
     int64_t seg_len = 1, blocks = 0, steps = 0;
 };
 
@@ -946,7 +946,7 @@ Cut cut(const ScanDesc& d) {
     if (c.rows) c.tile = c.sub * run / 4;
     auto warps = [&](int64_t t) {  // along time
         int w = 1;
-        while (w < NW && w * t < len) w *= 2;
+        while (w < kWarps && w * t < len) w *= 2;
         return w;
     };
     auto padded = [&](int64_t t) { return (len + warps(t) * t - 1) / (warps(t) * t) * warps(t) * t; };
@@ -956,12 +956,18 @@ Cut cut(const ScanDesc& d) {
     const int64_t tile = c.tile;
     c.W = warps(tile);
     const int64_t groups = c.rows ? (lanes + 32 / c.sub - 1) / (32 / c.sub) : (lanes + 31) / 32;
-    c.blocks = (groups + NW / c.W - 1) / (NW / c.W);
-    // more CTAs along time while three quarters of the SMs would have none and every CTA has a step of its
-    // own (T = 2048, 1024 lanes a sequence: 4 sequences 23 us with 1 CTA, 27 with 2; 2 sequences 22 with
-    // 1, 18 with 4; 1 sequence 22 with 1, 14 with 8)
+    c.blocks = (groups + kWarps / c.W - 1) / (kWarps / c.W);
+    // More CTAs along time while the blocks leave a quarter of the SMs idle and every CTA has a step of its
+    // own, and only as many as run at the same time (two an SM, in clusters within the GPCs).  T = 2048,
+    // 1024 lanes a sequence: 4 sequences 23 us with 1 CTA, 27 with 2; 2 sequences 22 with 1, 18 with 4;
+    // 1 sequence 22 with 1, 14 with 8.
     if (c.blocks < 112)
-        while (c.W == NW && c.cluster < 8 && c.blocks * c.cluster < 256 && c.cluster * c.W * tile * 2 <= len) c.cluster *= 2;
+        while (c.W == kWarps && c.cluster < 8 && c.blocks * c.cluster * 2 <= (c.cluster < 4 ? 280 : 256) &&
+               c.cluster * c.W * tile * 2 <= len)
+            c.cluster *= 2;
+    // backward, a CTA an SM: 16 warps a CTA, twice the steps in flight (4 x 2048 x 1024: 33 against 38 us;
+    // forward, with 24 steps a tile, 25 against 23)
+    if (d.backward && c.V == 4 && c.W == kWarps && c.blocks >= 112 && c.blocks <= 148 && 16 * tile <= len) c.warps = c.W = 16;
     c.seg_len = len;
     if (c.blocks * c.cluster < 112 && len > c.cluster * c.W * tile) {
         c.cluster = 1;
@@ -976,7 +982,7 @@ Cut cut(const ScanDesc& d) {
     return c;
 }
 
-template <auto Kernel>
+template <auto Kernel, int NW = kWarps>
 cudaError_t launch_kernel(size_t smem, const Cut& c, const ScanArgs& a, cudaStream_t stream) {
     static std::atomic<int> resident[64];  // CTAs that run at the same time, by device; 0: not found yet
     int dev = 0;
@@ -1010,10 +1016,14 @@ cudaError_t launch_kernel(size_t smem, const Cut& c, const ScanArgs& a, cudaStre
 
 template <bool BACKWARD, int PASS, int TILE>
 cudaError_t launch_cols(const Cut& c, const ScanArgs& a, cudaStream_t stream) {
-    constexpr size_t smem = sizeof(ColTile<BACKWARD, TILE>);
-    if (c.V == 4) return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 4, TILE>>(smem, c, a, stream);
-    if (c.V == 2) return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 2, TILE>>(smem, c, a, stream);
-    return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 1, TILE>>(smem, c, a, stream);
+    constexpr size_t smem = sizeof(ColTile<BACKWARD, TILE, kWarps>);
+    if constexpr (PASS == ONLY && BACKWARD) {
+        if (c.warps == 16)
+            return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 4, TILE, 16>, 16>(sizeof(ColTile<BACKWARD, TILE, 16>), c, a, stream);
+    }
+    if (c.V == 4) return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 4, TILE, kWarps>>(smem, c, a, stream);
+    if (c.V == 2) return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 2, TILE, kWarps>>(smem, c, a, stream);
+    return launch_kernel<scan_cols_kernel<BACKWARD, PASS, 1, TILE, kWarps>>(smem, c, a, stream);
 }
 
 template <bool BACKWARD, int PASS>
