@@ -201,7 +201,9 @@ int tt_compile(const tt_graph* g, const tt_compile_options* opt, tt_program** ou
 int tt_program_info(const tt_program* p, int32_t what, char* buf, size_t cap, size_t* needed);
 int tt_program_num_io(const tt_program* p, int32_t* num_inputs, int32_t* num_outputs);
 int tt_program_output_shape(const tt_program* p, int32_t index, int32_t* rank, int64_t* shape);
-/* Runs once.  TT_HOST: inputs/outputs are host pointers; the call copies inputs in,
+/* Runs once.  Runs of one program share its arena: order them (on one stream, or with events);
+ * so are CUDA graphs that hold runs of the same program.  Buffers of a run must not overlap,
+ * except inputs with one another.  TT_HOST: inputs/outputs are host pointers; the call copies inputs in,
  * runs, copies outputs out and synchronises (Executable::run semantics).
  * TT_DEVICE: device pointers; the work is queued on `stream` and the call returns
  * without synchronising (check tt_program_status after a sync). */

@@ -431,6 +431,70 @@ def test_token_operands_as_views(cache_dir):
     R.assert_within(out[1], tuple(np.transpose(v, (1, 0)) for v in want[1]))
 
 
+@pytest.mark.parametrize("V", [41, 1501, 3001, 9001, 40003, 140001])
+def test_rows_that_lie_differently_than_their_gradient(cache_dir, V):
+    """Rows in another order than the gradient's, an odd vocabulary: the two start differently within
+    16 bytes.  Tokens whose order no two strides describe are copied."""
+    rng = np.random.default_rng(V)
+    xv, kv = _f32(2 * rng.standard_normal([3, 2, 2, V])), rng.integers(0, V, [3, 2, 2]).astype(np.int32)
+    kv[1, 0, 1] = -1
+    gv = _f32(rng.standard_normal([2, 3, 2]))
+    g = tt.Graph()
+    x, k, s = g.input(xv.shape), g.input(kv.shape, dtype=tt.int32), g.input(gv.shape)
+    y = tt.token_logprob(tt.transpose(x, 0, 1), tt.transpose(k, 0, 1))  # rows [2, 3, 2]
+    out = [o.numpy() for o in tt.compile_gradients(g, y, [x], outputs=[y], seed=s, cache_dir=cache_dir).run({x: xv, k: kv, s: gv})]
+    want = R.logprob(xv.transpose(1, 0, 2, 3), kv.transpose(1, 0, 2), gv)
+    R.assert_within(out[0], want[0])
+    R.assert_within(out[1], tuple(np.transpose(v, (1, 0, 2, 3)) for v in want[1]))
+    # rows [3, 2] transposed: two strides, read in place
+    g = tt.Graph()
+    x, k, s = g.input([3, 2, V]), g.input([3, 2], dtype=tt.int32), g.input([2, 3])
+    y = tt.token_logprob(tt.transpose(x, 0, 1), tt.transpose(k, 0, 1))
+    xv, kv, gv = xv[:, :, 0], kv[:, :, 0], gv[:, :, 0]
+    out = [o.numpy() for o in tt.compile_gradients(g, y, [x], outputs=[y], seed=s, cache_dir=cache_dir).run({x: xv, k: kv, s: gv})]
+    want = R.logprob(xv.transpose(1, 0, 2), kv.T, gv)
+    R.assert_within(out[0], want[0])
+    R.assert_within(out[1], tuple(np.transpose(v, (1, 0, 2)) for v in want[1]))
+
+
+def test_scan_of_one_sequence(cache_dir):
+    rng = np.random.default_rng(0)
+    for T in (5, 1000, 70001):
+        av, xv = _f32(rng.random([T])), _f32(rng.standard_normal([T]))
+        g = tt.Graph()
+        a, x, s = g.input([T]), g.input([T]), g.input([])
+        h = tt.gated_scan(a, x, init=s, axis=0)
+        out = [o.numpy() for o in tt.compile_gradients(g, tt.sum(h), [a, x, s], outputs=[h], cache_dir=cache_dir)
+               .run({a: av, x: xv, s: 2.0})]
+        R.assert_within(out[0], R.scan(av, xv, np.float32(2.0), 0)[0])
+        for o, r in zip(out[1:], R.scan_grad(av, xv, np.float32(2.0), 0, np.ones([T]), None)):
+            R.assert_within(o, r)
+
+
+def test_scan_last_twice_without_cse(cache_dir):
+    gate, x, s, _, _ = _scan_data([2, 100, 40], 1, True, 3)
+    g = tt.Graph()
+    a, b, c = g.input(gate.shape), g.input(x.shape), g.input(s.shape)
+    h = tt.gated_scan(a, b, init=c)
+    l1, l2 = tt.scan_last(h), tt.scan_last(h)
+    out = [o.numpy() for o in tt.compile(g, [l1 * 1.0, l2, l1], optimize=False, cache_dir=cache_dir).run({a: gate, b: x, c: s})]
+    want = R.scan(gate, x, s, 1)[1]
+    for o in out:
+        R.assert_within(o, want)
+
+
+def test_gradient_of_an_expanded_gate_itself(cache_dir):
+    gate, x, _, dh, _ = _scan_data([2, 50, 3, 64], 1, False, 3, [2, 50, 3, 1])
+    g = tt.Graph()
+    a, b, d = g.input(gate.shape), g.input(x.shape), g.input(dh.shape)
+    h = tt.gated_scan(a, b, axis=1)
+    out = [o.numpy() for o in tt.compile_gradients(g, h, [h.inputs[0], a], outputs=[], seed=d, cache_dir=cache_dir)
+           .run({a: gate, b: x, d: dh})]
+    v, tol = R.scan_grad(gate, x, None, 1, dh, None)[0]
+    R.assert_within(out[0], (v, tol))
+    R.assert_within(out[1], (v.sum(-1, keepdims=True), tol.sum(-1, keepdims=True) + 2 * R.U * np.abs(v).sum(-1, keepdims=True)))
+
+
 def test_gradient_that_needs_the_loss(cache_dir):
     """A loss that is not linear in the values: the gradient has its own launch."""
     rng = np.random.default_rng(5)

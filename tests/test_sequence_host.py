@@ -271,6 +271,39 @@ def test_broadcast_and_transposed_operands_are_not_copied(cache_dir):
     assert _launches(tt.compile(g, [y], cache_dir=cache_dir, flags=HOST))[0] == 2
 
 
+def test_steps_of_scan_and_loss_outputs(cache_dir):
+    g = tt.Graph()
+    a, x, w = g.input([2, 50, 8]), g.input([2, 50, 8]), g.input([8, 40])
+    k, s = g.input([2, 50], dtype=tt.int32), g.input([2, 50])
+    h = tt.gated_scan(a, x)
+    y = tt.token_logprob(h @ w, k)
+    p = tt.compile_gradients(g, y, [w, a], outputs=[y, tt.scan_last(h)], seed=s, cache_dir=cache_dir, flags=HOST)
+    n = _launches(p)[0]
+    out, ins = p.output_steps(), p.input_steps()
+    assert out[1] == 0 and 0 < out[0] < min(out[2], out[3]) and max(out) == n - 1
+    assert ins[3] == ins[4] == out[0] and ins[1] == 0 and ins[0] == out[3]  # tokens, seed, x, gate
+
+
+def test_scan_last_twice_without_cse(cache_dir):
+    g = tt.Graph()
+    a, x = g.input([2, 50, 3]), g.input([2, 50, 3])
+    h = tt.gated_scan(a, x)
+    l1, l2 = tt.scan_last(h), tt.scan_last(h)
+    p = tt.compile(g, [l1 + 1.0, l2, l1], optimize=False, cache_dir=cache_dir, flags=HOST)
+    lines = _launches(p)[1]
+    assert sum("gated_scan" in ln for ln in lines) == 1 and lines[0].count("scan_last") == 1
+
+
+def test_gradient_of_an_expanded_gate_itself(cache_dir):
+    """A gate that is broadcast is a gradient target too (the C ABI can name the expand node)."""
+    g = tt.Graph()
+    a, x, d = g.input([2, 50, 3, 1]), g.input([2, 50, 3, 64]), g.input([2, 50, 3, 64])
+    h = tt.gated_scan(a, x, axis=1)
+    p = tt.compile_gradients(g, h, [h.inputs[0], a], outputs=[], seed=d, cache_dir=cache_dir, flags=HOST)
+    assert any("gated_scan_dgate" in ln for ln in _launches(p)[1])
+    assert p.output_shapes == [[2, 50, 3, 64], [2, 50, 3, 1]]
+
+
 def test_equal_nodes_merge_only_with_equal_numbers(cache_dir):
     g, x, k = _loss_graph()
     f = g.input([2, 3])

@@ -276,7 +276,8 @@ void append_gradients(Graph& g, int loss, const std::vector<int>& wrt, int seed)
                 {
                     const Node& e = g.nodes[static_cast<size_t>(gate)];
                     const Shape src = e.op == TT_OP_EXPAND ? b.shape(e.in[0]) : Shape{};
-                    if (e.op == TT_OP_EXPAND && src.size() == e.shape.size()) {
+                    // (not where the expanded gate itself is a gradient target)
+                    if (e.op == TT_OP_EXPAND && src.size() == e.shape.size() && std::find(wrt.begin(), wrt.end(), gate) == wrt.end()) {
                         size_t s = src.size();
                         while (s > static_cast<size_t>(n.dim0) + 1 && src[s - 1] == 1) --s;
                         const bool same = std::equal(src.begin(), src.begin() + static_cast<long>(s), e.shape.begin());

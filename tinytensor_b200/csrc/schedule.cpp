@@ -376,6 +376,13 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
                 if (is_elementwise(n.op)) {
                     if (stored[i]) p.st[i] = make_root(i);
                     else p.st[i].kind = SK_REG;
+                } else if (n.op == TT_OP_SCAN_LAST) {  // one buffer for all scan_last nodes of a scan
+                    p.st[i] = make_root(i);
+                    for (int k : users[static_cast<size_t>(n.in[0])])
+                        if (g.nodes[static_cast<size_t>(k)].op == TT_OP_SCAN_LAST && k < static_cast<int>(i)) {
+                            p.st[i] = p.st[static_cast<size_t>(k)];
+                            break;
+                        }
                 } else if (is_scan(n.op) || is_token_op(n.op)) {
                     p.st[i] = make_root(i);
                 } else {
@@ -715,6 +722,7 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
             bool stored_h = out_pos[static_cast<size_t>(i)] >= 0;
             for (int k : users[static_cast<size_t>(i)]) {
                 if (g.nodes[static_cast<size_t>(k)].op == TT_OP_SCAN_LAST) {
+                    if (p.st[static_cast<size_t>(k)].root != k) continue;  // another one's buffer
                     u.nodes.push_back(k);
                     u.writes.push_back(k);
                 } else {
