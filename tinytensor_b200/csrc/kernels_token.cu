@@ -70,7 +70,7 @@ struct Part {
 // exp(d), d <= 0, as 2^(d log2 e): two instructions instead of a library exp, which made these
 // kernels issue-bound (37 instructions a value; now about 10).  Relative error 2^-22.5 from ex2
 // and at most 2.25 |d| 2^-24 from rounding d, the product and the constant; results below the
-// normal range become 0.
+// normal range become 0.  Sums of values use exp_sum below instead.
 __device__ __forceinline__ float exp2_part(float d) {
     float e;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d));
@@ -78,8 +78,9 @@ __device__ __forceinline__ float exp2_part(float d) {
 }
 __device__ __forceinline__ float exp_part(float d) { return exp2_part(d * 1.44269504f); }
 
-// exp(a - b) for the maxima of a part and a whole: 0 for a part of -inf alone, whose sum is 0 too
+// exp(a - b) for the maxima of a part and a whole: 0 for a part of -inf alone
 __device__ __forceinline__ float part_weight(float m, float whole) { return m == -INFINITY ? 0.0f : exp_part(m - whole); }
+__device__ __forceinline__ float part_weight_exact(float m, float whole) { return m == -INFINITY ? 0.0f : expf(m - whole); }
 
 // What a row's scalars are formed from: the token's logit and the row's operands.
 struct RowNumbers {
@@ -175,13 +176,17 @@ __device__ __forceinline__ RowNumbers row_numbers(const TokenArgs& a, const Row&
 }
 
 // The token's log-probability.  log s of s = 2^k f, 0.75 <= f < 1.5, is k log 2 (in double) + logf(f):
-// |log f| < 0.41, so that float is off by 3e-8 at most, where logf(s) would be by 1e-6.
+// |log f| < 0.41, so that float is off by 3e-8 at most, where logf(s) would be by 1e-6.  The
+// preference loss, which sums many of them, takes a double log.
 __device__ __forceinline__ double token_logp(float xk, Part all) {
     const int bits = __float_as_int(all.s), k = (bits - 0x3f400000) >> 23;
     const double log_s = bits >= 0x00800000 && bits < 0x7f800000
                              ? k * 0.69314718055994530942 + static_cast<double>(logf(__int_as_float(bits - (k << 23))))
                              : static_cast<double>(logf(all.s));  // 0 (a row of -inf), inf, NaN
     return static_cast<double>(xk) - static_cast<double>(all.m) - log_s;
+}
+__device__ __forceinline__ double token_logp_exact(float xk, Part all) {
+    return static_cast<double>(xk) - static_cast<double>(all.m) - log(static_cast<double>(all.s));
 }
 
 // The gradient's factor c = g * d value / d p.  Ratios are expf of differences formed in double
@@ -259,9 +264,39 @@ __device__ __forceinline__ Pair operator*(Pair a, Pair b) {
     return r;
 }
 
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
+// exp(d) of two d <= 0, for sums without a gradient.  exp2_part's mean error is not 0 (about 4e-8
+// with its constant's), which all rows share and the preference loss adds up over a sequence's
+// tokens: an answer against an empty one was off by 1.3e-6, four times what it is with these.
+// d log2 e = n + f, |f| <= 1/2: n is rounded off by adding 1.5 * 2^23, f is formed by fused
+// multiply-adds with log2 e in two floats, 2^f is its interpolant of degree 6 at the Chebyshev
+// points of [-1/2, 1/2] (2.5e-9; 7.6e-8 with its roundings, whose mean is 1e-9), and n is added to
+// the exponent.  d below -87.3 (-inf: outside the row) counts as that: at most 2^30 terms of
+// 2^-126 beside a term of 1.  NaN and infinite maxima are the caller's.
+__device__ __forceinline__ Pair exp_sum(Pair d) {
+    float2 h = halves(d);
+    d = pair(fmaxf(h.x, -87.3f), fmaxf(h.y, -87.3f));
+    const Pair log2e = pair(1.44269502f, 1.44269502f), rest = pair(1.92596300e-8f, 1.92596300e-8f);
+    const Pair magic = pair(12582912.0f, 12582912.0f), n = fma(d, log2e, magic);
+    const Pair f = fma(d, rest, fma(d, log2e, fma(n, pair(-1.0f, -1.0f), magic)));
+    Pair y = pair(1.54614449e-4f, 1.54614449e-4f);
+    const float c[6] = {1.0f, 0.693147182f, 0.240226507f, 0.0555032715f, 0.00961805694f, 0.00134004280f};
+#pragma unroll
+    for (int q = 5; q >= 0; --q) y = fma(y, f, pair(c[q], c[q]));
+    const float2 a = halves(y), e = halves(n);
+    return pair(__int_as_float(__float_as_int(a.x) + (__float_as_int(e.x) << 23)),
+                __int_as_float(__float_as_int(a.y) + (__float_as_int(e.y) << 23)));
+}
+
 // The part of a warp from its threads' values: v becomes exp(v - maximum).  Maxima and sums
 // run in four chains a thread: one chain of 32 dependent operations cost more than their number.
-template <int NV>
+// EXACT: for sums without a gradient; v is left as it was.
+template <int NV, bool EXACT>
 __device__ __forceinline__ Part warp_part(float (*v)[4]) {
     float m4[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
 #pragma unroll
@@ -274,6 +309,11 @@ __device__ __forceinline__ Part warp_part(float (*v)[4]) {
     Pair s0 = pair(0.0f, 0.0f), s1 = s0;
 #pragma unroll
     for (int q = 0; q < NV; ++q) {
+        if (EXACT) {
+            s0 = s0 + exp_sum(pair(v[q][0], v[q][1]) + shift);
+            s1 = s1 + exp_sum(pair(v[q][2], v[q][3]) + shift);
+            continue;
+        }
         const float2 a = halves((pair(v[q][0], v[q][1]) + shift) * log2e), b = halves((pair(v[q][2], v[q][3]) + shift) * log2e);
         v[q][0] = exp2_part(a.x);
         v[q][1] = exp2_part(a.y);
@@ -283,15 +323,17 @@ __device__ __forceinline__ Part warp_part(float (*v)[4]) {
         s1 = s1 + pair(v[q][2], v[q][3]);
     }
     const float2 s = halves(s0 + s1);
-    return Part{m, warp_sum(s.x + s.y)};
+    const float sum = warp_sum(s.x + s.y);
+    return Part{m, EXACT ? fmaf(0.0f, from, sum) : sum};  // a maximum of NaN or inf: NaN
 }
 
 // Joins N parts (a multiple of 32 or less than 32), the same in every thread of the warp.
+template <bool EXACT>
 __device__ __forceinline__ Part join_parts(const Part* parts, int n, int l) {
     Part all{-INFINITY, 0.0f};
     for (int q = l; q < n; q += 32) all.m = max_nan(all.m, parts[q].m);
     all.m = warp_max(all.m);
-    for (int q = l; q < n; q += 32) all.s += parts[q].s * part_weight(parts[q].m, all.m);
+    for (int q = l; q < n; q += 32) all.s += parts[q].s * (EXACT ? part_weight_exact(parts[q].m, all.m) : part_weight(parts[q].m, all.m));
     all.s = warp_sum(all.s);
     return all;
 }
@@ -314,7 +356,7 @@ __device__ __forceinline__ void hand_part(Parts& sh, int size, int slot, int l, 
 // ---- short rows: a warp holds a row of at most 128*NV values, 8 rows a CTA.  Without a gradient a
 // row may be longer: the warp walks it, joining maximum and sum as it goes.
 template <int NV, bool GRAD>
-__global__ void __launch_bounds__(256, NV == 16 ? 2 : GRAD ? 4 : 5) token_warp_kernel(TokenArgs a) {
+__global__ void __launch_bounds__(256, NV == 16 ? 2 : GRAD || NV == 8 ? 4 : 5) token_warp_kernel(TokenArgs a) {
     const int l = threadIdx.x & 31;
     const int64_t index = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
     if (index >= a.rows) return;
@@ -327,18 +369,18 @@ __global__ void __launch_bounds__(256, NV == 16 ? 2 : GRAD ? 4 : 5) token_warp_k
     float v[NV][4];
 #pragma unroll
     for (int q = 0; q < NV; ++q) load_vec(r.x, 4 * (l + 32 * q) - r.shift, a.V, GRAD, v[q]);
-    Part all = warp_part<NV>(v);
+    Part all = warp_part<NV, !GRAD>(v);
     if constexpr (!GRAD) {
         for (int j = 128 * NV - r.shift; j < a.V; j += 128 * NV) {
 #pragma unroll
             for (int q = 0; q < NV; ++q) load_vec(r.x, j + 4 * (l + 32 * q), a.V, false, v[q]);
-            const Part next = warp_part<NV>(v);
+            const Part next = warp_part<NV, true>(v);
             const float m = max_nan(all.m, next.m);
-            all.s = all.s * part_weight(all.m, m) + next.s * part_weight(next.m, m);
+            all.s = all.s * part_weight_exact(all.m, m) + next.s * part_weight_exact(next.m, m);
             all.m = m;
         }
     }
-    const double p = token_logp(k.xk, all);
+    const double p = GRAD ? token_logp(k.xk, all) : token_logp_exact(k.xk, all);
     if (l == 0) write_value(a, r.row, k, all, p);
     if (!GRAD) return;
     const float c = row_slope(a, k, p);
@@ -386,21 +428,25 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(TokenArgs a) {
 #pragma unroll
             for (int u = 0; u < 4; ++u) m = max_nan(m, v[q][u]);
         const float from = m == -INFINITY ? 0.0f : m;
-        t.s *= part_weight(t.m, from);
+        const Pair shift = pair(-from, -from);
+        Pair s0 = pair(0.0f, 0.0f), s1 = s0;
 #pragma unroll
-        for (int q = 0; q < kStreamVec; ++q)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) t.s += exp_part(v[q][u] - from);
+        for (int q = 0; q < kStreamVec; ++q) {
+            s0 = s0 + exp_sum(pair(v[q][0], v[q][1]) + shift);
+            s1 = s1 + exp_sum(pair(v[q][2], v[q][3]) + shift);
+        }
+        const float2 s = halves(s0 + s1);
+        t.s = t.s * part_weight_exact(t.m, from) + fmaf(0.0f, from, s.x + s.y);  // a maximum of NaN or inf: NaN
         t.m = m;
     }
     Part w;
     w.m = warp_max(t.m);
-    w.s = warp_sum(t.s * part_weight(t.m, w.m));
+    w.s = warp_sum(t.s * part_weight_exact(t.m, w.m));
     if (size > 1) cl.barrier_wait();
     hand_part(sh, size, rank * (kStream / 32) + warp, l, w);
     if (!GRAD && (warp > 0 || rank > 0)) return;
-    const Part all = join_parts(sh.of, size * (kStream / 32), l);
-    const double p = token_logp(k.xk, all);
+    const Part all = join_parts<true>(sh.of, size * (kStream / 32), l);
+    const double p = token_logp_exact(k.xk, all);
     if (l == 0 && rank == 0 && warp == 0) write_value(a, r.row, k, all, p);
     if (!GRAD) return;
     const float c = row_slope(a, k, p);
@@ -449,8 +495,7 @@ __device__ __forceinline__ void named_sync(int id) { asm volatile("bar.sync %0, 
 // its own to have all of them.  (A cluster barrier instead held every warp of the cluster to the
 // slowest: 3.4 us a row and SM where the bytes take 3.0.)  The wait is bounded: about 2 s, or
 // until another kernel of the program gave up; then status word 0 has a code and the rows' results
-// are wrong.  Nobody writes to a CTA that has left: it leaves after it received the last row's
-// parts of all the others.
+// are wrong.  The cluster leaves together, so that nobody writes to a CTA that has left.
 constexpr int kTimeout = 0x500;
 constexpr long long kWaitBudget = 4000000000LL;  // SM cycles
 __device__ __forceinline__ void exchange_expect(uint32_t bar, int bytes) {
@@ -537,7 +582,7 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
             RowNumbers k;
             double logp = 0.0;
             if (computed(r)) {  // (the same for the whole cluster)
-                all = join_parts(warp_parts[p], G / 32, l);
+                all = join_parts<false>(warp_parts[p], G / 32, l);
                 if (size > 1) {
                     const int x = rows_done & 1;
                     const uint32_t bar = static_cast<uint32_t>(__cvta_generic_to_shared(&bars[x]));
@@ -545,7 +590,7 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
                     if (l < size) exchange_send(static_cast<uint32_t>(__cvta_generic_to_shared(&cta_parts[x][rank])), bar, l, all);
                     if (!failed) failed = !exchange_wait(bar, rows_done >> 1 & 1, a.status);
                     failed = __any_sync(0xffffffffu, failed);
-                    all = join_parts(cta_parts[x], size, l);
+                    all = join_parts<false>(cta_parts[x], size, l);
                     ++rows_done;
                 }
                 k.xk = __shfl_sync(0xffffffffu, mine, 0);
@@ -628,7 +673,7 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
                     for (int u = 0; u < 4; ++u)
                         if (static_cast<unsigned>(j0 + 4 * q * G + u) >= static_cast<unsigned>(a.V)) v[q][u] = -INFINITY;
             }
-            const Part own = warp_part<NV>(v);
+            const Part own = warp_part<NV, false>(v);
 #pragma unroll
             for (int q = 0; q < NV; ++q) *slot(n, q) = make_float4(v[q][0], v[q][1], v[q][2], v[q][3]);
             if (l == 0) warp_parts[n & 1][warp] = own;
@@ -749,12 +794,12 @@ __global__ void __launch_bounds__(256, 4) preference_cluster_kernel(TokenArgs a)
             float v[NV][4];
 #pragma unroll
             for (int q = 0; q < NV; ++q) load_vec(r.x, j + 4 * (l + 32 * q), a.V, false, v[q]);
-            const Part next = warp_part<NV>(v);
+            const Part next = warp_part<NV, true>(v);
             const float m = max_nan(all.m, next.m);
-            all.s = all.s * part_weight(all.m, m) + next.s * part_weight(next.m, m);
+            all.s = all.s * part_weight_exact(all.m, m) + next.s * part_weight_exact(next.m, m);
             all.m = m;
         }
-        const double diff = token_logp(k.xk, all) - static_cast<double>(k.ref);
+        const double diff = token_logp_exact(k.xk, all) - static_cast<double>(k.ref);
         sum += i < T ? diff : -diff;
         if (l == 0 && a.dlogits) write_value(a, r.row, k, all, diff + static_cast<double>(k.ref));
     }
