@@ -189,6 +189,35 @@ def test_device_buffer_refuses_other_dtypes():
         tt.PinnedBuffer([2], dtype="int64")
 
 
+class _At(tt.DeviceBuffer):  # a buffer without its allocation
+    def __init__(self, ptr, dtype):
+        self.ptr, self.dtype, self.shape = ptr, dtype, [1]
+
+    def free(self):
+        pass
+
+
+def test_device_runs_refuse_buffers_of_the_other_dtype(cache_dir):
+    """Also where a buffer lies at the address of one that an earlier run had."""
+    g, x, k = _loss_graph()
+    prog = tt.compile(g, outputs=[tt.token_logprob(x, k)], cache_dir=cache_dir, flags=HOST)
+    xb, kb, y = _At(0x1000, tt.float32), _At(0x2000, tt.int32), _At(0x3000, tt.float32)
+    prog._dev_args = ([0x1000, 0x2000], [0x3000], None, None)
+    for ins, out in [([xb, _At(0x2000, tt.float32)], y), ([_At(0x1000, tt.int32), kb], y), ([xb, kb], _At(0x3000, tt.int32))]:
+        with pytest.raises(tt.TypeError):
+            prog.run_device(ins, [out])
+
+
+def test_int32_tensors():
+    k = tt.tensor([[1, 2**31 - 1]], dtype=tt.int32)
+    assert k.dtype == tt.int32 and k.numpy().dtype == np.int32 and k.numpy().tolist() == [[1, 2**31 - 1]]
+    assert tt.tensor([1, 2]).dtype == tt.float32
+    with pytest.raises(tt.TypeError):
+        tt.tensor([0.5], dtype=tt.int32)
+    with pytest.raises(tt.TypeError):
+        tt.tensor([2**31], dtype=tt.int32)
+
+
 # ---- schedule --------------------------------------------------------------------------------
 
 

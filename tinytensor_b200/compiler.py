@@ -56,21 +56,24 @@ class Tensor:
 
     @property
     def dtype(self):
-        return "float32"
+        return int32 if self._a.dtype == np.int32 else float32
 
     def item(self):
         if self._a.size != 1:
             raise ShapeError(f"item() requires a single element, got {self._a.size}")
-        return float(self._a.reshape(-1)[0])
+        v = self._a.reshape(-1)[0]
+        return int(v) if self.dtype == int32 else float(v)
 
     def __array__(self, dtype=None, copy=None):
         return self._a if dtype is None else self._a.astype(dtype)
 
     def __repr__(self):
-        return f"Tensor(shape={self.shape}, dtype=float32)"
+        return f"Tensor(shape={self.shape}, dtype={self.dtype})"
 
 
 def tensor(data, dtype=None) -> Tensor:
+    if dtype == int32:  # token ids
+        return Tensor(_to_int32(data))
     return Tensor(np.array(data, dtype=np.float32, order="C"))
 
 
@@ -261,6 +264,7 @@ class CompiledProgram:
         self._grad_nodes = list(grad_nodes)
         self._h = handle
         self._inputs = graph.inputs
+        self._in_dtypes = [int32 if n.dtype == int32 else float32 for n in self._inputs]
         self._dev_args = None  # (input pointers, output pointers, their ctypes arrays) of the last run_device
         ni, no = ctypes.c_int32(), ctypes.c_int32()
         _lib.check(_lib.lib.tt_program_num_io(self._h, ctypes.byref(ni), ctypes.byref(no)))
@@ -337,11 +341,15 @@ class CompiledProgram:
         # generators
         ki = [getattr(x, "ptr", x) for x in inputs]
         ko = [getattr(x, "ptr", x) for x in outputs]
+        # (each call: a buffer may lie where a freed one of the other dtype was)
+        for x, dt in zip(inputs, self._in_dtypes):
+            if isinstance(x, DeviceBuffer) and x.dtype != dt:
+                raise TypeError(f"an input is {dt}, its buffer {x.dtype}")
+        for x in outputs:
+            if isinstance(x, DeviceBuffer) and x.dtype != float32:
+                raise TypeError(f"outputs are float32, a buffer is {x.dtype}")
         cached = self._dev_args
         if cached is None or cached[0] != ki or cached[1] != ko:
-            for n, x in zip(self._inputs, inputs):
-                if (getattr(x, "dtype", n.dtype) == int32) != (n.dtype == int32):
-                    raise TypeError(f"Input %{n.id} is {n.dtype}, its buffer {x.dtype}")
             ip = (ctypes.c_void_p * max(1, len(ki)))(*ki)
             op = (ctypes.c_void_p * max(1, len(ko)))(*ko)
             cached = self._dev_args = (ki, ko, ip, op)

@@ -153,9 +153,10 @@ class DataParallelSGD:
         buffer unchanged until the next step_host call (or a synchronize) — e.g.
         alternate two host buffers."""
         from .compiler import DeviceBuffer, Event, Stream
+        from .graph import float32
 
         if getattr(self, "_slots", None) is None:
-            self._slots = [[DeviceBuffer(h.shape, dtype=h.dtype) for h in host_inputs] for _ in range(2)]
+            self._slots = [[DeviceBuffer(h.shape, dtype=getattr(h, "dtype", float32)) for h in host_inputs] for _ in range(2)]
             self._copy_stream = Stream()
             self._copied = [Event(), Event()]
             self._consumed = [Event(), Event()]
