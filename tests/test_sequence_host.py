@@ -189,23 +189,58 @@ def test_device_buffer_refuses_other_dtypes():
         tt.PinnedBuffer([2], dtype="int64")
 
 
-class _At(tt.DeviceBuffer):  # a buffer without its allocation
-    def __init__(self, ptr, dtype):
-        self.ptr, self.dtype, self.shape = ptr, dtype, [1]
+class _FakeDevice:
+    """The library with an allocator that hands out the addresses it is told to, and runs that do nothing."""
 
-    def free(self):
-        pass
+    def __init__(self, lib):
+        self.lib, self.next, self.runs = lib, None, 0
+
+    def __getattr__(self, name):
+        return getattr(self.lib, name)
+
+    def tt_device_alloc(self, nbytes, p):
+        p._obj.value = self.next
+        return 0
+
+    def tt_device_free(self, p):
+        return 0
+
+    def tt_program_run(self, *args):
+        self.runs += 1
+        return 0
 
 
-def test_device_runs_refuse_buffers_of_the_other_dtype(cache_dir):
+def test_device_runs_refuse_buffers_of_the_other_dtype(cache_dir, monkeypatch):
     """Also where a buffer lies at the address of one that an earlier run had."""
     g, x, k = _loss_graph()
     prog = tt.compile(g, outputs=[tt.token_logprob(x, k)], cache_dir=cache_dir, flags=HOST)
-    xb, kb, y = _At(0x1000, tt.float32), _At(0x2000, tt.int32), _At(0x3000, tt.float32)
-    prog._dev_args = ([0x1000, 0x2000], [0x3000], None, None)
-    for ins, out in [([xb, _At(0x2000, tt.float32)], y), ([_At(0x1000, tt.int32), kb], y), ([xb, kb], _At(0x3000, tt.int32))]:
-        with pytest.raises(tt.TypeError):
-            prog.run_device(ins, [out])
+    fake = _FakeDevice(_lib.lib)
+    monkeypatch.setattr(_lib, "lib", fake)
+
+    def buffer(address, shape, dtype=tt.float32):
+        fake.next = address
+        return tt.DeviceBuffer(shape, dtype=dtype)
+
+    xb, kb, y = buffer(0x1000, [2, 3, 7]), buffer(0x2000, [2, 3], tt.int32), buffer(0x3000, [2, 3])
+    for _ in range(2):
+        prog.run_device([xb, kb], [y])
+    prog.run_device([0x1000, 0x2000], [0x3000])
+    assert fake.runs == 3
+    kb.free()
+    with pytest.raises(tt.TypeError):
+        prog.run_device([xb, buffer(0x2000, [2, 3])], [y])
+    kb = buffer(0x2000, [2, 3], tt.int32)
+    prog.run_device([xb, kb], [y])
+    xb.free()
+    with pytest.raises(tt.TypeError):
+        prog.run_device([buffer(0x1000, [2, 3, 7], tt.int32), kb], [y])
+    xb = buffer(0x1000, [2, 3, 7])
+    prog.run_device([xb, kb], [y])
+    y.free()
+    with pytest.raises(tt.TypeError):
+        prog.run_device([xb, kb], [buffer(0x3000, [2, 3], tt.int32)])
+    assert fake.runs == 5
+    xb = kb = None  # (freed through the fake)
 
 
 def test_int32_tensors():

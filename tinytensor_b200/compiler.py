@@ -185,6 +185,8 @@ def _to_int32(a):
 class DeviceBuffer:
     """A float32 (or int32, for token ids) device allocation (cudaMalloc) with a shape."""
 
+    _int32_changes = 0  # int32 buffers allocated and freed so far
+
     def __init__(self, shape, pinned_host=False, dtype=float32):
         self._np = _numpy_dtype(dtype)
         self.dtype = dtype
@@ -193,6 +195,8 @@ class DeviceBuffer:
         p = ctypes.c_void_p()
         _lib.check(_lib.lib.tt_device_alloc(self.nbytes, ctypes.byref(p)))
         self.ptr = p.value
+        if dtype == int32:
+            DeviceBuffer._int32_changes += 1
 
     def _host(self, arr):
         return _to_int32(arr) if self.dtype == int32 else np.ascontiguousarray(arr, dtype=np.float32)
@@ -222,6 +226,8 @@ class DeviceBuffer:
         if self.ptr:
             _lib.lib.tt_device_free(self.ptr)
             self.ptr = None
+            if self.dtype == int32:
+                DeviceBuffer._int32_changes += 1
 
     def __del__(self):
         try:
@@ -264,8 +270,7 @@ class CompiledProgram:
         self._grad_nodes = list(grad_nodes)
         self._h = handle
         self._inputs = graph.inputs
-        self._in_dtypes = [int32 if n.dtype == int32 else float32 for n in self._inputs]
-        self._dev_args = None  # (input pointers, output pointers, their ctypes arrays) of the last run_device
+        self._dev_args = None  # (input pointers, output pointers, their ctypes arrays, int32 buffers' count of changes) of the last run_device
         ni, no = ctypes.c_int32(), ctypes.c_int32()
         _lib.check(_lib.lib.tt_program_num_io(self._h, ctypes.byref(ni), ctypes.byref(no)))
         self.num_inputs, self.num_outputs = ni.value, no.value
@@ -341,18 +346,18 @@ class CompiledProgram:
         # generators
         ki = [getattr(x, "ptr", x) for x in inputs]
         ko = [getattr(x, "ptr", x) for x in outputs]
-        # (each call: a buffer may lie where a freed one of the other dtype was)
-        for x, dt in zip(inputs, self._in_dtypes):
-            if isinstance(x, DeviceBuffer) and x.dtype != dt:
-                raise TypeError(f"an input is {dt}, its buffer {x.dtype}")
-        for x in outputs:
-            if isinstance(x, DeviceBuffer) and x.dtype != float32:
-                raise TypeError(f"outputs are float32, a buffer is {x.dtype}")
+        # (checked again whenever an int32 buffer came or went: one may lie where another type's was)
         cached = self._dev_args
-        if cached is None or cached[0] != ki or cached[1] != ko:
+        if cached is None or cached[0] != ki or cached[1] != ko or cached[4] != DeviceBuffer._int32_changes:
+            for x, n in zip(inputs, self._inputs):
+                if isinstance(x, DeviceBuffer) and (x.dtype == int32) != (n.dtype == int32):
+                    raise TypeError(f"Input %{n.id} is {n.dtype}, its buffer {x.dtype}")
+            for x in outputs:
+                if isinstance(x, DeviceBuffer) and x.dtype != float32:
+                    raise TypeError(f"outputs are float32, a buffer is {x.dtype}")
             ip = (ctypes.c_void_p * max(1, len(ki)))(*ki)
             op = (ctypes.c_void_p * max(1, len(ko)))(*ko)
-            cached = self._dev_args = (ki, ko, ip, op)
+            cached = self._dev_args = (ki, ko, ip, op, DeviceBuffer._int32_changes)
         h = stream.handle if isinstance(stream, Stream) else stream
         _lib.check(_lib.lib.tt_program_run(self._h, cached[2], cached[3], _lib.DEVICE, h))
 
