@@ -148,6 +148,13 @@ __device__ __forceinline__ void split_lane(const ScanArgs& a, int64_t lane, int6
     }
 }
 
+__device__ __forceinline__ void split_inner(const ScanArgs& a, int64_t i, int64_t& i1, int64_t& i2) {
+    if (a.n2 == a.inner) i1 = 0;
+    else if (a.inner <= 0x7fffffff) i1 = static_cast<unsigned>(i) / static_cast<unsigned>(a.n2);
+    else i1 = i / a.n2;
+    i2 = i - i1 * a.n2;
+}
+
 // The state before segment `seg` of a lane, from the maps of the segments before it and the lane's
 // first state.  The warps of the CTA (all on the same lanes) join a share of the maps each,
 // loading 8 at a time; LW lanes a warp, `writer` one thread of a lane.
@@ -272,8 +279,8 @@ __device__ __forceinline__ void store_vec(float* p, const float* v, bool stream)
 // in 4*V bytes a thread and 128 bytes a row whatever V is; the V threads of a lane join their
 // maps by shuffles.  Operands whose lanes are adjacent move as V-vectors, operands broadcast over
 // the lanes behind n1 as one value (V > 1 is only cut where each operand is one or the other);
-// V = 1 takes any strides.  A thread reads back only what it copied itself, so the ring needs
-// no barrier.
+// V = 1 takes any strides.  A thread reads back what it copied itself, or a thread of its warp
+// (broadcast values), so the ring needs no block barrier.
 template <bool BACKWARD>
 constexpr int kArrays = BACKWARD ? 3 : 2;
 
@@ -294,46 +301,57 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a)
     const int wt = warp % W, wr = warp / W;
     const int col = l % COLS, sub = l / COLS;
     const bool want_gate = BACKWARD && PASS != MAPS && a.out[SO_GATE];
-    const int64_t stride = static_cast<int64_t>(at.size) * W * TILE;  // of this warp's tiles
-    const int64_t own = (static_cast<int64_t>(at.rank) * W + wt) * TILE + sub * TS;
+    // Places on the axis count from the segment's begin, in scan order; a segment has less than 2^31 steps.
+    const int stride = at.size * W * TILE;  // of this warp's tiles
+    const int own = (at.rank * W + wt) * TILE + sub * TS;
     auto block_of = [&](int64_t unit) { return a.segments == 1 ? unit : unit / a.segments; };
     auto first_lane = [&](int64_t unit) { return (block_of(unit) * (NW / W) + wr) * 32; };
-    // this thread's steps from r0 on
-    auto run_len = [&](bool live, int64_t r0, int64_t end) {
-        return live ? static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(TS), end - r0))) : 0;
-    };
-    auto slot = [&](int stage, int k) { return &sh.in[stage][k][warp][l * V]; };
+    auto run_len = [&](int r0, int end) { return min(max(end - r0, 0), TS); };  // this thread's steps from r0 on
+    // A thread's values of an operand in the ring: V a step, or one of an operand that is broadcast over the
+    // lanes.  That one is copied by the first thread that shares it and read by all of them (each copying its
+    // own, 32 threads from one address are served one after the other: 33 instead of 9 wavefronts a tile).
+    auto slot = [&](int stage, int k, bool one) { return &sh.in[stage][k][warp][one ? l : l * V]; };
+    auto is_one = [&](int k) { return a.n2 > 1 && a.in[k].s2 == 0; };
+    auto leader = [&](int64_t i2) { return static_cast<int>(max(static_cast<int64_t>(0), col * V - i2)) / V; };  // its column
 
-    // ---- the ring: a place ahead of the computation
+    // ---- the ring: a place ahead of the computation.  Pointers move on by a step, not by multiplications:
+    // 64-bit products and comparisons were a third of the kernel's instructions.
     struct {
-        int64_t unit, r0, end;
-        int step;
-        bool live;
-        const float *gate, *x, *h, *init;
+        int64_t unit;
+        int r0, end, hend, step;     // hend: the end of the steps with a state before them
+        bool leads;
+        const float *gate, *x, *h, *init;  // of the thread's first step at r0 (h: of the step before it)
     } ahead;
     auto aim = [&](int64_t unit) {
         ahead.unit = unit;
         ahead.step = 0;
         if (unit >= a.units) return;
         const int64_t lane = first_lane(unit) + col * V, begin = (unit - block_of(unit) * a.segments) * a.seg_len;
-        ahead.live = lane < a.lanes;
-        ahead.r0 = begin + own;
-        ahead.end = min(a.T, begin + a.seg_len);
-        int64_t o = 0, i = 0;
-        if (ahead.live) split_lane(a, lane, o, i);
-        const int64_t i1 = a.n2 == a.inner ? 0 : i / a.n2, i2 = i - i1 * a.n2;
-        auto ptr = [&](int k) { return a.in[k].p ? a.in[k].p + o * a.in[k].so + i1 * a.in[k].s1 + i2 * a.in[k].s2 : nullptr; };
-        ahead.gate = ptr(SI_GATE);
-        ahead.x = ptr(SI_X);
-        ahead.h = ptr(SI_H);
-        ahead.init = ptr(SI_INIT);
+        const bool live = lane < a.lanes;
+        ahead.r0 = own;
+        ahead.end = live ? static_cast<int>(min(a.seg_len, a.T - begin)) : 0;
+        ahead.hend = live ? static_cast<int>(min(a.seg_len, a.T - 1 - begin)) : 0;
+        int64_t o = 0, i = 0, i1, i2;
+        if (live) split_lane(a, lane, o, i);
+        split_inner(a, i, i1, i2);
+        ahead.leads = leader(i2) == col;
+        const int64_t t = BACKWARD ? a.T - 1 - begin - own : begin + own;
+        auto ptr = [&](int k, int64_t time) {
+            const Operand& q = a.in[k];
+            return q.p ? q.p + o * q.so + i1 * q.s1 + i2 * q.s2 + time * q.st : nullptr;
+        };
+        ahead.gate = ptr(SI_GATE, t);
+        ahead.x = ptr(SI_X, t);
+        ahead.h = ptr(SI_H, t - 1);
+        ahead.init = ptr(SI_INIT, 0);
     };
-    // copies of one operand: n steps in scan order from time t on
-    auto fetch = [&](const float* p, int k, int stage, int arr, int64_t t, int n) {
+    // copies of one operand: n steps in scan order from q on
+    auto fetch = [&](const float* q, int k, int stage, int arr, int n) {
         const int64_t step = BACKWARD ? -a.in[k].st : a.in[k].st;
-        const float* q = p + t * a.in[k].st;
-        const uint32_t dst = smem_addr(slot(stage, arr));
-        if (V > 1 && (a.vec >> k & 1)) {
+        const bool one = is_one(k);
+        if (one && !ahead.leads) return;
+        const uint32_t dst = smem_addr(slot(stage, arr, one));
+        if (V > 1 && !one) {
 #pragma unroll
             for (int j = 0; j < TS; ++j, q += step)
                 if (j < n) copy_async<4 * V>(dst + j * 128 * V, q);
@@ -343,17 +361,18 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a)
                 if (j < n) copy_async<4>(dst + j * 128 * V, q);
         }
     };
+    auto moved = [&](const float*& q, int k) { q += BACKWARD ? -stride * a.in[k].st : stride * a.in[k].st; };
     auto issue = [&](int stage) {
         if (ahead.unit < a.units) {
-            const int n = run_len(ahead.live, ahead.r0, ahead.end);
-            const int64_t t = BACKWARD ? a.T - 1 - ahead.r0 : ahead.r0;
+            const int n = run_len(ahead.r0, ahead.end);
             if (n > 0) {
-                fetch(ahead.gate, SI_GATE, stage, 0, t, n);
-                if (ahead.x) fetch(ahead.x, SI_X, stage, 1, t, n);
+                fetch(ahead.gate, SI_GATE, stage, 0, n);
+                if (a.in[SI_X].p) fetch(ahead.x, SI_X, stage, 1, n);
                 if (want_gate) {  // the states before each step; before t = 0 there is init
-                    fetch(ahead.h, SI_H, stage, NA - 1, t - 1, static_cast<int>(min(static_cast<int64_t>(n), t)));
-                    if (t < n && ahead.init) {
-                        const uint32_t dst = smem_addr(slot(stage, NA - 1)) + static_cast<int>(t) * 128 * V;
+                    const int nh = run_len(ahead.r0, ahead.hend);
+                    fetch(ahead.h, SI_H, stage, NA - 1, nh);
+                    if (nh < n && ahead.init) {
+                        const uint32_t dst = smem_addr(slot(stage, NA - 1, false)) + nh * 128 * V;
 #pragma unroll
                         for (int v = 0; v < V; ++v) copy_async<4>(dst + 4 * v, ahead.init + v * a.in[SI_INIT].s2);
                     }
@@ -362,14 +381,17 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a)
             if (PASS == ONLY && ahead.step == 0 && a.in[SI_CARRY].p) {  // the unit's first states, lane by lane
                 const int64_t lane = first_lane(ahead.unit) + l;
                 if (lane < a.lanes) {
-                    int64_t o, i;
+                    int64_t o, i, i1, i2;
                     split_lane(a, lane, o, i);
-                    const int64_t i1 = a.n2 == a.inner ? 0 : i / a.n2, i2 = i - i1 * a.n2;
+                    split_inner(a, i, i1, i2);
                     copy_async<4>(smem_addr(&sh.carry[stage][warp][l]),
                                   a.in[SI_CARRY].p + o * a.in[SI_CARRY].so + i1 * a.in[SI_CARRY].s1 + i2 * a.in[SI_CARRY].s2);
                 }
             }
             ahead.r0 += stride;
+            moved(ahead.gate, SI_GATE);
+            moved(ahead.x, SI_X);
+            if (want_gate) moved(ahead.h, SI_H);
             if (++ahead.step == a.steps) aim(ahead.unit + at.clusters);
         }
         copies_commit();
@@ -380,16 +402,26 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a)
     if (at.size > 1) cg::this_cluster().sync();  // every CTA runs before another writes to it
 
     Joiner<NW, 32> joiner{sh.ex, at, W, wt, wr, warp, l};
-    const bool splat_gate = V > 1 && !(a.vec >> SI_GATE & 1), splat_x = V > 1 && !(a.vec >> SI_X & 1);
-    const bool splat_h = V > 1 && !(a.vec >> SI_H & 1);
+    const bool one_gate = is_one(SI_GATE), one_x = is_one(SI_X), one_h = is_one(SI_H);
+    const bool shares = one_gate || one_x || one_h;
     int stage = 0;
     for (int64_t unit = at.first; unit < a.units; unit += at.clusters) {
         const int seg = static_cast<int>(unit - block_of(unit) * a.segments);
         const int64_t lane0 = first_lane(unit), lane = lane0 + col * V;
         const bool live = lane < a.lanes;
-        const int64_t begin = seg * a.seg_len, end = min(a.T, begin + a.seg_len);
+        const int64_t begin = seg * a.seg_len;
+        const int end = live ? static_cast<int>(min(a.seg_len, a.T - begin)) : 0;
+        const int hend = live ? static_cast<int>(min(a.seg_len, a.T - 1 - begin)) : 0;
+        const int last_end = live && begin + end == a.T ? end : -1;  // the axis ends here
         int64_t o = 0, i = 0;
         if (live) split_lane(a, lane, o, i);
+        int64_t i1, i2;
+        split_inner(a, i, i1, i2);
+        const int shared_by = leader(i2) - col;  // where the thread that copies a broadcast value is
+        // results of the thread's first step
+        const int64_t row = o * a.T + (BACKWARD ? a.T - 1 - begin - own : begin + own);
+        float* ym0 = a.out[SO_MAIN] + row * a.inner + i;
+        float* yg0 = a.out[SO_GATE] + row * (a.inner >> a.group) + (i >> a.group);
         float c = 0.0f, gates = 1.0f;
         if constexpr (PASS == JOINED) {
             const bool in = lane0 + l < a.lanes;
@@ -400,15 +432,17 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a)
             }
             c = segment_state<NW, 32>(a, sh.ex, seg, lane0 + l, in, c, warp, l, true);
         }
-        int64_t r0 = begin + own;
+        int r0 = own;
         for (int k = 0; k < a.steps; ++k, r0 += stride, stage ^= 1) {
-            const int n = run_len(live, r0, end);
+            const int n = run_len(r0, end);
             float ga[TS][V], xv[TS][V], hv[BACKWARD ? TS : 1][V];
             copies_wait_one();
-            auto read = [&](const float* q, bool splat, int count, float none, float (*dst)[V]) {
+            if (shares) __syncwarp();  // (broadcast values come from another thread's copies)
+            auto read = [&](const float* q, bool one, int count, float none, float (*dst)[V]) {
+                if (one) q += shared_by;
 #pragma unroll
                 for (int j = 0; j < TS; ++j) {
-                    if (splat) {
+                    if (one) {
                         const float f = q[j * 32 * V];
 #pragma unroll
                         for (int v = 0; v < V; ++v) dst[j][v] = f;
@@ -424,19 +458,19 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a)
                             if (j >= count) dst[j][v] = none;
                 }
             };
-            read(slot(stage, 0), splat_gate, n, 1.0f, ga);
-            read(slot(stage, 1), splat_x, a.in[SI_X].p ? n : 0, 0.0f, xv);
+            read(slot(stage, 0, one_gate), one_gate, n, 1.0f, ga);
+            read(slot(stage, 1, one_x), one_x, a.in[SI_X].p ? n : 0, 0.0f, xv);
             if constexpr (BACKWARD) {
-                const int64_t t0 = a.T - 1 - r0;
-                const int nh = static_cast<int>(max(static_cast<int64_t>(0), min(static_cast<int64_t>(n), t0)));
-                read(slot(stage, NA - 1), splat_h, want_gate ? (a.in[SI_INIT].p ? n : nh) : 0, 0.0f, hv);
-                if (splat_h && want_gate && a.in[SI_INIT].p && nh < n) {  // init need not be broadcast where h is
+                const int nh = run_len(r0, hend);
+                read(slot(stage, NA - 1, one_h), one_h, want_gate ? (a.in[SI_INIT].p ? n : nh) : 0, 0.0f, hv);
+                if (one_h && want_gate && a.in[SI_INIT].p && nh < n) {  // init need not be broadcast where h is
 #pragma unroll
                     for (int j = 0; j < TS; ++j)
-                        if (j == nh) load_shared<V>(slot(stage, NA - 1) + j * 32 * V, hv[j]);
+                        if (j == nh) load_shared<V>(slot(stage, NA - 1, false) + j * 32 * V, hv[j]);
                 }
             }
             if (PASS == ONLY && k == 0) c = a.in[SI_CARRY].p && lane0 + l < a.lanes ? sh.carry[stage][warp][l] : 0.0f;
+            if (shares) __syncwarp();
             issue(stage);
             // this thread's maps, those of the threads before it in time, and the tile's
             float2 m[V], before[V];
@@ -485,13 +519,13 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a)
                     s[v] = V > 1 ? __shfl_sync(0xffffffffu, first, col * V + v) : first;
                     if (V > 1) s[v] = sub > 0 ? apply(before[v], s[v]) : s[v];
                 }
-                const int64_t step = BACKWARD ? -a.inner : a.inner;
-                const int64_t y = (o * a.T + (BACKWARD ? a.T - 1 - r0 : r0)) * a.inner + i;
-                float* ym = a.out[SO_MAIN] + y;
-                float* yg = a.out[SO_GATE] + y;
+                const int64_t step = BACKWARD ? -a.inner : a.inner, step_g = BACKWARD ? -(a.inner >> a.group) : 0;
+                float *ym = ym0, *yg = yg0;
+                ym0 += stride * step;
+                if (want_gate) yg0 += stride * step_g;
                 const int nm = a.out[SO_MAIN] ? n : 0, ng = want_gate ? n : 0;
 #pragma unroll
-                for (int j = 0; j < TS; ++j, ym += step, yg += step) {  // (past the end: gate 1, x 0, the state stays)
+                for (int j = 0; j < TS; ++j, ym += step, yg += step_g) {  // (past the end: gate 1, x 0, the state stays)
                     float main[V], dg[V];
 #pragma unroll
                     for (int v = 0; v < V; ++v) {
@@ -515,12 +549,11 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a)
                             const float w = __shfl_xor_sync(0xffffffffu, t, d);
                             if (d * V >> a.group == 0) t += w;
                         }
-                        if (j < ng && (col * V & ((1 << a.group) - 1)) == 0)
-                            a.out[SO_GATE][(o * a.T + a.T - 1 - r0 - j) * (a.inner >> a.group) + (i >> a.group)] = t;
+                        if (j < ng && (col * V & ((1 << a.group) - 1)) == 0) *yg = t;
                     }
                 }
                 // the thread of the last step has the last state as it was stored
-                if (n > 0 && r0 + n == a.T && a.out[SO_LANE]) store_vec<V>(a.out[SO_LANE] + lane, s, false);
+                if (n > 0 && r0 + n == last_end && a.out[SO_LANE]) store_vec<V>(a.out[SO_LANE] + lane, s, false);
                 float behind = s[0];  // the state behind the tile, of lane l
                 if (V > 1) {
 #pragma unroll
@@ -847,7 +880,8 @@ __global__ void __launch_bounds__(256) scan_short_kernel(ScanArgs a) {
     if (lane >= a.lanes) return;
     int64_t o, i;
     split_lane(a, lane, o, i);
-    const int64_t i1 = a.n2 == a.inner ? 0 : i / a.n2, i2 = i - i1 * a.n2;
+    int64_t i1, i2;
+    split_inner(a, i, i1, i2);
     auto ptr = [&](int k) { return a.in[k].p ? a.in[k].p + o * a.in[k].so + i1 * a.in[k].s1 + i2 * a.in[k].s2 : nullptr; };
     const float *gate = ptr(SI_GATE), *x = ptr(SI_X), *carry = ptr(SI_CARRY), *h = ptr(SI_H), *init = ptr(SI_INIT);
     auto load = [&](const float* p, int k, float* v) {
@@ -1087,7 +1121,7 @@ int launch_scan(const ScanDesc& d, const float* const* in, float* const* out, vo
     const int64_t lanes = d.outer * d.n1 * d.n2;
     if (lanes == 0) return 0;
     const Cut c = cut(d);
-    if (c.blocks * c.segments > 0x7fffffff / 8 || c.steps > 0x7fffffff) return static_cast<int>(cudaErrorInvalidConfiguration);
+    if (c.blocks * c.segments > 0x7fffffff / 8 || c.steps > 0x7fffffff || c.seg_len > 0x7f000000) return static_cast<int>(cudaErrorInvalidConfiguration);
     ScanArgs a;
     a.vec = 0;
     for (int k = 0; k < SI_COUNT; ++k) {
