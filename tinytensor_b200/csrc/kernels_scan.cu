@@ -573,9 +573,12 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a)
 // run of 20 (12) adjacent steps per thread (an odd number of 16-byte vectors, so that the
 // threads' runs lie in different banks), the runs' maps joined by shuffles.  Rows of up to
 // SUB runs less 3 steps take SUB threads, 32/SUB rows a warp.  Tiles move between global and shared memory in coalesced
-// vectors, in and out.  Rows need not start on 16 bytes: vectors are cut at the row's own 16-byte
-// boundaries (`shift` steps before its first one), so whole vectors move as 16 bytes and only
-// ragged ends value by value.
+// vectors, in and out.  Rows need not start on 16 bytes: vectors are cut at the result's 16-byte
+// boundaries (`shift` steps before the row's first one), so whole vectors move as 16 bytes and only
+// ragged ends value by value.  Rows of whole warps are cut at 128-byte boundaries, so that tiles do not
+// share lines (2000 rows of 8191: 38.0 us forward and 61.4 backward against 38.8 and 63.1).
+template <int SUB>
+constexpr int kRowCut = SUB == 32 ? 32 : 4;
 template <bool BACKWARD>
 constexpr int kRowRun = BACKWARD ? 12 : 20;
 
@@ -636,8 +639,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(ScanArgs a) {
     };
     auto cutout = [&](int64_t row, Count end, Count r0) {
         Cutout q;
-        q.shift = static_cast<int>(static_cast<unsigned>(row) * static_cast<unsigned>(a.T) & 3);
-        q.vectors = (static_cast<Count>(a.T) + q.shift + 3) / 4;
+        q.shift = static_cast<int>(static_cast<unsigned>(row) * static_cast<unsigned>(a.T) & (kRowCut<SUB> - 1));
+        q.vectors = (static_cast<Count>(a.T) + q.shift + kRowCut<SUB> - 1) / kRowCut<SUB> * (kRowCut<SUB> / 4);
         const Count last = row < a.lanes ? min(q.vectors, end) : r0;
         q.n = static_cast<int>(max(static_cast<Count>(0), min(static_cast<Count>(VR), last - r0)));
         q.v0 = BACKWARD ? q.vectors - r0 - VR : r0;  // may be negative where n < VR
@@ -647,6 +650,26 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(ScanArgs a) {
     // all of the tile is inside the row: nothing to check vector by vector
     auto whole_tile = [&](const Cutout& q) {
         return q.n == VR && 4 * q.v0 >= q.shift && 4 * (q.v0 + VR) - q.shift <= a.T;
+    };
+    // A tile that is not (rows of whole warps): bit q says whether the thread's vector l + 32*q is inside the row.
+    auto inside_vectors = [&](const Cutout& q) {
+        unsigned m = 0;
+#pragma unroll
+        for (int u = 0; u < kVectors / 32; ++u) {
+            const int v = l + 32 * u;
+            const Count t = 4 * (q.v0 + v) - q.shift;
+            if (v >= q.lo && v < q.lo + q.n && t >= 0 && t + 3 < a.T) m |= 1u << u;
+        }
+        return m;
+    };
+    // The steps of a row outside whole vectors, at most three at each end, are moved by eight threads: this
+    // thread's step t, returned is its place in the tile (-1: none).
+    auto edge = [&](const Cutout& q, Count& t) {
+        const Count tail = static_cast<Count>(a.T) - ((static_cast<int>(a.T & 3) + q.shift) & 3);
+        t = l < 4 ? l : tail + (l - 4);
+        const bool is = l < 4 ? l < (-q.shift & 3) : l < 8 && t < a.T;
+        const Count at_t = t + q.shift - 4 * q.v0;
+        return is && at_t >= 4 * q.lo && at_t < 4 * (q.lo + q.n) ? static_cast<int>(at_t) : -1;
     };
     auto h_row = [&](int stage, int r) { return &tile.h[BACKWARD ? stage : 0][BACKWARD ? 4 + r * (SUB * kRun + 4) : 0]; };
     const int need = 1 << SI_GATE | (a.in[SI_X].p ? 1 << SI_X : 0) | (want_gate ? 1 << SI_H : 0);
@@ -664,6 +687,22 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(ScanArgs a) {
                     const uint32_t to = smem_addr(dst + 4 * l);
 #pragma unroll
                     for (int q = 0; q < kVectors / 32; ++q) copy_async<16>(to + 512 * q, p + 128 * q);
+                };
+                copy(SI_GATE, tile.in[stage][0]);
+                if (a.in[SI_X].p) copy(SI_X, tile.in[stage][1]);
+                if (want_gate) copy(SI_H, h_row(stage, 0));
+            } else if (SUB == 32 && (a.vec & need) == need) {
+                const unsigned in = inside_vectors(mine);
+                Count t;
+                const int e = edge(mine, t);
+                auto copy = [&](int op, float* dst) {
+                    const float* row = a.in[op].p + ahead.row0 * a.in[op].so;
+                    const float* p = row + at_t + 4 * l;
+                    const uint32_t to = smem_addr(dst + 4 * l);
+#pragma unroll
+                    for (int q = 0; q < kVectors / 32; ++q)
+                        if (in >> q & 1) copy_async<16>(to + 512 * q, p + 128 * q);
+                    if (e >= 0) copy_async<4>(smem_addr(dst + e), row + t);
                 };
                 copy(SI_GATE, tile.in[stage][0]);
                 if (a.in[SI_X].p) copy(SI_X, tile.in[stage][1]);
@@ -698,9 +737,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(ScanArgs a) {
             if (ls == 0 && row < a.lanes) {
                 if (PASS == ONLY && ahead_step == 0 && a.in[SI_CARRY].p)
                     copy_async<4>(smem_addr(&tile.carry[stage][sr]), a.in[SI_CARRY].p + row * a.in[SI_CARRY].so);
-                if (want_gate && mine.n > 0) {
+                const int64_t t = at_t + 4 * mine.lo;
+                if (want_gate && t > -4 * mine.n) {  // (otherwise none of the vectors is inside the row)
                     // the state before the tile's first step in memory, in front of it: init before t = 0
-                    const int64_t t = at_t + 4 * mine.lo;
                     float* dst = h_row(stage, sr) + 4 * mine.lo + (t < 0 ? -static_cast<int>(t) : 0) - 1;
                     if (t > 0) copy_async<4>(smem_addr(dst), a.in[SI_H].p + row * a.in[SI_H].so + (t - 1) * a.in[SI_H].st);
                     else if (a.in[SI_INIT].p) copy_async<4>(smem_addr(dst), a.in[SI_INIT].p + row * a.in[SI_INIT].so);
@@ -828,32 +867,41 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(ScanArgs a) {
 #pragma unroll
                 for (int j = 0; j < kRun; j += 4) *reinterpret_cast<float4*>(to + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
                 __syncwarp();
-                if (SUB == 32 && whole_tile(cut)) {
+                if constexpr (SUB == 32) {
                     float* to_g = out + row * a.T + 4 * cut.v0 - cut.shift + 4 * l;
+                    auto move = [&](unsigned in) {
 #pragma unroll
-                    for (int u = 0; u < kVectors / 32; ++u) {
-                        float f[4];
-                        load_shared<4>(&tile.out[4 * l + 128 * u], f);
-                        store_vec<4>(to_g + 128 * u, f, BACKWARD);
-                    }
-                    __syncwarp();
-                    return;
-                }
-#pragma unroll 1
-                for (int u = 0; u < kVectors / 32; ++u) {
-                    const int at_v = l + 32 * u, v = at_v % VR;
-                    const int64_t r = row0 + at_v / VR;
-                    const Cutout e = SUB == 32 ? cut : cutout(r, static_cast<Count>(here.end), r0);
-                    if (v < e.lo || v >= e.lo + e.n) continue;
-                    const Count t = 4 * (e.v0 + v) - e.shift;
-                    float f[4];
-                    load_shared<4>(&tile.out[4 * at_v], f);
-                    if (t >= 0 && t + 3 < a.T) {
-                        store_vec<4>(out + r * a.T + t, f, BACKWARD);
+                        for (int u = 0; u < kVectors / 32; ++u) {
+                            float f[4];
+                            load_shared<4>(&tile.out[4 * l + 128 * u], f);
+                            if (in >> u & 1) store_vec<4>(to_g + 128 * u, f, BACKWARD);
+                        }
+                    };
+                    if (whole_tile(cut)) {
+                        move(~0u);
                     } else {
+                        move(inside_vectors(cut));
+                        Count t;
+                        const int e = edge(cut, t);
+                        if (e >= 0) out[row * a.T + t] = tile.out[e];
+                    }
+                } else {
+#pragma unroll 1
+                    for (int u = 0; u < kVectors / 32; ++u) {
+                        const int at_v = l + 32 * u, v = at_v % VR;
+                        const int64_t r = row0 + at_v / VR;
+                        const Cutout e = cutout(r, static_cast<Count>(here.end), r0);
+                        if (v < e.lo || v >= e.lo + e.n) continue;
+                        const Count t = 4 * (e.v0 + v) - e.shift;
+                        float f[4];
+                        load_shared<4>(&tile.out[4 * at_v], f);
+                        if (t >= 0 && t + 3 < a.T) {
+                            store_vec<4>(out + r * a.T + t, f, BACKWARD);
+                        } else {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (t + j >= 0 && t + j < a.T) out[r * a.T + t + j] = f[j];
+                            for (int j = 0; j < 4; ++j)
+                                if (t + j >= 0 && t + j < a.T) out[r * a.T + t + j] = f[j];
+                        }
                     }
                 }
                 __syncwarp();
@@ -974,10 +1022,18 @@ Cut cut(const ScanDesc& d) {
         c.blocks = (lanes + 256 * c.V - 1) / (256 * c.V);
         return c;
     }
-    const int64_t len = c.rows ? (d.T + 6) / 4 : d.T;  // rows count time in vectors of four
+    // rows count time in vectors of four, from the boundary at or before their first step on: at most `cut` less
+    // the power of two that divides both T and it
+    auto row_vectors = [&](int64_t cut) {
+        int64_t two = cut;
+        while (d.T % two != 0) two /= 2;
+        return (d.T + cut - two + cut - 1) / cut * (cut / 4);
+    };
+    int64_t len = c.rows ? row_vectors(kRowCut<4>) : d.T;
     const int run = d.backward ? kRowRun<true> : kRowRun<false>;
     while (c.rows && c.sub > 4 && len <= c.sub / 2 * run / 4) c.sub /= 2;
     if (c.rows) c.tile = c.sub * run / 4;
+    if (c.rows && c.sub == 32) len = row_vectors(kRowCut<32>);
     auto warps = [&](int64_t t) {  // along time
         int w = 1;
         while (w < kWarps && w * t < len) w *= 2;
