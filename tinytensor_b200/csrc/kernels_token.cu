@@ -7,7 +7,7 @@
 //
 // What bounds them is the logits: 4 bytes a value read, 4 written where the gradient is
 // wanted.  A loss and its gradient are one kernel that reads a row once: its values stay in
-// registers between the row's maximum and sum and the gradient's write.  A row that no CTA
+// registers or shared memory between the row's maximum and sum and the gradient's write.  A row that no CTA
 // can hold is held by a cluster of up to 8, whose parts' (maximum, sum) are joined through
 // distributed shared memory; so are rows that are too few to fill the card.
 // The preference loss's slope depends on all rows of its pair, so its gradient is a second
@@ -354,7 +354,9 @@ __device__ __forceinline__ void hand_part(Parts& sh, int size, int slot, int l, 
 }
 
 // ---- short rows: a warp holds a row of at most 128*NV values, 8 rows a CTA.  Without a gradient a
-// row may be longer: the warp walks it, joining maximum and sum as it goes.
+// row may be longer: the warp walks it, joining maximum and sum as it goes: 8192 rows of 16384, a fifth
+// of them padding, take 84 us (5.0 TB/s; the rows are 1.4 rounds of the card's warps).  A CTA a row took
+// 90, a warp that loads ahead of its sums 88.
 template <int NV, bool GRAD>
 __global__ void __launch_bounds__(256, NV == 16 ? 2 : GRAD || NV == 8 ? 4 : 5) token_warp_kernel(TokenArgs a) {
     const int l = threadIdx.x & 31;
@@ -395,7 +397,8 @@ __global__ void __launch_bounds__(256, NV == 16 ? 2 : GRAD || NV == 8 ? 4 : 5) t
 
 // ---- values without a gradient, and rows longer than a cluster can hold: every CTA walks its
 // share of a row once, joining maximum and sum as it goes; for the gradient it reads it a second
-// time (mostly from L2, latest first).  Few rows are shared by a cluster.
+// time (mostly from L2, latest first).  Few rows are shared by a cluster: 8 rows of 131072 take 10 us on
+// 8 CTAs each, a launch, three loads' latencies and the cluster's exchange.
 constexpr int kStream = 256, kStreamVec = 8;
 constexpr int kWalk = 4096;  // vectors of the longest row that one warp walks
 
@@ -474,6 +477,9 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(TokenArgs a) {
 //   join:  info(n + 4), parts full(n) -> exchange -> scalars(n) -> scalars full(n)
 // What bounds it besides the bytes is the instructions a row costs on top of its values, so warps
 // whose vectors all lie inside the row move them without checks.
+// Clusters of 4 (71 run at a time: 284 of the 296 places) take 336 us for 8192 rows of 32768 with a ninth of
+// them padding (5.7 TB/s), 164 us for 4096 of 32001 (5.5); clusters of 7 (37: 259 places) 154 us for
+// 2177 of 50001 (4.8).
 struct RowInfo {
     const float* x;
     float* dx;
@@ -735,7 +741,9 @@ __global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(To
     if (size > 1) cl.sync();  // nobody writes to a CTA that has left
 }
 
-// ---- preference loss.  A pair's loss and slope from S(0) - S(1), by one thread.
+// ---- preference loss: the rows' stats, the pairs, the rows again.  8 pairs of 2x512x16384 take 84, 4 and
+// 146 us: the gradient's pass runs at the copy bandwidth.  A pair's loss and slope
+// from S(0) - S(1), by one thread.
 __device__ __forceinline__ float pair_value(const TokenArgs& a, int64_t n, double diff, bool write) {
     const double beta = a.f0, eps = a.f1, z = beta * diff;
     const double e = exp(-fabs(z)), soft = log1p(e);  // soft = -log sigmoid(|z|)
@@ -768,7 +776,8 @@ __global__ void __launch_bounds__(kPair) preference_pair_kernel(TokenArgs a) {
 }
 
 // A pair in one cluster and one launch: its warps walk the pair's rows, the CTAs' sums of p - ref are
-// joined, and each warp walks its rows again, latest first, for the gradient.
+// joined, and each warp walks its rows again, latest first, for the gradient.  3 pairs of 2x37x257: 14 us in a
+// stream that is flushed before it, 10 us a call; latency.
 constexpr int kPairCluster = 8;
 template <int NV>
 __global__ void __launch_bounds__(256, 4) preference_cluster_kernel(TokenArgs a) {
