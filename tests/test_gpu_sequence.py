@@ -269,6 +269,15 @@ def test_token_logprob(cache_dir, V):
     _check(out, R.logprob(x, k, g))
 
 
+@pytest.mark.parametrize("V, rows", [(9200, 300), (9216, 300), (9217, 150), (35001, 80), (73728, 40), (73725, 3), (73729, 3)])
+def test_token_logprob_at_most_vectors_a_thread(cache_dir, V, rows):
+    """Rows that just fit a cluster's threads, or just do not, and enough of them for the fewest CTAs."""
+    rng = np.random.default_rng(V)
+    x, k, g = _f32(rng.standard_normal([rows, V])), _tokens(rng, [rows], V), _f32(rng.standard_normal([rows]))
+    out = _run_tokens(cache_dir, tt.token_logprob, x, k, [], g)
+    _check(out, R.logprob(x, k, g))
+
+
 @pytest.mark.parametrize("rows", [1, 2, 9, 149, 600, 3000])
 @pytest.mark.parametrize("V", [7, 300])
 def test_token_logprob_rows(cache_dir, rows, V):

@@ -478,8 +478,8 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(TokenArgs a) {
 // What bounds it besides the bytes is the instructions a row costs on top of its values, so warps
 // whose vectors all lie inside the row move them without checks.
 // Clusters of 4 (71 run at a time: 284 of the 296 places) take 336 us for 8192 rows of 32768 with a ninth of
-// them padding (5.7 TB/s), 164 us for 4096 of 32001 (5.5); clusters of 7 (37: 259 places) 154 us for
-// 2177 of 50001 (4.8).
+// them padding (5.7 TB/s), 164 us for 4096 of 32001 (5.5); clusters of 6 147 us for 2177 of
+// 50001 (5.0).
 struct RowInfo {
     const float* x;
     float* dx;
@@ -962,14 +962,17 @@ cudaError_t launch_row_kernel(const TokenArgs& a, cudaStream_t stream) {
         else token_warp_kernel<GRAD ? 16 : 8, GRAD><<<grid, 256, 0, stream>>>(a);
         return cudaGetLastError();
     }
-    // as many CTAs a row as hold it, and more while the rows do not fill the card
+    // As many CTAs a row as hold it, and more while the rows do not fill the card.  Of 256 threads with up to 9
+    // vectors each, for which two CTAs an SM have the shared memory (2^27 values, 9 vectors at most against 8:
+    // rows of 36000 167 us on 4 CTAs, 178 on 5; 50001 175 on 6, 182 on 7; 9000 177 on 1, 187 on 2; 66000 183,
+    // 231 with 512 threads; rows of 18000 are slower, 178 on 2, 175 on 3), then of 512.
     const bool held = GRAD && vectors <= kMaxCluster * 512 * 8;
-    const int G = held && vectors > kMaxCluster * 256 * 8 ? 512 : 256;
-    int cluster = held ? (vectors + G * 8 - 1) / (G * 8) : GRAD ? kMaxCluster : 1;
+    const int G = held && vectors > kMaxCluster * 256 * 9 ? 512 : 256, most = G == 256 ? 9 : 8;
+    int cluster = held ? (vectors + G * most - 1) / (G * most) : GRAD ? kMaxCluster : 1;
     while (cluster < kMaxCluster && a.rows * cluster < 296 && cluster * G < vectors) ++cluster;
     if constexpr (GRAD) {
         if (held) {
-            // no more vectors a thread than it takes: rows of 33000 are 7 a thread of 5 CTAs (8 left the
+            // no more vectors a thread than it takes: rows of 40000 are 8 a thread of 5 CTAs (9 left the
             // fifth nearly empty and its ring as large as the others')
             if (G == 512) return launch_grad<512, 8>(a, cluster, stream);
             switch ((vectors + cluster * G - 1) / (cluster * G)) {
@@ -979,7 +982,8 @@ cudaError_t launch_row_kernel(const TokenArgs& a, cudaStream_t stream) {
                 case 5: return launch_grad<256, 5>(a, cluster, stream);
                 case 6: return launch_grad<256, 6>(a, cluster, stream);
                 case 7: return launch_grad<256, 7>(a, cluster, stream);
-                default: return launch_grad<256, 8>(a, cluster, stream);
+                case 8: return launch_grad<256, 8>(a, cluster, stream);
+                default: return launch_grad<256, 9>(a, cluster, stream);
             }
         }
     }
