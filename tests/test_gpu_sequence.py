@@ -345,6 +345,20 @@ def test_preference_loss(cache_dir, T, V):
         _check(out, R.preference(np.nan_to_num(x, neginf=-np.inf), k, ref, beta, smoothing, g))
 
 
+@pytest.mark.parametrize("N, T, V", [(200, 4, 300), (150, 5, 1025), (149, 1, 77), (40, 40, 1500), (2, 300, 701), (2, 290, 701), (33, 40, 2049)])
+def test_preference_loss_of_many_short_rows(cache_dir, N, T, V):
+    """Sizes around which the gradient's form changes."""
+    rng = np.random.default_rng(N + T + V)
+    shape, beta = [N, 2, T], 0.2
+    x, k = _f32(3 * rng.standard_normal(shape + [V])), _tokens(rng, shape, V, empty=False)
+    k[1, 0], k[N - 1, 1] = -1, -1
+    x[1, 0] = np.nan
+    x0 = np.nan_to_num(x)
+    ref, g = _f32(R.logprob(x0, k)[0][0] + 0.3 * rng.standard_normal(shape)), _f32(rng.standard_normal([N]))
+    out = _run_tokens(cache_dir, lambda a, b, r: tt.preference_loss(a, b, r, beta=beta, smoothing=0.125), x, k, [ref], g)
+    _check(out, R.preference(x0, k, ref, beta, 0.125, g))
+
+
 def test_preference_loss_saturates(cache_dir):
     """Sums far apart: the loss is -z or 0 and its slope -beta or 0, without overflow."""
     x = np.zeros([2, 2, 1, 4], np.float32)

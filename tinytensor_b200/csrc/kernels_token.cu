@@ -775,6 +775,31 @@ __global__ void __launch_bounds__(kPair) preference_pair_kernel(TokenArgs a) {
     if (a.slopes) a.slopes[n] = slope;
 }
 
+// The gradient of a row from its stats, by one warp.
+__device__ __forceinline__ void row_gradient(const TokenArgs& a, const Row& r, float c, int l) {
+    constexpr int NV = 4;
+    if (r.token < 0 || r.token >= a.V) {
+        const float f = r.token < 0 ? 0.0f : __int_as_float(0x7fc00000), v[4] = {f, f, f, f};
+        const int out = static_cast<int>(reinterpret_cast<uintptr_t>(r.dx) / 4 % 4);
+        for (int j = 4 * l - out; j < a.V; j += 128) store_vec(r.dx, j, a.V, true, v);
+        return;
+    }
+    const float m = __ldcg(a.stats + 3 * r.row), scale = -c * __ldcg(a.stats + 3 * r.row + 1);
+    for (int j = -r.shift; j < a.V; j += 128 * NV) {
+        float v[NV][4];
+#pragma unroll
+        for (int q = 0; q < NV; ++q) load_vec(r.x, j + 4 * (l + 32 * q), a.V, true, v[q]);
+#pragma unroll
+        for (int q = 0; q < NV; ++q) {
+            const int at = j + 4 * (l + 32 * q);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[q][u] = exp_part(v[q][u] - m);
+            grad_vec(v[q], at, r.token, scale, c);
+            store_vec(r.dx, at, a.V, r.dx_vec, v[q]);
+        }
+    }
+}
+
 // A pair in one cluster and one launch: its warps walk the pair's rows, the CTAs' sums of p - ref are
 // joined, and each warp walks its rows again, latest first, for the gradient.  3 pairs of 2x37x257: 14 us in a
 // stream that is flushed before it, 10 us a call; latency.
@@ -830,32 +855,21 @@ __global__ void __launch_bounds__(256, 4) preference_cluster_kernel(TokenArgs a)
     __syncthreads();
     const float slope = sh_slope;
     for (i -= step; i >= 0; i -= step) {
-        const Row r(a, n * a.n1 + i);
-        if (r.token < 0 || r.token >= a.V) {
-            const float f = r.token < 0 ? 0.0f : __int_as_float(0x7fc00000), v[4] = {f, f, f, f};
-            const int out = static_cast<int>(reinterpret_cast<uintptr_t>(r.dx) / 4 % 4);
-            for (int j = 4 * l - out; j < a.V; j += 128) store_vec(r.dx, j, a.V, true, v);
-            continue;
-        }
-        // (the warp's own stats: written by lane 0 above)
-        const float m = __ldcg(a.stats + 3 * r.row), c = i < T ? slope : -slope, scale = -c * __ldcg(a.stats + 3 * r.row + 1);
-        for (int j = -r.shift; j < a.V; j += 128 * NV) {
-            float v[NV][4];
-#pragma unroll
-            for (int q = 0; q < NV; ++q) load_vec(r.x, j + 4 * (l + 32 * q), a.V, true, v[q]);
-#pragma unroll
-            for (int q = 0; q < NV; ++q) {
-                const int at = j + 4 * (l + 32 * q);
-#pragma unroll
-                for (int u = 0; u < 4; ++u) v[q][u] = exp_part(v[q][u] - m);
-                grad_vec(v[q], at, r.token, scale, c);
-                store_vec(r.dx, at, a.V, r.dx_vec, v[q]);
-            }
-        }
+        row_gradient(a, Row(a, n * a.n1 + i), i < T ? slope : -slope, l);  // (the warp's own stats, written by lane 0 above)
     }
 }
 
-// The preference loss's gradient from the rows' stats: a CTA takes kGradVec*kGrad vectors of a row.
+// The preference loss's gradient from the rows' stats, a warp a row: many short rows, which leave most of a CTA
+// idle (1000 pairs of 2x64x300 133 us, 498 with a CTA a row; 768 rows of 1000 20 against 15).
+__global__ void __launch_bounds__(256) preference_grad_rows_kernel(TokenArgs a) {
+    const int64_t index = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (index >= a.rows) return;
+    const Row r(a, a.rows - 1 - index);
+    const float slope = __ldg(a.slopes + r.i0);
+    row_gradient(a, r, r.i1 < a.n1 / 2 ? slope : -slope, threadIdx.x & 31);
+}
+
+// The same of longer or few rows: a CTA takes kGradVec*kGrad vectors of a row.
 constexpr int kGrad = 256, kGradVec = 4;
 __global__ void __launch_bounds__(kGrad) preference_grad_kernel(TokenArgs a, int per_row) {
     const Row r(a, a.rows - 1 - blockIdx.x / per_row);
@@ -886,13 +900,14 @@ int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 // A pair in one cluster (one launch) or all rows, then all pairs, then all rows again (three).
 bool pairs_in_clusters(const TokenDesc& d) {
     if (d.n0 == 0 || d.n1 == 0 || d.n0 > 0x7fffffff / kPairCluster) return false;
-    // Clusters save two launches where the pairs are small, and a read from memory where the pairs that
-    // run at the same time stay in L2: 64 pairs of 2x64x4096 65 us against 93, 1000 of 2x16x1000 113
-    // against 149; but 8 clusters do not fill the card, and a warp per row is slow on long rows:
-    // 8 of 2x512x16384 669 against 262, 24 of 2x3x41309 109 against 26.
-    const int64_t pair = d.n1 * d.V;
-    if (d.n0 * pair <= 1 << 20) return d.V <= 4096;
-    return d.n0 >= 16 && d.n1 >= 16 && d.V <= 8192 && pair * (d.n0 < 74 ? d.n0 : 74) <= 40000000;
+    // Clusters save two launches where pairs are few and small (us, a cluster a pair against three launches: 3 of
+    // 2x37x257 11 against 13, 60 of 2x32x250 11 against 17, 16 of 2x64x1000 15 against 17; but 16 of 2x128x1000 25
+    // against 19, 128 of 2x64x250 29 against 25), and a read from memory where the pairs that run at the same time
+    // stay in L2 and their rows are long (64 of 2x64x4096 60 against 87, 100 of 2x64x2000 51 against 54; but 16 of
+    // 2x256x4000 113 against 64, 1000 of 2x16x1000 117 against 70, 16 of 2x128x8000 116 against 65).
+    const int64_t passes = (d.n1 + 63) / 64;  // rows of a warp
+    if (passes <= 2 && passes * ((d.V + 1023) / 1024) <= 4 && d.n0 * passes <= 148) return true;
+    return d.n0 >= 32 && d.n0 <= 256 && d.n1 >= 64 && d.n1 <= 256 && d.V > 1024 && d.V <= 4096;
 }
 
 // Launch configuration of `blocks` CTAs in clusters.
@@ -1049,7 +1064,9 @@ int launch_token(const TokenDesc& d, const void* const* in, float* y, float* dlo
         if (e != cudaSuccess) return static_cast<int>(e);
     }
     preference_pair_kernel<<<static_cast<unsigned>(d.n0), kPair, 0, st>>>(a);
-    if (dlogits && a.rows > 0)
+    if (dlogits && a.rows > 0 && per_row == 1 && a.rows >= 148 * 8)
+        preference_grad_rows_kernel<<<static_cast<unsigned>((a.rows + 7) / 8), 256, 0, st>>>(a);
+    else if (dlogits && a.rows > 0)
         preference_grad_kernel<<<static_cast<unsigned>(a.rows * per_row), kGrad, 0, st>>>(a, static_cast<int>(per_row));
     return static_cast<int>(cudaGetLastError());
 }
