@@ -88,7 +88,9 @@ def test_scan_broadcast_gates(cache_dir, gate_shape):
     ([2, 40, 3, 32], [2, 40, 3, 1], 1), ([2, 300, 2, 64], [2, 300, 2, 1], 1), ([1, 17, 5, 96], [1, 17, 5, 1], 1),
     ([2, 33, 3, 2], [2, 33, 3, 1], 1), ([2, 33, 3, 4], [2, 33, 3, 1], 1), ([3, 33, 1, 16], [3, 33, 1, 1], 1),
     ([2, 50, 128], [2, 50, 1], 1), ([2, 50, 2, 2, 16], [2, 50, 2, 1, 1], 1), ([2, 50, 3, 5], [2, 50, 3, 1], 1),
-    ([50, 3, 64], [50, 3, 1], 0), ([2, 5, 3, 64], [2, 5, 3, 1], 1), ([1, 9000, 64], [1, 9000, 1], 1)])
+    ([50, 3, 64], [50, 3, 1], 0), ([2, 5, 3, 64], [2, 5, 3, 1], 1), ([1, 9000, 64], [1, 9000, 1], 1),
+    ([2, 40, 3, 7], [2, 40, 3, 1], 1), ([2, 33, 1, 100], [2, 33, 1, 1], 1), ([2, 5, 3, 3], [2, 5, 3, 1], 1), ([1, 2, 2, 130], [1, 2, 2, 1], 1),
+    ([1, 9000, 2, 37], [1, 9000, 2, 1], 1), ([1, 40, 2, 1139], [1, 40, 2, 1], 1), ([1, 20, 4128], [1, 20, 1], 1)])
 def test_scan_shared_gates(cache_dir, shape, gate_shape, axis):
     _check_scan(cache_dir, shape, axis, gate_shape=gate_shape, seed=sum(shape))
 

@@ -300,12 +300,12 @@ def test_scan_gradients_share_a_launch(cache_dir):
 
 
 def test_a_shared_gates_gradient_is_summed_in_the_scan(cache_dir):
-    for dh, sums in ((64, True), (5, False)):
+    for gate, dh, sums in (([2, 50, 3, 1], 64, True), ([2, 50, 3, 1], 5, True), ([2, 50, 1, 64], 64, False)):
         g = tt.Graph()
-        a, x, d = g.input([2, 50, 3, 1]), g.input([2, 50, 3, dh]), g.input([2, 50, 3, dh])
+        a, x, d = g.input(gate), g.input([2, 50, 3, dh]), g.input([2, 50, 3, dh])
         p = tt.compile_gradients(g, tt.gated_scan(a, x, axis=1), [a, x], outputs=[], seed=d, cache_dir=cache_dir, flags=HOST)
         assert any("reduce_sum" in ln for ln in _launches(p)[1]) != sums
-        assert p.output_shapes == [[2, 50, 3, 1], [2, 50, 3, dh]]
+        assert p.output_shapes == [gate, [2, 50, 3, dh]]
 
 
 def test_states_only_scan_last_reads_are_not_stored(cache_dir):

@@ -993,11 +993,18 @@ __global__ void __launch_bounds__(256) scan_short_kernel(ScanArgs a) {
     if (a.out[SO_LANE]) store_vec<V>(a.out[SO_LANE] + lane, s, false);
 }
 
+// Of the lanes that dgate is summed over, those that a warp sums: groups that do not line up with warps are
+// summed by a second launch alone.
+int64_t warp_group(const ScanDesc& d) {
+    const int64_t g = d.group;
+    return g % 32 == 0 ? 32 : g == 2 || g == 4 || g == 8 || g == 16 ? g : 1;
+}
+
 // The widest vectors of lanes: every operand has adjacent lanes behind n1 whose vectors are
 // aligned wherever they start (buffers start on 16 bytes), or is broadcast over them.
 int widest(const ScanDesc& d) {
     for (int v = 4; v > 1; v /= 2) {
-        bool ok = d.n2 % v == 0 && (d.group == 1 || d.group % v == 0);
+        bool ok = d.n2 % v == 0 && (warp_group(d) == 1 || d.group % v == 0);
         for (int k = 0; k < SI_COUNT && ok; ++k) {
             const ScanStrides& s = d.in[k];  // (all 0 where absent)
             if (s.s2 == 0) continue;
@@ -1019,7 +1026,7 @@ struct Cut {
 Cut cut(const ScanDesc& d) {
     Cut c;
     const int64_t inner = d.n1 * d.n2, lanes = d.outer * inner;
-    c.direct = d.T <= kShort && d.group == 1;
+    c.direct = d.T <= kShort && warp_group(d) == 1;
     c.rows = inner == 1 && !c.direct;  // (no groups there: they are lanes)
     if (inner > 1) c.V = widest(d);
     if (c.direct) {
@@ -1152,8 +1159,9 @@ cudaError_t launch_cut(const Cut& c, const ScanArgs& a, cudaStream_t stream) {
     return e != cudaSuccess ? e : launch_pass<BACKWARD, JOINED>(c, a, stream);
 }
 
-// dgate of groups of more than 32 lanes: the sums of 32 lanes each, added in order (4 us for 4 x 2048 x 16 heads
-// of 64: a launch).
+// dgate of groups of lanes from the sums of a warp's lanes, or from all lanes, in order and in double: a thread
+// a sum, or a warp where a thread would walk far.  4 x 2048 x 16 heads of 64: 4 us, a launch; 26 x 4487 x 8 heads
+// of 3 8 us, 4 x 56527 heads of 37 14 us.
 __global__ void __launch_bounds__(256) gate_group_kernel(const float* __restrict__ part, float* __restrict__ out, int64_t n, int parts) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (i >= n) return;
@@ -1161,17 +1169,41 @@ __global__ void __launch_bounds__(256) gate_group_kernel(const float* __restrict
     for (int k = 0; k < parts; ++k) s += static_cast<double>(__ldg(part + i * parts + k));
     out[i] = static_cast<float>(s);
 }
+__global__ void __launch_bounds__(256) gate_group_warp_kernel(const float* __restrict__ part, float* __restrict__ out, int64_t n, int64_t parts) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (i >= n) return;
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    const float* p = part + i * parts;
+    int64_t k = threadIdx.x & 31;
+    for (; k + 96 < parts; k += 128)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s[u] += static_cast<double>(__ldg(p + k + 32 * u));
+    for (; k < parts; k += 32) s[0] += static_cast<double>(__ldg(p + k));
+    double t = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) t += __shfl_xor_sync(0xffffffffu, t, d);
+    if ((threadIdx.x & 31) == 0) out[i] = static_cast<float>(t);
+}
+cudaError_t sum_groups(const float* part, float* out, int64_t n, int64_t parts, cudaStream_t stream) {
+    const bool thread = parts <= 64;
+    const int64_t blocks = thread ? (n + 255) / 256 : (n + 7) / 8;
+    if (blocks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    const dim3 grid(static_cast<unsigned>(blocks));
+    if (thread) gate_group_kernel<<<grid, 256, 0, stream>>>(part, out, n, static_cast<int>(parts));
+    else gate_group_warp_kernel<<<grid, 256, 0, stream>>>(part, out, n, parts);
+    return cudaGetLastError();
+}
 
 int64_t maps_bytes(const ScanDesc& d, const Cut& c) {
     const int64_t b = c.segments > 1 ? c.segments * d.outer * d.n1 * d.n2 * static_cast<int64_t>(sizeof(float2)) : 0;
     return (b + 255) / 256 * 256;
 }
-int64_t group_parts(const ScanDesc& d) { return d.group > 32 ? d.group / 32 : 1; }
+int64_t group_parts(const ScanDesc& d) { return d.group / warp_group(d); }
 
 }  // namespace
 
 int64_t scan_scratch_bytes(const ScanDesc& d) {
-    const int64_t sums = group_parts(d) > 1 ? d.outer * d.T * (d.n1 * d.n2 / 32) * static_cast<int64_t>(sizeof(float)) : 0;
+    const int64_t sums = group_parts(d) > 1 ? d.outer * d.T * (d.n1 * d.n2 / warp_group(d)) * static_cast<int64_t>(sizeof(float)) : 0;
     return maps_bytes(d, cut(d)) + sums;
 }
 
@@ -1204,17 +1236,14 @@ int launch_scan(const ScanDesc& d, const float* const* in, float* const* out, vo
     a.seg_len = c.seg_len;
     a.segments = c.segments;
     a.group = 0;
-    while (a.group < 5 && (2 << a.group) <= d.group) ++a.group;
+    while (1 << a.group < warp_group(d)) ++a.group;
     a.units = c.blocks * c.segments;
     a.steps = static_cast<int>(c.steps);
     a.W = c.W;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e = d.backward ? launch_cut<true>(c, a, st) : launch_cut<false>(c, a, st);
     if (e == cudaSuccess && sums && d.T > 0) {
-        const int64_t n = lanes / d.group * d.T, blocks = (n + 255) / 256;
-        if (blocks > 0x7fffffff) return static_cast<int>(cudaErrorInvalidConfiguration);
-        gate_group_kernel<<<static_cast<unsigned>(blocks), 256, 0, st>>>(a.out[SO_GATE], out[SO_GATE], n, static_cast<int>(group_parts(d)));
-        e = cudaGetLastError();
+        e = sum_groups(a.out[SO_GATE], out[SO_GATE], lanes / d.group * d.T, group_parts(d), st);
     }
     return static_cast<int>(e);
 }

@@ -115,7 +115,7 @@ struct ScanDesc {
     // backward: gate, x = upstream g (absent: 0), carry = upstream gradient of the last
     // state (absent: 0), h, init -> main = dx, lane = dinit, gate = dgate.
     bool backward = false;
-    int64_t group = 1;  // backward: dgate is summed over this many adjacent lanes (sums_gate_group)
+    int64_t group = 1;  // backward: dgate is summed over this many adjacent lanes
     int64_t outer = 1, T = 0, n1 = 1, n2 = 1;
     ScanStrides in[SI_COUNT];
 };

@@ -73,10 +73,6 @@ enum BackwardOp {
     BOP_POLICY_GRAD = 68,
     BOP_PREFERENCE_GRAD = 69
 };
-// Adjacent lanes that a scan's launch can sum a shared gate's gradient over.
-inline bool sums_gate_group(int64_t group) {
-    return group > 1 && (group % 32 == 0 || group == 2 || group == 4 || group == 8 || group == 16);
-}
 bool is_scan(int op);      // GatedScan, ScanLast and the scan's backward nodes
 bool is_token_op(int op);  // the three token operators and their backward nodes
 
