@@ -271,7 +271,8 @@ def test_token_logprob(cache_dir, V):
     _check(out, R.logprob(x, k, g))
 
 
-@pytest.mark.parametrize("V, rows", [(9200, 300), (9216, 300), (9217, 150), (35001, 80), (73728, 40), (73725, 3), (73729, 3)])
+@pytest.mark.parametrize("V, rows", [(9200, 300), (9216, 300), (9217, 150), (35001, 80), (73728, 40), (73725, 3), (73729, 3),
+                                     (2049, 600), (2560, 592), (2561, 600), (3069, 592), (3077, 600)])
 def test_token_logprob_at_most_vectors_a_thread(cache_dir, V, rows):
     """Rows that just fit a cluster's threads, or just do not, and enough of them for the fewest CTAs."""
     rng = np.random.default_rng(V)

@@ -535,7 +535,7 @@ __device__ __forceinline__ bool exchange_wait(uint32_t bar, uint32_t parity, int
 }
 
 template <int G, int NV>
-__global__ void __launch_bounds__(G + 32, G == 512 ? 1 : 2) token_grad_kernel(TokenArgs a, int clusters) {
+__global__ void __launch_bounds__(G + 32, 512 / G) token_grad_kernel(TokenArgs a, int clusters) {
     constexpr int N = G + 32, FULL = 1, SCALARS = 3;  // barrier ids (+ parity)
     extern __shared__ __align__(16) float ring[];     // [stage][vector][thread][4]
     __shared__ Part warp_parts[2][G / 32], cta_parts[2][kMaxCluster];
@@ -987,9 +987,14 @@ cudaError_t launch_row_kernel(const TokenArgs& a, cudaStream_t stream) {
     while (cluster < kMaxCluster && a.rows * cluster < 296 && cluster * G < vectors) ++cluster;
     if constexpr (GRAD) {
         if (held) {
+            if (G == 512) return launch_grad<512, 8>(a, cluster, stream);
+            // Rows that 128 threads hold, and enough of them: four small CTAs an SM have more rows under way than
+            // two (32768 rows of 2500 107 us against 134, 6000 of 2132 29 against 35; but rows of 4000, at 8 vectors
+            // a thread, 180 against 154).
+            if (vectors <= 128 * 6 && a.rows >= 4 * 148)
+                return vectors <= 128 * 5 ? launch_grad<128, 5>(a, 1, stream) : launch_grad<128, 6>(a, 1, stream);
             // no more vectors a thread than it takes: rows of 40000 are 8 a thread of 5 CTAs (9 left the
             // fifth nearly empty and its ring as large as the others')
-            if (G == 512) return launch_grad<512, 8>(a, cluster, stream);
             switch ((vectors + cluster * G - 1) / (cluster * G)) {
                 case 1: case 2: return launch_grad<256, 2>(a, cluster, stream);
                 case 3: return launch_grad<256, 3>(a, cluster, stream);
