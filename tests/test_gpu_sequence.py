@@ -206,6 +206,33 @@ def test_scan_is_deterministic(cache_dir):
         assert [o.numpy().tobytes() for o in p.run({a: gate, b: x, c: s, d: dh})] == first
 
 
+@pytest.mark.parametrize("dense_first", [True, False])
+def test_scans_that_share_an_expanded_operand(cache_dir, dense_first):
+    """One scan takes the expanded node as a dense x, the other as its gate beside a transposed x."""
+    rng = np.random.default_rng(16)
+    av, yv, dv = _f32(rng.random([2, 5, 3, 1])), _f32(rng.standard_normal([2, 5, 4, 3])), _f32(rng.random([2, 5, 3, 4]))
+    for steps in (5, 50):  # (the thread-a-lane kernel and the tiled one)
+        n = steps // 5
+        av2, yv2, dv2 = (np.tile(v, [1, n, 1, 1]) for v in (av, yv, dv))
+        g = tt.Graph()
+        a, y, d = g.input(av2.shape), g.input(yv2.shape), g.input(dv2.shape)
+        if dense_first:
+            h1 = tt.gated_scan(d, a, axis=1)
+            h2 = tt.gated_scan(a, tt.transpose(y, 2, 3), axis=1)
+        else:
+            h2 = tt.gated_scan(a, tt.transpose(y, 2, 3), axis=1)
+            h1 = tt.gated_scan(d, a, axis=1)
+        out = [o.numpy() for o in tt.compile_gradients(g, tt.sum(h1) + tt.sum(h2), [y, d], outputs=[h1, h2], cache_dir=cache_dir)
+               .run({a: av2, y: yv2, d: dv2})]
+        full = np.broadcast_to(av2, dv2.shape)
+        yt = yv2.transpose(0, 1, 3, 2)
+        R.assert_within(out[0], R.scan(dv2, full, None, 1)[0])
+        R.assert_within(out[1], R.scan(av2, yt, None, 1)[0])
+        dx = R.scan_grad(av2, yt, None, 1, np.ones(yt.shape), None)[1]
+        R.assert_within(out[2], tuple(v.transpose(0, 1, 3, 2) for v in dx))
+        R.assert_within(out[3], R.scan_grad(dv2, full, None, 1, np.ones(yt.shape), None)[0])
+
+
 # ---- token operators ---------------------------------------------------------------------------
 
 

@@ -437,3 +437,74 @@ def test_loss_definitions_against_differences(kind):
     got = f(x, g)[1][0]
     want = _differences(lambda v: (f(v)[0][0] * g).sum(), x)
     assert np.allclose(got, want, atol=1e-7)
+
+
+# ---- operands as the kernels address them --------------------------------------------------------
+
+
+def _addressed(line):
+    """(extents, {operand: (strides, offset)}) of a scan's line in the plan."""
+    def ints(t):
+        return [int(v) for v in t.split(",")]
+
+    over = ints(line.split("over=[")[1].split("]")[0])
+    words = line.split("over=")[1].split(" ->")[0].split()[1:]
+    ops = {w.split("=")[0]: (ints(w.split("[")[1].split("]")[0]), int(w.split("+")[1])) for w in words}
+    return over, ops
+
+
+def _last_index(over, strides, offset):
+    return offset + sum((n - 1) * s for n, s in zip(over, strides) if n > 0)
+
+
+@pytest.mark.parametrize("dense_first", [True, False])
+def test_scans_that_share_an_expanded_operand(cache_dir, dense_first):
+    """One scan needs a dense copy of the expanded node (as its x: no split of the dense gate's dims fits it),
+    the other reads it in place as its gate: neither's split or strides depend on the other."""
+    g = tt.Graph()
+    a, y, d = g.input([2, 5, 3, 1]), g.input([2, 5, 4, 3]), g.input([2, 5, 3, 4])
+
+    def dense():
+        return tt.gated_scan(d, a, axis=1)
+
+    def shared():
+        return tt.gated_scan(a, tt.transpose(y, 2, 3), axis=1)
+
+    h = [dense(), shared()] if dense_first else [shared(), dense()][::-1]
+    lines = [ln for ln in _launches(tt.compile(g, h, cache_dir=cache_dir, flags=HOST))[1] if "gated_scan" in ln]
+    seen = {}
+    for ln in lines:
+        over, ops = _addressed(ln)
+        seen[ln.split("output:")[1].split()[0]] = (over, ops)
+        assert int(np.prod(over)) == 120
+        assert all(_last_index(over, s, o) < 120 for s, o in ops.values())
+    assert seen["0"] == ([2, 5, 1, 12], {"gate": ([60, 12, 0, 1], 0), "x": ([60, 12, 0, 1], 0)})
+    assert seen["1"] == ([2, 5, 3, 4], {"gate": ([15, 3, 1, 0], 0), "x": ([60, 12, 1, 3], 0)})
+
+
+def test_scans_over_shared_views_stay_inside_their_operands(cache_dir):
+    """Scans and their gradients over one pool of expanded and transposed nodes, in random roles and orders."""
+    rng = np.random.default_rng(0)
+    for _ in range(40):
+        g = tt.Graph()
+        full = [2, 5, 3, 4]
+        leaves = [g.input([2, 5, 3, 1]), g.input([2, 5, 4, 3]), g.input(full), g.input([1, 5, 1, 4]), g.input([2, 3, 5, 4])]
+        pool = [leaves[0], tt.transpose(leaves[1], 2, 3), leaves[2], leaves[3], tt.transpose(leaves[4], 1, 2)]
+        hs = []
+        for _ in range(4):
+            i, j = rng.integers(0, len(pool), 2)
+            if pool[i].shape != full and pool[j].shape != full:
+                j = 2
+            hs.append(tt.gated_scan(pool[i], pool[j], axis=int(rng.integers(0, 4))))
+        loss = hs[0] * hs[1]
+        for h in hs[2:]:
+            loss = loss + h
+        p = tt.compile_gradients(g, tt.sum(loss), leaves, outputs=hs, cache_dir=cache_dir, flags=HOST)
+        lines = [ln for ln in _launches(p)[1] if "gated_scan" in ln]
+        assert lines
+        for ln in lines:
+            over, ops = _addressed(ln)
+            assert int(np.prod(over)) == 120
+            for name, (s, o) in ops.items():
+                extents = [over[0], 1, over[2], over[3]] if name in ("carry", "init") else over
+                assert _last_index(extents, s, o) < 120, ln

@@ -517,12 +517,15 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
     };
     // Operands of scans and token losses.  A scalar constant becomes a one-element buffer
     // read with zero strides; a view whose strides the kernel cannot take becomes a dense
-    // copy.  Both are made once per node, so launches that share an operand still do.
+    // copy.  Both are made once per node, so launches that share an operand still do.  A view
+    // that fits is read where it is, though another launch may have needed a copy of it.
     std::map<int, int> dense_copy;
     auto operand = [&](int src, bool fits) {
+        const bool imm = p.st[static_cast<size_t>(src)].kind == SK_IMM;
+        if (fits && !imm) return src;
         auto it = dense_copy.find(src);
         if (it != dense_copy.end()) return it->second;
-        if (p.st[static_cast<size_t>(src)].kind == SK_IMM) {
+        if (imm) {
             Node c;
             c.op = TT_OP_CONSTANT;
             c.shape = g.nodes[static_cast<size_t>(src)].shape;  // the operand's shape, one stored value
@@ -537,7 +540,7 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
             p.region_of.push_back(-1);
             return dense_copy[src] = idx;
         }
-        return fits ? src : dense_copy[src] = materialise(src);
+        return dense_copy[src] = materialise(src);
     };
     // Flattened stride of dims [lo, hi) of a view: dims of size 1 carry none, broadcast
     // dims stride 0; false when the dims are not one arithmetic sequence.
@@ -604,6 +607,9 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
     };
 
     std::vector<int> launch_nodes;  // reduce / matmul / scan / token nodes, original order
+    // Where a scan's dims behind the axis are split: chosen once, before operands are replaced by copies
+    // (a copy fits any split, but another split need not fit the operands that were checked).
+    std::map<int, size_t> split_of;
     g.nodes.reserve(N0 * 6 + 8);      // materialise() appends nodes: no reference is held across it
     for (size_t i = 0; i < N0; ++i) {
         const int op = g.nodes[i].op;
@@ -639,7 +645,7 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
             launch_nodes.push_back(static_cast<int>(i));
         } else if (is_scan(op) && op != TT_OP_SCAN_LAST) {
             const size_t axis = static_cast<size_t>(g.nodes[i].dim0);
-            const size_t split = scan_split(g.nodes[i].in[0], axis);
+            const size_t split = split_of[static_cast<int>(i)] = scan_split(g.nodes[i].in[0], axis);
             for (size_t k = 0; k < g.nodes[i].in.size(); ++k) {
                 ScanStrides o;
                 const int src = g.nodes[i].in[k];
@@ -753,7 +759,7 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
                 for (int j : b.nodes)
                     if (g.nodes[static_cast<size_t>(i)].op == g.nodes[static_cast<size_t>(j)].op) return false;
             const size_t common = 1 + static_cast<size_t>(x.axes[0] != 0) + static_cast<size_t>(x.axes[1] != 0);
-            return x.dim0 == y.dim0 && x.axes == y.axes &&
+            return x.dim0 == y.dim0 && x.axes == y.axes && split_of.at(a.idx) == split_of.at(b.idx) &&
                    std::equal(x.in.begin(), x.in.begin() + static_cast<long>(common), y.in.begin());
         };
         auto reaches = [&](size_t from, size_t to) {
@@ -932,14 +938,16 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
             L.out_nodes.assign(SO_COUNT, -1);
             const Node& first = g.nodes[static_cast<size_t>(un.idx)];
             const Shape& sh = g.nodes[static_cast<size_t>(first.in[0])].shape;
-            const size_t axis = static_cast<size_t>(first.dim0), split = scan_split(first.in[0], axis);
+            const size_t axis = static_cast<size_t>(first.dim0), split = split_of.at(un.idx);
             d.backward = first.op != TT_OP_GATED_SCAN;
             d.T = sh[axis];
             for (size_t k = 0; k < axis; ++k) d.outer *= sh[k];
             for (size_t k = axis + 1; k < split; ++k) d.n1 *= sh[k];
             for (size_t k = split; k < sh.size(); ++k) d.n2 *= sh[k];
             auto bind = [&](const Node& n, size_t k, int slot) {
-                scan_strides(n.in[k], axis, split, lane_operand(n, k), d.in[slot]);
+                if (!scan_strides(n.in[k], axis, split, lane_operand(n, k), d.in[slot]))
+                    fail(TT_ERR_COMPILE, std::string("internal: the strides of operand ") + std::to_string(k) + " of " +
+                                             op_name(n.op) + " do not fit its launch");
                 L.in_nodes[static_cast<size_t>(slot)] = p.st[static_cast<size_t>(n.in[k])].root;
             };
             std::ostringstream lb;
@@ -995,7 +1003,9 @@ Plan schedule(const Graph& gin, const ScheduleOptions& opt) {
                     size_t slot = k;  // logits, tokens, old, advantage, ref
                     if (d.kind == TK_PREFERENCE && k == 2) slot = TI_REF;
                     if (bw && k + 1 == n.in.size()) slot = TI_GRAD;
-                    token_strides(n, k, d.s0[slot], d.s1[slot]);
+                    if (!token_strides(n, k, d.s0[slot], d.s1[slot]))
+                        fail(TT_ERR_COMPILE, std::string("internal: the strides of operand ") + std::to_string(k) + " of " +
+                                                 op_name(n.op) + " do not fit its launch");
                     d.off[slot] = p.st[static_cast<size_t>(n.in[k])].offset;
                     L.in_nodes[slot] = p.st[static_cast<size_t>(n.in[k])].root;
                 }
@@ -1393,6 +1403,22 @@ std::string plan_text(const Plan& p) {
                 ss << " copies=" << split_copies_bytes(r.copy_R, r.copy_C, r.copy_rows, r.copy_t) << "@"
                    << L.split_ref.offset;
         } else if (L.type == LT_SCAN || L.type == LT_TOKEN) {
+            // operands as the kernel addresses them: element strides over (outer, time, n1, n2) or (n0, n1)
+            static const char* const scan_in[SI_COUNT] = {"gate", "x", "carry", "h", "init"};
+            static const char* const token_in[TI_COUNT] = {"logits", "tokens", "old", "advantage", "ref", "g"};
+            if (L.type == LT_SCAN)
+                ss << " over=[" << L.sd.outer << "," << L.sd.T << "," << L.sd.n1 << "," << L.sd.n2 << "]";
+            else
+                ss << " over=[" << L.td.n0 << "," << L.td.n1 << "]";
+            for (size_t k = 0; k < L.in_refs.size(); ++k) {
+                if (L.in_refs[k].kind == BK_NONE) continue;
+                if (L.type == LT_SCAN) {
+                    const ScanStrides& q = L.sd.in[k];
+                    ss << " " << scan_in[k] << "=[" << q.so << "," << q.st << "," << q.s1 << "," << q.s2 << "]+" << q.off;
+                } else {
+                    ss << " " << token_in[k] << "=[" << L.td.s0[k] << "," << L.td.s1[k] << "]+" << L.td.off[k];
+                }
+            }
             ss << " ->";
             for (const BufRef& b : L.out_refs)
                 if (b.kind != BK_NONE) ss << " " << kind_name(b.kind) << ":" << (b.kind == BK_ARENA ? b.offset : b.index);
