@@ -233,6 +233,29 @@ def test_scans_that_share_an_expanded_operand(cache_dir, dense_first):
         R.assert_within(out[3], R.scan_grad(dv2, full, None, 1, np.ones(yt.shape), None)[0])
 
 
+@pytest.mark.parametrize("shape,axis", [([2, 5, 3], 1), ([2, 40, 5], 1), ([3, 50], 1), ([50, 3, 2], 0), ([4], 0), ([2, 1, 3], 1)])
+def test_gradient_of_the_states_themselves(cache_dir, shape, axis):
+    """d loss / d h takes in what the loss reads through scan_last, at the last step."""
+    gate, x, s, w, wl = _scan_data(shape, axis, True, 5)
+    for direct in (False, True):
+        for targets in (1, 2):  # (2: the target named twice, and x beside it)
+            g = tt.Graph()
+            a, b, c, nw, nl = g.input(shape), g.input(shape), g.input(s.shape), g.input(shape), g.input(wl.shape)
+            h = tt.gated_scan(a, b, init=c, axis=axis)
+            loss = tt.sum(tt.scan_last(h) * nl)
+            if direct:
+                loss = loss + tt.sum(h * nw)
+            wrt = [h] if targets == 1 else [h, b, h]
+            out = [o.numpy() for o in tt.compile_gradients(g, loss, wrt, outputs=[tt.scan_last(h)], cache_dir=cache_dir)
+                   .run({a: gate, b: x, c: s, nw: w, nl: wl})][1:]
+            want = w.astype(np.float64) if direct else np.zeros(shape)
+            np.moveaxis(want, axis, 0)[-1] += wl
+            for o in out[::2]:
+                R.assert_within(o, (want, R.U * np.abs(want)))
+            if targets == 2:
+                R.assert_within(out[1], R.scan_grad(gate, x, s, axis, w if direct else None, wl)[1])
+
+
 # ---- token operators ---------------------------------------------------------------------------
 
 

@@ -387,6 +387,26 @@ def test_existing_schedules_hold_a_scan_between_regions(cache_dir):
     assert [("gated_scan" in ln) for ln in lines].index(True) == n - 2
 
 
+def test_the_last_states_gradient_is_the_states_own_too(cache_dir):
+    """d loss / d h where the loss reads h through scan_last alone, and beside it."""
+    def plan(loss, wrt):
+        g = tt.Graph()
+        a, x, w = g.input([2, 5, 3]), g.input([2, 5, 3]), g.input([2, 3])
+        h = tt.gated_scan(a, x)
+        nodes = {"h": h, "x": x}
+        p = tt.compile_gradients(g, loss(h, w), [nodes[n] for n in wrt], outputs=[], cache_dir=cache_dir, flags=HOST)
+        assert p.output_shapes == [[2, 5, 3]] * len(wrt)
+        return _launches(p)[1]
+
+    last = lambda h, w: tt.sum(tt.scan_last(h) * w)  # noqa: E731
+    both = lambda h, w: tt.sum(tt.scan_last(h) * w) + tt.sum(h * h)  # noqa: E731
+    for loss in (last, both):
+        lines = plan(loss, ["h"])
+        assert "mul" in lines[-1] and "output:0" in lines[-1] and not any("gated_scan_d" in ln for ln in lines)
+    lines = plan(both, ["h", "x", "h"])
+    assert sum("gated_scan_d" in ln for ln in lines) == 1
+
+
 # ---- the definitions themselves -----------------------------------------------------------------
 
 

@@ -30,14 +30,16 @@ struct Builder {
         infer_shape(g, n);
         return g.add(std::move(n));
     }
-    int scalar(float v, int dtype) {
+    int constant(std::vector<float> values, Shape s, int dtype) {
         Node n;
         n.op = TT_OP_CONSTANT;
         n.dtype = dtype;
-        n.cdata = {v};
+        n.shape = std::move(s);
+        n.cdata = std::move(values);
         n.id = g.next_id;
         return g.add(std::move(n));
     }
+    int scalar(float v, int dtype) { return constant({v}, {}, dtype); }
     int view(int op, int a, const Shape s) {
         const Node& an = g.nodes[static_cast<size_t>(a)];
         if (an.shape == s) return a;
@@ -312,6 +314,23 @@ void append_gradients(Graph& g, int loss, const std::vector<int>& wrt, int seed)
 
     for (int w : wrt) {
         if (w < 0 || static_cast<size_t>(w) >= nfwd) fail(TT_ERR_INVALID, "gradient target out of range");
+        // A scan's states as the target: their last one's gradient is theirs too, at the axis's last step
+        // (times 1 there and 0 before it: where it is not finite, so are its lane's steps before).
+        const auto last = last_grads.find(w);
+        if (last != last_grads.end()) {
+            const Shape sh = b.shape(w);
+            if (numel(sh) > 0) {
+                const size_t axis = static_cast<size_t>(g.nodes[static_cast<size_t>(w)].dim0);
+                Shape steps(sh.size(), 1), lane = sh;
+                steps[axis] = sh[axis];
+                lane[axis] = 1;
+                std::vector<float> one(static_cast<size_t>(sh[axis]), 0.0f);
+                one.back() = 1.0f;
+                const int at = b.view(TT_OP_EXPAND, b.constant(std::move(one), steps, b.dtype(w)), sh);
+                accumulate(w, b.mk(TT_OP_MUL, {b.view(TT_OP_EXPAND, b.view(TT_OP_RESHAPE, last->second, lane), sh), at}));
+            }
+            last_grads.erase(last);
+        }
         auto it = grads.find(w);
         int out;
         if (it != grads.end()) {
