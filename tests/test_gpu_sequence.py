@@ -130,6 +130,23 @@ def test_scan_empty(cache_dir, shape, axis):
     assert out[1].shape == tuple(lane)
 
 
+@pytest.mark.parametrize("dh", [2, 3, 4, 5, 8, 16, 32, 64, 96])
+def test_scan_without_steps_and_a_shared_gate(cache_dir, dh):
+    """No steps: dinit is the last state's gradient, also where the launch is one that sums groups of lanes."""
+    lane = [2, 3, dh]
+    g = tt.Graph()
+    a, x, s, w = g.input([2, 0, 3, 1]), g.input([2, 0, 3, dh]), g.input(lane), g.input(lane)
+    last = tt.scan_last(tt.gated_scan(a, x, init=s, axis=1))
+    prog = tt.compile_gradients(g, last, [a, s], outputs=[last], seed=w, cache_dir=cache_dir)
+    rng = np.random.default_rng(dh)
+    sv, wv = _f32(rng.standard_normal(lane)), _f32(rng.standard_normal(lane))
+    ins = [tt.DeviceBuffer.from_numpy(v) for v in (np.zeros([2, 0, 3, 1]), np.zeros([2, 0, 3, dh]), sv, wv)]
+    outs = [tt.DeviceBuffer.from_numpy(np.full(v, 7.0)) for v in prog.output_shapes]
+    prog.run_device(ins, outs)
+    got = [b.numpy() for b in outs]
+    assert np.array_equal(got[0], sv) and got[1].size == 0 and np.array_equal(got[2], wv)
+
+
 def test_scan_last_without_states(cache_dir):
     gate, x, s, _, _ = _scan_data([2, 900, 40], 1, True, 3)
     g = tt.Graph()

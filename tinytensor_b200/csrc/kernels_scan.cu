@@ -1026,7 +1026,8 @@ struct Cut {
 Cut cut(const ScanDesc& d) {
     Cut c;
     const int64_t inner = d.n1 * d.n2, lanes = d.outer * inner;
-    c.direct = d.T <= kShort && warp_group(d) == 1;
+    // (no steps: the first state alone is handed through, whatever the groups)
+    c.direct = d.T == 0 || (d.T <= kShort && warp_group(d) == 1);
     c.rows = inner == 1 && !c.direct;  // (no groups there: they are lanes)
     if (inner > 1) c.V = widest(d);
     if (c.direct) {
