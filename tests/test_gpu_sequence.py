@@ -500,6 +500,33 @@ def test_token_outside_the_vocabulary(cache_dir, V):
         assert np.isfinite(out[1].numpy()).all() and prog.status() == 0
 
 
+def test_a_reports_clear_does_not_hide_the_next_one(cache_dir):
+    """The status is cleared when its report is raised, whatever the default stream is busy with (streams of
+    the framework are not ordered with it): the next run's report is not lost."""
+    from tinytensor_b200 import _lib
+
+    V = 64
+    g = tt.Graph()
+    nx, nk = g.input([4, V]), g.input([4], dtype=tt.int32)
+    prog = tt.compile(g, [tt.token_logprob(nx, nk)], cache_dir=cache_dir)
+    x, k = np.zeros([4, V], np.float32), np.array([0, V, 1, 2], np.int32)
+    ins = [tt.DeviceBuffer.from_numpy(x), tt.DeviceBuffer.from_numpy(k, dtype=tt.int32)]
+    out, st = tt.DeviceBuffer([4]), tt.Stream()
+    big = [tt.DeviceBuffer([1 << 28]) for _ in range(2)]
+    for _ in range(3):
+        for _ in range(40):  # some 30 ms of copies on the default stream
+            _lib.check(_lib.lib.tt_memcpy(big[0].ptr, big[1].ptr, big[0].nbytes, _lib.D2D, None))
+        prog.run_device(ins, [out], st)
+        with pytest.raises(tt.DeviceStatusError, match="token id"):
+            prog.status()
+        prog.run_device(ins, [out], st)
+        st.synchronize()
+        _lib.check(_lib.lib.tt_stream_sync(None))
+        with pytest.raises(tt.DeviceStatusError, match="token id"):
+            prog.status()
+        assert prog.status() == 0
+
+
 def test_token_operands_as_views(cache_dir):
     """Transposed rows, a broadcast advantage, logits whose vocabulary is not adjacent."""
     rng = np.random.default_rng(4)

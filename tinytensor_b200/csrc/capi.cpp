@@ -128,6 +128,13 @@ static std::string status_text(int32_t status) {
     return "a kernel gave up a bounded wait (status " + std::to_string(status) + ")";
 }
 
+// Clears both words before the caller hears of them: on the stream of the run, which is not ordered with the
+// default one, and waited for, since the next run may take another stream and set them again.
+static void clear_status(tt_program* p, cudaStream_t stream) {
+    check_cuda(cudaMemsetAsync(p->arena + p->plan.status_offset, 0, 2 * sizeof(int32_t), stream), "status clear");
+    check_cuda(cudaStreamSynchronize(stream), "status clear");
+}
+
 static int launches_of(const Plan& p, const Launch& L) {
     if (L.type == LT_REGION) return p.regions[static_cast<size_t>(L.region)].grid > 0 ? 1 : 0;
     if (L.type == LT_REDUCE) return L.rd.outer == 0 ? 0 : (L.rd.R == 0 ? 1 : (L.rd.splits > 1 ? 2 : 1));
@@ -513,7 +520,7 @@ int tt_program_run(tt_program* p, const void* const* inputs, void* const* output
             collect_profile(p);
             const int32_t status = words[0] ? words[0] : words[1];
             if (status != 0) {
-                cudaMemsetAsync(p->arena + p->plan.status_offset, 0, sizeof(words), stream);
+                clear_status(p, stream);
                 fail(TT_ERR_DEVICE_STATUS, status_text(status));
             }
         }
@@ -658,7 +665,7 @@ int tt_program_status(tt_program* p, int32_t* device_status) {
         const int32_t status = words[0] ? words[0] : words[1];
         if (device_status) *device_status = status;
         if (status != 0) {
-            cudaMemset(p->arena + p->plan.status_offset, 0, sizeof(words));
+            clear_status(p, p->last_stream);
             fail(TT_ERR_DEVICE_STATUS, status_text(status));
         }
     });
