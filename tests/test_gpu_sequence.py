@@ -66,6 +66,19 @@ def test_scan_lengths(cache_dir, T, D):
     _check_scan(cache_dir, [2, T, D], 1, init=T % 2 == 1, seed=T * 100 + D)
 
 
+# Several blocks of lanes a CTA: far more blocks than run at the same time, so that the ring of tiles runs on from
+# one block to the next: columns of 4, 2 and 1 lanes a thread, one tile and several a block, rows of whole warps,
+# short rows several a warp, and a gate a head.
+@pytest.mark.parametrize("shape,axis,gate_shape", [
+    ([4, 200, 30016], 1, None), ([4, 40, 60002], 1, None), ([3, 130, 30011], 1, None), ([1000, 700], 1, None),
+    ([700, 4099], 1, None), ([20000, 33], 1, None), ([9000, 130], 1, None), ([6, 70, 400, 64], 1, [6, 70, 400, 1]),
+    ([30, 33, 90, 24], 1, [30, 33, 90, 1])])
+def test_scan_of_many_blocks_a_cta(cache_dir, shape, axis, gate_shape):
+    _check_scan(cache_dir, shape, axis, seed=sum(shape), gate_shape=gate_shape)
+    if gate_shape is None:
+        _check_scan(cache_dir, shape, axis, init=False, seed=sum(shape) + 1)
+
+
 @pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 31, 127, 128, 129, 511, 513, 1000, 2047, 4099])
 @pytest.mark.parametrize("rows", [1, 7, 40])
 def test_scan_time_last(cache_dir, T, rows):
@@ -346,6 +359,53 @@ def test_token_logprob_at_most_vectors_a_thread(cache_dir, V, rows):
     x, k, g = _f32(rng.standard_normal([rows, V])), _tokens(rng, [rows], V), _f32(rng.standard_normal([rows]))
     out = _run_tokens(cache_dir, tt.token_logprob, x, k, [], g)
     _check(out, R.logprob(x, k, g))
+
+
+# Rows that a gradient's clusters (1 to 8 CTAs of 256 or 512 threads) and small CTAs walk about ten or more each: ring
+# stages and row records come round several times, barriers and mbarriers go through their phases, and padding
+# rows shift the exchange's parity against the rows'.  Rows that all start on 16 bytes, and rows that do not.
+@pytest.mark.parametrize("V, rows", [(2500, 6500), (3001, 6500), (5000, 3000), (9217, 1500), (9220, 1500), (18501, 1000),
+                                     (35001, 720), (50004, 500), (73725, 380), (80003, 300)])
+def test_token_gradient_of_many_rows_a_cluster(cache_dir, V, rows):
+    rng = np.random.default_rng(V)
+    x = 2 * rng.standard_normal([rows, V], dtype=np.float32)
+    k, g = rng.integers(0, V, [rows]).astype(np.int32), _f32(rng.standard_normal([rows]))
+    # single padding rows, a run of them, and a stretch without any
+    k[rng.random(rows) < 0.15] = -1
+    k[rows // 3:rows // 3 + rows // 20] = -1
+    k[rows // 2:rows // 2 + rows // 5] = np.abs(k[rows // 2:rows // 2 + rows // 5])
+    x[k < 0] = np.nan
+    gr = tt.Graph()
+    nx, nk, ng = gr.input(x.shape), gr.input([rows], dtype=tt.int32), gr.input([rows])
+    y = tt.token_logprob(nx, nk)
+    out = [o.numpy() for o in tt.compile_gradients(gr, y, [nx], outputs=[y], seed=ng, cache_dir=cache_dir)
+           .run({nx: x, nk: k, ng: g})]
+    x[k < 0] = 0
+    for i in range(0, rows, 250):  # (the definition in blocks of rows, for its 64-bit copies)
+        b = slice(i, i + 250)
+        want = R.logprob(x[b], k[b], g[b])
+        R.assert_within(out[0][b], want[0])
+        R.assert_within(out[1][b], want[1])
+
+
+@pytest.mark.parametrize("kl", [0.0, 0.1])
+def test_policy_gradient_of_many_rows_a_cluster(cache_dir, kl):
+    """The joining warp's operands of the rows ahead, over many rows of a cluster."""
+    rng = np.random.default_rng(3)
+    rows, V, clip = 1400, 9300, (0.2, 0.3)
+    x = rng.standard_normal([rows, V], dtype=np.float32)
+    k = rng.integers(0, V, [rows]).astype(np.int32)
+    k[rng.random(rows) < 0.2] = -1
+    p = R.logprob(x, k)[0][0]
+    ratio = np.exp(0.3 * rng.standard_normal(rows))
+    for border in (0.8, 1.3):
+        ratio = np.where(np.abs(ratio - border) < 1e-3, border + 5e-3, ratio)
+    old, adv, g = _f32(p - np.log(ratio)), _f32(rng.standard_normal(rows)), _f32(rng.standard_normal(rows))
+    ref = _f32(p + 0.3 * rng.standard_normal(rows))
+    data = [old, adv] + ([ref] if kl else [])
+    out = _run_tokens(cache_dir, lambda a, b, o, d, r=None: tt.policy_loss(a, b, o, d, ref_logp=r, clip=clip, kl=kl),
+                      x, k, data, g)
+    _check(out, R.policy(x, k, old, adv, ref if kl else None, clip, kl, g))
 
 
 @pytest.mark.parametrize("rows", [1, 2, 9, 149, 600, 3000])
