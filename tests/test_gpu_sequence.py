@@ -205,6 +205,88 @@ def test_scan_special_values(cache_dir):
     assert np.array_equal(got[fin], _f32(want)[fin])  # powers of two: exact
 
 
+def _wild_scan(shape, axis, kind, seed, gate_shape=None):
+    """Gates whose products leave float32's range many times over, on states that do not: every lane's state
+    follows a path of magnitudes within 1e-30 .. 1e30, and the upstream gradient the inverse of it."""
+    rng = np.random.default_rng(seed)
+    lanes = list(gate_shape or shape)
+    T = lanes.pop(axis)
+    u = np.linspace(0.0, 1.0, T + 1).reshape([-1] + [1] * len(lanes))
+    if kind == "paths":  # a reflected random walk
+        p = np.cumsum(3.0 * rng.standard_normal([T + 1] + lanes), 0) + 28
+        p = np.abs(p - 112.0 * np.round(p / 112.0)) - 28
+    else:
+        p = {"grow": 60 * u - 30, "decay": 30 - 60 * u, "there and back": 58 * np.sin(2 * np.pi * u) / 2,
+             "up and down": 29 - 58 * np.abs(2 * u - 1)}[kind] + rng.uniform(-0.5, 0.5, lanes)
+    sign = np.where(rng.random([T + 1] + lanes) < 0.1, -1.0, 1.0)
+    gate = _f32(10.0 ** (p[1:] - p[:-1]) * sign[1:])
+    size = 10.0 ** np.broadcast_to(p, [T + 1] + [d for i, d in enumerate(shape) if i != axis])
+    noise = [0.1 * rng.standard_normal(size[1:].shape) * (rng.random(size[1:].shape) < 0.5) for _ in range(2)]
+    if kind != "paths":
+        noise = [0.0 * n for n in noise]
+    back = lambda v: np.moveaxis(v, 0, axis)  # noqa: E731
+    return (back(gate), _f32(back(noise[0] * size[1:])), _f32(size[0] * rng.choice([-1, 1], size[0].shape)),
+            _f32(back(noise[1] / size[1:])), _f32(1 / size[-1]))
+
+
+_WILD = [([7, 60], 1, None), ([9, 130], 1, None), ([5, 600], 1, None), ([5, 4001], 1, None), ([3, 30000], 1, None),
+         ([1, 70001], 1, None), ([300, 4100], 1, None), ([2, 12, 40], 1, None), ([2, 50, 7], 1, None), ([2, 300, 5], 1, None),
+         ([2, 301, 6], 1, None), ([2, 900, 40], 1, None), ([1, 5000, 40], 1, None), ([1, 20000, 64], 1, None),
+         ([1, 70000, 3], 1, None), ([1, 70000, 40], 1, None), ([1, 300, 3584], 1, None), ([2, 200, 12000], 1, None),
+         ([300, 10, 7], 0, None), ([2, 300, 3, 64], 1, [2, 300, 3, 1]), ([1, 9000, 2, 24], 1, [1, 9000, 2, 1])]
+
+
+@pytest.mark.parametrize("kind", ["paths", "grow", "decay", "there and back", "up and down"])
+@pytest.mark.parametrize("shape,axis,gate_shape", _WILD)
+def test_scan_where_products_of_gates_leave_the_range(cache_dir, shape, axis, gate_shape, kind):
+    """A tile's map cannot hold such a product, the states are ordinary: at every cut of the axis (threads, warps,
+    clusters, segments), forward and backward."""
+    gate, x, s, dh, dl = _wild_scan(shape, axis, kind, sum(shape), gate_shape)
+    g = tt.Graph()
+    na, nx, ns, nd, nl = (g.input(v.shape) for v in (gate, x, s, dh, dl))
+    h = tt.gated_scan(na, nx, init=ns, axis=axis)
+    last = tt.scan_last(h)
+    loss = tt.sum(h * nd) + tt.sum(last * nl)
+    out = [o.numpy() for o in tt.compile_gradients(g, loss, [na, nx, ns], outputs=[h, last], cache_dir=cache_dir)
+           .run({na: gate, nx: x, ns: s, nd: dh, nl: dl})]
+    full = np.broadcast_to(gate, shape)
+    (rh, rlast), rg = R.scan(full, x, s, axis), R.scan_grad(full, x, s, axis, dh, dl)
+    assert np.isfinite(rh[0]).all() and np.abs(rh[0]).max() < 1e37 and np.abs(rg[1][0]).max() < 1e37
+    R.assert_within(out[0], rh)
+    R.assert_within(out[1], rlast)
+    if gate_shape is None:
+        R.assert_within(out[2], rg[0])
+    else:  # (the bound of a shared gate's sum: see _check_scan)
+        ax = tuple(i for i in range(len(shape)) if gate_shape[i] != shape[i])
+        v, tol = rg[0]
+        R.assert_within(out[2], (v.sum(ax, keepdims=True), tol.sum(ax, keepdims=True) + 7 * R.U * np.abs(v).sum(ax, keepdims=True)))
+    R.assert_within(out[3], rg[1])
+    R.assert_within(out[4], rg[2])
+    # the last state alone: the states are not stored, the maps are the same
+    g = tt.Graph()
+    na, nx, ns = (g.input(v.shape) for v in (gate, x, s))
+    alone = tt.compile(g, [tt.scan_last(tt.gated_scan(na, nx, init=ns, axis=axis))], cache_dir=cache_dir)
+    R.assert_within(alone.run({na: gate, nx: x, ns: s}).numpy(), rlast)
+
+
+@pytest.mark.parametrize("shape,axis", [([3, 640], 1), ([2, 700, 40], 1), ([1, 70000, 5], 1), ([1, 70001], 1)])
+def test_scan_in_windows_equals_the_whole_where_gates_grow(cache_dir, shape, axis):
+    """Single windows, and their states handed on: no cut of the axis changes a state."""
+    gate, x, s, _, _ = _wild_scan(shape, axis, "paths", 3)
+    (rh, tol), _ = R.scan(gate, x, s, axis)
+    T, at = shape[axis], 0
+    cut = lambda v, i, j: np.ascontiguousarray(np.moveaxis(np.moveaxis(v, axis, 0)[i:j], 0, axis))  # noqa: E731
+    for n in (T // 2 + 1, T - T // 2 - 4, 1, 1, 1):
+        w = [cut(v, at, at + n) for v in (gate, x)]
+        g = tt.Graph()
+        a, b, c = g.input(w[0].shape), g.input(w[1].shape), g.input(s.shape)
+        h = tt.gated_scan(a, b, init=c, axis=axis)
+        got, s = (o.numpy() for o in tt.compile(g, [h, tt.scan_last(h)], cache_dir=cache_dir).run({a: w[0], b: w[1], c: s}))
+        R.assert_within(got, (cut(rh, at, at + n), cut(tol, at, at + n)))
+        at += n
+    assert at == T
+
+
 def test_scan_in_windows_and_tokens_equals_the_whole(cache_dir):
     """Windows that hand their last state on, then single tokens: the states of one long scan."""
     gate, x, _, _, _ = _scan_data([3, 64, 20], 1, False, 6)

@@ -20,6 +20,9 @@
 //                         where there are too few lanes to fill the card;
 //   segments of the axis  through device scratch, by a first launch that finds the segments'
 //                         maps, where clusters are not enough (the data is read twice).
+// Maps hold the products of their gates, which may leave float's range where no state does (growing gates and a
+// small state, a state of 1e30 that decays).  A CTA watches for that (Watch) and, where it may have happened,
+// walks its lanes once more, step by step as the recurrence is written.
 // Time runs in scan order r: t = r forward, t = T-1-r backward.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -58,21 +61,40 @@ struct ScanArgs {
 
 enum Pass { ONLY = 0, MAPS = 1, JOINED = 2 };  // the whole scan; its segments' maps; the scan from them
 
-// Maps (A, H) keep A finite unless a gate is not: an overflowing product is held at the largest
-// float, so that 0 * A stays 0 (a state of 0, or a gate of 0 behind it) where inf would make it
-// NaN.  (A underflowing product is 0: an infinite state may become NaN behind it.)
 __device__ __forceinline__ float apply(float2 m, float c) { return fmaf(m.x, c, m.y); }
 
-__device__ __forceinline__ float join_gates(float a, float b) {
-    constexpr float kMax = 3.402823466e38f;
-    float p = a * b;
-    asm("min.NaN.f32 %0, %0, %1;" : "+f"(p) : "f"(kMax));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(p) : "f"(-kMax));
-    return p;
+// First m, then n.
+__device__ __forceinline__ float2 join(float2 m, float2 n) { return make_float2(m.x * n.x, apply(n, m.y)); }
+
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN propagates
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
 }
 
-// First m, then n.
-__device__ __forceinline__ float2 join(float2 m, float2 n) { return make_float2(join_gates(m.x, n.x), apply(n, m.y)); }
+// What a thread has seen of the maps (A, H) and the states, and whether the maps do.  Products must not overflow: a
+// thread's run of steps has |A| <= 2 and a tile |A| <= 16, else it is GROWN (a step's tiles are 2^32 at most then).  A
+// product below the normal range has lost some 2^-146 at most, which is next to nothing (2^-119) of states of 2^27,
+// unless a run behind it grows.  So maps do unless one is GROWN, or one is TINY (|A| < 2^-90; part of a tile may
+// have 2^-121) and one LARGE: a run grows, or an H or a state is above 2^20 (states between tiles may then be
+// 2^27).  The two need not be one lane's: that costs time only.  States that are NaN are NaN either way.
+enum Range { GROWN = 1, TINY = 2, LARGE = 4 };
+constexpr float kTiny = 8.077935669e-28f, kLarge = 1048576.0f;  // 2^-90, 2^20
+struct Watch {
+    float run = 0.0f, tile = 0.0f, least = 1.0f, most = 0.0f;  // largest |A| of runs, of tiles, least |A|, largest |H|
+    __device__ __forceinline__ void run_of(float a) { run = max_nan(run, fabsf(a)); }
+    __device__ __forceinline__ void product(float a) { least = fminf(least, fabsf(a)); }
+    __device__ __forceinline__ void state(float c) { most = fmaxf(most, fabsf(c)); }
+    __device__ __forceinline__ void tile_of(float2 m) {
+        tile = max_nan(tile, fabsf(m.x));
+        product(m.x);
+        state(m.y);
+    }
+    __device__ __forceinline__ int range() const {
+        return (run <= 2.0f && tile <= 16.0f ? 0 : GROWN) | (least < kTiny ? TINY : 0) | (run <= 1.0f && most <= kLarge ? 0 : LARGE);
+    }
+};
+__device__ __forceinline__ bool maps_do(int range) { return (range & GROWN) == 0 && (range & (TINY | LARGE)) != (TINY | LARGE); }
 
 // The map of N steps in scan order, its gates' product as it comes.
 template <bool BACKWARD, int N, class G, class X>
@@ -84,19 +106,6 @@ __device__ __forceinline__ float2 tile_map(G gate, X x) {
         m.y = BACKWARD ? gate(j) * (x(j) + m.y) : fmaf(gate(j), m.y, x(j));
     }
     return m;
-}
-__device__ __forceinline__ bool finite(float a) { return fabsf(a) <= 3.402823466e38f; }
-// Settles a product that is not finite: 0 where a gate is 0 (after an overflow 0 * inf), the largest float
-// where it overflowed, NaN or infinite where a gate is.
-template <int N, class G>
-__device__ __forceinline__ float settle(float a, G gate) {
-    bool zero = false, all = true;
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-        zero |= gate(j) == 0.0f;
-        all &= finite(gate(j));
-    }
-    return !all ? a : zero ? 0.0f : a != a ? a : copysignf(3.402823466e38f, a);
 }
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -119,7 +128,19 @@ struct Exchange {
     // only where W = NW (otherwise one step covers the axis):
     float2 cta[2][8][LW];  // by rank in the cluster
     float state[2][LW];    // the last warp's state behind a step, for the next one
+    int range[NW], cta_range[8];  // Range bits of the warps, and of the cluster's CTAs
 };
+// The Range bits of all warps of the CTA.
+template <int NW, int LW>
+__device__ __forceinline__ int block_range(Exchange<NW, LW>& ex, int range) {
+    range = __reduce_or_sync(0xffffffffu, range);
+    __syncthreads();  // (they may still be read for the unit before)
+    if ((threadIdx.x & 31) == 0) ex.range[threadIdx.x >> 5] = range;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) range |= ex.range[w];
+    return range;
+}
 
 // A CTA's place: its rank in its cluster, the cluster's first unit and how many clusters walk them.
 struct Place {
@@ -155,12 +176,17 @@ __device__ __forceinline__ void split_inner(const ScanArgs& a, int64_t i, int64_
     i2 = i - i1 * a.n2;
 }
 
+// A segment's map as the first launch leaves it: NaN for A where it does not do.
+__device__ __forceinline__ float2 segment_map(float gates, float h, int range) {
+    return make_float2(maps_do(range) && fabsf(gates) <= 4294967296.0f ? gates : __int_as_float(0x7fc00000), h);
+}
+
 // The state before segment `seg` of a lane, from the maps of the segments before it and the lane's
 // first state.  The warps of the CTA (all on the same lanes) join a share of the maps each,
 // loading 8 at a time; LW lanes a warp, `writer` one thread of a lane.
 template <int NW, int LW>
 __device__ __forceinline__ float segment_state(const ScanArgs& a, Exchange<NW, LW>& ex, int seg, int64_t lane, bool live,
-                                               float c, int warp, int l, bool writer) {
+                                               float c, int warp, int l, bool writer, Watch& watch) {
     const int share = (seg + NW - 1) / NW, begin = min(seg, warp * share), end = min(seg, begin + share);
     float2 m = make_float2(1.0f, 0.0f);
     for (int s0 = begin; s0 < end; s0 += 8) {
@@ -169,8 +195,13 @@ __device__ __forceinline__ float segment_state(const ScanArgs& a, Exchange<NW, L
         for (int u = 0; u < 8; ++u)
             q[u] = live && s0 + u < end ? __ldcg(a.maps + (s0 + u) * a.lanes + lane) : make_float2(1.0f, 0.0f);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) m = join(m, q[u]);
+        for (int u = 0; u < 8; ++u) {
+            m = join(m, q[u]);
+            watch.run = fabsf(q[u].x) <= 4294967296.0f ? fmaxf(watch.run, fminf(fabsf(q[u].x), 1.5f)) : INFINITY;  // (grows: LARGE)
+            watch.tile_of(make_float2(fabsf(m.x) <= 4294967296.0f ? fminf(fabsf(m.x), 1.0f) : INFINITY, q[u].y));
+        }
     }
+    watch.state(c);
     __syncthreads();  // (the unit before may still be reading)
     if (writer) ex.warp[0][warp][l] = m;
     __syncthreads();
@@ -191,7 +222,8 @@ struct Joiner {
 
     // m: the map of this warp's tile.  Returns the state before the tile; c is the state before
     // the first step (later steps find theirs in the exchange).
-    __device__ __forceinline__ float first(float2 m, float c, bool first_step, bool writer) {
+    __device__ __forceinline__ float first(float2 m, float c, bool first_step, bool writer, Watch& watch) {
+        watch.tile_of(m);
         if (writer) ex.warp[buf][warp][l] = m;
         __syncthreads();
         if (at.size > 1) {
@@ -200,6 +232,7 @@ struct Joiner {
                 float2 all = m;
 #pragma unroll
                 for (int w = 1; w < NW; ++w) all = join(all, ex.warp[buf][w][l]);
+                watch.product(all.x);
                 for (int q = 0; q < at.size; ++q) cl.map_shared_rank(&ex, q)->cta[buf][at.rank][l] = all;
             }
             cl.sync();
@@ -219,6 +252,7 @@ struct Joiner {
         } else {
             for (int w = 0; w < wt; ++w) s = apply(ex.warp[buf][wr * W + w][l], s);
         }
+        watch.state(s);
         return s;
     }
     // s: the state behind this warp's tile.  The step's last tile hands it to the next step
@@ -235,11 +269,118 @@ struct Joiner {
         buf ^= 1;
     }
     // The product of all gates of a step (for a segment's map; one lane group a CTA).
-    __device__ __forceinline__ void gates_of_step(float& gates) const {
+    __device__ __forceinline__ void gates_of_step(float& gates, Watch& watch) const {
 #pragma unroll
-        for (int w = 0; w < NW; ++w) gates = join_gates(gates, ex.warp[buf][w][l].x);
+        for (int w = 0; w < NW; ++w) gates *= ex.warp[buf][w][l].x;
+        watch.product(gates);
     }
 };
+
+// The steps of a row before its vector v of four (in scan order), cut at CUT steps' boundaries.
+template <bool BACKWARD, int CUT>
+__device__ __forceinline__ int64_t steps_before(const ScanArgs& a, int64_t row, int64_t v) {
+    const int shift = static_cast<int>(static_cast<unsigned>(row) * static_cast<unsigned>(a.T) & (CUT - 1));
+    const int64_t vectors = (a.T + shift + CUT - 1) / CUT * (CUT / 4);
+    const int64_t t = min(max(4 * (BACKWARD ? vectors - v : v) - shift, static_cast<int64_t>(0)), a.T);
+    return BACKWARD ? a.T - t : t;
+}
+
+// The units of a CTA (a cluster's first one) once more, `lanes` lanes a unit, a thread a lane: the recurrence step by
+// step, from the axis's begin to the unit's end.  CUT: of rows; 0 for lanes side by side, 32 of which are a warp's.
+// Two batches of loads under way, so latency bounds it: 1 x 65536 x 1024 takes 8.6 ms instead of 0.15, 2000 rows of
+// 8191 1.0 ms instead of 0.04.  (Steps without maps inside the tiles' loop, the warps in turn, were faster where
+// they happened, and the loop's code slower where they did not: 4 to 19 %.)
+template <bool BACKWARD, int CUT>
+__device__ __noinline__ void walk_again(const ScanArgs& a, int64_t first, int64_t clusters, int lanes) {
+    const int64_t all = (a.units - first + clusters - 1) / clusters * lanes;
+    const bool want_gate = BACKWARD && a.out[SO_GATE];
+    for (int64_t q = threadIdx.x; q - (threadIdx.x & 31) < all; q += blockDim.x) {
+        const int64_t unit = first + q / lanes * clusters, block = unit / a.segments, seg = unit - block * a.segments;
+        const int64_t lane = block * lanes + q % lanes;
+        const bool live = q < all && lane < a.lanes;
+        int64_t begin = seg * a.seg_len, end = begin + a.seg_len;
+        if (CUT > 0) {
+            begin = live ? steps_before<BACKWARD, CUT < 4 ? 4 : CUT>(a, lane, begin) : 0;
+            end = live ? steps_before<BACKWARD, CUT < 4 ? 4 : CUT>(a, lane, end) : 0;
+        } else {
+            end = min(end, a.T);
+        }
+        int64_t o = 0, i = 0, i1, i2;
+        if (live) split_lane(a, lane, o, i);
+        split_inner(a, i, i1, i2);
+        const int64_t t0 = BACKWARD ? a.T - 1 : 0;
+        auto ptr = [&](int k, int64_t t) {
+            const Operand& p = a.in[k];
+            return live && p.p ? p.p + o * p.so + i1 * p.s1 + i2 * p.s2 + t * p.st : nullptr;
+        };
+        auto per_step = [&](int k) { return BACKWARD ? -a.in[k].st : a.in[k].st; };
+        const float *gate = ptr(SI_GATE, t0), *x = ptr(SI_X, t0), *h = ptr(SI_H, t0 - 1), *init = ptr(SI_INIT, 0);
+        const int64_t gs = per_step(SI_GATE), xs = per_step(SI_X), hs = per_step(SI_H);
+        const float* carry = ptr(SI_CARRY, 0);
+        float c = carry ? __ldg(carry) : 0.0f;
+        constexpr int N = 16;
+        struct Batch {
+            float g[N], x[N], h[N];
+        };
+        // the steps r0 .. r0 + N - 1 before r1 (the others: gate 1, x 0), and the states before them
+        auto load = [&](Batch& b, int64_t r0, int64_t r1, bool states) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const bool in = live && r0 + j < r1;
+                b.g[j] = in ? __ldg(gate + (r0 + j) * gs) : 1.0f;
+                b.x[j] = in && x ? __ldg(x + (r0 + j) * xs) : 0.0f;
+                if constexpr (BACKWARD) {
+                    const float* q = r0 + j == a.T - 1 ? init : h + (r0 + j) * hs;
+                    b.h[j] = in && states && q ? __ldg(q) : 0.0f;
+                }
+            }
+        };
+        auto walk = [&](int64_t r0, int64_t r1, bool write) {
+            const bool states = write && want_gate;
+            Batch now, next;
+            load(now, r0, r1, states);
+            for (; r0 < r1; r0 += N) {
+                load(next, r0 + N, r1, states);
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const float main = BACKWARD ? now.x[j] + c : fmaf(now.g[j], c, now.x[j]);
+                    c = BACKWARD ? now.g[j] * main : main;
+                    if (!write || r0 + j >= r1) continue;
+                    const int64_t row = o * a.T + (BACKWARD ? a.T - 1 - r0 - j : r0 + j);
+                    if (live && a.out[SO_MAIN]) a.out[SO_MAIN][row * a.inner + i] = main;
+                    if constexpr (BACKWARD) {
+                        if (!want_gate) continue;
+                        float dg = main * now.h[j];
+                        for (int d = 1; d >> a.group == 0; d *= 2) dg += __shfl_xor_sync(0xffffffffu, dg, d);
+                        if (live && (i & ((1 << a.group) - 1)) == 0) a.out[SO_GATE][row * (a.inner >> a.group) + (i >> a.group)] = dg;
+                    }
+                }
+                now = next;
+            }
+        };
+        walk(0, begin, false);
+        walk(begin, end, true);
+        if (live && end == a.T && a.out[SO_LANE]) a.out[SO_LANE][lane] = c;
+    }
+}
+
+// At a CTA's end: its units again where a thread of the cluster has seen maps that do not do.
+template <bool BACKWARD, int CUT, int NW, int LW>
+__device__ __forceinline__ void settle(const ScanArgs& a, Exchange<NW, LW>& ex, const Place& at, const Watch& watch, int lanes) {
+    int range = watch.range();
+    if (at.size == 1) {
+        if (!__syncthreads_or(range & (GROWN | LARGE))) return;
+        range = block_range(ex, range);
+    } else {
+        cg::cluster_group cl = cg::this_cluster();
+        range = block_range(ex, range);
+        if (threadIdx.x == 0) cl.map_shared_rank(&ex, 0)->cta_range[at.rank] = range;
+        cl.sync();  // (the cluster's results are written, too)
+        if (at.rank > 0) return;
+        for (int q = 0; q < at.size; ++q) range |= ex.cta_range[q];
+    }
+    if (!maps_do(range)) walk_again<BACKWARD, CUT>(a, at.first, at.clusters, lanes);
+}
 
 template <int V>
 __device__ __forceinline__ void load_shared(const float* p, float* v) {
@@ -296,7 +437,7 @@ struct ColTile {
 };
 
 template <bool BACKWARD, int PASS, int V, int TILE, int NW>
-__global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(const __grid_constant__ ScanArgs a) {
     constexpr int TS = TILE / V, COLS = 32 / V, NA = kArrays<BACKWARD>;
     extern __shared__ __align__(16) unsigned char raw[];
     ColTile<BACKWARD, TILE, NW>& sh = *reinterpret_cast<ColTile<BACKWARD, TILE, NW>*>(raw);
@@ -408,6 +549,7 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a)
     Joiner<NW, 32> joiner{sh.ex, at, W, wt, wr, warp, l};
     const bool one_gate = is_one(SI_GATE), one_x = is_one(SI_X), one_h = is_one(SI_H);
     const bool shares = one_gate || one_x || one_h;
+    Watch watch;
     int stage = 0;
     for (int64_t unit = at.first; unit < a.units; unit += at.clusters) {
         const int seg = static_cast<int>(unit - block_of(unit) * a.segments);
@@ -427,6 +569,7 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a)
         float* ym0 = a.out[SO_MAIN] + row * a.inner + i;
         float* yg0 = a.out[SO_GATE] + row * (a.inner >> a.group) + (i >> a.group);
         float c = 0.0f, gates = 1.0f;
+        if constexpr (PASS == MAPS) watch = Watch();  // (a unit's own)
         if constexpr (PASS == JOINED) {
             const bool in = lane0 + l < a.lanes;
             if (in && a.in[SI_CARRY].p) {
@@ -434,7 +577,7 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a)
                 split_lane(a, lane0 + l, oc, ic);
                 c = __ldg(a.in[SI_CARRY].p + oc * a.in[SI_CARRY].so + ic / a.n2 * a.in[SI_CARRY].s1 + ic % a.n2 * a.in[SI_CARRY].s2);
             }
-            c = segment_state<NW, 32>(a, sh.ex, seg, lane0 + l, in, c, warp, l, true);
+            c = segment_state<NW, 32>(a, sh.ex, seg, lane0 + l, in, c, warp, l, true, watch);
         }
         int r0 = own;
         for (int k = 0; k < a.steps; ++k, r0 += stride, stage ^= 1) {
@@ -478,16 +621,10 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a)
             issue(stage);
             // this thread's maps, those of the threads before it in time, and the tile's
             float2 m[V], before[V];
-            bool settled = true;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 m[v] = tile_map<BACKWARD, TS>([&](int j) { return ga[j][v]; }, [&](int j) { return xv[j][v]; });
-                settled &= finite(m[v].x);
-            }
-            if (!settled) {
-#pragma unroll
-                for (int v = 0; v < V; ++v)
-                    if (!finite(m[v].x)) m[v].x = settle<TS>(m[v].x, [&](int j) { return ga[j][v]; });
+                watch.run_of(m[v].x);
             }
 #pragma unroll
             for (int d = COLS; d < 32; d *= 2) {
@@ -510,11 +647,12 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a)
                 }
             }
             const bool last = k + 1 == a.steps;
-            const float first = joiner.first(tile, c, k == 0, true);
+            const float first = joiner.first(tile, c, k == 0, true, watch);
             if constexpr (PASS == MAPS) {
-                joiner.gates_of_step(gates);
+                joiner.gates_of_step(gates, watch);
                 const float s = apply(tile, first);
-                if (last && lane0 + l < a.lanes && wt == W - 1) a.maps[seg * a.lanes + lane0 + l] = make_float2(gates, s);
+                const int range = last ? block_range(sh.ex, watch.range()) : 0;
+                if (last && lane0 + l < a.lanes && wt == W - 1) a.maps[seg * a.lanes + lane0 + l] = segment_map(gates, s, range);
                 joiner.hand_on(s, last, true);
             } else {
                 float s[V];
@@ -571,6 +709,7 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(ScanArgs a)
         }
     }
     copies_wait_all();
+    if constexpr (PASS != MAPS) settle<BACKWARD, 0>(a, sh.ex, at, watch, NW / W * 32);
 }
 
 // ---- time adjacent in memory ([.., T]): a warp's tile is 640 (backward 384) steps of one row, a
@@ -609,7 +748,7 @@ struct Select<false, A, B> {
 };
 
 template <bool BACKWARD, int PASS, int SUB>
-__global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(const __grid_constant__ ScanArgs a) {
     constexpr int NW = kWarps, NA = kArrays<BACKWARD>, kRun = kRowRun<BACKWARD>, kTile = 32 * kRun, kVectors = kTile / 4;
     constexpr int R = 32 / SUB, VR = SUB * kRun / 4;  // rows a warp, vectors of a row's tile
     extern __shared__ __align__(16) unsigned char raw[];
@@ -766,6 +905,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(ScanArgs a) {
     if (at.size > 1) cg::this_cluster().sync();  // every CTA runs before another writes to it
     Joiner<NW, 1> joiner{ex, at, W, wt, wr, warp, 0};
     const int run = (BACKWARD ? SUB - 1 - ls : ls) * kRun;  // this thread's run within its row's tile
+    Watch watch;
     int stage = 0;
     for (int64_t unit = at.first; unit < a.units; unit += at.clusters) {
         const Rows here = rows_of(unit);
@@ -773,9 +913,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(ScanArgs a) {
         const int64_t row0 = here.row0, row = row0 + sr;
         const bool live = row < a.lanes;
         float c = 0.0f, gates = 1.0f;
+        if constexpr (PASS == MAPS) watch = Watch();  // (a unit's own)
         if constexpr (PASS == JOINED) {
             if (live && a.in[SI_CARRY].p) c = __ldg(a.in[SI_CARRY].p + row * a.in[SI_CARRY].so);
-            c = segment_state<NW, 1>(a, ex, seg, row, live, c, warp, 0, l == 0);
+            c = segment_state<NW, 1>(a, ex, seg, row, live, c, warp, 0, l == 0, watch);
         }
         Count r0 = static_cast<Count>(here.begin + own);
         for (int k = 0; k < a.steps; ++k, stage ^= 1, r0 += static_cast<Count>(stride)) {
@@ -787,10 +928,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(ScanArgs a) {
                 if (PASS == ONLY && k == 0) c = a.in[SI_CARRY].p && live ? tile.carry[stage][0] : 0.0f;
                 __syncwarp();
                 issue(stage);
-                const float s = joiner.first(make_float2(1.0f, 0.0f), c, k == 0, l == 0);
+                const float s = joiner.first(make_float2(1.0f, 0.0f), c, k == 0, l == 0, watch);
                 if constexpr (PASS == MAPS) {
-                    joiner.gates_of_step(gates);
-                    if (k + 1 == a.steps && live && wt == W - 1 && l == 0) a.maps[seg * a.lanes + row] = make_float2(gates, s);
+                    joiner.gates_of_step(gates, watch);
+                    const int range = k + 1 == a.steps ? block_range(ex, watch.range()) : 0;
+                    if (k + 1 == a.steps && live && wt == W - 1 && l == 0) a.maps[seg * a.lanes + row] = segment_map(gates, s, range);
                 }
                 joiner.hand_on(s, k + 1 == a.steps, l == 0);
                 continue;
@@ -833,7 +975,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(ScanArgs a) {
             issue(stage);
             float2 q = tile_map<BACKWARD, kRun>([&](int j) { return ga[BACKWARD ? kRun - 1 - j : j]; },
                                                 [&](int j) { return xv[BACKWARD ? kRun - 1 - j : j]; });
-            if (!finite(q.x)) q.x = settle<kRun>(q.x, [&](int j) { return ga[j]; });
+            watch.run_of(q.x);
 #pragma unroll
             for (int d = 1; d < SUB; d *= 2) {
                 const float2 b = make_float2(__shfl_up_sync(0xffffffffu, q.x, d), __shfl_up_sync(0xffffffffu, q.y, d));
@@ -845,14 +987,19 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(ScanArgs a) {
             float s = c;
             if constexpr (SUB == 32) {
                 const float2 m = make_float2(__shfl_sync(0xffffffffu, q.x, 31), __shfl_sync(0xffffffffu, q.y, 31));
-                s = joiner.first(m, c, k == 0, l == 0);
+                s = joiner.first(m, c, k == 0, l == 0, watch);
                 if constexpr (PASS == MAPS) {
-                    joiner.gates_of_step(gates);
+                    joiner.gates_of_step(gates, watch);
                     s = apply(m, s);
-                    if (last && live && wt == W - 1 && l == 0) a.maps[seg * a.lanes + row] = make_float2(gates, s);
+                    const int range = last ? block_range(ex, watch.range()) : 0;
+                    if (last && live && wt == W - 1 && l == 0) a.maps[seg * a.lanes + row] = segment_map(gates, s, range);
                     joiner.hand_on(s, last, l == 0);
                     continue;
                 }
+            }
+            if constexpr (SUB < 32) {
+                watch.tile_of(q);
+                watch.state(s);
             }
             float y = ls > 0 ? apply(b, s) : s;
             // results over the inputs' registers: x becomes h or dx, h becomes dgate
@@ -922,6 +1069,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(ScanArgs a) {
         }
     }
     copies_wait_all();
+    if constexpr (PASS != MAPS) settle<BACKWARD, kRowCut<SUB>>(a, ex, at, watch, NW / W * R);
 }
 
 // ---- a few steps (a token for each of many sequences): a thread walks V lanes, nothing to join.

@@ -263,7 +263,9 @@ class Graph:
         without the axis.  The gradient reaches all three.  One step (an axis of size 1)
         with the last state as init is the form for serving one token at a time; a gate
         of 0 starts anew there, e.g. at a document's first token.  A state that is NaN stays
-        NaN, an infinite one infinite or NaN, through gates of 0 too (0 * inf)."""
+        NaN, an infinite one infinite or NaN, through gates of 0 too (0 * inf).  Gates may have any
+        size; where their products overflow, or underflow beside states above 10^6, the lanes
+        are walked step by step, which is slower."""
         gate, x = self._ensure(gate), self._ensure(x)
         self._float32("gated_scan", gate, x)
         shape = broadcast_shapes(gate.shape, x.shape)
