@@ -825,6 +825,87 @@ def _scan_program(cache_dir, shape=(3, 3000, 48), axis=1, seed=11):
     return prog, [tt.DeviceBuffer.from_numpy(v) for v in (gate, x, s, dh)], want
 
 
+def test_equal_outputs_and_gradients_keep_their_places(cache_dir):
+    rng = np.random.default_rng(17)
+    av, bv, cv = (_f32(rng.standard_normal([2, 3])) for _ in range(3))
+    g = tt.Graph()
+    a, b = g.input([2, 3]), g.input([2, 3])
+    out = tt.compile(g, [tt.relu(a + b), a + b, a * b, a + b], cache_dir=cache_dir).run({a: av, b: bv})
+    for o, w in zip(out, (np.maximum(av + bv, 0), av + bv, av * bv, av + bv), strict=True):
+        assert np.array_equal(o.numpy(), w)
+    g = tt.Graph()
+    a, b, c = g.input([2, 3]), g.input([2, 3]), g.input([2, 3])
+    grads = tt.gradients(g, tt.sum(c * c), {a: av, b: bv, c: cv}, cache_dir=cache_dir)
+    assert not grads[a].numpy().any() and not grads[b].numpy().any() and np.array_equal(grads[c].numpy(), 2 * cv)
+    # equal gradients of different targets: the two initial states of a scan over equal gates
+    g = tt.Graph()
+    gate, x, s1, s2 = g.input([2, 3]), g.input([2, 3]), g.input([3]), g.input([3])
+    h1, h2 = (tt.gated_scan(gate, x, init=s, axis=0) for s in (s1, s2))
+    res = tt.compile_gradients(g, tt.sum(tt.scan_last(h1)) + tt.sum(tt.scan_last(h2)), [s1, x, s2], outputs=[], cache_dir=cache_dir)
+    got = [o.numpy() for o in res.run({gate: av, x: bv, s1: cv[0], s2: cv[1]})]
+    want = av[0].astype(np.float64) * av[1]
+    assert [o.shape for o in got] == [(3,), (2, 3), (3,)]
+    for o in (got[0], got[2]):
+        R.assert_within(o, (want, 2 * R.U * np.abs(want)))
+
+
+def test_random_graphs_of_scans(cache_dir):
+    """Scans, last states and losses over one pool of views, in random roles, against torch's autodiff in 64 bits:
+    operands and launches shared in every way the schedule knows.  Gates are at most 1, so a step of
+    at most 40 adds a few roundings: 100 in all, 6e-6 of a result's norm."""
+    import torch
+
+    def scan(a, x, s, axis):
+        a, x = torch.broadcast_tensors(a, x)
+        a, x = a.movedim(axis, 0), x.movedim(axis, 0)
+        c = torch.zeros_like(x[0]) if s is None else torch.broadcast_to(s, x[0].shape)
+        h = []
+        for t in range(x.shape[0]):
+            c = a[t] * c + x[t]
+            h.append(c)
+        return torch.stack(h).movedim(0, axis), c
+
+    rng = np.random.default_rng(11)
+    for case in range(40):
+        T, H, D = int(rng.choice([3, 18, 40])), int(rng.integers(1, 4)), int(rng.choice([1, 3, 4, 8]))
+        full = [2, T, H, D]
+        shapes = [[2, T, H, 1], [2, T, D, H], full, [1, T, 1, D], [2, H, T, D], [T, H, 1]]
+        vals = [_f32(rng.uniform(-1, 1, s)) for s in shapes]
+        g = tt.Graph()
+        leaves = [g.input(s) for s in shapes]
+        ref = [torch.tensor(v, dtype=torch.float64, requires_grad=True) for v in vals]
+        pool = [leaves[0], tt.transpose(leaves[1], 2, 3), leaves[2], leaves[3], tt.transpose(leaves[4], 1, 2), leaves[5]]
+        rpool = [ref[0], ref[1].transpose(2, 3), ref[2], ref[3], ref[4].transpose(1, 2), ref[5]]
+        loss, rloss, outs, routs = 0.0, 0.0, [], []
+        for _ in range(3):
+            i, j = (int(v) for v in rng.integers(0, len(pool), 2))
+            if pool[i].shape != full and pool[j].shape != full:
+                j = int(rng.choice([1, 2, 4]))
+            init = None
+            if rng.random() < 0.5:
+                init = int(rng.integers(0, len(outs) + 1)) if outs else None
+            s, rs = (None, None) if init is None or init >= len(outs) else (outs[init], routs[init])
+            h = tt.gated_scan(pool[i], pool[j], init=s, axis=1)
+            rh, rlast = scan(rpool[i], rpool[j], rs, 1)
+            if rng.random() < 0.6:
+                loss, rloss = tt.sum(h * pool[2]) + loss, (rh * rpool[2]).sum() + rloss
+            last = tt.scan_last(h)
+            loss, rloss = tt.sum(last * last) + loss, (rlast * rlast).sum() + rloss
+            outs.append(last)
+            routs.append(rlast)
+            if rng.random() < 0.4 and T > 1:  # (the states as another scan's operand)
+                pool.append(h)
+                rpool.append(rh)
+        for flags in (0, tt.FLAG_NO_FUSION):
+            got = [o.numpy() for o in tt.compile_gradients(g, loss, leaves, outputs=[loss], cache_dir=cache_dir, flags=flags)
+                   .run(dict(zip(leaves, vals)))]
+            want = [rloss] + list(torch.autograd.grad(rloss, ref, allow_unused=True, retain_graph=True))
+            for o, r in zip(got, want):
+                r = np.zeros(o.shape) if r is None else r.detach().numpy()
+                assert o.shape == r.shape
+                assert np.linalg.norm(o - r) <= 6e-6 * max(np.linalg.norm(r), 1e-30), (case, flags)
+
+
 def test_on_streams_captured_and_replayed(cache_dir):
     runs = [_token_program(cache_dir), _scan_program(cache_dir), _scan_program(cache_dir, (5, 4000), 1, 12)]
     streams = [tt.Stream() for _ in runs]

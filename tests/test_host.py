@@ -222,6 +222,26 @@ def test_gradient_graph_structure(cache_dir):
     assert p.num_outputs == 2 and p.output_shapes == [[], [4, 3]]
 
 
+def test_equal_outputs_stay_apart(cache_dir):
+    """Outputs that are the same expression, or gradients that are the same values, keep their places."""
+    g = tt.Graph()
+    a, b = g.input([2, 3]), g.input([2, 3])
+    x, y, z = a + b, a + b, tt.relu(a)
+    p = tt.compile(g, [x, z, y], cache_dir=cache_dir, flags=HOST)
+    assert p.num_outputs == 3 and p.output_shapes == [[2, 3]] * 3
+    assert p.execution_plan().count("fused") + p.execution_plan().count("copy") >= 2
+    g = tt.Graph()
+    a, b, c, d = g.input([2, 3]), g.input([2, 3]), g.input([2, 3]), g.input([5])
+    # no path to a and b: two zeros of one shape; c is reached, d is not
+    p = tt.compile_gradients(g, tt.sum(c * c), [a, c, b, d], cache_dir=cache_dir, flags=HOST)
+    assert p.output_shapes == [[], [2, 3], [2, 3], [2, 3], [5]]
+    # an output that merges into a node that is none
+    g = tt.Graph()
+    a, b = g.input([2, 3]), g.input([2, 3])
+    p = tt.compile(g, [tt.relu(a + b), a + b, a + b], cache_dir=cache_dir, flags=HOST)
+    assert p.num_outputs == 3 and p.output_shapes == [[2, 3]] * 3
+
+
 def test_run_validates_inputs_before_device(cache_dir):
     g = tt.Graph()
     a = g.input([4])

@@ -578,11 +578,13 @@ Graph dce(const Graph& g, size_t* removed) {
 }
 
 // Common subexpression elimination keyed like src/optimizer/cse.cpp:9-40
-// (op, operand ids, shape, dtype, attributes); constants merge only on equal bits.
+// (op, operand ids, shape, dtype, attributes); constants merge only on equal bits.  Every output
+// stays one: an output equal to an earlier one becomes a copy of it (an identity reshape).
 Graph cse(const Graph& g, size_t* removed) {
     std::map<std::string, int> seen;
     std::vector<int> remap(g.nodes.size());
-    std::vector<bool> keep(g.nodes.size(), true);
+    std::vector<bool> keep(g.nodes.size(), true), is_output(g.nodes.size(), false), copied(g.nodes.size(), false);
+    for (int o : g.outputs) is_output[static_cast<size_t>(o)] = true;
     size_t cnt = 0;
     for (size_t i = 0; i < g.nodes.size(); ++i) {
         const Node& n = g.nodes[i];
@@ -610,6 +612,11 @@ Graph cse(const Graph& g, size_t* removed) {
         auto it = seen.find(key.str());
         if (it != seen.end()) {
             remap[i] = it->second;
+            if (is_output[i] && is_output[static_cast<size_t>(it->second)]) {
+                copied[i] = true;
+                continue;
+            }
+            if (is_output[i]) is_output[static_cast<size_t>(it->second)] = true;
             keep[i] = false;
             ++cnt;
         } else {
@@ -619,9 +626,21 @@ Graph cse(const Graph& g, size_t* removed) {
     if (removed) *removed = cnt;
     // Inputs of kept nodes must be remapped before rebuild sees them.
     Graph tmp = g;
-    for (size_t i = 0; i < tmp.nodes.size(); ++i)
-        for (int& k : tmp.nodes[i].in) k = remap[static_cast<size_t>(k)];
-    for (int& o : tmp.outputs) o = remap[static_cast<size_t>(o)];
+    for (size_t i = 0; i < tmp.nodes.size(); ++i) {
+        Node& n = tmp.nodes[i];
+        if (copied[i]) {
+            Node c;
+            c.op = TT_OP_RESHAPE;
+            c.dtype = n.dtype;
+            c.in = {static_cast<int>(i)};  // (its own place, which remap leads to the earlier output)
+            c.shape = n.shape;
+            c.id = n.id;
+            n = std::move(c);
+        }
+        for (int& k : n.in) k = remap[static_cast<size_t>(k)];
+    }
+    for (int& o : tmp.outputs)
+        if (!copied[static_cast<size_t>(o)]) o = remap[static_cast<size_t>(o)];
     std::vector<int> ident(g.nodes.size());
     for (size_t i = 0; i < ident.size(); ++i) ident[i] = static_cast<int>(i);
     return rebuild(tmp, ident, keep);
