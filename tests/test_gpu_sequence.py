@@ -269,6 +269,29 @@ def test_scan_where_products_of_gates_leave_the_range(cache_dir, shape, axis, ga
     R.assert_within(alone.run({na: gate, nx: x, ns: s}).numpy(), rlast)
 
 
+@pytest.mark.parametrize("shape,axis", [([3, 20], 1), ([3, 100], 1), ([2, 900], 1), ([5, 9000], 1), ([1, 70001], 1), ([2, 50, 7], 1),
+                                        ([2, 700, 40], 1), ([1, 5000, 40], 1), ([1, 70000, 3], 1)])
+@pytest.mark.parametrize("gate", [1.0, -1.0])
+def test_scan_of_states_near_the_largest_float(cache_dir, shape, axis, gate):
+    """A run of addends that overflows by itself, on a state that it brings from one end of the range to the other."""
+    T = shape[axis]
+    lane = list(shape)
+    del lane[axis]
+    sign = np.where(np.arange(T) // 6 % 2 == 0, 1.0, -1.0) * np.where(np.arange(T) % 2 == 1, np.sign(gate), 1.0)
+    if gate < 0:  # h[t] = -h[t-1] + x[t]: the same path with every other state's sign turned
+        sign = -sign
+    x = _f32(np.broadcast_to((1e38 * sign).reshape([T if i == axis else 1 for i in range(len(shape))]), shape))
+    init = np.full(lane, -3e38, np.float32)
+    g = tt.Graph()
+    nx, ns = g.input(shape), g.input(lane)
+    h = tt.gated_scan(gate, nx, init=ns, axis=axis)
+    out = [o.numpy() for o in tt.compile(g, [h, tt.scan_last(h)], cache_dir=cache_dir).run({nx: x, ns: init})]
+    rh, rlast = R.scan(np.full([1] * len(shape), gate), x, init, axis)
+    assert np.abs(rh[0]).max() < 3.1e38
+    R.assert_within(out[0], rh)
+    R.assert_within(out[1], rlast)
+
+
 @pytest.mark.parametrize("shape,axis", [([3, 640], 1), ([2, 700, 40], 1), ([1, 70000, 5], 1), ([1, 70001], 1)])
 def test_scan_in_windows_equals_the_whole_where_gates_grow(cache_dir, shape, axis):
     """Single windows, and their states handed on: no cut of the axis changes a state."""

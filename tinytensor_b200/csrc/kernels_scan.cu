@@ -66,9 +66,9 @@ __device__ __forceinline__ float apply(float2 m, float c) { return fmaf(m.x, c, 
 // First m, then n.
 __device__ __forceinline__ float2 join(float2 m, float2 n) { return make_float2(m.x * n.x, apply(n, m.y)); }
 
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN propagates
+__device__ __forceinline__ float max_abs(float a, float b, float c) {  // NaN propagates
     float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 
@@ -77,21 +77,21 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN propagates
 // product below the normal range has lost some 2^-146 at most, which is next to nothing (2^-119) of states of 2^27,
 // unless a run behind it grows.  So maps do unless one is GROWN, or one is TINY (|A| < 2^-90; part of a tile may
 // have 2^-121) and one LARGE: a run grows, or an H or a state is above 2^20 (states between tiles may then be
-// 2^27).  The two need not be one lane's: that costs time only.  States that are NaN are NaN either way.
+// 2^27).  An H that is not finite is GROWN too: the state it stands for starts from 0 and may overflow where the
+// true one, from another, does not.  The bits need not be one lane's: that costs time only.
 enum Range { GROWN = 1, TINY = 2, LARGE = 4 };
 constexpr float kTiny = 8.077935669e-28f, kLarge = 1048576.0f;  // 2^-90, 2^20
 struct Watch {
     float run = 0.0f, tile = 0.0f, least = 1.0f, most = 0.0f;  // largest |A| of runs, of tiles, least |A|, largest |H|
-    __device__ __forceinline__ void run_of(float a) { run = max_nan(run, fabsf(a)); }
-    __device__ __forceinline__ void product(float a) { least = fminf(least, fabsf(a)); }
-    __device__ __forceinline__ void state(float c) { most = fmaxf(most, fabsf(c)); }
-    __device__ __forceinline__ void tile_of(float2 m) {
-        tile = max_nan(tile, fabsf(m.x));
-        product(m.x);
-        state(m.y);
+    __device__ __forceinline__ void runs(float a, float b) { run = max_abs(run, a, b); }
+    __device__ __forceinline__ void tile_of(float a) {
+        tile = max_abs(tile, a, a);
+        product(a);
     }
+    __device__ __forceinline__ void product(float a) { least = fminf(least, fabsf(a)); }
+    __device__ __forceinline__ void states(float h, float s) { most = max_abs(most, h, s); }
     __device__ __forceinline__ int range() const {
-        return (run <= 2.0f && tile <= 16.0f ? 0 : GROWN) | (least < kTiny ? TINY : 0) | (run <= 1.0f && most <= kLarge ? 0 : LARGE);
+        return (run <= 2.0f && tile <= 16.0f && most <= 3.402823466e38f ? 0 : GROWN) | (least < kTiny ? TINY : 0) | (run <= 1.0f && most <= kLarge ? 0 : LARGE);
     }
 };
 __device__ __forceinline__ bool maps_do(int range) { return (range & GROWN) == 0 && (range & (TINY | LARGE)) != (TINY | LARGE); }
@@ -197,11 +197,13 @@ __device__ __forceinline__ float segment_state(const ScanArgs& a, Exchange<NW, L
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
             m = join(m, q[u]);
-            watch.run = fabsf(q[u].x) <= 4294967296.0f ? fmaxf(watch.run, fminf(fabsf(q[u].x), 1.5f)) : INFINITY;  // (grows: LARGE)
-            watch.tile_of(make_float2(fabsf(m.x) <= 4294967296.0f ? fminf(fabsf(m.x), 1.0f) : INFINITY, q[u].y));
+            // (a segment that grows is LARGE; one whose map does not do, and joins that would overflow, GROWN)
+            const float grows = fabsf(q[u].x) <= 4294967296.0f ? fminf(fabsf(q[u].x), 1.5f) : INFINITY;
+            watch.runs(grows, fabsf(m.x) <= 4294967296.0f ? 0.0f : INFINITY);
+            watch.product(m.x);
+            watch.states(q[u].y, c);
         }
     }
-    watch.state(c);
     __syncthreads();  // (the unit before may still be reading)
     if (writer) ex.warp[0][warp][l] = m;
     __syncthreads();
@@ -223,7 +225,7 @@ struct Joiner {
     // m: the map of this warp's tile.  Returns the state before the tile; c is the state before
     // the first step (later steps find theirs in the exchange).
     __device__ __forceinline__ float first(float2 m, float c, bool first_step, bool writer, Watch& watch) {
-        watch.tile_of(m);
+        watch.tile_of(m.x);
         if (writer) ex.warp[buf][warp][l] = m;
         __syncthreads();
         if (at.size > 1) {
@@ -252,7 +254,7 @@ struct Joiner {
         } else {
             for (int w = 0; w < wt; ++w) s = apply(ex.warp[buf][wr * W + w][l], s);
         }
-        watch.state(s);
+        watch.states(m.y, s);
         return s;
     }
     // s: the state behind this warp's tile.  The step's last tile hands it to the next step
@@ -318,7 +320,7 @@ __device__ __noinline__ void walk_again(const ScanArgs& a, int64_t first, int64_
         const int64_t gs = per_step(SI_GATE), xs = per_step(SI_X), hs = per_step(SI_H);
         const float* carry = ptr(SI_CARRY, 0);
         float c = carry ? __ldg(carry) : 0.0f;
-        constexpr int N = 16;
+        constexpr int N = CUT > 0 ? 8 : 16;  // (16 steps of rows spill registers)
         struct Batch {
             float g[N], x[N], h[N];
         };
@@ -622,10 +624,9 @@ __global__ void __launch_bounds__(NW * 32, 16 / NW) scan_cols_kernel(const __gri
             // this thread's maps, those of the threads before it in time, and the tile's
             float2 m[V], before[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                m[v] = tile_map<BACKWARD, TS>([&](int j) { return ga[j][v]; }, [&](int j) { return xv[j][v]; });
-                watch.run_of(m[v].x);
-            }
+            for (int v = 0; v < V; ++v) m[v] = tile_map<BACKWARD, TS>([&](int j) { return ga[j][v]; }, [&](int j) { return xv[j][v]; });
+#pragma unroll
+            for (int v = 0; v < V; v += 2) watch.runs(m[v].x, m[V > 1 ? v + 1 : 0].x);
 #pragma unroll
             for (int d = COLS; d < 32; d *= 2) {
 #pragma unroll
@@ -975,7 +976,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(const __grid_
             issue(stage);
             float2 q = tile_map<BACKWARD, kRun>([&](int j) { return ga[BACKWARD ? kRun - 1 - j : j]; },
                                                 [&](int j) { return xv[BACKWARD ? kRun - 1 - j : j]; });
-            watch.run_of(q.x);
+            watch.runs(q.x, q.x);
 #pragma unroll
             for (int d = 1; d < SUB; d *= 2) {
                 const float2 b = make_float2(__shfl_up_sync(0xffffffffu, q.x, d), __shfl_up_sync(0xffffffffu, q.y, d));
@@ -998,8 +999,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) scan_rows_kernel(const __grid_
                 }
             }
             if constexpr (SUB < 32) {
-                watch.tile_of(q);
-                watch.state(s);
+                watch.tile_of(q.x);
+                watch.states(q.y, s);
             }
             float y = ls > 0 ? apply(b, s) : s;
             // results over the inputs' registers: x becomes h or dx, h becomes dgate
