@@ -594,6 +594,19 @@ def test_preference_loss_of_many_short_rows(cache_dir, N, T, V):
     _check(out, R.preference(x0, k, ref, beta, 0.125, g))
 
 
+@pytest.mark.parametrize("N, T, V", [(32, 32, 1281), (31, 32, 1281), (33, 31, 1283), (300, 32, 1301), (32, 128, 1290), (32, 129, 1290),
+                                     (32, 32, 6144), (32, 32, 6145), (400, 33, 1280)])
+def test_preference_loss_of_many_pairs(cache_dir, N, T, V):
+    """Sizes around which pairs go to a cluster each or to three launches."""
+    rng = np.random.default_rng(N + T + V)
+    shape = [N, 2, T]
+    x, k = 3 * rng.standard_normal(shape + [V], dtype=np.float32), _tokens(rng, shape, V, empty=False)
+    k[1, 0], k[N - 1, 1] = -1, -1
+    ref, g = _f32(R.logprob(x, k)[0][0] + 0.3 * rng.standard_normal(shape)), _f32(rng.standard_normal([N]))
+    out = _run_tokens(cache_dir, lambda a, b, r: tt.preference_loss(a, b, r, beta=0.2, smoothing=0.125), x, k, [ref], g)
+    _check(out, R.preference(x, k, ref, 0.2, 0.125, g))
+
+
 def test_preference_loss_saturates(cache_dir):
     """Sums far apart: the loss is -z or 0 and its slope -beta or 0, without overflow."""
     x = np.zeros([2, 2, 1, 4], np.float32)

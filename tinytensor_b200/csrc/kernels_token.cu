@@ -900,14 +900,19 @@ int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 // A pair in one cluster (one launch) or all rows, then all pairs, then all rows again (three).
 bool pairs_in_clusters(const TokenDesc& d) {
     if (d.n0 == 0 || d.n1 == 0 || d.n0 > 0x7fffffff / kPairCluster) return false;
-    // Clusters save two launches where pairs are few and small (us, a cluster a pair against three launches: 3 of
-    // 2x37x257 11 against 13, 60 of 2x32x250 11 against 17, 16 of 2x64x1000 15 against 17; but 16 of 2x128x1000 25
-    // against 19, 128 of 2x64x250 29 against 25), and a read from memory where the pairs that run at the same time
-    // stay in L2 and their rows are long (64 of 2x64x4096 60 against 87, 100 of 2x64x2000 51 against 54; but 16 of
-    // 2x256x4000 113 against 64, 1000 of 2x16x1000 117 against 70, 16 of 2x128x8000 116 against 65).
+    // us, a cluster a pair against three launches, L2 flushed before each.  Few and small pairs save two launches: 3
+    // of 2x37x257 11 against 13, 60 of 2x32x250 11 against 17, 16 of 2x64x1000 15 against 17; but 16 of 2x128x1000
+    // 25 against 19, 128 of 2x64x250 29 against 25.
     const int64_t passes = (d.n1 + 63) / 64;  // rows of a warp
     if (passes <= 2 && passes * ((d.V + 1023) / 1024) <= 4 && d.n0 * passes <= 148) return true;
-    return d.n0 >= 32 && d.n0 <= 256 && d.n1 >= 64 && d.n1 <= 256 && d.V > 1024 && d.V <= 4096;
+    // More pairs, while their clusters fill the card and a warp has one to four rows, gain where a row is two to six
+    // steps of a warp's walk of 1024 values, so that loads hide its sums and the second read comes partly from L2:
+    // 48 of 2x64x4096 51 against 76, 320 of 2x32x4096 143 against 205, 256 of 2x96x4096 348 against 459, 1000 of
+    // 2x64x1500 358 against 426, 64 of 2x32x6000 47 against 61; but 16 of 2x128x2000 41 against 29 (SMs without a
+    // CTA), 1000 of 2x24x1025 184 against 143 (warps without a row), 74 of 2x192x2000 139 against 125 (six rows a
+    // warp), 148 of 2x48x1025 61 against 51 (short rows), 16 of 2x128x8000 126 against 72, 32 of 2x48x8000 70
+    // against 56 (long ones).
+    return d.n0 * kPairCluster >= 256 && d.n1 >= 64 && passes <= 4 && d.V > 1280 && d.V <= 6144;
 }
 
 // Launch configuration of `blocks` CTAs in clusters.
