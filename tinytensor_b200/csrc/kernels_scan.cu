@@ -425,7 +425,7 @@ __device__ __forceinline__ void store_vec(float* p, const float* v, bool stream)
 // V = 1 takes any strides.  A thread reads back what it copied itself, or a thread of its warp
 // (broadcast values), so the ring needs no block barrier.
 // 8 x 2048 x 1024: 33 us forward (6.1 TB/s), 61 us backward with all gradients (5.5 TB/s: 256 CTAs on the
-// 296 places of the card); 1 x 65536 x 1024 147 us (5.5 TB/s, a cluster barrier a step).  Where there are fewer
+// 296 places of the card); 1 x 65536 x 1024 150 us (5.4 TB/s, a cluster barrier a step).  Where there are fewer
 // lanes a step's latency bounds it, not the bytes: a gate per head of 64 lanes, 4 x 2048 x 1024, 23 and
 // 35 us (3.0 and 2.9 TB/s).
 template <bool BACKWARD>

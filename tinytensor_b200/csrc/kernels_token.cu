@@ -477,9 +477,9 @@ __global__ void __launch_bounds__(kStream, 4) token_stream_kernel(TokenArgs a) {
 //   join:  info(n + 4), parts full(n) -> exchange -> scalars(n) -> scalars full(n)
 // What bounds it besides the bytes is the instructions a row costs on top of its values, so warps
 // whose vectors all lie inside the row move them without checks.
-// Clusters of 4 (71 run at a time: 284 of the 296 places) take 336 us for 8192 rows of 32768 with a ninth of
-// them padding (5.7 TB/s), 164 us for 4096 of 32001 (5.5); clusters of 6 147 us for 2177 of
-// 50001 (5.0).
+// Clusters of 4 (71 run at a time: 284 of the 296 places) take 336 to 360 us for 8192 rows of 32768 with a
+// ninth of them padding (5.7 to 5.3 TB/s, by box), 164 to 168 us for 4096 of 32001 (5.5 to 5.4); clusters of 6 147 us
+// for 2177 of 50001 (5.0).
 struct RowInfo {
     const float* x;
     float* dx;

@@ -319,7 +319,8 @@ class Graph:
 
         Padding is a negative token: its logits are not read (whatever they hold), its value
         and its gradient are 0.  A token of V or more gives NaN and DeviceStatusError.  With
-        seed = -weights it is the cross-entropy's gradient."""
+        seed = -weights it is the cross-entropy's gradient.  Programs with a gradient and without
+        one round differently: the same value from both differs in its last bits."""
         logits, tokens = self._token_operands("token_logprob", logits, tokens)
         return self._token_node(_lib.OP_TOKEN_LOGPROB, tokens.shape, [logits, tokens], ())
 
@@ -331,7 +332,8 @@ class Graph:
               + kl * (exp(ref_logp - p) - (ref_logp - p) - 1)
 
         old_logp, advantage and ref_logp broadcast to the tokens' shape and count as data:
-        the gradient reaches the logits only.  kl > 0 takes ref_logp, kl = 0 does not.
+        the gradient reaches the logits only.  kl > 0 takes ref_logp, kl = 0 does not.  With
+        old_logp from a program of its own, r of the same policy is 1 up to that rounding.
         Padding as in token_logprob, whatever the other operands hold there."""
         logits, tokens = self._token_operands("policy_loss", logits, tokens)
         if len(clip) != 2 or not 0.0 <= clip[0] <= 1.0 or not 0.0 <= clip[1] < float("inf"):
